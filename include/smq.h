@@ -360,6 +360,121 @@ smq_status smq_argmax_advance_embed(const float *logits, uint32_t vocab, const u
                                     int32_t *pos, uint32_t *count, uint32_t *history, uint32_t capacity,
                                     const smq_qmat *embed, float *x);
 
+/* ---- paged KV cache: several sequences at once -----------------------------
+ * No reference counterpart (the reference holds one sequence in one f32 or f16
+ * cache, src/model.h:59-61): the caches of many sequences in pages of one
+ * pool, and batches of sequences that bring different numbers of new tokens
+ * (one while decoding, a chunk of a prompt). One pool pair holds one layer.
+ *
+ * A page holds page_size positions of every KV head: keys as
+ * [kv_head][position][head_dim], values as [kv_head][head_dim][position].
+ * SMQ_KV_Q8 holds int8 codes and an f32 scale per position and 32-wide block
+ * of a head, [kv_head][ceil(head_dim / 32)][position] per page: the activation
+ * quantizer's rule (smq_quantize_q8) over each head's dims, the last block
+ * shorter where head_dim is no multiple of 32. */
+#define SMQ_KV_F32 0u
+#define SMQ_KV_F16 1u
+#define SMQ_KV_Q8 2u
+typedef struct smq_paged_kv {
+    void *keys, *values;              /* device, 16-byte aligned: `pages` pages each */
+    float *key_scales, *value_scales; /* device, 16-byte aligned, SMQ_KV_Q8 only */
+    uint32_t type;                    /* SMQ_KV_* */
+    uint32_t page_size;               /* positions of a page: 16, 32, 64, 128 or 256 */
+    uint32_t pages;
+} smq_paged_kv;
+/* A batch of seqs sequences. The new tokens' rows lie one after another: those
+ * of sequence s are rows begin[s] .. begin[s + 1] - 1, n of them (0 allowed),
+ * and row begin[s] + i stands at position length[s] - n + i. Positions x of
+ * sequence s lie in page table[s * table_stride + x / page_size]. The arrays
+ * are read on the device, so a captured launch replays with new contents.
+ * Rows before begin[0] and from begin[seqs] on are padding: never read, never
+ * written.
+ *
+ * What the host cannot check raises the sticky numeric flag on the device and
+ * touches nothing out of range: a page id outside [0, pages) (only of a page
+ * that the call needs), a row whose position is negative, at or past
+ * shape->context or past the table (not stored, not read, its attention is
+ * 0), a begin that does not ascend within 0 .. tokens (which rows are computed
+ * is then unspecified). Rows in such pages are not stored and not read,
+ * positions in them not seen. */
+typedef struct smq_paged_batch {
+    const int32_t *begin;  /* device, seqs + 1 */
+    const int32_t *length; /* device, seqs: positions including the new tokens */
+    const int32_t *table;  /* device, seqs * table_stride page ids */
+    uint32_t seqs, tokens, table_stride;
+} smq_paged_batch;
+/* smq_rope_kv for a paged cache: every new token's k (kv_heads * head_dim
+ * floats a row) rotated by its position's table row (rotary_pairs floats each,
+ * shape->context rows) and v into the cache as kv->type holds them; k itself
+ * is left as it is. q's rows, rotated, go to q_out (q_out == q rotates in
+ * place; both NULL: none). Rotation as smq_rope_kv's, bit for bit; f16
+ * rounds to nearest even. A value that the type cannot hold as a finite number
+ * raises the numeric flag (f16: infinite; Q8: its block gets a NaN scale).
+ * Sequences must not share a page that the call writes to. shape: head_dim a
+ * multiple of 16, at most 256, context at most 1,048,576. Asynchronous. */
+smq_status smq_paged_rope_kv(const float *q, float *q_out, const float *k, const float *v,
+                             const smq_paged_batch *batch, const smq_attn_shape *shape, const float *cos_table,
+                             const float *sin_table, const smq_paged_kv *kv);
+/* The batch's rows out of the cache as f32: keys and values row r =
+ * kv_heads * head_dim floats, what the cache holds at the row's position (f16
+ * exactly, Q8 code * scale). With begin the running sum of length, whole
+ * sequences, for instance into contiguous caches. Asynchronous. */
+smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *shape, const smq_paged_kv *kv,
+                          float *keys, float *values);
+/* Attention of the new tokens (their keys and values are in the cache): head h
+ * of the row at position p over the positions j <= p of its sequence, with
+ * shape->window w > 0 only those with j > p - w or j < sinks:
+ *   att[h] = sum_j softmax_j(q[h] . k[j] / sqrt(head_dim)) v[j]
+ * (KV head h / (heads / kv_heads)); f32 sums and statistics, each product of
+ * f32 accuracy, no order of the sums promised beyond: the same call gives the
+ * same bits. A row that sees nothing is 0. Keys and values at positions that a
+ * row does not see, and slots past a sequence's length, never matter, NaN and
+ * infinities included; a visible one that is not finite leaves the row's result
+ * unspecified. Pages that no row sees may have any id. att must not overlap q.
+ * workspace (device, 16-byte aligned, may be NULL): where the call splits long
+ * sequences over workgroups, their partial results;
+ * smq_paged_attention_workspace gives the bytes that allow the widest split,
+ * fewer bytes split less. Calls that may overlap in time, replays of different
+ * graphs among them, must not share one. Asynchronous, capturable. */
+size_t smq_paged_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape);
+smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                               uint32_t sinks, const smq_paged_kv *kv, void *workspace, size_t workspace_bytes);
+
+/* ---- logits of several rows before the choice of a token -------------------
+ * No reference counterpart (sampler.c:57-63 only skips banned ids). For each
+ * row, with c the times id v stands in the row's history:
+ *   l = logits[v]
+ *   c > 0: l = (l > 0 ? l / repetition : l * repetition) - (c * frequency + presence)
+ *   l += the sum of the row's biases for v
+ *   l = -inf where the row's mask does not allow v
+ * and the greedy token: smq_argmax's choice (the lowest id on ties; a NaN only
+ * where it is the first candidate) among the allowed ids, UINT32_MAX if there
+ * is none. Ids at or past vocab in history and bias_ids are skipped. Lists end
+ * at history_count and bias_count whatever the begin arrays say. */
+typedef struct smq_logit_rules {
+    const uint32_t *history;      /* device; NULL: no penalties */
+    const int32_t *history_begin; /* device, rows + 1: row r's ids are history[history_begin[r]] .. */
+    uint32_t history_count;
+    const float *penalty;         /* device, rows x 3: repetition, presence, frequency (1, 0, 0: none) */
+    const uint32_t *bias_ids;     /* device; NULL: no biases */
+    const float *bias;            /* device: one for each of bias_ids */
+    const int32_t *bias_begin;    /* device, rows + 1 */
+    uint32_t bias_count;
+    const uint32_t *allowed;      /* device, allowed_rows x ceil(vocab / 32) words, bit v % 32 of word v / 32; NULL: none */
+    uint32_t allowed_rows;
+    const int32_t *mask_row;      /* device, rows: the row of `allowed`, negative: no mask; NULL: row r of allowed.
+                                   * An index at or past allowed_rows raises the numeric flag and allows nothing. */
+} smq_logit_rules;
+/* Row r of logits at logits + r * stride, of out at out + r * out_stride (out
+ * may be logits with the same stride; NULL: only the tokens); token (rows, may
+ * be NULL when out is not). rules NULL: only the choice. workspace (device,
+ * 16-byte aligned, smq_logits_workspace bytes) is needed with token; calls that
+ * may overlap in time must not share one. Asynchronous, capturable. */
+size_t smq_logits_workspace(uint32_t rows, uint32_t vocab);
+smq_status smq_logits_adjust(const float *logits, size_t stride, uint32_t rows, uint32_t vocab,
+                             const smq_logit_rules *rules, float *out, size_t out_stride, uint32_t *token,
+                             void *workspace, size_t workspace_bytes);
+
 /* ---- Q5 weight conversion (src/kernels.h:205, kernels.c:1064-1117) -------
  * quantize_q5_row: cols floats x -> ceil(cols/32) Q5 blocks (22 B each) at
  * out, byte for byte the reference's: signed extreme, the first minimum of 21

@@ -66,6 +66,22 @@ class _AttnShape(ctypes.Structure):
                 ("context", _u32)]
 
 
+class _PagedKv(ctypes.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp), ("key_scales", _vp), ("value_scales", _vp), ("type", _u32),
+                ("page_size", _u32), ("pages", _u32)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("begin", _vp), ("length", _vp), ("table", _vp), ("seqs", _u32), ("tokens", _u32),
+                ("table_stride", _u32)]
+
+
+class _LogitRules(ctypes.Structure):
+    _fields_ = [("history", _vp), ("history_begin", _vp), ("history_count", _u32), ("penalty", _vp),
+                ("bias_ids", _vp), ("bias", _vp), ("bias_begin", _vp), ("bias_count", _u32), ("allowed", _vp),
+                ("allowed_rows", _u32), ("mask_row", _vp)]
+
+
 _SIGS = {
     "smq_last_status": (ctypes.c_int, []),
     "smq_last_error": (ctypes.c_char_p, []),
@@ -125,6 +141,15 @@ _SIGS = {
     "smq_argmax_advance": (ctypes.c_int, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32]),
     "smq_argmax_advance_embed": (ctypes.c_int, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, ctypes.POINTER(_QMat),
                                                 _vp]),
+    "smq_paged_rope_kv": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape),
+                                         _vp, _vp, ctypes.POINTER(_PagedKv)]),
+    "smq_paged_read": (ctypes.c_int, [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape),
+                                      ctypes.POINTER(_PagedKv), _vp, _vp]),
+    "smq_paged_attention_workspace": (_sz, [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape)]),
+    "smq_paged_attention": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape), _u32,
+                                           ctypes.POINTER(_PagedKv), _vp, _sz]),
+    "smq_logits_workspace": (_sz, [_u32, _u32]),
+    "smq_logits_adjust": (ctypes.c_int, [_vp, _sz, _u32, _u32, ctypes.POINTER(_LogitRules), _vp, _sz, _vp, _vp, _sz]),
     "smq_quantize_q5_row": (None, [_vp, _u32, _vp]),
     "smq_quantize_q5_rows": (ctypes.c_int, [_vp, _u32, _u32, _vp]),
     "smq_dequantize_q8_row": (None, [_vp, _u32, _vp]),
@@ -552,6 +577,74 @@ def argmax_advance_embed(logits, vocab, banned, token, pos, count, history, capa
     e = embed._c()
     _check(load().smq_argmax_advance_embed(_p(logits), vocab, _p(banned), _p(token), _p(pos), _p(count),
                                            _p(history), capacity, ctypes.byref(e), _p(x)))
+
+
+# ---- paged KV cache: several sequences at once
+KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+
+
+def paged_kv(keys, values, key_scales, value_scales, kv_type, page_size, pages):
+    """The pool of a layer's pages (smq_paged_kv); holds its buffers."""
+    kv = _PagedKv(_p(keys), _p(values), _p(key_scales), _p(value_scales), kv_type, page_size, pages)
+    kv._keep = (keys, values, key_scales, value_scales)
+    return kv
+
+
+def paged_batch(begin, length, table, seqs, tokens, table_stride):
+    """The sequences of a call and their new tokens' rows (smq_paged_batch); holds its buffers."""
+    b = _PagedBatch(_p(begin), _p(length), _p(table), seqs, tokens, table_stride)
+    b._keep = (begin, length, table)
+    return b
+
+
+def paged_rope_kv(q, q_out, k, v, batch, shape, cos_table, sin_table, kv):
+    """smq_paged_rope_kv: RoPE, and the new tokens' keys and values into their pages as kv holds them."""
+    _check(load().smq_paged_rope_kv(_p(q), _p(q_out), _p(k), _p(v), batch, shape, _p(cos_table), _p(sin_table), kv))
+
+
+def paged_read(batch, shape, kv, keys, values):
+    """smq_paged_read: the batch's rows out of the pages as f32."""
+    _check(load().smq_paged_read(batch, shape, kv, _p(keys), _p(values)))
+
+
+def paged_attention_workspace(batch, shape):
+    """Bytes of workspace that allow paged_attention its widest split."""
+    n = load().smq_paged_attention_workspace(batch, shape)
+    if not n:
+        _check()
+    return n
+
+
+def paged_attention(q, att, batch, shape, sinks, kv, workspace=None, workspace_bytes=0):
+    """smq_paged_attention: the new tokens over their sequences' pages, causal, with shape's window and `sinks` first
+    positions that stay visible."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+        workspace_bytes = workspace.nbytes
+    _check(load().smq_paged_attention(_p(q), _p(att), batch, shape, sinks, kv, _p(workspace), workspace_bytes))
+
+
+# ---- logits of several rows before the choice of a token
+def logit_rules(history=None, history_begin=None, history_count=0, penalty=None, bias_ids=None, bias=None,
+                bias_begin=None, bias_count=0, allowed=None, allowed_rows=0, mask_row=None):
+    """Penalties over a history, biases and grammar masks (smq_logit_rules); holds its buffers."""
+    r = _LogitRules(_p(history), _p(history_begin), history_count, _p(penalty), _p(bias_ids), _p(bias),
+                    _p(bias_begin), bias_count, _p(allowed), allowed_rows, _p(mask_row))
+    r._keep = (history, history_begin, penalty, bias_ids, bias, bias_begin, allowed, mask_row)
+    return r
+
+
+def logits_workspace(rows, vocab):
+    return load().smq_logits_workspace(rows, vocab)
+
+
+def logits_adjust(logits, rows, vocab, rules, out, token, workspace=None, workspace_bytes=0, stride=None,
+                  out_stride=None):
+    """smq_logits_adjust: rows of logits under the rules into out (None: not wanted), and each row's greedy token."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+        workspace_bytes = workspace.nbytes
+    _check(load().smq_logits_adjust(_p(logits), vocab if stride is None else stride, rows, vocab, rules, _p(out),
+                                    vocab if out_stride is None else out_stride, _p(token), _p(workspace),
+                                    workspace_bytes))
 
 
 def numeric_check():

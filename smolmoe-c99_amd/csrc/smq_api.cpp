@@ -1436,6 +1436,210 @@ smq_status smq_decode_advance(int32_t *pos, uint32_t *count, const uint32_t *tok
                : t_status;
 }
 
+static bool paged_args(const smq_paged_batch *b, const smq_attn_shape *shape, const smq_paged_kv *kv, const char *who,
+                       smq::PagedArgs *out) {
+    if (!b || !shape) {
+        set_status(SMQ_ERR_RANGE, "%s: NULL argument", who);
+        return false;
+    }
+    smq::PagedArgs a;
+    memset(&a, 0, sizeof(a));
+    if (!shape->heads || !shape->kv_heads || shape->heads % shape->kv_heads || !shape->head_dim ||
+        shape->head_dim % 16 || shape->head_dim > smq::MAX_HEAD_DIM || shape->rotary_pairs > shape->head_dim / 2 ||
+        shape->heads > 65535 || !shape->context || shape->context > smq::MAX_PAGED_CONTEXT) {
+        set_status(SMQ_ERR_RANGE,
+                   "%s: unsupported shape (heads %u, kv_heads %u, head_dim %u, a multiple of 16 <= %u, pairs %u, "
+                   "context %u <= %u)",
+                   who, shape->heads, shape->kv_heads, shape->head_dim, smq::MAX_HEAD_DIM, shape->rotary_pairs,
+                   shape->context, smq::MAX_PAGED_CONTEXT);
+        return false;
+    }
+    if (b->seqs > (1u << 20) || b->tokens > (1u << 24) || (b->seqs && !b->table_stride) || b->table_stride > (1u << 20)) {
+        set_status(SMQ_ERR_RANGE, "%s: unsupported batch (%u sequences <= 2^20, %u tokens <= 2^24, table stride %u of 1 .. 2^20)",
+                   who, b->seqs, b->tokens, b->table_stride);
+        return false;
+    }
+    a.begin = b->begin;
+    a.length = b->length;
+    a.table = b->table;
+    a.seqs = b->seqs;
+    a.tokens = b->tokens;
+    a.table_stride = b->table_stride;
+    a.heads = shape->heads;
+    a.kv_heads = shape->kv_heads;
+    a.head_dim = shape->head_dim;
+    a.nb = (shape->head_dim + smq::QK - 1) / smq::QK;
+    a.pairs = shape->rotary_pairs;
+    a.window = shape->window;
+    a.context = shape->context;
+    a.limit = a.context;
+    a.flag = g.flag;
+    if (kv) {
+        if (kv->type > SMQ_KV_Q8 || kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)) ||
+            kv->pages > 0x7fffffffu) {
+            set_status(SMQ_ERR_RANGE, "%s: unsupported cache (type %u, page size %u of 16, 32, 64, 128 or 256, %u pages)",
+                       who, kv->type, kv->page_size, kv->pages);
+            return false;
+        }
+        a.keys = kv->keys;
+        a.values = kv->values;
+        a.ks = kv->key_scales;
+        a.vs = kv->value_scales;
+        a.type = kv->type;
+        a.pages = kv->pages;
+        while ((1u << a.shift) < kv->page_size) ++a.shift;
+        if ((uint64_t)a.table_stride << a.shift < a.limit) a.limit = a.table_stride << a.shift;
+    }
+    *out = a;
+    return true;
+}
+
+/* The descriptors' arrays, of a batch that is not empty. */
+static bool paged_extents(const smq::PagedArgs &a, const char *who) {
+    static const size_t bytes[3] = {4, 2, 1};
+    const size_t positions = (size_t)a.pages << a.shift, kd = (size_t)a.kv_heads * a.head_dim;
+    const size_t scales = a.type == SMQ_KV_Q8 ? positions * a.kv_heads * a.nb * 4 : 0;
+    if (!a.pages) {
+        set_status(SMQ_ERR_RANGE, "%s: a cache without pages", who);
+        return false;
+    }
+    if (((uintptr_t)a.keys | (uintptr_t)a.values | (scales ? (uintptr_t)a.ks | (uintptr_t)a.vs : 0)) & 15) {
+        set_status(SMQ_ERR_RANGE, "%s: the pools must be 16-byte aligned", who);
+        return false;
+    }
+    return extent_ok(a.begin, ((size_t)a.seqs + 1) * 4, "begin") && extent_ok(a.length, (size_t)a.seqs * 4, "length") &&
+           extent_ok(a.table, (size_t)a.seqs * a.table_stride * 4, "table") &&
+           extent_ok(a.keys, positions * kd * bytes[a.type], "keys") &&
+           extent_ok(a.values, positions * kd * bytes[a.type], "values") && extent_ok(a.ks, scales, "key scales") &&
+           extent_ok(a.vs, scales, "value scales");
+}
+
+smq_status smq_paged_rope_kv(const float *q, float *q_out, const float *k, const float *v,
+                             const smq_paged_batch *batch, const smq_attn_shape *shape, const float *cos_table,
+                             const float *sin_table, const smq_paged_kv *kv) {
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!kv) return set_status(SMQ_ERR_RANGE, "paged_rope_kv: the cache is NULL");
+    if (!paged_args(batch, shape, kv, "paged_rope_kv", &a)) return t_status;
+    if (!q != !q_out) return set_status(SMQ_ERR_RANGE, "paged_rope_kv: q without q_out, or q_out without q");
+    if (!a.seqs || !a.tokens) return SMQ_OK;
+    const size_t table = (size_t)a.context * a.pairs * 4, qd = (size_t)a.heads * a.head_dim,
+                 kd = (size_t)a.kv_heads * a.head_dim;
+    if (!paged_extents(a, "paged_rope_kv") || !extent_ok(q, q ? a.tokens * qd * 4 : 0, "q") ||
+        !extent_ok(q_out, q ? a.tokens * qd * 4 : 0, "q_out") || !extent_ok(k, a.tokens * kd * 4, "k") ||
+        !extent_ok(v, a.tokens * kd * 4, "v") || !extent_ok(cos_table, table, "cos table") ||
+        !extent_ok(sin_table, table, "sin table"))
+        return t_status;
+    return hip_ok(smq::launch_paged_rope_kv(a, q, q_out, k, v, cos_table, sin_table, g.cur), "paged_rope_kv") ? SMQ_OK
+                                                                                                            : t_status;
+}
+
+smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *shape, const smq_paged_kv *kv,
+                          float *keys, float *values) {
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!kv) return set_status(SMQ_ERR_RANGE, "paged_read: the cache is NULL");
+    if (!paged_args(batch, shape, kv, "paged_read", &a)) return t_status;
+    if (!a.seqs || !a.tokens) return SMQ_OK;
+    const size_t rows = (size_t)a.tokens * a.kv_heads * a.head_dim * 4;
+    if (!paged_extents(a, "paged_read") || !extent_ok(keys, rows, "key rows") || !extent_ok(values, rows, "value rows"))
+        return t_status;
+    return hip_ok(smq::launch_paged_read(a, keys, values, g.cur), "paged_read") ? SMQ_OK : t_status;
+}
+
+size_t smq_paged_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape) {
+    smq::PagedArgs a;
+    return paged_args(batch, shape, nullptr, "paged_attention_workspace", &a) ? smq::paged_attention_workspace(a) : 0;
+}
+
+smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                               uint32_t sinks, const smq_paged_kv *kv, void *workspace, size_t workspace_bytes) {
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!kv) return set_status(SMQ_ERR_RANGE, "paged_attention: the cache is NULL");
+    if (!paged_args(batch, shape, kv, "paged_attention", &a)) return t_status;
+    if (!a.seqs || !a.tokens) return SMQ_OK;
+    a.sinks = sinks;
+    const size_t rows = (size_t)a.tokens * a.heads * a.head_dim * 4;
+    if (!workspace) workspace_bytes = 0;
+    if ((uintptr_t)workspace & 15)
+        return set_status(SMQ_ERR_RANGE, "paged_attention: the workspace must be 16-byte aligned");
+    if (!paged_extents(a, "paged_attention") || !extent_ok(q, rows, "q") || !extent_ok(att, rows, "att") ||
+        !extent_ok(workspace, workspace_bytes, "workspace"))
+        return t_status;
+    return hip_ok(smq::launch_paged_attention(a, q, att, workspace, workspace_bytes, g.cur), "paged_attention")
+               ? SMQ_OK
+               : t_status;
+}
+
+size_t smq_logits_workspace(uint32_t rows, uint32_t vocab) { return smq::logits_workspace(rows, vocab); }
+
+smq_status smq_logits_adjust(const float *logits, size_t stride, uint32_t rows, uint32_t vocab,
+                             const smq_logit_rules *rules, float *out, size_t out_stride, uint32_t *token,
+                             void *workspace, size_t workspace_bytes) {
+    if (!ready()) return t_status;
+    if (!vocab || vocab > (1u << 30)) return set_status(SMQ_ERR_RANGE, "logits_adjust: vocabulary of %u ids", vocab);
+    if (rows > 65535) return set_status(SMQ_ERR_RANGE, "logits_adjust: %u rows exceed 65535", rows);
+    if (!out && !token) return set_status(SMQ_ERR_RANGE, "logits_adjust: neither out nor token");
+    if (!rows) return SMQ_OK;
+    if (rows > 1 && (stride < vocab || (out && out_stride < vocab)))
+        return set_status(SMQ_ERR_RANGE, "logits_adjust: row strides %zu, %zu below the vocabulary", stride, out_stride);
+    if (out == logits && rows > 1 && out_stride != stride)
+        return set_status(SMQ_ERR_RANGE, "logits_adjust: in place with another stride");
+    smq::LogitArgs a;
+    memset(&a, 0, sizeof(a));
+    a.logits = logits;
+    a.out = out;
+    a.stride = stride;
+    a.out_stride = out_stride;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.flag = g.flag;
+    const size_t begins = ((size_t)rows + 1) * 4;
+    if (!extent_ok(logits, ((size_t)(rows - 1) * stride + vocab) * 4, "logits") ||
+        !extent_ok(out, out ? ((size_t)(rows - 1) * out_stride + vocab) * 4 : 0, "out") ||
+        !extent_ok(token, token ? (size_t)rows * 4 : 0, "token"))
+        return t_status;
+    if (rules && rules->history && rules->history_count) {
+        if (!extent_ok(rules->history, (size_t)rules->history_count * 4, "history") ||
+            !extent_ok(rules->history_begin, begins, "history_begin") ||
+            !extent_ok(rules->penalty, (size_t)rows * 12, "penalty"))
+            return t_status;
+        a.history = rules->history;
+        a.history_begin = rules->history_begin;
+        a.history_count = rules->history_count;
+        a.penalty = rules->penalty;
+    }
+    if (rules && rules->bias_ids && rules->bias_count) {
+        if (!extent_ok(rules->bias_ids, (size_t)rules->bias_count * 4, "bias_ids") ||
+            !extent_ok(rules->bias, (size_t)rules->bias_count * 4, "bias") ||
+            !extent_ok(rules->bias_begin, begins, "bias_begin"))
+            return t_status;
+        a.bias_ids = rules->bias_ids;
+        a.bias = rules->bias;
+        a.bias_begin = rules->bias_begin;
+        a.bias_count = rules->bias_count;
+    }
+    if (rules && rules->allowed) {
+        if (!rules->mask_row && rules->allowed_rows < rows)
+            return set_status(SMQ_ERR_RANGE, "logits_adjust: %u masks for %u rows", rules->allowed_rows, rows);
+        if (!extent_ok(rules->allowed, (size_t)rules->allowed_rows * ((vocab + 31) / 32) * 4, "allowed") ||
+            !extent_ok(rules->mask_row, rules->mask_row ? (size_t)rows * 4 : 0, "mask_row"))
+            return t_status;
+        a.allowed = rules->allowed;
+        a.allowed_rows = rules->allowed_rows;
+        a.mask_row = rules->mask_row;
+    }
+    if (token) {
+        const size_t need = smq::logits_workspace(rows, vocab);
+        if (workspace_bytes < need || ((uintptr_t)workspace & 15))
+            return set_status(SMQ_ERR_RANGE, "logits_adjust: the workspace has %zu bytes of %zu, 16-byte aligned",
+                              workspace_bytes, need);
+        if (!extent_ok(workspace, need, "workspace")) return t_status;
+    }
+    return hip_ok(smq::launch_logits(a, token, workspace, g.cur), "logits_adjust") ? SMQ_OK : t_status;
+}
+
 smq_status smq_quantize_q5_rows(const float *x, uint32_t rows, uint32_t cols, unsigned char *out) {
     if (!ready()) return t_status;
     if (!rows || !cols) return SMQ_OK;

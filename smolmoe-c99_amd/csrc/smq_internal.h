@@ -269,6 +269,48 @@ hipError_t launch_embed(const unsigned char *w, size_t row_bytes, bool q5, uint3
 hipError_t launch_quantize_q5(const float *x, uint32_t rows, uint32_t cols, unsigned char *out, hipStream_t s);
 hipError_t launch_dequantize_row(const unsigned char *w, uint32_t cols, float *out, bool q5, hipStream_t s);
 
+/* Paged KV cache (csrc/smq_paged.hip): checked descriptors. page = 1 << shift positions; limit: positions
+ * that the table and the context can address. */
+constexpr uint32_t MAX_PAGED_CONTEXT = 1u << 20;
+struct PagedArgs {
+    const int32_t *begin, *length, *table;
+    uint32_t seqs, tokens, table_stride;
+    void *keys, *values;
+    float *ks, *vs;
+    uint32_t type, shift, pages;
+    uint32_t heads, kv_heads, head_dim, nb, pairs, window, sinks, context, limit;
+    int *flag;
+};
+hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out, const float *k, const float *v,
+                                const float *cs, const float *sn, hipStream_t s);
+hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s);
+/* The workspace of the widest split that the kernel would take. */
+size_t paged_attention_workspace(const PagedArgs &a);
+hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
+                                  hipStream_t s);
+
+/* Penalties, biases, masks and the greedy choice on rows of logits (csrc/smq_logits.hip). */
+struct LogitArgs {
+    const float *logits;
+    float *out;
+    size_t stride, out_stride;
+    uint32_t rows, vocab;
+    const uint32_t *history;
+    const int32_t *history_begin;
+    uint32_t history_count;
+    const float *penalty;
+    const uint32_t *bias_ids;
+    const float *bias;
+    const int32_t *bias_begin;
+    uint32_t bias_count;
+    const uint32_t *allowed;
+    uint32_t allowed_rows;
+    const int32_t *mask_row;
+    int *flag;
+};
+size_t logits_workspace(uint32_t rows, uint32_t vocab);
+hipError_t launch_logits(const LogitArgs &a, uint32_t *token, void *ws, hipStream_t s);
+
 /* Grid barrier probe (csrc/smq_anchor.hip): clears `words` (GRID_BARRIER_WORDS of them), then one launch
  * of wgs workgroups (one per CU, wgs <= the CU count) passing `episodes` barriers of the given kind;
  * words[GRID_BARRIER_TIMEOUTS] counts the workgroups that gave up a wait. */
