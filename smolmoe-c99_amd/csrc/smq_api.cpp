@@ -1454,9 +1454,9 @@ static bool paged_args(const smq_paged_batch *b, const smq_attn_shape *shape, co
                    shape->context, smq::MAX_PAGED_CONTEXT);
         return false;
     }
-    if (b->seqs > (1u << 20) || b->tokens > (1u << 24) || (b->seqs && !b->table_stride) || b->table_stride > (1u << 20)) {
-        set_status(SMQ_ERR_RANGE, "%s: unsupported batch (%u sequences <= 2^20, %u tokens <= 2^24, table stride %u of 1 .. 2^20)",
-                   who, b->seqs, b->tokens, b->table_stride);
+    if (b->seqs > (1u << 20) || (uint64_t)b->tokens * shape->heads > (1u << 23) || (b->seqs && !b->table_stride) || b->table_stride > (1u << 20)) {
+        set_status(SMQ_ERR_RANGE, "%s: unsupported batch (%u sequences <= 2^20, %u tokens of %u heads <= 2^23, table stride %u of 1 .. 2^20)",
+                   who, b->seqs, b->tokens, shape->heads, b->table_stride);
         return false;
     }
     a.begin = b->begin;

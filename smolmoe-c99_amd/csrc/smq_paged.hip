@@ -1,70 +1,11 @@
 /* Paged KV cache on gfx950: RoPE and the store of new tokens (f32, f16, Q8), rows read back, and the attention of a
  * ragged batch of new tokens over the pages (include/smq.h has the layout of a page). */
 #include <hip/hip_fp16.h>
-#include <float.h>
 
-#include "smq_device.h"
+#include "smq_paged_attend.h"
 
 namespace smq {
 namespace {
-
-/* A page id of the table or -1 with the flag raised where it names no page. */
-__device__ __forceinline__ int page_of(const PagedArgs &a, uint32_t s, uint32_t pos) {
-    const int id = a.table[(size_t)s * a.table_stride + (pos >> a.shift)];
-    if ((uint32_t)id < a.pages) return id;
-    *a.flag = 1;
-    return -1;
-}
-
-/* Sequence s's new tokens: rows begin .. begin + n at positions first .. first + n, of `length` positions. False, with
- * the flag raised, where begin does not ascend within 0 .. tokens. */
-struct Seq {
-    int begin, n, length;
-    int64_t first;
-};
-__device__ __forceinline__ bool sequence(const PagedArgs &a, uint32_t s, Seq &q) {
-    const int b0 = a.begin[s], b1 = a.begin[s + 1];
-    if (b0 < 0 || b1 < b0 || (uint32_t)b1 > a.tokens) {
-        *a.flag = 1;
-        return false;
-    }
-    const int len = a.length[s];
-    q.begin = b0;
-    q.n = b1 - b0;
-    q.length = len < 0 ? 0 : (uint32_t)len > a.limit ? (int)a.limit : len;
-    q.first = (int64_t)len - q.n;
-    return true;
-}
-
-/* Raises the flag where begin does not ascend within 0 .. tokens (rows may then belong to no sequence); by one workgroup
- * of a launch. */
-__device__ __forceinline__ void check_begin(const PagedArgs &a, uint32_t tid, uint32_t threads) {
-    for (uint32_t s = tid; s < a.seqs; s += threads) {
-        const int b0 = a.begin[s], b1 = a.begin[s + 1];
-        if (b0 < 0 || b1 < b0 || (uint32_t)b1 > a.tokens) *a.flag = 1;
-    }
-}
-
-/* The sequence and position of row r; false where the row is padding or has no place (then with the flag). */
-__device__ __forceinline__ bool place_of(const PagedArgs &a, uint32_t r, uint32_t &s, uint32_t &pos) {
-    uint32_t lo = 0, hi = a.seqs; /* the first sequence that begins past r */
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.begin[mid] <= (int)r) lo = mid + 1;
-        else hi = mid;
-    }
-    Seq q;
-    if (!lo || a.begin[lo] <= (int)r) return false; /* behind the last sequence (lo == seqs) */
-    s = lo - 1;
-    if (!sequence(a, s, q)) return false;
-    const int64_t p = q.first + (int)(r - (uint32_t)q.begin);
-    if (p < 0 || p >= (int64_t)a.limit) {
-        *a.flag = 1;
-        return false;
-    }
-    pos = (uint32_t)p;
-    return true;
-}
 
 /* Coordinate d of a rotated head row x (smq_rope_kv's products and order). */
 __device__ __forceinline__ float rotated(const float *x, uint32_t d, uint32_t pairs, const float *c, const float *s) {
@@ -160,68 +101,57 @@ __global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, 
     }
 }
 
-/* One wave per row and head: 64 positions at a time, a running maximum and sum of the softmax in one pass. */
-template <uint32_t TYPE>
-__global__ __launch_bounds__(64) void k_paged_attend(PagedArgs a, const float *q, float *att) {
-    __shared__ float qs[MAX_HEAD_DIM], ps[64];
-    __shared__ size_t at_v[64];
-    const uint32_t r = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, h = head / (a.heads / a.kv_heads);
-    const uint32_t P = 1u << a.shift, hd = a.head_dim;
-    uint32_t s, pos;
-    float *out = att + ((size_t)r * a.heads + head) * hd;
-    if (r == 0 && head == 0) check_begin(a, lane, 64);
-    if (!place_of(a, r, s, pos)) {
-        if ((int)r < a.begin[a.seqs])
-            for (uint32_t d = lane; d < hd; d += 64) out[d] = 0.0f;
-        return;
-    }
-    for (uint32_t d = lane; d < hd; d += 64) qs[d] = q[((size_t)r * a.heads + head) * hd + d];
-    const float scale = 1.0f / sqrtf((float)hd);
-    float m = -INFINITY, l = 0.0f, o[MAX_HEAD_DIM / 64] = {};
-    const uint32_t low = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0;
-    __syncthreads();
-    for (uint32_t j0 = 0; j0 <= pos; j0 += 64) {
-        if (j0 + 64 <= low && j0 >= a.sinks) continue;
-        const uint32_t j = j0 + lane;
-        bool sees = j <= pos && (j >= low || j < a.sinks);
-        const int page = sees ? page_of(a, s, j) : -1;
-        sees = page >= 0;
-        float x = -INFINITY;
-        if (sees) {
-            const uint32_t slot = j & (P - 1);
-            const size_t ph = (size_t)page * a.kv_heads + h;
-            float dot = 0.0f;
-            for (uint32_t d = 0; d < hd; ++d)
-                dot += qs[d] * element<TYPE>(a.keys, (ph * P + slot) * hd + d, a.ks, (ph * a.nb + d / 32) * P + slot);
-            x = dot * scale;
-            at_v[lane] = ph * hd * P + slot;
+/* Joins the splits of a tile and KV head: the weights of their maxima, in the order of the splits. */
+__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, float *att, uint32_t tile_rows, uint32_t tiles,
+                                                    uint32_t splits, const uint32_t *used, const float *part) {
+    const uint32_t kh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, G = a.heads / a.kv_heads, hd = a.head_dim;
+    const size_t slot = (size_t)tile * a.kv_heads + kh;
+    const uint32_t parts = used[slot];
+    if (parts < 2) return;
+    uint32_t seq, row0;
+    Seq sq;
+    if (!find_tile(a, tile, tile_rows, seq, row0) || !sequence(a, seq, sq)) return;
+    const uint32_t n = min(tile_rows, (uint32_t)sq.n * G - row0);
+    const size_t r0 = slot * splits * tile_rows;
+    const float *po = part + r0 * hd, *pml = part + (size_t)tiles * a.kv_heads * splits * tile_rows * hd + 2 * r0;
+    for (uint32_t i = threadIdx.x; i < n * (hd / 4); i += 256) {
+        const uint32_t r = i / (hd / 4), d = 4 * (i % (hd / 4));
+        float m = -FLT_MAX, l = 0.0f;
+        for (uint32_t x = 0; x < parts; ++x) m = fmaxf(m, pml[2 * (x * tile_rows + r)]);
+        f4 o = {};
+        for (uint32_t x = 0; x < parts; ++x) {
+            const size_t y = (size_t)x * tile_rows + r;
+            const float e = __builtin_amdgcn_exp2f(pml[2 * y] - m);
+            l += e * pml[2 * y + 1];
+            o += e * *(const f4 *)(po + y * hd + d);
         }
-        float mx = x;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-        const float mn = fmaxf(m, mx);
-        if (mn == -INFINITY) continue; /* nothing seen so far: uniform */
-        const float alpha = __expf(m - mn), p = sees ? __expf(x - mn) : 0.0f;
-        float sum = p;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
-        l = l * alpha + sum;
-        m = mn;
-        ps[lane] = sees ? p : -1.0f;
-        __syncthreads();
-        for (uint32_t u = 0; u * 64 + lane < hd; ++u) {
-            const uint32_t d = u * 64 + lane;
-            float acc = o[u] * alpha;
-            for (uint32_t i = 0; i < 64; ++i) {
-                if (ps[i] < 0.0f) continue; /* not seen: its value never matters */
-                const size_t sh = at_v[i] / ((size_t)hd * P), slot = at_v[i] % P;
-                acc += ps[i] * element<TYPE>(a.values, at_v[i] + (size_t)d * P, a.vs, (sh * a.nb + d / 32) * P + slot);
-            }
-            o[u] = acc;
-        }
-        __syncthreads();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *(f4u *)(att + row_at(a, sq, kh, row0 + r) + d) = o * inv;
     }
-    for (uint32_t u = 0; u * 64 + lane < hd; ++u) out[u * 64 + lane] = l > 0.0f ? o[u] / l : m == -INFINITY ? 0.0f : l;
+}
+
+/* Tiles and splits. Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a
+ * workgroup's waves own theirs. Splits: as many workgroups as fill the chip, each with PA_MIN_STEPS steps at least. */
+AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
+    AttendPlan p;
+    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
+    p.owns = rows > 32 * seqs;
+    p.tile_rows = p.owns ? 64 * attend_rt(a.type, attend_ks(a.head_dim)) : 16;
+    p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) / p.tile_rows);
+    uint64_t most = a.limit;
+    if (a.window) { /* what a tile can see: its tokens, their windows, the sinks */
+        const uint64_t w = (uint64_t)a.window + p.tile_rows + 2 * PA_STEP + a.sinks;
+        most = w < most ? w : most;
+    }
+    p.steps = (uint32_t)((most + PA_STEP - 1) / PA_STEP);
+    const uint64_t groups = (uint64_t)p.tiles * a.kv_heads, want = p.owns ? 512 : 1024;
+    uint64_t splits = groups ? (want + groups - 1) / groups : 1;
+    if (splits > p.steps / PA_MIN_STEPS) splits = p.steps / PA_MIN_STEPS;
+    if (splits > PA_MAX_SPLITS) splits = PA_MAX_SPLITS;
+    const size_t head = attend_used_bytes(a, p), each = attend_part_bytes(a, p);
+    if (splits > 1 && (ws_bytes < head || splits > (ws_bytes - head) / each)) splits = ws_bytes < head ? 1 : (ws_bytes - head) / each;
+    p.splits = splits > 1 ? (uint32_t)splits : 1;
+    return p;
 }
 
 }  // namespace
@@ -244,10 +174,31 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
     return hipGetLastError();
 }
 
-size_t paged_attention_workspace(const PagedArgs &) { return 0; }
 
-hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *, size_t, hipStream_t s) {
-    SMQ_PAGED(k_paged_attend, dim3(a.tokens, a.heads), dim3(64), q, att);
+/* Over the types, whose tiles differ: the cache is not known yet. */
+size_t paged_attention_workspace(const PagedArgs &a0) {
+    size_t most = 0;
+    for (uint32_t type = 0; type < 3; ++type) {
+        PagedArgs a = a0;
+        a.type = type;
+        const AttendPlan p = attend_plan(a, ~(size_t)0);
+        const size_t n = p.splits > 1 ? attend_used_bytes(a, p) + p.splits * attend_part_bytes(a, p) : 0;
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
+                                  hipStream_t s) {
+    const AttendPlan p = attend_plan(a, ws_bytes);
+    uint32_t *used = p.splits > 1 ? (uint32_t *)ws : nullptr;
+    float *part = p.splits > 1 ? (float *)((char *)ws + attend_used_bytes(a, p)) : nullptr;
+    hipError_t e = a.type == 0 ? launch_attend<0>(a, p, q, att, used, part, s)
+                 : a.type == 1 ? launch_attend<1>(a, p, q, att, used, part, s)
+                               : launch_attend<2>(a, p, q, att, used, part, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    hipLaunchKernelGGL(k_paged_join, dim3(a.kv_heads * p.tiles), dim3(256), 0, s, a, att, p.tile_rows, p.tiles, p.splits,
+                       used, part);
     return hipGetLastError();
 }
 
