@@ -17,10 +17,10 @@ __device__ __forceinline__ int page_of(const PagedArgs &a, uint32_t s, uint32_t 
     return -1;
 }
 
-/* Sequence s's new tokens: rows begin .. begin + n at positions first .. first + n, of `length` positions. False, with
- * the flag raised, where begin does not ascend within 0 .. tokens. */
+/* Sequence s's new tokens: rows begin .. begin + n at positions first .. first + n. False, with the flag raised, where
+ * begin does not ascend within 0 .. tokens. */
 struct Seq {
-    int begin, n, length;
+    int begin, n;
     int64_t first;
 };
 __device__ __forceinline__ bool sequence(const PagedArgs &a, uint32_t s, Seq &q) {
@@ -29,11 +29,9 @@ __device__ __forceinline__ bool sequence(const PagedArgs &a, uint32_t s, Seq &q)
         *a.flag = 1;
         return false;
     }
-    const int len = a.length[s];
     q.begin = b0;
     q.n = b1 - b0;
-    q.length = len < 0 ? 0 : (uint32_t)len > a.limit ? (int)a.limit : len;
-    q.first = (int64_t)len - q.n;
+    q.first = (int64_t)a.length[s] - q.n;
     return true;
 }
 
@@ -67,44 +65,14 @@ __device__ __forceinline__ bool place_of(const PagedArgs &a, uint32_t r, uint32_
     return true;
 }
 
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
-/* Tile t of the batch: sequence and first row. Uniform; false behind the last tile. */
-__device__ __forceinline__ bool find_tile(const PagedArgs &a, uint32_t t, uint32_t tile_rows, uint32_t &seq, uint32_t &row0) {
-    const uint32_t lane = threadIdx.x % 64, G = a.heads / a.kv_heads;
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        uint32_t n = 0;
-        if (s < a.seqs) {
-            const int b0 = a.begin[s], b1 = a.begin[s + 1];
-            if (b0 < 0 || b1 < b0 || (uint32_t)b1 > a.tokens) *a.flag = 1;
-            else n = ((uint32_t)(b1 - b0) * G + tile_rows - 1) / tile_rows;
-        }
-        uint32_t sum = n;
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) {
-            const uint32_t x = __shfl_up(sum, off);
-            sum += (int)lane >= off ? x : 0;
-        }
-        const uint64_t past = __ballot(before + sum > t);
-        if (past) {
-            const int w = __ffsll((unsigned long long)past) - 1;
-            const uint32_t upto = before + __builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(n, w);
-            seq = s0 + (uint32_t)w;
-            row0 = (t - upto) * tile_rows;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-    }
-    return false;
-}
-
-/* Row r of a sequence and KV head, in q and att. */
-__device__ __forceinline__ size_t row_at(const PagedArgs &a, const Seq &sq, uint32_t kh, uint32_t r) {
+/* Row r of a sequence (its first token: begin) and KV head, in q and att. */
+__device__ __forceinline__ size_t row_at(const PagedArgs &a, int begin, uint32_t kh, uint32_t r) {
     const uint32_t G = a.heads / a.kv_heads;
-    return ((size_t)(sq.begin + (int)(r / G)) * a.heads + (size_t)kh * G + r % G) * a.head_dim;
+    return ((size_t)(begin + (int)(r / G)) * a.heads + (size_t)kh * G + r % G) * a.head_dim;
 }
 
 }  // namespace

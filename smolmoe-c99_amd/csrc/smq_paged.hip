@@ -101,56 +101,65 @@ __global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, 
     }
 }
 
-/* Joins the splits of a tile and KV head: the weights of their maxima, in the order of the splits. */
-__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, float *att, uint32_t tile_rows, uint32_t tiles,
-                                                    uint32_t splits, const uint32_t *used, const float *part) {
-    const uint32_t kh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, G = a.heads / a.kv_heads, hd = a.head_dim;
-    const size_t slot = (size_t)tile * a.kv_heads + kh;
-    const uint32_t parts = used[slot];
-    if (parts < 2) return;
-    uint32_t seq, row0;
-    Seq sq;
-    if (!find_tile(a, tile, tile_rows, seq, row0) || !sequence(a, seq, sq)) return;
-    const uint32_t n = min(tile_rows, (uint32_t)sq.n * G - row0);
-    const size_t r0 = slot * splits * tile_rows;
-    const float *po = part + r0 * hd, *pml = part + (size_t)tiles * a.kv_heads * splits * tile_rows * hd + 2 * r0;
-    for (uint32_t i = threadIdx.x; i < n * (hd / 4); i += 256) {
-        const uint32_t r = i / (hd / 4), d = 4 * (i % (hd / 4));
-        float m = -FLT_MAX, l = 0.0f;
-        for (uint32_t x = 0; x < parts; ++x) m = fmaxf(m, pml[2 * (x * tile_rows + r)]);
-        f4 o = {};
-        for (uint32_t x = 0; x < parts; ++x) {
-            const size_t y = (size_t)x * tile_rows + r;
-            const float e = __builtin_amdgcn_exp2f(pml[2 * y] - m);
-            l += e * pml[2 * y + 1];
-            o += e * *(const f4 *)(po + y * hd + d);
+/* Joins what several workgroups have of a tile and KV head: the weights of their maxima, in their order. head_dim / 4 lanes
+ * per row. A lane requests its part of O and the maxima and sums of eight workgroups at once: after the tile's four words
+ * one round trip to memory joins up to eight. */
+constexpr uint32_t JOIN_WG = 256, JOIN_AT_ONCE = 8;
+__global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att, AttendPlan p, const i4 *used,
+                                                        const float *part) {
+    const uint32_t hd = a.head_dim, lanes = hd / 4, per = JOIN_WG / lanes;
+    const uint32_t groups = (p.tile_rows + per - 1) / per, tile = blockIdx.x / groups, kh = tile % a.kv_heads;
+    const uint32_t r = blockIdx.x % groups * per + threadIdx.x / lanes, d = 4 * (threadIdx.x % lanes);
+    const i4 u = used[tile];
+    const uint32_t parts = (uint32_t)u[0] & 0xffff, n = (uint32_t)u[0] >> 16, slot = (uint32_t)u[3];
+    if (parts < 2 || r >= n || threadIdx.x / lanes >= per) return;
+    const f2 *pml = (const f2 *)(part + (size_t)2 * p.stream * a.kv_heads * p.tile_rows * hd);
+    float m = -FLT_MAX, l = 0.0f;
+    f4 o = {};
+    for (uint32_t i0 = 0; i0 < parts; i0 += JOIN_AT_ONCE) {
+        f2 ml[JOIN_AT_ONCE];
+        f4 x[JOIN_AT_ONCE];
+        float top = m;
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_AT_ONCE; ++i) {
+            const uint32_t k = min(i0 + i, parts - 1); /* the first one's slot, then slots 0 of the next workgroups */
+            const size_t y = ((size_t)(k ? (slot & ~1u) + 2 * k : slot) * a.kv_heads + kh) * p.tile_rows + r;
+            ml[i] = pml[y];
+            x[i] = *(const f4 *)(part + y * hd + d);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *(f4u *)(att + row_at(a, sq, kh, row0 + r) + d) = o * inv;
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_AT_ONCE; ++i) top = fmaxf(top, ml[i][0]);
+        const float old = __builtin_amdgcn_exp2f(m - top);
+        l *= old;
+        o *= old;
+        m = top;
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_AT_ONCE; ++i) {
+            const float e = i0 + i < parts ? __builtin_amdgcn_exp2f(ml[i][0] - m) : 0.0f;
+            l += e * ml[i][1];
+            o += e * x[i];
+        }
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *(f4u *)(att + row_at(a, u[1], kh, (uint32_t)u[2] + r) + d) = o * inv;
 }
 
-/* Tiles and splits. Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a
- * workgroup's waves own theirs. Splits: as many workgroups as fill the chip, each with PA_MIN_STEPS steps at least. */
+/* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own
+ * theirs. Workgroups: one a CU while decoding, whose rate is then that of the memory, two a CU for products. */
 AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     AttendPlan p;
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
     p.owns = rows > 32 * seqs;
-    p.tile_rows = p.owns ? 64 * attend_rt(a.type, attend_ks(a.head_dim)) : 16;
+    p.tile_rows = p.owns ? 64 * attend_rt(attend_ks(a.head_dim)) : 16;
     p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) / p.tile_rows);
-    uint64_t most = a.limit;
-    if (a.window) { /* what a tile can see: its tokens, their windows, the sinks */
-        const uint64_t w = (uint64_t)a.window + p.tile_rows + 2 * PA_STEP + a.sinks;
-        most = w < most ? w : most;
-    }
-    p.steps = (uint32_t)((most + PA_STEP - 1) / PA_STEP);
-    const uint64_t groups = (uint64_t)p.tiles * a.kv_heads, want = p.owns ? 512 : 1024;
-    uint64_t splits = groups ? (want + groups - 1) / groups : 1;
-    if (splits > p.steps / PA_MIN_STEPS) splits = p.steps / PA_MIN_STEPS;
-    if (splits > PA_MAX_SPLITS) splits = PA_MAX_SPLITS;
-    const size_t head = attend_used_bytes(a, p), each = attend_part_bytes(a, p);
-    if (splits > 1 && (ws_bytes < head || splits > (ws_bytes - head) / each)) splits = ws_bytes < head ? 1 : (ws_bytes - head) / each;
-    p.splits = splits > 1 ? (uint32_t)splits : 1;
+    p.stream = ((p.owns ? 512 : 256) + a.kv_heads - 1) / a.kv_heads;
+    p.unit = 0; /* all units (at most this many) and the last workgroup's end below 2^31 */
+    while (((uint64_t)p.tiles * (2 * (uint64_t)a.limit + 128) >> p.unit) + p.tiles + 64 * 512 >= 1u << 30) ++p.unit;
+    if (a.limit <= PA_MIN_STEPS * PA_STEP && p.tiles >= p.stream) p.stream = 0; /* short sequences: a tile each */
+    if (a.limit <= PA_MIN_STEPS * PA_STEP && !p.owns) p.stream = 0;
+    const size_t used = attend_used_bytes(a, p), each = attend_part_bytes(a, p.tile_rows);
+    const uint64_t room = ws_bytes > used ? (ws_bytes - used) / each : 0;
+    if (room < p.stream) p.stream = room > p.tiles ? (uint32_t)room : 0;
     return p;
 }
 
@@ -175,30 +184,22 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
 }
 
 
-/* Over the types, whose tiles differ: the cache is not known yet. */
-size_t paged_attention_workspace(const PagedArgs &a0) {
-    size_t most = 0;
-    for (uint32_t type = 0; type < 3; ++type) {
-        PagedArgs a = a0;
-        a.type = type;
-        const AttendPlan p = attend_plan(a, ~(size_t)0);
-        const size_t n = p.splits > 1 ? attend_used_bytes(a, p) + p.splits * attend_part_bytes(a, p) : 0;
-        most = n > most ? n : most;
-    }
-    return most;
+size_t paged_attention_workspace(const PagedArgs &a) {
+    const AttendPlan p = attend_plan(a, ~(size_t)0);
+    return p.stream ? attend_used_bytes(a, p) + p.stream * attend_part_bytes(a, p.tile_rows) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
                                   hipStream_t s) {
     const AttendPlan p = attend_plan(a, ws_bytes);
-    uint32_t *used = p.splits > 1 ? (uint32_t *)ws : nullptr;
-    float *part = p.splits > 1 ? (float *)((char *)ws + attend_used_bytes(a, p)) : nullptr;
+    i4 *used = p.stream ? (i4 *)ws : nullptr;
+    float *part = p.stream ? (float *)((char *)ws + attend_used_bytes(a, p)) : nullptr;
     hipError_t e = a.type == 0 ? launch_attend<0>(a, p, q, att, used, part, s)
                  : a.type == 1 ? launch_attend<1>(a, p, q, att, used, part, s)
                                : launch_attend<2>(a, p, q, att, used, part, s);
-    if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL(k_paged_join, dim3(a.kv_heads * p.tiles), dim3(256), 0, s, a, att, p.tile_rows, p.tiles, p.splits,
-                       used, part);
+    if (e != hipSuccess || !p.stream) return e;
+    const uint32_t per = JOIN_WG / (a.head_dim / 4), groups = (p.tile_rows + per - 1) / per;
+    hipLaunchKernelGGL(k_paged_join, dim3(a.kv_heads * p.tiles * groups), dim3(JOIN_WG), 0, s, a, att, p, used, part);
     return hipGetLastError();
 }
 

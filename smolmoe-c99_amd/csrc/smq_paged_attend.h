@@ -24,34 +24,43 @@
 
 namespace smq {
 
-constexpr int PA_WG = 256, PA_WAVES = 4;
+constexpr int PA_WAVES = 4; /* of a workgroup */
 constexpr uint32_t PA_STEP = 32;      /* positions */
-constexpr uint32_t PA_MIN_STEPS = 8;  /* of a split, at least */
-constexpr uint32_t PA_MAX_SPLITS = 64;
+constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps are dealt out */
 
 /* How a launch covers the rows: tiles of tile_rows rows of one sequence and KV head (`tiles`: as many as the batch can
- * need), each over splits workgroups. owns: a wave owns 16 * RT of the tile's rows over all positions; else the tile has
- * 16 rows and the four waves share the positions out. */
+ * need). owns: a wave owns 16 * RT of the tile's rows over all positions; else the tile has 16 rows and the waves share
+ * the positions out.
+ *
+ * stream > 0: stream workgroups per KV head take equal runs of all tiles' steps laid end to end, so a run ends and the
+ * next begins inside a tile, whose partial results k_paged_join joins. Lengths are known on the device only: each
+ * workgroup finds its run there. A tile counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the
+ * sequence: its steps nearly, and with sums that need no loop. stream 0 (no workspace): a workgroup per tile. */
+typedef int i4 __attribute__((ext_vector_type(4)));
 struct AttendPlan {
     bool owns;
-    uint32_t tile_rows, tiles, splits, steps;
+    uint32_t tile_rows, tiles, stream, unit;
 };
-/* Partial results of one split tile: per tile and KV head the splits in use (a word), then per split, row: the maximum,
- * the sum, O. */
-inline size_t attend_used_bytes(const PagedArgs &a, const AttendPlan &p) {
-    return ((size_t)p.tiles * a.kv_heads * 4 + 15) & ~(size_t)15;
-}
-inline size_t attend_part_bytes(const PagedArgs &a, const AttendPlan &p) {
-    return (size_t)p.tiles * a.kv_heads * p.tile_rows * (a.head_dim + 2) * 4;
+/* The workspace: per tile and KV head four words (the workgroups that share it, its rows << 16; the sequence's first
+ * token; the first row; the first one's slot), then per workgroup two slots of tile_rows rows: O, and behind all of them
+ * the maxima and sums. A workgroup's first tile, if it shares that one, has slot 0, its last slot 1; the tiles between are
+ * its own. */
+inline size_t attend_used_bytes(const PagedArgs &a, const AttendPlan &p) { return (size_t)p.tiles * a.kv_heads * 16; }
+inline size_t attend_part_bytes(const PagedArgs &a, uint32_t tile_rows) { /* for a workgroup per KV head */
+    return (size_t)2 * a.kv_heads * tile_rows * (a.head_dim + 2) * 4;
 }
 
 template <uint32_t TYPE>
-hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, uint32_t *used, float *part,
+hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
                          hipStream_t s);
 
-/* RT of the kernels whose waves own rows, by the head size's 32-wide steps: what fits two waves per SIMD. */
-constexpr uint32_t attend_rt(uint32_t type, uint32_t ks) { return type == 0 ? (ks <= 2 ? 2 : 1) : ks <= 2 ? 4 : ks <= 4 ? 2 : 1; }
-constexpr int attend_waves(uint32_t type, uint32_t ks) { return ks == 8 || (type == 0 && ks > 2) ? 1 : 2; }
+/* RT of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles and two
+ * waves: each fragment read from LDS serves twice, the registers hold without spills, one wave's softmax runs beside the
+ * other's products. Useful rate over 64 sequences of 128 tokens at 4096, 32 heads on 8 (RT 1 / 2 / 3 or 4): f16 heads of
+ * 64 403 / 445 / 409 TFLOP/s, of 128 488 / 586 / 215; Q8 252 / 298 / 301, 301 / 363 / 195; f32 123 / 129 / 115, 99 / 127 /
+ * 114. Three waves of RT 2: the same or spills. */
+constexpr uint32_t attend_rt(uint32_t ks) { return ks <= 4 ? 2 : 1; }
+constexpr int attend_waves(uint32_t ks) { return ks == 8 ? 1 : 2; }
 constexpr uint32_t attend_ks(uint32_t hd) { return hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : hd <= 128 ? 4 : 8; }
 
 #ifdef SMQ_ATTEND_KERNELS
@@ -59,7 +68,6 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float wave_max_quads(float x) { /* over the lanes of one column */
@@ -71,8 +79,9 @@ __device__ __forceinline__ float wave_sum_quads(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-/* x[0..8) as two f16, value and remainder. The rounded pair is opaque to the compiler: it would round the value a second
- * time elsewhere, from a product that it has not rounded to f32, and the remainder would belong to another value. */
+/* x[0..8) as two f16, value and remainder (one v_fma_mix each: the remainder is exact). The rounded pair is opaque to
+ * the compiler: it would round the value a second time elsewhere, from a product that it has not rounded to f32, and the
+ * remainder would belong to another value. */
 __device__ __forceinline__ void split8(const float *x, h8 &hi, h8 &lo) {
     union {
         h8 h;
@@ -86,13 +95,24 @@ __device__ __forceinline__ void split8(const float *x, h8 &hi, h8 &lo) {
         } p, q;
         p.h = __builtin_convertvector(f2{x[2 * j], x[2 * j + 1]}, h2);
         asm("" : "+v"(p.u));
-        q.h = __builtin_convertvector(f2{__builtin_fmaf((float)p.h[0], -1.0f, x[2 * j]),
-                                         __builtin_fmaf((float)p.h[1], -1.0f, x[2 * j + 1])}, h2);
+        float r0, r1;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(p.u), "v"(x[2 * j]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(p.u), "v"(x[2 * j + 1]));
+        q.h = __builtin_convertvector(f2{r0, r1}, h2);
         r.u[j] = p.u;
         s.u[j] = q.u;
     }
     hi = r.h;
     lo = s.h;
+}
+/* The largest of three, in one instruction: the compiler's fmaxf makes every input canonical first. A NaN loses. */
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+__device__ __forceinline__ float max8(const float *x) {
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
 }
 
 /* Eight int8 as f16, exactly: the byte plus 128 in the mantissa of 1024 + byte, less 1152. */
@@ -164,6 +184,128 @@ __device__ __forceinline__ Steps tile_steps(const PagedArgs &a, int64_t pmin, in
     return s;
 }
 
+/* A tile: sequence, its number in it, its number in the batch, its first unit and its units. */
+struct Tile {
+    uint32_t seq, j, t, first, units;
+    Seq sq;
+};
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t x) { /* x plus the lane's neighbour by CTRL, in the rows of the mask */
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x) { /* inclusive, over the 64 lanes */
+    x = dpp_add<0x111, 0xf>(x); /* row_shr 1, 2, 4, 8: in rows of 16 */
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x); /* row_bcast 15 into rows 1 and 3 */
+    return dpp_add<0x143, 0xc>(x); /* row_bcast 31 into rows 2 and 3 */
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int w) { return (uint32_t)__builtin_amdgcn_readlane(x, w); }
+
+/* The batch's tiles; a wave looks at 64 sequences at a time, one per lane, their lengths requested with their begins. */
+struct Tiles {
+    const PagedArgs &a;
+    uint32_t rows, unit;
+    int b0, b1, len;
+    uint32_t n, c0, c1, cw; /* the lane's sequence: its tiles and their units */
+    uint32_t mine, upto, tiles_upto; /* its units, and those and the tiles of the sequences up to it, of the 64 */
+    uint32_t at;                     /* the first of the 64 */
+
+    __device__ __forceinline__ Tiles(const PagedArgs &a_, const AttendPlan &p) : a(a_), rows(p.tile_rows), unit(p.unit) { look(0); }
+    __device__ __forceinline__ void look(uint32_t s0) {
+        const uint32_t s = s0 + threadIdx.x % 64, G = a.heads / a.kv_heads;
+        at = s0;
+        b0 = b1 = len = 0;
+        if (s < a.seqs) {
+            b0 = a.begin[s];
+            b1 = a.begin[s + 1];
+            len = a.length[s];
+        }
+        const bool fine = b0 >= 0 && b1 > b0 && (uint32_t)b1 <= a.tokens; /* else no tile; check_begin raises the flag */
+        const uint32_t tokens = fine ? (uint32_t)(b1 - b0) : 0, tok = rows / G + 1; /* of the sequence, of a tile */
+        n = (tokens * G + rows - 1) / rows;
+        const uint32_t p = len > (int)tokens ? min((uint32_t)len - tokens, a.limit) : 0;
+        const uint64_t w = (uint64_t)a.window + a.sinks + tok + 64;
+        const uint32_t most = a.limit + 32;
+        cw = max(1u, 2 * (a.window && w < most ? (uint32_t)w : most) >> unit);
+        c0 = max(1u, min(2 * (p + min(tok, tokens)) + 64 >> unit, cw));
+        c1 = 2 * rows / G >> unit;
+        mine = sum(n, c0, c1, cw);
+        upto = scan_wave(mine);
+        tiles_upto = scan_wave(n);
+    }
+    /* Units of the first j tiles of a sequence. */
+    static __device__ __forceinline__ uint32_t sum(uint32_t j, uint32_t c0, uint32_t c1, uint32_t cw) {
+        const uint32_t k = c1 ? min(j, (cw - c0 + c1 - 1) / c1) : j; /* those below cw */
+        return k * c0 + (uint32_t)((uint64_t)k * (k - (k ? 1 : 0)) / 2 * c1) + (j - k) * cw;
+    }
+    __device__ __forceinline__ void total(uint32_t &units, uint32_t &tiles) {
+        units = tiles = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+            if (s0 != at) look(s0);
+            units += lane_of(upto, 63);
+            tiles += lane_of(tiles_upto, 63);
+        }
+    }
+    __device__ __forceinline__ void take(Tile &t, int w, uint32_t tiles_before) {
+        t.seq = at + (uint32_t)w;
+        t.t = tiles_before;
+        t.sq.begin = (int)lane_of((uint32_t)b0, w);
+        t.sq.n = (int)lane_of((uint32_t)b1, w) - t.sq.begin;
+        t.sq.first = (int64_t)(int)lane_of((uint32_t)len, w) - t.sq.n;
+    }
+    /* The tile of number x. False behind the last. */
+    __device__ __forceinline__ bool by_number(uint32_t x, Tile &t) {
+        uint32_t before = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+            if (s0 != at) look(s0);
+            const uint64_t past = __ballot(before + tiles_upto > x);
+            if (past) {
+                const int w = __ffsll((unsigned long long)past) - 1;
+                const uint32_t first = before + lane_of(tiles_upto, w) - lane_of(n, w);
+                take(t, w, x);
+                t.j = x - first;
+                return true;
+            }
+            before += lane_of(tiles_upto, 63);
+        }
+        return false;
+    }
+    /* The last tile whose first unit u and number t have key(u, t) <= x; key grows with both. False if x is behind all of
+     * them (key of the batch's end <= x). */
+    template <typename Key>
+    __device__ __forceinline__ bool last_with(uint32_t x, Key key, Tile &t) {
+        uint32_t before = 0, tiles = 0;
+        for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+            if (s0 != at) look(s0);
+            const uint64_t past = __ballot(key(before + upto, tiles + tiles_upto) > x);
+            if (past) {
+                const int w = __ffsll((unsigned long long)past) - 1;
+                before += lane_of(upto, w) - lane_of(mine, w);
+                tiles += lane_of(tiles_upto, w) - lane_of(n, w);
+                const uint32_t N = lane_of(n, w), d0 = lane_of(c0, w), d1 = lane_of(c1, w), dw = lane_of(cw, w);
+                uint32_t lo = 0, span = N; /* the last j of [lo, lo + span) */
+                while (span > 1) {
+                    const uint32_t step = (span + 63) / 64, j = lo + threadIdx.x % 64 * step;
+                    const uint64_t fit = __ballot(j < lo + span && key(before + sum(j, d0, d1, dw), tiles + j) <= x);
+                    const uint32_t k = 63 - (uint32_t)__builtin_clzll(fit); /* lane 0 fits */
+                    span = min(step, span - k * step);
+                    lo += k * step;
+                }
+                t.j = lo;
+                t.first = before + sum(lo, d0, d1, dw);
+                t.units = sum(lo + 1, d0, d1, dw) - sum(lo, d0, d1, dw);
+                take(t, w, tiles + lo);
+                return true;
+            }
+            before += lane_of(upto, 63);
+            tiles += lane_of(tiles_upto, 63);
+        }
+        return false;
+    }
+};
+
 /* Positions that some rows see: [0, sinks) and [low, high]. */
 struct Span {
     int high;
@@ -181,54 +323,66 @@ __device__ __forceinline__ Span span_of(const PagedArgs &a, int pmin, int pmax) 
     return s;
 }
 
-/* Where the two halves of 16 positions of a step lie. */
-struct Place {
-    uint32_t page[2], slot[2];
-    uint32_t ok; /* bit h: half h has a page */
-};
-/* A sequence's page ids, 64 of them in the lanes of a wave. */
-struct Table {
+/* A sequence's pages for one KV head. SMALL: pages of 16 positions, so that a step of 32 lies in two; else in one. The
+ * page ids are read 64 at a time, one per lane. */
+template <uint32_t TYPE, bool SMALL>
+struct Pages {
+    static constexpr uint32_t EB = Elem<TYPE>::bytes;
+    static constexpr int N = SMALL ? 2 : 1;
+    /* Where a step lies, for each of its N parts: its first position's key and dim 0 of its value, and the scales of
+     * block 0. Uniform. */
+    struct Place {
+        const unsigned char *k[N], *v[N], *kw[N], *vw[N];
+        uint32_t ok; /* bit h: the half of 16 positions has a page */
+    };
+    const PagedArgs &a;
     const int32_t *table;
+    const unsigned char *k0, *v0, *kw0, *vw0; /* page 0 */
+    size_t stride, wstride;                   /* bytes of a page */
     uint32_t base, ids;
-    __device__ __forceinline__ void open(const PagedArgs &a, uint32_t seq) {
+
+    __device__ __forceinline__ Pages(const PagedArgs &a_, uint32_t seq, uint32_t kh) : a(a_) {
         table = a.table + (size_t)seq * a.table_stride;
         base = 0x7fffffff;
         ids = 0;
+        const size_t head = ((size_t)a.head_dim << a.shift) * EB, whead = ((size_t)a.nb << a.shift) * 4;
+        stride = head * a.kv_heads;
+        wstride = whead * a.kv_heads;
+        k0 = (const unsigned char *)a.keys + head * kh;
+        v0 = (const unsigned char *)a.values + head * kh;
+        if constexpr (TYPE == 2) {
+            kw0 = (const unsigned char *)a.ks + whead * kh;
+            vw0 = (const unsigned char *)a.vs + whead * kh;
+        }
     }
     /* A page that is none and that `span` needs raises the flag; page 0 then stands in, its positions unseen. */
-    __device__ __forceinline__ Place locate(const PagedArgs &a, uint32_t step, const Span &span) {
-        const uint32_t p0 = step * PA_STEP, i0 = p0 >> a.shift, i1 = (p0 + 16) >> a.shift, P = 1u << a.shift;
-        if (i0 < base || i1 >= base + 64) { /* uniform */
+    __device__ __forceinline__ Place locate(uint32_t step, const Span &span) {
+        const uint32_t p0 = step * PA_STEP, i0 = p0 >> a.shift;
+        if (i0 < base || i0 + N > base + 64) { /* uniform */
             base = i0;
             ids = (uint32_t)table[min(base + threadIdx.x % 64, a.table_stride - 1)];
         }
         Place pl;
-        pl.ok = 0;
+        pl.ok = 3;
+        const uint32_t slot = SMALL ? 0 : p0 & ((1u << a.shift) - 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            pl.page[h] = (uint32_t)__builtin_amdgcn_readlane(ids, (h ? i1 : i0) - base);
-            pl.slot[h] = (p0 + 16 * h) & (P - 1);
-            if (pl.page[h] < a.pages) {
-                pl.ok |= 1u << h;
-            } else {
-                if (span.meets(p0 + 16 * h, 16)) *a.flag = 1;
-                pl.page[h] = 0;
+        for (int h = 0; h < N; ++h) {
+            uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, i0 + h - base);
+            if (page >= a.pages) {
+                if (span.meets(p0 + 16 * h, SMALL ? 16 : 32)) *a.flag = 1;
+                page = 0;
+                pl.ok = SMALL ? pl.ok & ~(1u << h) : 0;
+            }
+            pl.k[h] = k0 + stride * page + slot * a.head_dim * EB;
+            pl.v[h] = v0 + stride * page + slot * EB;
+            if constexpr (TYPE == 2) {
+                pl.kw[h] = kw0 + wstride * page + slot * 4;
+                pl.vw[h] = vw0 + wstride * page + slot * 4;
             }
         }
         return pl;
     }
 };
-/* Byte offsets of a half's first position: of its keys (head_dim elements a position), of its values (dim 0), of its
- * scales (block 0). */
-__device__ __forceinline__ size_t key_at(const PagedArgs &a, uint32_t kh, uint32_t page, uint32_t slot, uint32_t bytes) {
-    return ((((size_t)page * a.kv_heads + kh) << a.shift) + slot) * a.head_dim * bytes;
-}
-__device__ __forceinline__ size_t value_at(const PagedArgs &a, uint32_t kh, uint32_t page, uint32_t slot, uint32_t bytes) {
-    return (((((size_t)page * a.kv_heads + kh) * a.head_dim) << a.shift) + slot) * bytes;
-}
-__device__ __forceinline__ size_t scale_at(const PagedArgs &a, uint32_t kh, uint32_t page, uint32_t slot) {
-    return (((((size_t)page * a.kv_heads + kh) * a.nb) << a.shift) + slot) * 4;
-}
 
 /* A wave's rows: queries, positions, and the running maximum, sum and O. */
 template <uint32_t TYPE, int KS, int RT>
@@ -246,7 +400,7 @@ struct Rows {
     Span span;
     uint32_t low_last; /* where the last row's window begins */
     f4 o[RT][DT];
-    float m[RT], l[RT];
+    float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
     float inv_e[TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values */
 
     /* `count` rows of the sequence from row0 on; columns past them see what the first one sees and are not stored. */
@@ -358,17 +512,17 @@ struct Rows {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const Frag k = src.k(t, i);
+                    if constexpr (TYPE == 0) {
 #pragma unroll
-                    for (int c = 0; c < RT; ++c) {
-                        if constexpr (TYPE == 0) {
+                        for (int j = 0; j < 8; ++j)
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                s[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(j < 4 ? k.a[j & 3] : k.b[j & 3],
-                                                                               qf[c][i].x[j], s[c][t], 0, 0, 0);
-                        } else {
-                            s[c][t] = mma(k, qf[c][i].lo, s[c][t]);
-                            s[c][t] = mma(k, qf[c][i].hi, s[c][t]);
-                        }
+                            for (int c = 0; c < RT; ++c)
+                                s[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(get(k, j), qf[c][i].x[j], s[c][t], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < RT; ++c) s[c][t] = mma(k, qf[c][i].lo, s[c][t]);
+#pragma unroll
+                        for (int c = 0; c < RT; ++c) s[c][t] = mma(k, qf[c][i].hi, s[c][t]);
                     }
                 }
 #pragma unroll
@@ -392,10 +546,7 @@ struct Rows {
         float mx[RT];
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
-            mx[c] = x[c][0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) mx[c] = fmaxf(mx[c], x[c][j]);
-            mx[c] *= factor[c];
+            mx[c] = max8(x[c]) * factor[c];
             up = up || mx[c] > m[c] + 8.0f;
         }
         if (__any(up)) {
@@ -460,27 +611,54 @@ struct Rows {
      * anything; a Q8 scale there must not set E either. */
     template <typename Src>
     __device__ __forceinline__ void product(uint32_t p0, uint32_t ok, bool full, const Src &src, const float (&x)[RT][8]) {
-        uint32_t bits = 0;
+        const bool have = ok >> (quad >> 1) & 1;
         if constexpr (TYPE == 2) {
+            f4 w[KS][2];
 #pragma unroll
             for (int b = 0; b < KS; ++b) {
-                f4 w0 = src.vscale(b, 0), w1 = src.vscale(b, 1);
-                if (!full) {
-                    const bool have = ok >> (quad >> 1) & 1;
+                w[b][0] = src.vscale(b, 0);
+                w[b][1] = src.vscale(b, 1);
+            }
+            if (!full) {
+                float r = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float &w = j < 4 ? *((float *)&w0 + j) : *((float *)&w1 + j - 4);
-                        w = have && span.holds(p0 + quad * 8 + j) ? w : 0.0f;
-                        bits |= odd(w) ? 1u << j : 0;
-                        w = odd(w) ? 0.0f : w;
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t in = have && span.holds(p0 + quad * 8 + j) ? 0xffffffffu : 0u;
+#pragma unroll
+                    for (int b = 0; b < KS; ++b) {
+                        float &y = ((float *)&w[b][j >> 2])[j & 3];
+                        y = __uint_as_float(__float_as_uint(y) & in);
+                        r = __builtin_fmaf(y, 0.0f, r);
                     }
                 }
-                float mx = fabsf(w0[0]);
+                if (__any(!(r == 0.0f))) {
+                    uint32_t bits = 0;
 #pragma unroll
-                for (int j = 1; j < 8; ++j) mx = fmaxf(mx, fabsf(j < 4 ? w0[j & 3] : w1[j & 3]));
-                if (__any(mx * inv_e[b] > 1.0f)) {
-                    const int e = max(-100, __builtin_amdgcn_frexp_expf(wave_max_quads(mx)));
-                    const float n = __builtin_ldexpf(1.0f, -e), r = n / inv_e[b]; /* a power of two <= 1 */
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int b = 0; b < KS; ++b)
+                            if (odd(w[b][j >> 2][j & 3])) {
+                                w[b][j >> 2][j & 3] = 0.0f;
+                                bits |= 1u << j;
+                            }
+                    spoil(p0, bits);
+                }
+            }
+            float mx[KS];
+            bool up = false;
+#pragma unroll
+            for (int b = 0; b < KS; ++b) {
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = fabsf(w[b][j >> 2][j & 3]);
+                mx[b] = max8(z);
+                up = up || mx[b] * inv_e[b] > 1.0f;
+            }
+            if (__any(up)) {
+#pragma unroll
+                for (int b = 0; b < KS; ++b) {
+                    const int e = max(-100, __builtin_amdgcn_frexp_expf(wave_max_quads(mx[b])));
+                    const float n = fminf(__builtin_ldexpf(1.0f, -e), inv_e[b]), r = n / inv_e[b]; /* a power of two <= 1 */
                     inv_e[b] = n;
 #pragma unroll
                     for (int c = 0; c < RT; ++c) {
@@ -488,31 +666,48 @@ struct Rows {
                         o[c][2 * b + 1] *= r;
                     }
                 }
-                w0 *= inv_e[b];
-                w1 *= inv_e[b];
+            }
+#pragma unroll
+            for (int b = 0; b < KS; ++b) {
+                w[b][0] *= inv_e[b];
+                w[b][1] *= inv_e[b];
                 const h8 v0 = codes8(src.v(2 * b)), v1 = codes8(src.v(2 * b + 1));
 #pragma unroll
                 for (int c = 0; c < RT; ++c) {
-                    float w[8];
+                    float y[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        w[j] = x[c][j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
-                        asm("" : "+v"(w[j])); /* rounded to f32, for both halves of the split */
+                        y[j] = x[c][j] * w[b][j >> 2][j & 3];
+                        asm("" : "+v"(y[j])); /* rounded to f32, for both halves of the split */
                     }
                     h8 hi, lo;
-                    split8(w, hi, lo);
-                    o[c][2 * b] = mma(v0, hi, mma(v0, lo, o[c][2 * b]));
-                    o[c][2 * b + 1] = mma(v1, hi, mma(v1, lo, o[c][2 * b + 1]));
+                    split8(y, hi, lo);
+                    o[c][2 * b] = mma(v0, lo, o[c][2 * b]);
+                    o[c][2 * b + 1] = mma(v1, lo, o[c][2 * b + 1]);
+                    o[c][2 * b] = mma(v0, hi, o[c][2 * b]);
+                    o[c][2 * b + 1] = mma(v1, hi, o[c][2 * b + 1]);
                 }
             }
-            if (!full && __any(bits)) spoil(p0, bits);
         } else {
-            bool some = false;
+            Frag v[DT];
+#pragma unroll
+            for (int t = 0; t < DT; ++t) v[t] = src.v(t);
             if (!full) {
                 float r = 0.0f;
 #pragma unroll
-                for (int t = 0; t < DT; ++t) r += test(src.v(t));
-                some = __any(!(r == 0.0f));
+                for (int t = 0; t < DT; ++t) r += test(v[t]);
+                if (__any(!(r == 0.0f))) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (odd(get(v[t], j))) {
+                                zero(v[t], j);
+                                bits |= 1u << j;
+                            }
+                    spoil(p0, have ? bits : 0);
+                }
             }
             h8 hi[RT], lo[RT];
             if constexpr (TYPE == 1) {
@@ -521,27 +716,19 @@ struct Rows {
             }
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                Frag v = src.v(t);
-                if (some) { /* uniform, rare */
+                if constexpr (TYPE == 0) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (odd(get(v, j))) {
-                            zero(v, j);
-                            bits |= 1u << j;
-                        }
-                }
 #pragma unroll
-                for (int c = 0; c < RT; ++c) {
-                    if constexpr (TYPE == 0) {
+                        for (int c = 0; c < RT; ++c)
+                            o[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(get(v[t], j), x[c][j], o[c][t], 0, 0, 0);
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            o[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(get(v, j), x[c][j], o[c][t], 0, 0, 0);
-                    } else {
-                        o[c][t] = mma(v, hi[c], mma(v, lo[c], o[c][t]));
-                    }
+                    for (int c = 0; c < RT; ++c) o[c][t] = mma(v[t], lo[c], o[c][t]);
+#pragma unroll
+                    for (int c = 0; c < RT; ++c) o[c][t] = mma(v[t], hi[c], o[c][t]);
                 }
             }
-            if (some) spoil(p0, ok >> (quad >> 1) & 1 ? bits : 0);
         }
     }
 
@@ -562,75 +749,60 @@ struct Rows {
     }
 };
 
-/* A step's keys and values in registers, loaded straight from the pages. SMALL: pages of 16, so a step lies in two;
- * else in one, whose address is uniform. Where head_dim ends inside 32 dims of keys the lanes past it read the 16 before
- * again (q is 0 there); value dims past it are read at 0 and not stored. */
+/* A step's keys and values in registers, loaded straight from the pages. Where head_dim ends inside 32 dims of keys the
+ * lanes past it read the 16 before again (q is 0 there); value dims past it are read at 0 and not stored. */
 template <uint32_t TYPE, int KS, bool SMALL>
 struct InRegisters {
     typedef typename Elem<TYPE>::Frag Frag;
+    typedef typename Pages<TYPE, SMALL>::Place Place;
     static constexpr uint32_t EB = Elem<TYPE>::bytes;
     static constexpr int DT = 2 * KS, NS = TYPE == 2 ? KS : 1;
     Frag kf[2][KS], vf[DT];
     f4 kw[NS][2], vw[NS][2];
+    uint32_t hd, shift, nb, kwhole, kpart, voff, woff; /* the lane's offsets */
+    bool second;                                       /* SMALL: of the second page; keys and values alike */
+    bool ksecond;
 
+    __device__ __forceinline__ InRegisters(const PagedArgs &a) : hd(a.head_dim), shift(a.shift), nb(a.nb) {
+        const uint32_t lane = threadIdx.x % 64, u = lane % 16 >> 2, quad = lane / 16;
+        ksecond = SMALL && u >> 1;
+        second = SMALL && quad >> 1;
+        const uint32_t r = ((SMALL ? u & 1 : u) * 8 + (lane & 3)) * hd * EB, q = SMALL ? quad & 1 : quad;
+        kwhole = r + quad * 8 * EB;
+        kpart = r + (quad & 1) * 8 * EB;
+        voff = ((lane % 16 << shift) + q * 8) * EB;
+        woff = q * 32;
+    }
     __device__ __forceinline__ Frag k(int t, int s) const { return kf[t][s]; }
     __device__ __forceinline__ Frag v(int t) const { return vf[t]; }
     __device__ __forceinline__ f4 kscale(int s, int h) const { return kw[s][h]; }
     __device__ __forceinline__ f4 vscale(int s, int h) const { return vw[s][h]; }
 
-    __device__ __forceinline__ void load_k(const PagedArgs &a, uint32_t kh, const Place &pl) {
-        const uint32_t lane = threadIdx.x % 64, u = lane % 16 >> 2, quad = lane / 16, hd = a.head_dim;
-        const uint32_t row = (u & 1) * 8 + (lane & 3);
-        const unsigned char *p = (const unsigned char *)a.keys;
-        uint32_t r;
-        if constexpr (SMALL) {
-            const size_t p0 = key_at(a, kh, pl.page[0], pl.slot[0], EB), p1 = key_at(a, kh, pl.page[1], pl.slot[1], EB);
-            p += u >> 1 ? p1 : p0;
-            r = row * hd * EB;
-        } else {
-            p += key_at(a, kh, pl.page[0], pl.slot[0], EB);
-            r = (row + (u >> 1) * 16) * hd * EB;
-        }
-        const uint32_t whole = r + quad * 8 * EB, part = r + (quad & 1) * 8 * EB;
+    static __device__ __forceinline__ const unsigned char *pick(const unsigned char *const (&p)[Pages<TYPE, SMALL>::N], bool second) {
+        if constexpr (SMALL) return second ? p[1] : p[0];
+        else return p[0];
+    }
+    __device__ __forceinline__ void load_k(const Place &pl) {
+        const unsigned char *p = pick(pl.k, ksecond);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const unsigned char *b = p + (((uint32_t)s * 32 < hd ? s * 32 : 0) + t * 4 * hd) * EB;
-                kf[t][s] = load_frag<TYPE>(b + ((uint32_t)s * 32 + 32 <= hd ? whole : part));
+                kf[t][s] = load_frag<TYPE>(b + ((uint32_t)s * 32 + 32 <= hd ? kwhole : kpart));
             }
-        if constexpr (TYPE == 2) load_scales(a, a.ks, kh, pl, kw);
+        if constexpr (TYPE == 2) load_scales(pick(pl.kw, second), kw);
     }
-    __device__ __forceinline__ void load_v(const PagedArgs &a, uint32_t kh, const Place &pl) {
-        const uint32_t lane = threadIdx.x % 64, quad = lane / 16;
-        const unsigned char *p = (const unsigned char *)a.values;
-        uint32_t r = (lane % 16 << a.shift) * EB;
-        if constexpr (SMALL) {
-            const size_t p0 = value_at(a, kh, pl.page[0], pl.slot[0], EB), p1 = value_at(a, kh, pl.page[1], pl.slot[1], EB);
-            p += quad >> 1 ? p1 : p0;
-            r += (quad & 1) * 8 * EB;
-        } else {
-            p += value_at(a, kh, pl.page[0], pl.slot[0], EB);
-            r += quad * 8 * EB;
-        }
+    __device__ __forceinline__ void load_v(const Place &pl) {
+        const unsigned char *p = pick(pl.v, second);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) vf[t] = load_frag<TYPE>(p + (((t * 16u < a.head_dim ? t * 16 : 0) << a.shift) * EB) + r);
-        if constexpr (TYPE == 2) load_scales(a, a.vs, kh, pl, vw);
+        for (int t = 0; t < DT; ++t) vf[t] = load_frag<TYPE>(p + (((t * 16u < hd ? t * 16 : 0) << shift) * EB) + voff);
+        if constexpr (TYPE == 2) load_scales(pick(pl.vw, second), vw);
     }
-    __device__ __forceinline__ void load_scales(const PagedArgs &a, const float *sc, uint32_t kh, const Place &pl, f4 (&x)[NS][2]) {
-        const uint32_t quad = threadIdx.x % 64 / 16;
-        const unsigned char *p = (const unsigned char *)sc;
-        uint32_t r = quad * 32;
-        if constexpr (SMALL) {
-            const size_t p0 = scale_at(a, kh, pl.page[0], pl.slot[0]), p1 = scale_at(a, kh, pl.page[1], pl.slot[1]);
-            p += quad >> 1 ? p1 : p0;
-            r = (quad & 1) * 32;
-        } else {
-            p += scale_at(a, kh, pl.page[0], pl.slot[0]);
-        }
+    __device__ __forceinline__ void load_scales(const unsigned char *p, f4 (&x)[NS][2]) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const f4 *y = (const f4 *)(p + (((uint32_t)s < a.nb ? s : 0) << a.shift) * 4 + r);
+            const f4 *y = (const f4 *)(p + (((uint32_t)s < nb ? s : 0) << shift) * 4 + woff);
             x[s][0] = y[0];
             x[s][1] = y[1];
         }
@@ -640,16 +812,17 @@ struct InRegisters {
 /* A step's keys and values in LDS, brought there by the whole workgroup without registers (global loads to LDS, 16
  * bytes a lane, the lanes' pieces one after another): pieces in the order in which the products read them, so that a
  * fragment's read is free of bank conflicts. f16 and f32: a piece is (half) a lane's fragment. Q8: a piece is 16 codes,
- * the fragments of two quads; one more KiB holds the scales of both, block by block. */
-template <uint32_t TYPE, int KS>
+ * the fragments of two quads; behind them the scales of both, block by block. */
+template <uint32_t TYPE, int KS, bool SMALL>
 struct InLds {
     typedef typename Elem<TYPE>::Frag Frag;
+    typedef typename Pages<TYPE, SMALL>::Place Place;
     static constexpr uint32_t EB = Elem<TYPE>::bytes;
     static constexpr int DT = 2 * KS;
-    static constexpr uint32_t K_BYTES = 32 * 32 * KS * EB, V_BYTES = K_BYTES;
+    static constexpr uint32_t K_BYTES = 32 * 32 * KS * EB;
     static constexpr uint32_t W_BYTES = TYPE == 2 ? 128 * KS : 0; /* the scales of keys or of values */
-    static constexpr uint32_t BYTES = K_BYTES + V_BYTES + 2 * W_BYTES;
-    static constexpr uint32_t K_LOADS = K_BYTES / 1024, LOADS = 2 * K_LOADS + (2 * W_BYTES + 1023) / 1024; /* of a wave */
+    static constexpr uint32_t K_LOADS = K_BYTES / 1024, W_LOADS = (2 * W_BYTES + 1023) / 1024; /* of a wave */
+    static constexpr uint32_t BUFFER = 2 * K_BYTES + W_LOADS * 1024, EACH = (K_LOADS + PA_WAVES - 1) / PA_WAVES;
     const unsigned char *b; /* the buffer of the step */
 
     __device__ __forceinline__ Frag k(int t, int s) const {
@@ -668,69 +841,85 @@ struct InLds {
         else return {*(const f4 *)(p + t * 2048 + lane * 16), *(const f4 *)(p + t * 2048 + 1024 + lane * 16)};
     }
     __device__ __forceinline__ f4 kscale(int s, int h) const {
-        return *(const f4 *)(b + K_BYTES + V_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
+        return *(const f4 *)(b + 2 * K_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
     }
     __device__ __forceinline__ f4 vscale(int s, int h) const {
-        return *(const f4 *)(b + K_BYTES + V_BYTES + W_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
+        return *(const f4 *)(b + 2 * K_BYTES + W_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
     }
 
-    /* The lane's piece of load i of a step. */
-    static __device__ __forceinline__ const unsigned char *source(const PagedArgs &a, uint32_t kh, const Place &pl, uint32_t i) {
-        const uint32_t lane = threadIdx.x % 64, hd = a.head_dim;
-        if (i < K_LOADS) {
-            uint32_t t, m, d; /* tile, row, first dim */
-            if constexpr (TYPE == 2) {
-                t = lane / 16 & 1;
-                m = lane % 16;
-                d = (i * 2 + lane / 32) * 16;
-            } else if constexpr (TYPE == 1) {
-                t = i & 1;
-                m = lane % 16;
-                d = i / 2 * 32 + lane / 16 * 8;
-            } else {
-                t = i / 2 & 1;
-                m = lane % 16;
-                d = i / 4 * 32 + lane / 16 * 8 + (i & 1) * 4;
-            }
-            d = d < hd ? d : 0; /* q is 0 there */
-            const uint32_t u = m >> 2, pos = u * 8 + t * 4 + (m & 3), h = pos >> 4;
-            return (const unsigned char *)a.keys + key_at(a, kh, h ? pl.page[1] : pl.page[0], h ? pl.slot[1] : pl.slot[0], EB) +
-                   ((pos & 15) * hd + d) * EB;
-        }
-        if (i < 2 * K_LOADS) {
-            i -= K_LOADS;
-            uint32_t d, pos;
-            if constexpr (TYPE == 2) {
-                d = (i * 2 + lane / 32) * 16 + lane % 16;
-                pos = (lane / 16 & 1) * 16;
-            } else if constexpr (TYPE == 1) {
-                d = i * 16 + lane % 16;
-                pos = lane / 16 * 8;
-            } else {
-                d = i / 2 * 16 + lane % 16;
-                pos = lane / 16 * 8 + (i & 1) * 4;
-            }
-            d = d < hd ? d : 0; /* not stored */
-            const uint32_t h = pos >> 4;
-            return (const unsigned char *)a.values + value_at(a, kh, h ? pl.page[1] : pl.page[0], h ? pl.slot[1] : pl.slot[0], EB) +
-                   ((d << a.shift) + (pos & 15)) * EB;
-        }
-        const uint32_t x = (i - 2 * K_LOADS) * 64 + lane, block = x / 8 % KS, pos = x % 8 * 4, h = pos >> 4;
-        const float *sc = x / 8 < KS ? a.ks : a.vs; /* past both (heads of 32): the values' again, not read */
-        return (const unsigned char *)sc + scale_at(a, kh, h ? pl.page[1] : pl.page[0], h ? pl.slot[1] : pl.slot[0]) +
-               ((block < a.nb ? block : 0) << a.shift) * 4 + (pos & 15) * 4;
-    }
-    /* The wave's share of a step's loads into `to`. */
-    static __device__ __forceinline__ void load(const PagedArgs &a, uint32_t kh, const Place &pl, uint32_t wave, unsigned char *to) {
+    /* A wave's part of a step's loads: every fourth piece of keys and of values, one wave the scales. The lane's
+     * offsets from the step's place, and which of two pages they are from. */
+    struct Loader {
+        uint32_t wave, koff[EACH], voff[EACH], woff[W_LOADS ? W_LOADS : 1];
+        bool ksecond, vsecond, wsecond, wvalues[W_LOADS ? W_LOADS : 1];
+
+        __device__ __forceinline__ Loader(const PagedArgs &a, uint32_t wave_) : wave(wave_) {
+            const uint32_t lane = threadIdx.x % 64, hd = a.head_dim, m = lane % 16, quad = lane / 16;
+            ksecond = SMALL && m >> 3;
+            vsecond = SMALL && (TYPE == 2 ? quad & 1 : quad >> 1);
+            wsecond = SMALL && lane % 8 / 4;
 #pragma unroll
-        for (uint32_t j = 0; j < (LOADS + PA_WAVES - 1) / PA_WAVES; ++j) {
-            const uint32_t i = j * PA_WAVES + wave;
-            if (i < LOADS)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)source(a, kh, pl, i),
-                                                 (__attribute__((address_space(3))) void *)(to + i * 1024), 16, 0, 0);
+            for (uint32_t j = 0; j < EACH; ++j) {
+                const uint32_t i = j * PA_WAVES + wave;
+                uint32_t t, d; /* keys: tile and first dim */
+                if constexpr (TYPE == 2) {
+                    t = quad & 1;
+                    d = (i * 2 + lane / 32) * 16;
+                } else if constexpr (TYPE == 1) {
+                    t = i & 1;
+                    d = i / 2 * 32 + quad * 8;
+                } else {
+                    t = i / 2 & 1;
+                    d = i / 4 * 32 + quad * 8 + (i & 1) * 4;
+                }
+                d = d < hd ? d : 0; /* q is 0 there */
+                uint32_t pos = (m >> 2) * 8 + t * 4 + (m & 3);
+                koff[j] = ((SMALL ? pos & 15 : pos) * hd + d) * EB;
+                if constexpr (TYPE == 2) { /* values: dim and first position */
+                    d = (i * 2 + lane / 32) * 16 + m;
+                    pos = (quad & 1) * 16;
+                } else if constexpr (TYPE == 1) {
+                    d = i * 16 + m;
+                    pos = quad * 8;
+                } else {
+                    d = i / 2 * 16 + m;
+                    pos = quad * 8 + (i & 1) * 4;
+                }
+                d = d < hd ? d : 0; /* not stored */
+                voff[j] = ((d << a.shift) + (SMALL ? pos & 15 : pos)) * EB;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < W_LOADS; ++j) {
+                const uint32_t x = j * 64 + lane, block = x / 8 % KS, pos = x % 8 * 4;
+                wvalues[j] = x / 8 >= KS; /* past both (heads of 32): the values' again, not read */
+                woff[j] = (((block < a.nb ? block : 0) << a.shift) + (SMALL ? pos & 15 : pos)) * 4;
+            }
         }
-    }
-    static constexpr uint32_t BUFFER = LOADS * 1024;
+        static __device__ __forceinline__ void move(const unsigned char *from, unsigned char *to) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                             (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+        }
+        __device__ __forceinline__ void load(const Place &pl, unsigned char *to) const {
+            typedef InRegisters<TYPE, KS, SMALL> Pick;
+            const unsigned char *k = Pick::pick(pl.k, ksecond), *v = Pick::pick(pl.v, vsecond);
+#pragma unroll
+            for (uint32_t j = 0; j < EACH; ++j) {
+                const uint32_t i = j * PA_WAVES + wave;
+                if (K_LOADS % PA_WAVES == 0 || i < K_LOADS) {
+                    move(k + koff[j], to + i * 1024);
+                    move(v + voff[j], to + K_BYTES + i * 1024);
+                }
+            }
+            if constexpr (TYPE == 2) {
+                if (wave == PA_WAVES - 1) {
+                    const unsigned char *kw = Pick::pick(pl.kw, wsecond), *vw = Pick::pick(pl.vw, wsecond);
+#pragma unroll
+                    for (uint32_t j = 0; j < W_LOADS; ++j)
+                        move((wvalues[j] ? vw : kw) + woff[j], to + 2 * K_BYTES + j * 1024);
+                }
+            }
+        }
+    };
     /* This wave's loads to LDS are done, then everyone's. */
     static __device__ __forceinline__ void wait() {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -753,13 +942,14 @@ struct Out {
             }
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l; /* a row that sees nothing is 0 */
-            *(f4u *)(att + row_at(a, sq, kh, row0 + r) + d) = o * inv;
+            *(f4u *)(att + row_at(a, sq.begin, kh, row0 + r) + d) = o * inv;
         }
     }
 };
 
-/* 16 rows or fewer: the four waves share the steps [u0, u1) out, each with its steps' keys and values in registers, and
- * join their results in LDS. The keys of a wave's next step are requested as soon as this step's are used. */
+/* 16 rows or fewer: the waves take the steps [u0, u1) in turn, each with its steps' keys and values in registers, and
+ * join their results in LDS. In turn, not in runs: a step's values are 64 bytes (f16) of each dim's row in the page, and
+ * the cache lines' other halves are the next steps'; with runs half of every line was fetched twice. The keys of a wave's next step are requested as soon as this step's are used. */
 template <uint32_t TYPE, int KS, bool SMALL>
 __device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
                                             uint32_t u0, uint32_t u1, uint32_t wave, const Out &out, unsigned char *lds) {
@@ -767,24 +957,22 @@ __device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, 
     float(*so)[16][LD] = (float(*)[16][LD])lds;
     float(*sml)[16][2] = (float(*)[16][2])(lds + PA_WAVES * 16 * LD * 4);
     Rows<TYPE, KS, 1> w(a, q, sq, out.kh, out.row0, (int)out.n);
-    const uint32_t n = u1 - u0, e = u0 + n * (wave + 1) / PA_WAVES;
-    u0 += n * wave / PA_WAVES;
-    if (u0 < e) {
-        Table table;
-        table.open(a, seq);
-        InRegisters<TYPE, KS, SMALL> src;
+    u0 += wave;
+    if (u0 < u1) {
+        Pages<TYPE, SMALL> pages(a, seq, out.kh);
+        InRegisters<TYPE, KS, SMALL> src(a);
         uint32_t at = st.at(u0);
-        Place pl = table.locate(a, at, w.span);
-        src.load_k(a, out.kh, pl);
-        for (uint32_t u = u0; u < e; ++u) {
+        auto pl = pages.locate(at, w.span);
+        src.load_k(pl);
+        for (uint32_t u = u0; u < u1; u += PA_WAVES) {
             const uint32_t p0 = at * PA_STEP;
-            at = st.at(min(u + 1, e - 1)); /* the last one's keys twice */
-            const Place next = table.locate(a, at, w.span);
+            at = st.at(u + PA_WAVES < u1 ? u + PA_WAVES : u); /* the last one's keys twice */
+            src.load_v(pl);
+            const auto next = pages.locate(at, w.span);
             const bool full = w.full(p0, pl.ok);
             float x[1][8];
-            src.load_v(a, out.kh, pl);
             w.scores(src, x);
-            src.load_k(a, out.kh, next);
+            src.load_k(next);
             w.weights(p0, pl.ok, full, x);
             w.product(p0, pl.ok, full, src, x);
             pl = next;
@@ -798,7 +986,7 @@ __device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, 
         sml[wave][w.col][1] = w.l[0];
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < out.n * (a.head_dim / 4); i += PA_WG) {
+    for (uint32_t i = threadIdx.x; i < out.n * (a.head_dim / 4); i += 64 * PA_WAVES) {
         const uint32_t r = i / (a.head_dim / 4), d = 4 * (i % (a.head_dim / 4));
         float m = sml[0][r][0], l = 0.0f;
 #pragma unroll
@@ -817,10 +1005,10 @@ constexpr uint32_t shared_lds(int ks) { return PA_WAVES * 16 * (32 * ks + 4) * 4
 
 /* Each wave has 16 * RT rows of the tile over the steps [u0, u1), whose keys and values the workgroup brings to LDS, the
  * next step's while this one is computed. A wave without rows (or whose rows do not see a step) only loads. */
-template <uint32_t TYPE, int KS, int RT>
+template <uint32_t TYPE, int KS, int RT, bool SMALL>
 __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
                                            uint32_t u0, uint32_t u1, uint32_t wave, const Out &out, unsigned char *lds) {
-    typedef InLds<TYPE, KS> Src;
+    typedef InLds<TYPE, KS, SMALL> Src;
     const uint32_t first = wave * 16 * RT, G = a.heads / a.kv_heads;
     const bool mine = first < out.n;
     /* the last wave's rows again where there are none: never stored */
@@ -829,30 +1017,28 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, c
     const int64_t tmin = sq.first + out.row0 / G, tmax = min(sq.first + (out.row0 + out.n - 1) / G, (int64_t)a.limit - 1);
     const Span span = span_of(a, (int)max((int64_t)-1, tmin), (int)max((int64_t)-1, tmax));
     if (u0 < u1) {
-        Table table;
-        table.open(a, seq);
+        Pages<TYPE, SMALL> pages(a, seq, out.kh);
+        const typename Src::Loader loader(a, wave);
         uint32_t at = st.at(u0);
-        Place pl = table.locate(a, at, span);
-        Src::load(a, out.kh, pl, wave, lds);
+        auto pl = pages.locate(at, span);
+        loader.load(pl, lds);
         Src::wait();
         for (uint32_t u = u0; u < u1; ++u) {
-            const uint32_t p0 = at * PA_STEP;
-            Place next = pl;
+            const uint32_t p0 = at * PA_STEP, ok = pl.ok;
             if (u + 1 < u1) {
                 at = st.at(u + 1);
-                next = table.locate(a, at, span);
-                Src::load(a, out.kh, next, wave, lds + ((u + 1 - u0) & 1) * Src::BUFFER);
+                pl = pages.locate(at, span);
+                loader.load(pl, lds + ((u + 1 - u0) & 1) * Src::BUFFER);
             }
             __builtin_amdgcn_sched_barrier(0); /* the loads first: the compiler would sink them behind the products */
             if (mine && w.span.meets(p0, PA_STEP)) {
                 const Src src = {lds + ((u - u0) & 1) * Src::BUFFER};
-                const bool full = w.full(p0, pl.ok);
+                const bool full = w.full(p0, ok);
                 float x[RT][8];
                 w.scores(src, x);
-                w.weights(p0, pl.ok, full, x);
-                w.product(p0, pl.ok, full, src, x);
+                w.weights(p0, ok, full, x);
+                w.product(p0, ok, full, src, x);
             }
-            pl = next;
             Src::wait(); /* the next step is there, and this one's buffer free */
         }
     }
@@ -870,57 +1056,103 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, c
     }
 }
 
-/* Workgroups by split, KV head, tile: those of one KV head and split follow each other at a distance of all heads and
- * splits, so where these are a multiple of the eight XCDs the tiles of a sequence that read the same pages share an L2.
- * Tiles run from the last to the first: the last rows of a chunk see the most. */
+/* The units [v, e) of a tile, which belong to workgroup i's run [i each, (i + 1) each) of a KV head; each 0: all of the
+ * tile, undivided. */
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
-__global__ __launch_bounds__(PA_WG, attend_waves(TYPE, KS)) void k_paged_attend(PagedArgs a, const float *q, float *att,
-                                                                                uint32_t tile_rows, uint32_t tiles, uint32_t splits,
-                                                                                uint32_t *used, float *part) {
-    constexpr uint32_t OWN_LDS = OWNS ? 2 * InLds<TYPE, KS>::BUFFER : 0;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[OWN_LDS > shared_lds(KS) ? OWN_LDS : shared_lds(KS)];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), split = blockIdx.x % splits;
-    const uint32_t kh = blockIdx.x / splits % a.kv_heads, tile = tiles - 1 - blockIdx.x / splits / a.kv_heads;
-    const uint32_t G = a.heads / a.kv_heads;
-    const size_t slot = (size_t)tile * a.kv_heads + kh;
-    uint32_t seq, row0;
-    Seq sq;
-    if (!find_tile(a, tile, tile_rows, seq, row0) || !sequence(a, seq, sq)) {
-        if (used && split == 0 && threadIdx.x == 0) used[slot] = 0;
-        return;
-    }
-    const uint32_t n = min(tile_rows, (uint32_t)sq.n * G - row0);
-    const Steps st = tile_steps(a, sq.first + row0 / G, sq.first + (row0 + n - 1) / G);
-    const uint32_t parts = max(1u, min(splits, st.total / PA_MIN_STEPS));
-    if (used && split == 0 && threadIdx.x == 0) used[slot] = parts;
-    if (split >= parts) return;
-    const uint32_t u0 = (uint32_t)((uint64_t)st.total * split / parts), u1 = (uint32_t)((uint64_t)st.total * (split + 1) / parts);
-    Out out = {a, sq, kh, row0, n, att, nullptr, nullptr};
-    if (parts > 1) {
-        const size_t r = (slot * splits + split) * tile_rows;
-        out.po = part + r * a.head_dim;
-        out.pml = part + (size_t)tiles * a.kv_heads * splits * tile_rows * a.head_dim + 2 * r;
+__device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used,
+                                          float *part, uint32_t kh, const Tile &t, uint32_t i, uint32_t each, uint32_t v,
+                                          uint32_t e, unsigned char *lds) {
+    const uint32_t G = a.heads / a.kv_heads, row0 = t.j * p.tile_rows, n = min(p.tile_rows, (uint32_t)t.sq.n * G - row0);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const Steps st = tile_steps(a, t.sq.first + row0 / G, t.sq.first + (row0 + n - 1) / G);
+    Out out = {a, t.sq, kh, row0, n, att, nullptr, nullptr};
+    uint32_t u0 = 0, u1 = st.total;
+    if (each) {
+        const uint32_t i0 = t.first / each, parts = (t.first + t.units - 1) / each - i0 + 1;
+        const uint32_t slot = 2 * i + (v == i * each ? 0 : 1);
+        if (i == i0 && threadIdx.x == 0)
+            used[(size_t)t.t * a.kv_heads + kh] = i4{(int)(parts | n << 16), t.sq.begin, (int)row0, (int)slot};
+        if (parts > 1) {
+            const size_t r = ((size_t)slot * a.kv_heads + kh) * p.tile_rows;
+            out.po = part + r * a.head_dim;
+            out.pml = part + (size_t)2 * p.stream * a.kv_heads * p.tile_rows * a.head_dim + 2 * r;
+            /* both sides of a cut round it alike; the tile's ends are 0 and all */
+            const float f = (float)t.units, all = (float)st.total;
+            u0 = (uint32_t)((float)(v - t.first) / f * all);
+            u1 = (uint32_t)((float)(e - t.first) / f * all);
+        }
     }
     if constexpr (OWNS) {
-        if (n > 16) tile_owned<TYPE, KS, RT>(a, q, sq, seq, st, u0, u1, wave, out, lds);
-        else tile_shared<TYPE, KS, SMALL>(a, q, sq, seq, st, u0, u1, wave, out, lds);
+        if (n > 16) {
+            tile_owned<TYPE, KS, RT, SMALL>(a, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
+            return;
+        }
+    }
+    tile_shared<TYPE, KS, SMALL>(a, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
+}
+
+/* Workgroups of one KV head follow each other at a distance of all heads, so where these are a multiple of the eight XCDs
+ * the tiles of a sequence that read the same pages share an L2.
+ *
+ * A run's tiles are taken one after another by one workgroup while decoding: as many workgroups as CUs stream without a
+ * pause, each its share. Where waves own rows every piece of a run is a workgroup of its own, in no loop: what a loop
+ * carries costs the products their registers (heads of 128: 40 spilled), and pieces are long. */
+template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
+__global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_attend(PagedArgs a, const float *q, float *att,
+                                                                                  AttendPlan p, i4 *used, float *part) {
+    constexpr uint32_t OWN_LDS = OWNS ? 2 * InLds<TYPE, KS, SMALL>::BUFFER : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[OWN_LDS > shared_lds(KS) ? OWN_LDS : shared_lds(KS)];
+    const uint32_t kh = blockIdx.x % a.kv_heads;
+    uint32_t i = blockIdx.x / a.kv_heads;
+    if (blockIdx.x == 0) check_begin(a, threadIdx.x, 64 * PA_WAVES);
+    Tile t;
+    if (!p.stream) { /* from the last tile to the first: the last rows of a chunk see the most */
+        Tiles tiles(a, p);
+        if (tiles.by_number(p.tiles - 1 - i, t))
+            tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, 0, 0, 0, lds);
+        return;
+    }
+    uint32_t units, count, each;
+    {
+        Tiles tiles(a, p);
+        tiles.total(units, count);
+        if (i == 0) /* tiles that the batch does not need */
+            for (uint32_t x = count + threadIdx.x; x < p.tiles; x += 64 * PA_WAVES) used[(size_t)x * a.kv_heads + kh] = i4{};
+        each = max((units + p.stream - 1) / p.stream, (PA_MIN_STEPS * 64 >> p.unit) + 1);
+        if constexpr (OWNS) { /* tile t's first piece has number t + its first unit / each, from the last to the first */
+            i = p.stream + p.tiles - 1 - i;
+            if (!tiles.last_with(i, [&](uint32_t u, uint32_t n) { return u / each + n; }, t)) return;
+            i -= t.t; /* the workgroup whose run it is */
+        }
+    }
+    if constexpr (OWNS) {
+        const uint32_t v = max(t.first, i * each), e = min(t.first + t.units, (i + 1) * each);
+        if (v < e) tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
     } else {
-        tile_shared<TYPE, KS, SMALL>(a, q, sq, seq, st, u0, u1, wave, out, lds);
+        const uint32_t end = min(units, (i + 1) * each); /* stream * each is below 2^31: see attend_plan */
+        for (uint32_t v = i * each; v < end;) {
+            Tiles tiles(a, p);
+            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
+            const uint32_t e = min(end, t.first + t.units);
+            tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
+            v = e;
+            if (v < end) __syncthreads(); /* LDS is free */
+        }
     }
 }
 
 }  // namespace
 
 template <uint32_t TYPE>
-hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, uint32_t *used, float *part,
+hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
                          hipStream_t s) {
-    const dim3 grid(a.kv_heads * p.splits * p.tiles);
-#define SMQ_ATTEND3(KS, RT, OWNS, SMALL)                                                                              \
-    hipLaunchKernelGGL((k_paged_attend<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(PA_WG), 0, s, a, q, att, p.tile_rows,  \
-                       p.tiles, p.splits, used, part)
+    const dim3 grid(a.kv_heads * (!p.stream ? p.tiles : p.owns ? p.tiles + p.stream : p.stream));
+#define SMQ_ATTEND3(KS, RT, OWNS, SMALL)                                                                               \
+    hipLaunchKernelGGL((k_paged_attend<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(64 * PA_WAVES), 0, s, a, q, att, p, used, \
+                       part)
 #define SMQ_ATTEND(KS)                                                            \
     do {                                                                          \
-        constexpr int RT = attend_rt(TYPE, KS);                                   \
+        constexpr int RT = attend_rt(KS);                                   \
         if (p.owns && a.shift > 4) SMQ_ATTEND3(KS, RT, true, false);              \
         else if (p.owns) SMQ_ATTEND3(KS, RT, true, true);                         \
         else if (a.shift > 4) SMQ_ATTEND3(KS, 1, false, false);                   \

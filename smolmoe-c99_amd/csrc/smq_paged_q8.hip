@@ -3,6 +3,6 @@
 #include "smq_paged_attend.h"
 
 namespace smq {
-template hipError_t launch_attend<2>(const PagedArgs &, const AttendPlan &, const float *, float *, uint32_t *, float *,
+template hipError_t launch_attend<2>(const PagedArgs &, const AttendPlan &, const float *, float *, i4 *, float *,
                                        hipStream_t);
 }  // namespace smq
