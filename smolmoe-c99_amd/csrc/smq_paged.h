@@ -20,9 +20,10 @@ __device__ __forceinline__ int page_of(const PagedArgs &a, uint32_t s, uint32_t 
 /* Sequence s's new tokens: rows begin .. begin + n at positions first .. first + n. False, with the flag raised, where
  * begin does not ascend within 0 .. tokens. */
 struct Seq {
-    int begin, n;
-    int64_t first;
+    int begin, n, first;
 };
+/* length - n without overflow: what no position of the n tokens (below 2^23) can make a place (0 .. 2^20) stays none. */
+__device__ __forceinline__ int first_position(int length, int n) { return min(max(length, -(1 << 25)), 1 << 30) - n; }
 __device__ __forceinline__ bool sequence(const PagedArgs &a, uint32_t s, Seq &q) {
     const int b0 = a.begin[s], b1 = a.begin[s + 1];
     if (b0 < 0 || b1 < b0 || (uint32_t)b1 > a.tokens) {
@@ -31,7 +32,7 @@ __device__ __forceinline__ bool sequence(const PagedArgs &a, uint32_t s, Seq &q)
     }
     q.begin = b0;
     q.n = b1 - b0;
-    q.first = (int64_t)a.length[s] - q.n;
+    q.first = first_position(a.length[s], q.n);
     return true;
 }
 
@@ -56,8 +57,8 @@ __device__ __forceinline__ bool place_of(const PagedArgs &a, uint32_t r, uint32_
     if (!lo || a.begin[lo] <= (int)r) return false; /* behind the last sequence (lo == seqs) */
     s = lo - 1;
     if (!sequence(a, s, q)) return false;
-    const int64_t p = q.first + (int)(r - (uint32_t)q.begin);
-    if (p < 0 || p >= (int64_t)a.limit) {
+    const int p = q.first + (int)(r - (uint32_t)q.begin);
+    if ((uint32_t)p >= a.limit) {
         *a.flag = 1;
         return false;
     }

@@ -145,18 +145,41 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
 }
 
 /* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own
- * theirs. Workgroups: one a CU while decoding, whose rate is then that of the memory, two a CU for products. */
+ * theirs.
+ *
+ * Workgroups that share the steps out: two a CU for products and for decoding heads of up to 64 (8 KiB of f16 a step and
+ * wave: 64 sequences at 5000, 8 KV heads, 134 us with one a CU, 94 with two), one a CU for wider ones (16 x 12000, 8 KV
+ * heads of 128: 145, 150; 32 x 3000 Q8, 2 KV heads: 31, 35).
+ *
+ * Sharing them out costs a second launch, which joins: not where there are tiles for every CU four times over, and not
+ * where a tile's steps at the longest length exceed an equal share by less than that (about 24 steps: 64 sequences at 700,
+ * 2 KV heads of 64: 11.8 us with a workgroup per tile, 15.4 shared out). */
 AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     AttendPlan p;
-    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
+    const uint32_t G = a.heads / a.kv_heads;
+    const uint64_t rows = (uint64_t)a.tokens * G, seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
     p.owns = rows > 32 * seqs;
     p.tile_rows = p.owns ? 64 * attend_rt(attend_ks(a.head_dim)) : 16;
-    p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) / p.tile_rows);
-    p.stream = ((p.owns ? 512 : 256) + a.kv_heads - 1) / a.kv_heads;
-    p.unit = 0; /* all units (at most this many) and the last workgroup's end below 2^31 */
-    while (((uint64_t)p.tiles * (2 * (uint64_t)a.limit + 128) >> p.unit) + p.tiles + 64 * 512 >= 1u << 30) ++p.unit;
-    if (a.limit <= PA_MIN_STEPS * PA_STEP && p.tiles >= p.stream) p.stream = 0; /* short sequences: a tile each */
-    if (a.limit <= PA_MIN_STEPS * PA_STEP && !p.owns) p.stream = 0;
+    p.row_shift = p.tile_rows == 128 ? 7 : p.tile_rows == 64 ? 6 : 4;
+    p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) >> p.row_shift);
+    const uint32_t groups = p.owns || a.head_dim <= 64 ? 512 : 256;
+    p.stream = (groups + a.kv_heads - 1) / a.kv_heads;
+    p.tile_tokens = p.tile_rows / G + 1;
+    p.fixed = 64 * (PA_FIXED + 1);
+    uint64_t most = a.limit + PA_STEP; /* positions of a tile's steps */
+    if (a.window) {
+        const uint64_t w = (uint64_t)a.window + a.sinks + p.tile_tokens + 2 * PA_STEP;
+        most = w < most ? w : most;
+    }
+    most = 2 * most + p.fixed;
+    p.unit = 0; /* all units and the last workgroup's end below 2^31 */
+    while (((uint64_t)(p.tiles + 512) * ((most >> p.unit) + 1)) >= 1u << 30) ++p.unit;
+    p.cw = (uint32_t)(most >> p.unit) + 1;
+    p.c1 = 2 * p.tile_rows / G >> p.unit;
+    /* tiles of an even batch, and by how many steps the longest could exceed an equal share */
+    const uint64_t tiles = seqs * ((rows / (seqs ? seqs : 1) + p.tile_rows - 1) >> p.row_shift) * a.kv_heads;
+    const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
+    if (tiles >= 1024 || (tiles < groups ? steps * (groups - tiles) / groups : 0) <= 24) p.stream = 0;
     const size_t used = attend_used_bytes(a, p), each = attend_part_bytes(a, p.tile_rows);
     const uint64_t room = ws_bytes > used ? (ws_bytes - used) / each : 0;
     if (room < p.stream) p.stream = room > p.tiles ? (uint32_t)room : 0;

@@ -27,6 +27,7 @@ namespace smq {
 constexpr int PA_WAVES = 4; /* of a workgroup */
 constexpr uint32_t PA_STEP = 32;      /* positions */
 constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps are dealt out */
+constexpr uint32_t PA_FIXED = 16;     /* steps that a tile costs beside its own */
 
 /* How a launch covers the rows: tiles of tile_rows rows of one sequence and KV head (`tiles`: as many as the batch can
  * need). owns: a wave owns 16 * RT of the tile's rows over all positions; else the tile has 16 rows and the waves share
@@ -35,11 +36,13 @@ constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps a
  * stream > 0: stream workgroups per KV head take equal runs of all tiles' steps laid end to end, so a run ends and the
  * next begins inside a tile, whose partial results k_paged_join joins. Lengths are known on the device only: each
  * workgroup finds its run there. A tile counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the
- * sequence: its steps nearly, and with sums that need no loop. stream 0 (no workspace): a workgroup per tile. */
+ * sequence: its steps nearly, with sums that need no loop, and PA_FIXED for what it costs beside its steps (the batch
+ * looked at, queries, the first keys, the join). stream 0 (no workspace): a workgroup per tile. */
 typedef int i4 __attribute__((ext_vector_type(4)));
 struct AttendPlan {
     bool owns;
-    uint32_t tile_rows, tiles, stream, unit;
+    uint32_t tile_rows, row_shift, tiles, stream;
+    uint32_t unit, fixed, c1, cw, tile_tokens; /* units; tokens of a tile, at most */
 };
 /* The workspace: per tile and KV head four words (the workgroups that share it, its rows << 16; the sequence's first
  * token; the first row; the first one's slot), then per workgroup two slots of tile_rows rows: O, and behind all of them
@@ -172,11 +175,11 @@ struct Steps {
     uint32_t sinks, first, total;
     __device__ __forceinline__ uint32_t at(uint32_t u) const { return u < sinks ? u : u - sinks + first; }
 };
-__device__ __forceinline__ Steps tile_steps(const PagedArgs &a, int64_t pmin, int64_t pmax) {
+__device__ __forceinline__ Steps tile_steps(const PagedArgs &a, int pmin, int pmax) {
     Steps s = {0, 0, 0};
-    pmax = min(pmax, (int64_t)a.limit - 1);
+    pmax = min(pmax, (int)a.limit - 1);
     if (pmax < 0) return s;
-    const uint32_t low = a.window && pmin + 1 > (int64_t)a.window ? (uint32_t)(pmin + 1 - a.window) : 0;
+    const uint32_t low = a.window && pmin >= 0 && (uint32_t)pmin + 1 > a.window ? (uint32_t)pmin + 1 - a.window : 0;
     if (a.window) s.sinks = (min(a.sinks, (uint32_t)pmax + 1) + PA_STEP - 1) / PA_STEP;
     s.first = max(low / PA_STEP, s.sinks);
     const uint32_t end = (uint32_t)pmax / PA_STEP + 1;
@@ -206,15 +209,15 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, int w) { return (uint32_
 /* The batch's tiles; a wave looks at 64 sequences at a time, one per lane, their lengths requested with their begins. */
 struct Tiles {
     const PagedArgs &a;
-    uint32_t rows, unit;
+    const AttendPlan &p;
     int b0, b1, len;
     uint32_t n, c0, c1, cw; /* the lane's sequence: its tiles and their units */
     uint32_t mine, upto, tiles_upto; /* its units, and those and the tiles of the sequences up to it, of the 64 */
     uint32_t at;                     /* the first of the 64 */
 
-    __device__ __forceinline__ Tiles(const PagedArgs &a_, const AttendPlan &p) : a(a_), rows(p.tile_rows), unit(p.unit) { look(0); }
+    __device__ __forceinline__ Tiles(const PagedArgs &a_, const AttendPlan &p_) : a(a_), p(p_) { look(0); }
     __device__ __forceinline__ void look(uint32_t s0) {
-        const uint32_t s = s0 + threadIdx.x % 64, G = a.heads / a.kv_heads;
+        const uint32_t s = s0 + threadIdx.x % 64;
         at = s0;
         b0 = b1 = len = 0;
         if (s < a.seqs) {
@@ -223,14 +226,12 @@ struct Tiles {
             len = a.length[s];
         }
         const bool fine = b0 >= 0 && b1 > b0 && (uint32_t)b1 <= a.tokens; /* else no tile; check_begin raises the flag */
-        const uint32_t tokens = fine ? (uint32_t)(b1 - b0) : 0, tok = rows / G + 1; /* of the sequence, of a tile */
-        n = (tokens * G + rows - 1) / rows;
-        const uint32_t p = len > (int)tokens ? min((uint32_t)len - tokens, a.limit) : 0;
-        const uint64_t w = (uint64_t)a.window + a.sinks + tok + 64;
-        const uint32_t most = a.limit + 32;
-        cw = max(1u, 2 * (a.window && w < most ? (uint32_t)w : most) >> unit);
-        c0 = max(1u, min(2 * (p + min(tok, tokens)) + 64 >> unit, cw));
-        c1 = 2 * rows / G >> unit;
+        const uint32_t tokens = fine ? (uint32_t)(b1 - b0) : 0;
+        n = (tokens * (a.heads / a.kv_heads) + p.tile_rows - 1) >> p.row_shift;
+        const uint32_t pos = len > (int)tokens ? min((uint32_t)len - tokens, a.limit) : 0;
+        cw = p.cw;
+        c1 = p.c1;
+        c0 = min((2 * (pos + min(p.tile_tokens, tokens)) + p.fixed >> p.unit) + 1, cw);
         mine = sum(n, c0, c1, cw);
         upto = scan_wave(mine);
         tiles_upto = scan_wave(n);
@@ -253,7 +254,7 @@ struct Tiles {
         t.t = tiles_before;
         t.sq.begin = (int)lane_of((uint32_t)b0, w);
         t.sq.n = (int)lane_of((uint32_t)b1, w) - t.sq.begin;
-        t.sq.first = (int64_t)(int)lane_of((uint32_t)len, w) - t.sq.n;
+        t.sq.first = first_position((int)lane_of((uint32_t)len, w), t.sq.n);
     }
     /* The tile of number x. False behind the last. */
     __device__ __forceinline__ bool by_number(uint32_t x, Tile &t) {
@@ -394,6 +395,7 @@ struct Rows {
     uint32_t lane, col, quad;
     /* What this lane's column sees: positions of [from, from + reach] and below first. */
     uint32_t from[RT], reach[RT], first[RT];
+    int row[RT]; /* of q and att; -1: none */
     float factor[RT];   /* of a product: the score's scale, log2 e, the row's power of two */
     QFrag<TYPE> qf[RT][KS];
     int pmin;
@@ -403,29 +405,51 @@ struct Rows {
     float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
     float inv_e[TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values */
 
-    /* `count` rows of the sequence from row0 on; columns past them see what the first one sees and are not stored. */
-    __device__ __forceinline__ Rows(const PagedArgs &a_, const float *q, const Seq &sq, uint32_t kh, uint32_t row0, int count)
-        : a(a_) {
+    /* `count` rows of the sequence from row0 on; columns past them see what the first one sees and are not stored. First
+     * what they see, then (queries) their values, so that loads of keys can run beside those. */
+    __device__ __forceinline__ Rows(const PagedArgs &a_, const Seq &sq, uint32_t kh, uint32_t row0, int count) : a(a_) {
         lane = threadIdx.x % 64;
         col = lane % 16;
         quad = lane / 16;
-        const uint32_t G = a.heads / a.kv_heads, hd = a.head_dim;
-        const float scale = 1.44269504088896340736f / sqrtf((float)hd);
+        const uint32_t G = a.heads / a.kv_heads, tok0 = row0 / G, rest = row0 - tok0 * G;
+        const float inv = 1.0f / (float)G;
         int lo = 0x7fffffff, hi = -1;
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
             const bool in = c * 16 + (int)col < count;
-            const uint32_t r = row0 + (in ? c * 16 + col : 0), tok = r / G, g = r % G;
-            const int64_t p = sq.first + tok;
-            const bool place = p >= 0 && p < (int64_t)a.limit;
+            const uint32_t r = rest + (in ? c * 16 + col : 0);
+            const uint32_t up = (uint32_t)(((float)r + 0.5f) * inv); /* r / G: r is below 2^17, where this is exact */
+            const uint32_t tok = tok0 + up, g = r - up * G;
+            const uint32_t p = (uint32_t)(sq.first + (int)tok);
+            const bool place = p < a.limit;
             if (in && !place) *a.flag = 1;
             const int pc = place ? (int)p : -1;
-            from[c] = !place ? 0xffffffffu : a.window && p + 1 > (int64_t)a.window ? (uint32_t)(p + 1 - a.window) : 0;
-            reach[c] = place ? (uint32_t)pc - from[c] : 0;
+            from[c] = !place ? 0xffffffffu : a.window && p + 1 > a.window ? p + 1 - a.window : 0;
+            reach[c] = place ? p - from[c] : 0;
             first[c] = a.window ? min(a.sinks, (uint32_t)(pc + 1)) : 0;
             lo = min(lo, pc);
             hi = max(hi, pc);
-            const float *x = q + ((size_t)(sq.begin + (int)tok) * a.heads + (size_t)kh * G + g) * hd;
+            row[c] = in ? (int)(((uint32_t)sq.begin + tok) * a.heads + kh * G + g) : -1; /* below 2^23 */
+        }
+#pragma unroll
+        for (int off = 1; off < 16; off *= 2) {
+            lo = min(lo, __shfl_xor(lo, off));
+            hi = max(hi, __shfl_xor(hi, off));
+        }
+        pmin = __builtin_amdgcn_readfirstlane(lo);
+        const int pmax = __builtin_amdgcn_readfirstlane(hi);
+        span = span_of(a, pmin, pmax);
+        low_last = span_of(a, pmax, pmax).low;
+#pragma unroll
+        for (int b = 0; b < (TYPE == 2 ? KS : 1); ++b) inv_e[b] = __builtin_ldexpf(1.0f, 100);
+    }
+    __device__ __forceinline__ void queries(const float *q) {
+        const uint32_t hd = a.head_dim;
+        const float scale = 1.44269504088896340736f / sqrtf((float)hd);
+#pragma unroll
+        for (int c = 0; c < RT; ++c) {
+            const bool in = row[c] >= 0;
+            const float *x = q + (size_t)(in ? row[c] : 0) * hd;
             float t[KS][8], big = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -462,17 +486,6 @@ struct Rows {
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[c][d] = f4{};
         }
-#pragma unroll
-        for (int off = 1; off < 16; off *= 2) {
-            lo = min(lo, __shfl_xor(lo, off));
-            hi = max(hi, __shfl_xor(hi, off));
-        }
-        pmin = __builtin_amdgcn_readfirstlane(lo);
-        const int pmax = __builtin_amdgcn_readfirstlane(hi);
-        span = span_of(a, pmin, pmax);
-        low_last = span_of(a, pmax, pmax).low;
-#pragma unroll
-        for (int b = 0; b < (TYPE == 2 ? KS : 1); ++b) inv_e[b] = __builtin_ldexpf(1.0f, 100);
     }
 
     __device__ __forceinline__ bool sees(uint32_t pos, int c) const { return pos - from[c] <= reach[c] || pos < first[c]; }
@@ -956,14 +969,17 @@ __device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, 
     constexpr int LD = 32 * KS + 4;
     float(*so)[16][LD] = (float(*)[16][LD])lds;
     float(*sml)[16][2] = (float(*)[16][2])(lds + PA_WAVES * 16 * LD * 4);
-    Rows<TYPE, KS, 1> w(a, q, sq, out.kh, out.row0, (int)out.n);
+    Rows<TYPE, KS, 1> w(a, sq, out.kh, out.row0, (int)out.n);
     u0 += wave;
-    if (u0 < u1) {
+    if (u0 >= u1) {
+        w.queries(q);
+    } else {
         Pages<TYPE, SMALL> pages(a, seq, out.kh);
         InRegisters<TYPE, KS, SMALL> src(a);
         uint32_t at = st.at(u0);
         auto pl = pages.locate(at, w.span);
         src.load_k(pl);
+        w.queries(q);
         for (uint32_t u = u0; u < u1; u += PA_WAVES) {
             const uint32_t p0 = at * PA_STEP;
             at = st.at(u + PA_WAVES < u1 ? u + PA_WAVES : u); /* the last one's keys twice */
@@ -1012,16 +1028,19 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, c
     const uint32_t first = wave * 16 * RT, G = a.heads / a.kv_heads;
     const bool mine = first < out.n;
     /* the last wave's rows again where there are none: never stored */
-    Rows<TYPE, KS, RT> w(a, q, sq, out.kh, out.row0 + (mine ? first : 0), mine ? (int)min(16u * RT, out.n - first) : 1);
+    Rows<TYPE, KS, RT> w(a, sq, out.kh, out.row0 + (mine ? first : 0), mine ? (int)min(16u * RT, out.n - first) : 1);
     /* what the tile sees: the pages that the workgroup needs */
-    const int64_t tmin = sq.first + out.row0 / G, tmax = min(sq.first + (out.row0 + out.n - 1) / G, (int64_t)a.limit - 1);
-    const Span span = span_of(a, (int)max((int64_t)-1, tmin), (int)max((int64_t)-1, tmax));
-    if (u0 < u1) {
+    const int tmin = sq.first + (int)(out.row0 / G), tmax = min(sq.first + (int)((out.row0 + out.n - 1) / G), (int)a.limit - 1);
+    const Span span = span_of(a, max(-1, tmin), max(-1, tmax));
+    if (u0 >= u1) {
+        w.queries(q);
+    } else {
         Pages<TYPE, SMALL> pages(a, seq, out.kh);
         const typename Src::Loader loader(a, wave);
         uint32_t at = st.at(u0);
         auto pl = pages.locate(at, span);
         loader.load(pl, lds);
+        w.queries(q);
         Src::wait();
         for (uint32_t u = u0; u < u1; ++u) {
             const uint32_t p0 = at * PA_STEP, ok = pl.ok;
@@ -1064,7 +1083,7 @@ __device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &
                                           uint32_t e, unsigned char *lds) {
     const uint32_t G = a.heads / a.kv_heads, row0 = t.j * p.tile_rows, n = min(p.tile_rows, (uint32_t)t.sq.n * G - row0);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Steps st = tile_steps(a, t.sq.first + row0 / G, t.sq.first + (row0 + n - 1) / G);
+    const Steps st = tile_steps(a, t.sq.first + (int)(row0 / G), t.sq.first + (int)((row0 + n - 1) / G));
     Out out = {a, t.sq, kh, row0, n, att, nullptr, nullptr};
     uint32_t u0 = 0, u1 = st.total;
     if (each) {
@@ -1112,7 +1131,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
             tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, 0, 0, 0, lds);
         return;
     }
-    uint32_t units, count, each;
+    uint32_t units, count, each, v, e;
     {
         Tiles tiles(a, p);
         tiles.total(units, count);
@@ -1123,20 +1142,26 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
             i = p.stream + p.tiles - 1 - i;
             if (!tiles.last_with(i, [&](uint32_t u, uint32_t n) { return u / each + n; }, t)) return;
             i -= t.t; /* the workgroup whose run it is */
+            v = max(t.first, i * each);
+        } else {
+            v = i * each; /* stream * each is below 2^31: see attend_plan */
+            if (v >= units) return;
+            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
         }
     }
     if constexpr (OWNS) {
-        const uint32_t v = max(t.first, i * each), e = min(t.first + t.units, (i + 1) * each);
+        e = min(t.first + t.units, (i + 1) * each);
         if (v < e) tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
     } else {
-        const uint32_t end = min(units, (i + 1) * each); /* stream * each is below 2^31: see attend_plan */
-        for (uint32_t v = i * each; v < end;) {
-            Tiles tiles(a, p);
-            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
-            const uint32_t e = min(end, t.first + t.units);
+        const uint32_t end = min(units, (i + 1) * each);
+        for (;;) {
+            e = min(end, t.first + t.units);
             tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
             v = e;
-            if (v < end) __syncthreads(); /* LDS is free */
+            if (v >= end) break;
+            __syncthreads(); /* LDS is free */
+            Tiles tiles(a, p); /* again: carried along it took the products' registers */
+            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
         }
     }
 }
