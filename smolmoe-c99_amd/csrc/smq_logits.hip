@@ -1,28 +1,31 @@
 /* Rows of logits before the choice of a token on gfx950: penalties over a history, biases, grammar masks, and the
- * greedy choice (include/smq.h has the formulas). */
+ * greedy choice (include/smq.h has the formulas).
+ *
+ * One pass: a workgroup takes a span of ids of one row, requests its logits, counts the row's whole history (and adds up
+ * its biases) in LDS where they fall into the span meanwhile, and writes the adjusted logits with the span's best
+ * candidate; a second launch, a wave per row, joins the candidates. */
 #include "smq_device.h"
 
 namespace smq {
 namespace {
 
-constexpr uint32_t LG_WG = 256;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t LG_WG = 256, LG_WAVES = LG_WG / 64;
 constexpr uint32_t NONE = 0xffffffffu;
 
-/* The best of some ids: the first id that may be taken and whether its logit is a NaN, then the lowest id of the largest
- * logit among those that are no NaN. */
+/* Of some ids that may be taken: the lowest one and whether its logit is a NaN, and the lowest one of the largest logit
+ * above -inf. The choice: the lowest if its logit is a NaN or none is above -inf, else the largest. */
 struct Part {
     float best;
     uint32_t id, first, first_nan;
 };
 __device__ __forceinline__ void join(Part &a, const Part &b) {
-    if (b.id != NONE && (a.id == NONE || b.best > a.best || (b.best == a.best && b.id < a.id))) {
-        a.best = b.best;
-        a.id = b.id;
-    }
-    if (b.first < a.first) {
-        a.first = b.first;
-        a.first_nan = b.first_nan;
-    }
+    const bool take = b.best > a.best || (b.best == a.best && b.id < a.id);
+    a.best = take ? b.best : a.best;
+    a.id = take ? b.id : a.id;
+    a.first_nan = b.first < a.first ? b.first_nan : a.first_nan;
+    a.first = min(a.first, b.first);
 }
 __device__ __forceinline__ Part join_wave(Part p) {
 #pragma unroll
@@ -36,6 +39,7 @@ __device__ __forceinline__ Part join_wave(Part p) {
     }
     return p;
 }
+__device__ __forceinline__ Part nothing() { return {-INFINITY, NONE, NONE, 0}; }
 
 /* [begin[r], begin[r + 1]) cut to the list's count entries. */
 __device__ __forceinline__ void list_range(const int32_t *begin, uint32_t r, uint32_t count, uint32_t &b, uint32_t &e) {
@@ -44,62 +48,82 @@ __device__ __forceinline__ void list_range(const int32_t *begin, uint32_t r, uin
     e = y < 0 ? 0 : min((uint32_t)y, count);
 }
 
-/* One workgroup per span of SPAN ids of a row, one pass over the logits. The whole history of the row is read and
- * counted in LDS where it falls into the span (integers: no order), biases 256 entries at a time: the first entry of an
- * id adds up the later ones in the order of the list, so that the same id twice gives the same bits on every run. */
-template <uint32_t SPAN>
+/* A thread has ids v0 + 1024 u + 4 tid .. + 3 of the span, u < SPAN / 1024. WIDE: rows of 16-byte aligned quadruples;
+ * else single words. */
+template <uint32_t SPAN, bool WIDE>
 __global__ __launch_bounds__(LG_WG) void k_logits(LogitArgs a, Part *parts) {
-    __shared__ uint32_t count[SPAN];
-    __shared__ float add[SPAN];
-    __shared__ uint32_t ids[LG_WG];
+    constexpr uint32_t U = SPAN / (4 * LG_WG);
+    __shared__ __attribute__((aligned(16))) uint32_t count[SPAN];
+    __shared__ __attribute__((aligned(16))) float add[SPAN];
+    __shared__ uint32_t ids[LG_WG], found[LG_WAVES];
     __shared__ float vals[LG_WG];
-    __shared__ Part best[LG_WG / 64];
-    const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * SPAN;
-    constexpr uint32_t EPT = SPAN / LG_WG;
-    const float *row = a.logits + (size_t)r * a.stride;
-    float l[EPT];
+    __shared__ Part best[LG_WAVES];
+    const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * SPAN, left = a.vocab - v0; /* ids from v0 on */
+    const float *row = a.logits + (size_t)r * a.stride + v0;
+    f4 l[U];
 #pragma unroll
-    for (uint32_t u = 0; u < EPT; ++u) {
-        const uint32_t v = v0 + u * LG_WG + tid;
-        l[u] = v < a.vocab ? row[v] : 0.0f;
-        count[u * LG_WG + tid] = 0;
-        add[u * LG_WG + tid] = 0.0f;
-    }
-    uint32_t mb = 0;
-    bool masked = a.allowed != nullptr, none = false;
-    if (masked) {
-        const int mr = a.mask_row ? a.mask_row[r] : (int)r;
-        masked = mr >= 0;
-        none = masked && (uint32_t)mr >= a.allowed_rows;
-        mb = (uint32_t)mr;
-        if (none && tid == 0) *a.flag = 1;
-    }
-    __syncthreads();
-    uint32_t hb = 0, he = 0, bb = 0, be = 0;
-    if (a.history) {
-        list_range(a.history_begin, r, a.history_count, hb, he);
-        for (uint32_t i = hb + tid; i < he; i += LG_WG) {
-            const uint32_t v = a.history[i] - v0;
-            if (v < SPAN) atomicAdd(&count[v], 1u);
+    for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t i = u * 4 * LG_WG + 4 * tid;
+        if (WIDE && i + 4 <= left) {
+            l[u] = *(const f4 *)(row + i);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) l[u][e] = i + e < left ? row[i + e] : 0.0f;
         }
     }
-    if (a.bias_ids) {
-        list_range(a.bias_begin, r, a.bias_count, bb, be);
+    uint32_t hb = 0, he = 0, bb = 0, be = 0;
+    if (a.history) list_range(a.history_begin, r, a.history_count, hb, he);
+    if (a.bias_ids) list_range(a.bias_begin, r, a.bias_count, bb, be);
+    const uint32_t *mask = nullptr; /* the span's words */
+    bool none = false;
+    if (a.allowed) {
+        const int m = a.mask_row ? a.mask_row[r] : (int)r;
+        none = m >= 0 && (uint32_t)m >= a.allowed_rows;
+        if (none && tid == 0) *a.flag = 1;
+        if (m >= 0 && !none) mask = a.allowed + (size_t)m * ((a.vocab + 31) / 32) + v0 / 32;
+    }
+    if (he > hb) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) *(u4 *)&count[u * 4 * LG_WG + 4 * tid] = u4{};
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t i = hb + tid; i < he; i += LG_WG) {
+            const uint32_t v = a.history[i] - v0;
+            if (v < SPAN) atomicAdd(&count[v], 1u); /* integers: no order */
+        }
+    }
+    if (be > bb) {
+        /* 256 entries at a time, those of the span put together in the order of the list; the first one of an id adds up
+         * the later ones, so that the same id twice gives the same bits on every run */
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) *(f4 *)&add[u * 4 * LG_WG + 4 * tid] = f4{};
         for (uint32_t i0 = bb; i0 < be; i0 += LG_WG) {
             const uint32_t n = min(LG_WG, be - i0), id = tid < n ? a.bias_ids[i0 + tid] - v0 : NONE;
-            const float x = tid < n ? a.bias[i0 + tid] : 0.0f;
+            const uint64_t in = __ballot(id < SPAN);
             __syncthreads();
-            ids[tid] = id;
-            vals[tid] = x;
+            if (tid % 64 == 0) found[tid / 64] = (uint32_t)__popcll(in);
             __syncthreads();
+            uint32_t at = __popcll(in & ((1ull << tid % 64) - 1)), total = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < LG_WAVES; ++w) {
+                at += w < tid / 64 ? found[w] : 0;
+                total += found[w];
+            }
+            if (!total) continue; /* uniform */
             if (id < SPAN) {
+                ids[at] = id;
+                vals[at] = a.bias[i0 + tid];
+            }
+            __syncthreads();
+            if (tid < total) {
+                const uint32_t mine = ids[tid];
                 bool first = true;
-                for (uint32_t j = 0; j < tid; ++j) first = first && ids[j] != id;
+                for (uint32_t j = 0; j < tid; ++j) first = first & (ids[j] != mine);
                 if (first) {
-                    float sum = add[id] + x;
-                    for (uint32_t j = tid + 1; j < n; ++j)
-                        if (ids[j] == id) sum += vals[j];
-                    add[id] = sum;
+                    float sum = add[mine] + vals[tid];
+                    for (uint32_t j = tid + 1; j < total; ++j)
+                        if (ids[j] == mine) sum += vals[j];
+                    add[mine] = sum;
                 }
             }
         }
@@ -111,27 +135,47 @@ __global__ __launch_bounds__(LG_WG) void k_logits(LogitArgs a, Part *parts) {
         pres = a.penalty[3 * (size_t)r + 1];
         freq = a.penalty[3 * (size_t)r + 2];
     }
-    const uint32_t words = (a.vocab + 31) / 32;
-    Part p = {0.0f, NONE, NONE, 0};
+    Part p = nothing();
+    float *out = a.out ? a.out + (size_t)r * a.out_stride + v0 : nullptr;
 #pragma unroll
-    for (uint32_t u = 0; u < EPT; ++u) {
-        const uint32_t i = u * LG_WG + tid, v = v0 + i;
-        if (v >= a.vocab) continue;
-        float x = l[u];
-        const uint32_t c = count[i];
-        if (c) {
-            x = x > 0.0f ? x / rep : x * rep;
-            const float t = (float)c * freq;
-            x = x - (t + pres);
+    for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t i = u * 4 * LG_WG + 4 * tid;
+        f4 x = l[u];
+        if (he > hb) {
+            const u4 c = *(const u4 *)&count[i];
+            if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const float y = x[e] > 0.0f ? x[e] / rep : x[e] * rep, t = (float)c[e] * freq;
+                    x[e] = c[e] ? y - (t + pres) : x[e];
+                }
+            }
         }
-        if (be > bb) x = x + add[i];
-        const bool may = !masked || (!none && (a.allowed[(size_t)mb * words + v / 32] >> (v % 32) & 1u));
-        if (!may) x = -INFINITY;
-        if (a.out) a.out[(size_t)r * a.out_stride + v] = x;
-        if (may) {
-            const bool nan = x != x;
-            const Part o = {x, nan ? NONE : v, v, nan};
-            join(p, o);
+        if (be > bb) x += *(const f4 *)&add[i];
+        uint32_t may = none ? 0 : i + 4 <= left ? 15 : i < left ? (1u << (left - i)) - 1 : 0;
+        if (mask && may) may &= mask[i / 32] >> (i % 32);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const bool m = may >> e & 1;
+            x[e] = m ? x[e] : -INFINITY;
+            const bool take = x[e] > p.best; /* ids ascend: the lowest of equal ones stays; a NaN is not above */
+            p.best = take ? x[e] : p.best;
+            p.id = take ? v0 + i + e : p.id;
+        }
+        if (p.first == NONE && may) {
+            const uint32_t e = (uint32_t)__ffs(may) - 1;
+            const float y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
+            p.first = v0 + i + e;
+            p.first_nan = y != y;
+        }
+        if (out) {
+            if (WIDE && i + 4 <= left) {
+                *(f4 *)(out + i) = x;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (i + e < left) out[i + e] = x[e];
+            }
         }
     }
     if (!parts) return;
@@ -139,31 +183,44 @@ __global__ __launch_bounds__(LG_WG) void k_logits(LogitArgs a, Part *parts) {
     if (tid % 64 == 0) best[tid / 64] = p;
     __syncthreads();
     if (tid == 0) {
-        for (uint32_t w = 1; w < LG_WG / 64; ++w) join(p, best[w]);
+        for (uint32_t w = 1; w < LG_WAVES; ++w) join(p, best[w]);
         parts[(size_t)r * gridDim.x + blockIdx.x] = p;
     }
 }
 
 __global__ __launch_bounds__(64) void k_logits_pick(const Part *parts, uint32_t n, uint32_t *token) {
-    Part p = {0.0f, NONE, NONE, 0};
+    Part p = nothing();
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < n; i += 64) join(p, parts[(size_t)blockIdx.x * n + i]);
     p = join_wave(p);
-    if (threadIdx.x == 0) token[blockIdx.x] = p.first_nan ? p.first : p.id;
+    if (threadIdx.x == 0) token[blockIdx.x] = p.first_nan || p.id == NONE ? p.first : p.id;
 }
 
-constexpr uint32_t SPAN = 1024;
-uint32_t spans(uint32_t vocab) { return (vocab + SPAN - 1) / SPAN; }
+/* Spans of 4096 ids where they give two workgroups a CU or more (each reads the row's whole history), else of 1024. */
+uint32_t span_of(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + 4095) / 4096) >= 512 ? 4096 : 1024; }
 
 }  // namespace
 
-size_t logits_workspace(uint32_t rows, uint32_t vocab) { return (size_t)rows * spans(vocab) * sizeof(Part); }
+size_t logits_workspace(uint32_t rows, uint32_t vocab) {
+    const uint32_t span = span_of(rows, vocab);
+    return (size_t)rows * ((vocab + span - 1) / span) * sizeof(Part);
+}
 
 hipError_t launch_logits(const LogitArgs &a, uint32_t *token, void *ws, hipStream_t s) {
-    const uint32_t n = spans(a.vocab);
-    hipLaunchKernelGGL((k_logits<SPAN>), dim3(n, a.rows), dim3(LG_WG), 0, s, a, token ? (Part *)ws : nullptr);
+    const uint32_t span = span_of(a.rows, a.vocab), n = (a.vocab + span - 1) / span;
+    const bool wide = !(((uintptr_t)a.logits | (uintptr_t)a.out | (a.rows > 1 ? (a.stride | a.out_stride) * 4 : 0)) & 15);
+    Part *parts = token ? (Part *)ws : nullptr;
+    const dim3 grid(n, a.rows);
+    if (span == 4096) {
+        if (wide) hipLaunchKernelGGL((k_logits<4096, true>), grid, dim3(LG_WG), 0, s, a, parts);
+        else hipLaunchKernelGGL((k_logits<4096, false>), grid, dim3(LG_WG), 0, s, a, parts);
+    } else {
+        if (wide) hipLaunchKernelGGL((k_logits<1024, true>), grid, dim3(LG_WG), 0, s, a, parts);
+        else hipLaunchKernelGGL((k_logits<1024, false>), grid, dim3(LG_WG), 0, s, a, parts);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !token) return e;
-    hipLaunchKernelGGL(k_logits_pick, dim3(a.rows), dim3(64), 0, s, (const Part *)ws, n, token);
+    hipLaunchKernelGGL(k_logits_pick, dim3(a.rows), dim3(64), 0, s, parts, n, token);
     return hipGetLastError();
 }
 

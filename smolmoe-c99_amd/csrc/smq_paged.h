@@ -45,14 +45,16 @@ __device__ __forceinline__ void check_begin(const PagedArgs &a, uint32_t tid, ui
     }
 }
 
-/* The sequence and position of row r; false where the row is padding or has no place (then with the flag). */
+/* The sequence and position of row r (of a whole wave: uniform); false where the row is padding or has no place (then with the flag). */
 __device__ __forceinline__ bool place_of(const PagedArgs &a, uint32_t r, uint32_t &s, uint32_t &pos) {
-    uint32_t lo = 0, hi = a.seqs; /* the first sequence that begins past r */
-    while (lo < hi) {
+    uint32_t lo = 0, hi = a.seqs; /* the first sequence that begins past r: halved to 64, which the lanes look at */
+    while (hi - lo > 64) {
         const uint32_t mid = (lo + hi) / 2;
         if (a.begin[mid] <= (int)r) lo = mid + 1;
         else hi = mid;
     }
+    const uint32_t lane = threadIdx.x % 64;
+    lo += (uint32_t)__popcll(__ballot(lo + lane < hi && a.begin[lo + min(lane, hi - lo - 1)] <= (int)r));
     Seq q;
     if (!lo || a.begin[lo] <= (int)r) return false; /* behind the last sequence (lo == seqs) */
     s = lo - 1;

@@ -1,103 +1,304 @@
 /* Paged KV cache on gfx950: RoPE and the store of new tokens (f32, f16, Q8), rows read back, and the attention of a
  * ragged batch of new tokens over the pages (include/smq.h has the layout of a page). */
-#include <hip/hip_fp16.h>
-
 #include "smq_paged_attend.h"
 
 namespace smq {
 namespace {
 
-/* Coordinate d of a rotated head row x (smq_rope_kv's products and order). */
-__device__ __forceinline__ float rotated(const float *x, uint32_t d, uint32_t pairs, const float *c, const float *s) {
-    if (d >= 2 * pairs) return x[d];
-    const uint32_t i = d / 2;
-    const float p = x[2 * i], q = x[2 * i + 1];
-    const float pc = p * c[i], qs = q * s[i], ps = p * s[i], qc = q * c[i];
-    return d & 1 ? ps + qc : pc - qs;
+constexpr uint32_t ST_WG = 256;
+constexpr uint32_t ST_POS = 32; /* positions of a block */
+
+/* Blocks of ST_POS positions (from a multiple of it on) that the new tokens of the sequences touch: block x's sequence and
+ * positions [p0, p1), all of them places. Uniform over a wave; false behind the last. */
+struct Block {
+    uint32_t seq, p0, p1;
+    int row; /* of position 0: begin - first */
+};
+__device__ __forceinline__ bool find_block(const PagedArgs &a, uint32_t x, Block &b) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        int b0 = 0, n = 0, first = 0;
+        if (s < a.seqs) {
+            b0 = a.begin[s];
+            n = a.begin[s + 1] - b0;
+            if (b0 < 0 || n < 0 || (uint32_t)n > a.tokens - (uint32_t)min((uint32_t)b0, a.tokens)) n = 0; /* check_begin */
+            first = first_position(a.length[s], n);
+        }
+        const int from = max(first, 0), to = min(first + n, (int)a.limit);
+        if (n && (from != first || to != first + n)) *a.flag = 1; /* rows without a place */
+        const uint32_t blocks = to > from ? (uint32_t)(to - 1) / ST_POS - (uint32_t)from / ST_POS + 1 : 0;
+        uint32_t upto = blocks;
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) {
+            const uint32_t y = __shfl_up(upto, off);
+            upto += (int)lane >= off ? y : 0;
+        }
+        const uint64_t past = __ballot(before + upto > x);
+        if (past) {
+            const int w = __ffsll((unsigned long long)past) - 1;
+            const uint32_t k = x - before - (uint32_t)(__builtin_amdgcn_readlane(upto, w) - __builtin_amdgcn_readlane(blocks, w));
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane(from, w), hi = (uint32_t)__builtin_amdgcn_readlane(to, w);
+            const uint32_t at = (lo / ST_POS + k) * ST_POS;
+            b.seq = s0 + (uint32_t)w;
+            b.p0 = max(at, lo);
+            b.p1 = min(at + ST_POS, hi);
+            b.row = __builtin_amdgcn_readlane(b0, w) - __builtin_amdgcn_readlane(first, w);
+            return true;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+/* As many blocks as a batch can need. */
+uint32_t most_blocks(const PagedArgs &a) {
+    const uint32_t seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
+    return a.tokens / ST_POS + 2 * seqs;
+}
+/* The block's page ids of 16 positions each, one per lane of 0 .. 1 (blocks of one page have the same one twice); -1, with
+ * the flag, where a page that the block needs is none. */
+__device__ __forceinline__ void block_pages(const PagedArgs &a, const Block &b, int (&page)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t p = b.p0 / ST_POS * ST_POS + 16 * h;
+        page[h] = p < b.p1 && p + 16 > b.p0 ? page_of(a, b.seq, max(p, b.p0)) : -1;
+    }
+}
+/* Element of position 0, dim 0 of a page's head; slot of a position. */
+__device__ __forceinline__ size_t head_at(const PagedArgs &a, int page, uint32_t h) {
+    return (((size_t)page * a.kv_heads + h) * a.head_dim) << a.shift;
+}
+__device__ __forceinline__ size_t scales_at(const PagedArgs &a, int page, uint32_t h) {
+    return (((size_t)page * a.kv_heads + h) * a.nb) << a.shift;
 }
 
-constexpr int ST_WG = 256;
+/* Dims d .. d + 3 of a head row, rotated (smq_rope_kv's products and order). */
+__device__ __forceinline__ f4 rotated(f4 x, uint32_t d, uint32_t pairs, const float *c, const float *s) {
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e += 2) {
+        const uint32_t i = (d + e) / 2;
+        if (i >= pairs) continue;
+        const float p = x[e], q = x[e + 1];
+        const float pc = p * c[i], qs = q * s[i], ps = p * s[i], qc = q * c[i];
+        x[e] = pc - qs;
+        x[e + 1] = ps + qc;
+    }
+    return x;
+}
 
-/* One workgroup per row; 32 lanes per block of 32 dims of a head, so that a Q8 block's maximum is a shuffle. */
+template <uint32_t TYPE>
+struct Four; /* four elements as the cache holds them */
+template <>
+struct Four<0> {
+    typedef f4 T;
+};
+template <>
+struct Four<1> {
+    typedef uint32_t T __attribute__((ext_vector_type(2)));
+};
+template <>
+struct Four<2> {
+    typedef uint32_t T;
+};
+
+/* Four values to elements; Q8: eight lanes hold a 32-wide block (values past head_dim are 0), whose scale comes back.
+ * bad: a value that is not finite there (the block's, for Q8). */
+template <uint32_t TYPE>
+__device__ __forceinline__ typename Four<TYPE>::T encode(f4 x, float &scale, bool &bad) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bad = bad || !(fabsf(x[e]) <= FLT_MAX);
+        m = fmaxf(m, fabsf(x[e]));
+    }
+    if constexpr (TYPE == 0) {
+        return x;
+    } else if constexpr (TYPE == 1) {
+        union {
+            h4 h;
+            typename Four<1>::T u;
+        } r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r.h[e] = (_Float16)x[e];
+            bad = bad || !(fabsf((float)r.h[e]) <= FLT_MAX);
+        }
+        return r.u;
+    } else {
+        int any = bad;
+#pragma unroll
+        for (int off = 1; off < 8; off *= 2) {
+            m = fmaxf(m, __shfl_xor(m, off));
+            any |= __shfl_xor(any, off);
+        }
+        bad = any;
+        scale = any ? __builtin_nanf("") : m / 127.0f;
+        const float inv = !any && scale >= FLT_MIN ? 1.0f / scale : 0.0f;
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p = __builtin_rintf(any ? 0.0f : x[e] * inv);
+            r |= ((uint32_t)(int)fminf(fmaxf(p, -127.0f), 127.0f) & 255u) << (8 * e);
+        }
+        return r;
+    }
+}
+
+/* The first a.tokens workgroups: a row of q each (all heads). Then one per block and KV head: keys and values of up to
+ * ST_POS positions, four dims a thread, values turned through LDS so that a dim's positions are written together (few
+ * positions: straight, element by element). */
 template <uint32_t TYPE>
 __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float *q, float *q_out, const float *k,
                                                        const float *v, const float *cs, const float *sn) {
-    const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid % 32;
-    uint32_t s, pos;
-    if (r == 0) check_begin(a, tid, ST_WG);
-    if (!place_of(a, r, s, pos)) return;
-    const float *c = cs + (size_t)pos * a.pairs, *sr = sn + (size_t)pos * a.pairs;
-    if (q) {
-        const size_t row = (size_t)r * a.heads * a.head_dim;
-        for (uint32_t i = tid; i < a.heads * a.head_dim / 2; i += ST_WG) {
-            const uint32_t h = i / (a.head_dim / 2), d = 2 * (i % (a.head_dim / 2));
-            const float *x = q + row + (size_t)h * a.head_dim;
-            const float y0 = rotated(x, d, a.pairs, c, sr), y1 = rotated(x, d + 1, a.pairs, c, sr);
-            q_out[row + (size_t)h * a.head_dim + d] = y0; /* both read before either is written: q_out may be q */
-            q_out[row + (size_t)h * a.head_dim + d + 1] = y1;
-        }
+    typedef typename Four<TYPE>::T T;
+    constexpr uint32_t EB = sizeof(T) / 4;
+    __shared__ __attribute__((aligned(16))) unsigned char turn[MAX_HEAD_DIM * (ST_POS * EB + 4)];
+    const uint32_t tid = threadIdx.x, hd = a.head_dim, rows = q ? a.tokens : 0;
+    if (blockIdx.x == 0) check_begin(a, tid, ST_WG);
+    if (blockIdx.x < rows) {
+        uint32_t s, pos;
+        if (!place_of(a, blockIdx.x, s, pos)) return;
+        const float *c = cs + (size_t)pos * a.pairs, *sr = sn + (size_t)pos * a.pairs;
+        const size_t row = (size_t)blockIdx.x * a.heads * hd;
+        for (uint32_t i = tid; i < a.heads * hd / 4; i += ST_WG)
+            *(f4u *)(q_out + row + 4 * i) = rotated(*(const f4u *)(q + row + 4 * i), 4 * i % hd, a.pairs, c, sr);
+        return;
     }
-    const int page = page_of(a, s, pos);
-    if (page < 0) return;
-    const uint32_t P = 1u << a.shift, slot = pos & (P - 1);
-    const size_t krow = (size_t)r * a.kv_heads * a.head_dim;
-    for (uint32_t i = tid / 32; i < a.kv_heads * a.nb * 2; i += ST_WG / 32) {
-        const bool isv = i >= a.kv_heads * a.nb;
-        const uint32_t j = isv ? i - a.kv_heads * a.nb : i, h = j / a.nb, b = j % a.nb, d = b * 32 + lane;
-        const bool in = d < a.head_dim;
-        const float *x = (isv ? v : k) + krow + (size_t)h * a.head_dim;
-        const float y = !in ? 0.0f : isv ? x[d] : rotated(x, d, a.pairs, c, sr);
-        const size_t ph = (size_t)page * a.kv_heads + h;
-        const size_t at = isv ? (ph * a.head_dim + d) * P + slot : (ph * P + slot) * a.head_dim + d;
-        void *pool = isv ? a.values : a.keys;
-        bool bad = !(fabsf(y) <= FLT_MAX);
-        if constexpr (TYPE == 0) {
-            if (in) ((float *)pool)[at] = y;
-        } else if constexpr (TYPE == 1) {
-            const __half hv = __float2half_rn(y);
-            bad = bad || !(fabsf(__half2float(hv)) <= FLT_MAX);
-            if (in) ((__half *)pool)[at] = hv;
-        } else {
-            float m = fabsf(y);
-            int any = bad;
-#pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) {
-                m = fmaxf(m, __shfl_xor(m, off, 32));
-                any |= __shfl_xor(any, off, 32);
+    const uint32_t x = blockIdx.x - rows, h = x % a.kv_heads;
+    Block b;
+    if (!find_block(a, x / a.kv_heads, b)) return;
+    int page[2];
+    block_pages(a, b, page);
+    const uint32_t P = 1u << a.shift, lanes = a.nb * 8, n = b.p1 - b.p0; /* lanes of a row: whole 32-wide blocks */
+    const bool few = n <= 2;
+    for (uint32_t kind = 0; kind < 2; ++kind) { /* keys, values */
+        const float *from = kind ? v : k;
+        for (uint32_t i = tid; i < (n * lanes + ST_WG - 1) / ST_WG * ST_WG; i += ST_WG) { /* whole waves: encode shuffles */
+            const uint32_t j = i / lanes, d = 4 * (i - j * lanes), pos = b.p0 + min(j, n - 1), slot = pos & (P - 1);
+            const int pg = pos & 16 ? page[1] : page[0];
+            const bool in = j < n && d < hd;
+            f4 y = {};
+            if (in) {
+                y = *(const f4u *)(from + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d);
+                if (!kind) y = rotated(y, d, a.pairs, cs + (size_t)pos * a.pairs, sn + (size_t)pos * a.pairs);
             }
-            const float scale = m / 127.0f;
-            const float inv = scale >= FLT_MIN ? 1.0f / scale : 0.0f;
-            float p = __builtin_rintf(y * inv);
-            p = p > 127.0f ? 127.0f : p < -127.0f ? -127.0f : p;
-            if (in) ((int8_t *)pool)[at] = any ? 0 : (int8_t)(int)p;
-            if (lane == 0) (isv ? a.vs : a.ks)[(ph * a.nb + b) * P + slot] = any ? __builtin_nanf("") : scale;
-            bad = any;
+            float scale;
+            bool bad = false;
+            const T t = encode<TYPE>(y, scale, bad);
+            if (!in || pg < 0) continue;
+            if (bad) *a.flag = 1;
+            if (TYPE == 2 && d % 32 == 0) (kind ? a.vs : a.ks)[scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot] = scale;
+            if (!kind) {
+                *(T *)((unsigned char *)a.keys + (head_at(a, pg, h) + (size_t)slot * hd + d) * EB) = t;
+            } else {
+                unsigned char *to = few ? (unsigned char *)a.values + (head_at(a, pg, h) + ((size_t)d << a.shift) + slot) * EB
+                                        : turn + d * (ST_POS * EB + 4) + (pos % ST_POS) * EB;
+                const size_t step = few ? (size_t)EB << a.shift : ST_POS * EB + 4;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    if constexpr (TYPE == 0) *(float *)(to + e * step) = t[e];
+                    else if constexpr (TYPE == 1) *(uint16_t *)(to + e * step) = (uint16_t)(t[e / 2] >> (16 * (e & 1)));
+                    else *(to + e * step) = (unsigned char)(t >> (8 * e));
+                }
+            }
         }
-        if (bad) *a.flag = 1;
+    }
+    if (few) return;
+    __syncthreads();
+    for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) { /* four positions of a dim */
+        const uint32_t d = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), pos = b.p0 / ST_POS * ST_POS + j;
+        const int pg = j & 16 ? page[1] : page[0];
+        if (pg < 0 || pos >= b.p1 || pos + 4 <= b.p0) continue;
+        const unsigned char *t = turn + d * (ST_POS * EB + 4) + j * EB;
+        unsigned char *to = (unsigned char *)a.values + (head_at(a, pg, h) + ((size_t)d << a.shift) + (pos & (P - 1))) * EB;
+        if (pos >= b.p0 && pos + 4 <= b.p1) {
+            union {
+                uint32_t u[EB];
+                T t;
+            } y;
+#pragma unroll
+            for (uint32_t w = 0; w < EB; ++w) y.u[w] = ((const uint32_t *)t)[w];
+            *(T *)to = y.t;
+        } else {
+            for (uint32_t e = 0; e < 4; ++e)
+                if (pos + e >= b.p0 && pos + e < b.p1) {
+                    if constexpr (TYPE == 0) ((uint32_t *)to)[e] = ((const uint32_t *)t)[e];
+                    else if constexpr (TYPE == 1) ((uint16_t *)to)[e] = ((const uint16_t *)t)[e];
+                    else to[e] = t[e];
+                }
+        }
     }
 }
 
 template <uint32_t TYPE>
-__device__ __forceinline__ float element(const void *pool, size_t at, const float *scales, size_t sat) {
-    if constexpr (TYPE == 0) return ((const float *)pool)[at];
-    if constexpr (TYPE == 1) return __half2float(((const __half *)pool)[at]);
-    return (float)((const int8_t *)pool)[at] * scales[sat];
+__device__ __forceinline__ f4 decode(typename Four<TYPE>::T t) {
+    f4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (TYPE == 0) {
+            r[e] = t[e];
+        } else if constexpr (TYPE == 1) {
+            union {
+                uint16_t u;
+                _Float16 h;
+            } y = {(uint16_t)(t[e / 2] >> (16 * (e & 1)))};
+            r[e] = (float)y.h;
+        } else {
+            r[e] = (float)(int8_t)(t >> (8 * e));
+        }
+    }
+    return r;
 }
 
+/* A workgroup per run of `run` blocks and KV head: keys four dims a thread, values four positions of a dim a thread, turned
+ * through LDS. Several blocks a workgroup where there are many: a dim's positions of one block are a part (Q8: 32 bytes) of
+ * a cache line, the next blocks' the rest. */
 template <uint32_t TYPE>
-__global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, float *values) {
-    const uint32_t r = blockIdx.x;
-    uint32_t s, pos;
-    if (r == 0) check_begin(a, threadIdx.x, ST_WG);
-    if (!place_of(a, r, s, pos)) return;
-    const int page = page_of(a, s, pos);
-    if (page < 0) return;
-    const uint32_t P = 1u << a.shift, slot = pos & (P - 1), kd = a.kv_heads * a.head_dim;
-    for (uint32_t i = threadIdx.x; i < kd; i += ST_WG) {
-        const uint32_t h = i / a.head_dim, d = i % a.head_dim;
-        const size_t ph = (size_t)page * a.kv_heads + h, sc = (ph * a.nb + d / 32) * P + slot;
-        keys[(size_t)r * kd + i] = element<TYPE>(a.keys, (ph * P + slot) * a.head_dim + d, a.ks, sc);
-        values[(size_t)r * kd + i] = element<TYPE>(a.values, (ph * a.head_dim + d) * P + slot, a.vs, sc);
+__global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, float *values, uint32_t run) {
+    typedef typename Four<TYPE>::T T;
+    constexpr uint32_t EB = sizeof(T) / 4;
+    __shared__ __attribute__((aligned(16))) float turn[ST_POS * (MAX_HEAD_DIM + 4)];
+    const uint32_t tid = threadIdx.x, hd = a.head_dim, h = blockIdx.x % a.kv_heads, P = 1u << a.shift, q = hd / 4;
+    if (blockIdx.x == 0) check_begin(a, tid, ST_WG);
+    for (uint32_t x = blockIdx.x / a.kv_heads * run, end = x + run; x < end; ++x) {
+        Block b;
+        if (!find_block(a, x, b)) return;
+        int page[2];
+        block_pages(a, b, page);
+        const uint32_t n = b.p1 - b.p0, base = b.p0 / ST_POS * ST_POS;
+        for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) {
+            const uint32_t d = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), slot = (base + j) & (P - 1);
+            const int pg = j & 16 ? page[1] : page[0];
+            if (pg < 0 || base + j >= b.p1 || base + j + 4 <= b.p0) continue;
+            f4 y = decode<TYPE>(*(const T *)((const unsigned char *)a.values + (head_at(a, pg, h) + ((size_t)d << a.shift) + slot) * EB));
+            if constexpr (TYPE == 2) {
+                const f4 w = *(const f4 *)(a.vs + scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = y[e] * w[e];
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) turn[(j + e) * (hd + 4) + d] = y[e];
+        }
+        for (uint32_t i = tid; i < n * q; i += ST_WG) {
+            const uint32_t j = i / q, d = 4 * (i - j * q), pos = b.p0 + j, slot = pos & (P - 1);
+            const int pg = pos & 16 ? page[1] : page[0];
+            if (pg < 0) continue;
+            f4 y = decode<TYPE>(*(const T *)((const unsigned char *)a.keys + (head_at(a, pg, h) + (size_t)slot * hd + d) * EB));
+            if constexpr (TYPE == 2) {
+                const float w = a.ks[scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot];
+                y *= w;
+            }
+            *(f4u *)(keys + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d) = y;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < n * q; i += ST_WG) {
+            const uint32_t j = i / q, d = 4 * (i - j * q), pos = b.p0 + j;
+            if ((pos & 16 ? page[1] : page[0]) < 0) continue;
+            *(f4u *)(values + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d) = *(const f4 *)&turn[(pos - base) * (hd + 4) + d];
+        }
+        if (x + 1 < end) __syncthreads();
     }
 }
 
@@ -197,15 +398,15 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
 
 hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out, const float *k, const float *v,
                                 const float *cs, const float *sn, hipStream_t s) {
-    SMQ_PAGED(k_paged_store, dim3(a.tokens), dim3(ST_WG), q, q_out, k, v, cs, sn);
+    SMQ_PAGED(k_paged_store, dim3((q ? a.tokens : 0) + most_blocks(a) * a.kv_heads), dim3(ST_WG), q, q_out, k, v, cs, sn);
     return hipGetLastError();
 }
 
 hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s) {
-    SMQ_PAGED(k_paged_read, dim3(a.tokens), dim3(ST_WG), keys, values);
+    const uint32_t blocks = most_blocks(a), run = (uint64_t)blocks * a.kv_heads >= 4096 ? 4 : 1;
+    SMQ_PAGED(k_paged_read, dim3((blocks + run - 1) / run * a.kv_heads), dim3(ST_WG), keys, values, run);
     return hipGetLastError();
 }
-
 
 size_t paged_attention_workspace(const PagedArgs &a) {
     const AttendPlan p = attend_plan(a, ~(size_t)0);

@@ -78,7 +78,8 @@ def check(logits, rules, wants, stride=None, in_place=False, offset=0):
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 33), (2, 1000), (5, 1023), (4, 1024), (3, 1025), (2, 4099), (9, 32000),
-                                        (1, 151936), (7, 20000), (70, 5001)])
+                                        (1, 151936), (7, 20000), (70, 5001),
+                                        (260, 4099)])  # the last one in spans of 4096 ids
 def test_all_rules(rows, vocab):
     say("logits", rows, vocab)
     rng = np.random.default_rng(rows * vocab)
