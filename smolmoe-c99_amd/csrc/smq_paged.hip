@@ -146,47 +146,54 @@ __device__ __forceinline__ typename Four<TYPE>::T encode(f4 x, float &scale, boo
     }
 }
 
-/* The first a.tokens workgroups: a row of q each (all heads). Then one per block and KV head: keys and values of up to
- * ST_POS positions, four dims a thread, values turned through LDS so that a dim's positions are written together (few
- * positions: straight, element by element). */
+/* First two workgroups per block and KV head, one its keys, one its values: up to ST_POS positions, four dims a thread,
+ * the loads of four passes at once; values are turned through LDS so that a dim's positions are written together (few
+ * positions: straight, element by element). Then a workgroup per row of q (all heads). */
+constexpr uint32_t ST_PASSES = 4;
 template <uint32_t TYPE>
 __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float *q, float *q_out, const float *k,
-                                                       const float *v, const float *cs, const float *sn) {
+                                                       const float *v, const float *cs, const float *sn, uint32_t kv_groups) {
     typedef typename Four<TYPE>::T T;
     constexpr uint32_t EB = sizeof(T) / 4;
-    __shared__ __attribute__((aligned(16))) unsigned char turn[MAX_HEAD_DIM * (ST_POS * EB + 4)];
-    const uint32_t tid = threadIdx.x, hd = a.head_dim, rows = q ? a.tokens : 0;
+    extern __shared__ __attribute__((aligned(16))) unsigned char turn[]; /* [head_dim][ST_POS * EB + 4] */
+    const uint32_t tid = threadIdx.x, hd = a.head_dim;
     if (blockIdx.x == 0) check_begin(a, tid, ST_WG);
-    if (blockIdx.x < rows) {
+    if (blockIdx.x >= kv_groups) {
         uint32_t s, pos;
-        if (!place_of(a, blockIdx.x, s, pos)) return;
+        const uint32_t r = blockIdx.x - kv_groups;
+        if (!place_of(a, r, s, pos)) return;
         const float *c = cs + (size_t)pos * a.pairs, *sr = sn + (size_t)pos * a.pairs;
-        const size_t row = (size_t)blockIdx.x * a.heads * hd;
+        const size_t row = (size_t)r * a.heads * hd;
+#pragma unroll 2
         for (uint32_t i = tid; i < a.heads * hd / 4; i += ST_WG)
             *(f4u *)(q_out + row + 4 * i) = rotated(*(const f4u *)(q + row + 4 * i), 4 * i % hd, a.pairs, c, sr);
         return;
     }
-    const uint32_t x = blockIdx.x - rows, h = x % a.kv_heads;
+    const uint32_t kind = blockIdx.x & 1, x = blockIdx.x >> 1, h = x % a.kv_heads; /* kind 0: keys, 1: values */
     Block b;
     if (!find_block(a, x / a.kv_heads, b)) return;
     int page[2];
     block_pages(a, b, page);
     const uint32_t P = 1u << a.shift, lanes = a.nb * 8, n = b.p1 - b.p0; /* lanes of a row: whole 32-wide blocks */
     const bool few = n <= 2;
-    for (uint32_t kind = 0; kind < 2; ++kind) { /* keys, values */
-        const float *from = kind ? v : k;
-        for (uint32_t i = tid; i < (n * lanes + ST_WG - 1) / ST_WG * ST_WG; i += ST_WG) { /* whole waves: encode shuffles */
-            const uint32_t j = i / lanes, d = 4 * (i - j * lanes), pos = b.p0 + min(j, n - 1), slot = pos & (P - 1);
+    const float *from = kind ? v : k;
+    for (uint32_t i0 = tid; i0 < (n * lanes + ST_WG - 1) / ST_WG * ST_WG; i0 += ST_PASSES * ST_WG) { /* whole waves: encode shuffles */
+        f4 y[ST_PASSES];
+#pragma unroll
+        for (uint32_t u = 0; u < ST_PASSES; ++u) {
+            const uint32_t i = i0 + u * ST_WG, j = i / lanes, d = 4 * (i - j * lanes);
+            y[u] = f4{};
+            if (j < n && d < hd) y[u] = *(const f4u *)(from + ((size_t)(b.row + (int)(b.p0 + j)) * a.kv_heads + h) * hd + d);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < ST_PASSES; ++u) {
+            const uint32_t i = i0 + u * ST_WG, j = i / lanes, d = 4 * (i - j * lanes), pos = b.p0 + j, slot = pos & (P - 1);
             const int pg = pos & 16 ? page[1] : page[0];
             const bool in = j < n && d < hd;
-            f4 y = {};
-            if (in) {
-                y = *(const f4u *)(from + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d);
-                if (!kind) y = rotated(y, d, a.pairs, cs + (size_t)pos * a.pairs, sn + (size_t)pos * a.pairs);
-            }
+            if (!kind && in) y[u] = rotated(y[u], d, a.pairs, cs + (size_t)pos * a.pairs, sn + (size_t)pos * a.pairs);
             float scale;
             bool bad = false;
-            const T t = encode<TYPE>(y, scale, bad);
+            const T t = encode<TYPE>(y[u], scale, bad);
             if (!in || pg < 0) continue;
             if (bad) *a.flag = 1;
             if (TYPE == 2 && d % 32 == 0) (kind ? a.vs : a.ks)[scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot] = scale;
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float 
             }
         }
     }
-    if (few) return;
+    if (few || !kind) return;
     __syncthreads();
     for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) { /* four positions of a dim */
         const uint32_t d = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), pos = b.p0 / ST_POS * ST_POS + j;
@@ -252,53 +259,69 @@ __device__ __forceinline__ f4 decode(typename Four<TYPE>::T t) {
     return r;
 }
 
-/* A workgroup per run of `run` blocks and KV head: keys four dims a thread, values four positions of a dim a thread, turned
- * through LDS. Several blocks a workgroup where there are many: a dim's positions of one block are a part (Q8: 32 bytes) of
- * a cache line, the next blocks' the rest. */
+/* A workgroup per block and KV head: keys four dims a thread, values four positions of a dim a thread, turned through LDS.
+ * A block has as many of the ones as of the others; both are requested together, RD_PASSES of them at once. */
+constexpr uint32_t RD_PASSES = 2;
 template <uint32_t TYPE>
-__global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, float *values, uint32_t run) {
+__global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, float *values) {
     typedef typename Four<TYPE>::T T;
     constexpr uint32_t EB = sizeof(T) / 4;
-    __shared__ __attribute__((aligned(16))) float turn[ST_POS * (MAX_HEAD_DIM + 4)];
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    float *turn = (float *)lds; /* [ST_POS][head_dim + 4] */
     const uint32_t tid = threadIdx.x, hd = a.head_dim, h = blockIdx.x % a.kv_heads, P = 1u << a.shift, q = hd / 4;
     if (blockIdx.x == 0) check_begin(a, tid, ST_WG);
-    for (uint32_t x = blockIdx.x / a.kv_heads * run, end = x + run; x < end; ++x) {
-        Block b;
-        if (!find_block(a, x, b)) return;
-        int page[2];
-        block_pages(a, b, page);
-        const uint32_t n = b.p1 - b.p0, base = b.p0 / ST_POS * ST_POS;
-        for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) {
-            const uint32_t d = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), slot = (base + j) & (P - 1);
-            const int pg = j & 16 ? page[1] : page[0];
-            if (pg < 0 || base + j >= b.p1 || base + j + 4 <= b.p0) continue;
-            f4 y = decode<TYPE>(*(const T *)((const unsigned char *)a.values + (head_at(a, pg, h) + ((size_t)d << a.shift) + slot) * EB));
-            if constexpr (TYPE == 2) {
-                const f4 w = *(const f4 *)(a.vs + scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot);
+    Block b;
+    if (!find_block(a, blockIdx.x / a.kv_heads, b)) return;
+    int page[2];
+    block_pages(a, b, page);
+    const uint32_t base = b.p0 / ST_POS * ST_POS;
+    auto page_at = [&](uint32_t pos) { return pos >= b.p0 && pos < b.p1 ? (pos & 16 ? page[1] : page[0]) : -1; };
+    for (uint32_t i0 = tid; i0 < hd * (ST_POS / 4); i0 += RD_PASSES * ST_WG) {
+        T tv[RD_PASSES], tk[RD_PASSES];
+        f4 wv[RD_PASSES];
+        float wk[RD_PASSES];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = y[e] * w[e];
+        for (uint32_t u = 0; u < RD_PASSES; ++u) {
+            const uint32_t i = i0 + u * ST_WG;
+            if (i >= hd * (ST_POS / 4)) continue;
+            const uint32_t dv = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), sv = (base + j) & (P - 1);
+            const int pv = j & 16 ? page[1] : page[0];
+            if (pv >= 0) {
+                tv[u] = *(const T *)((const unsigned char *)a.values + (head_at(a, pv, h) + ((size_t)dv << a.shift) + sv) * EB);
+                if constexpr (TYPE == 2) wv[u] = *(const f4 *)(a.vs + scales_at(a, pv, h) + ((size_t)(dv / 32) << a.shift) + sv);
             }
+            const uint32_t pos = base + i / q, dk = 4 * (i % q), sk = pos & (P - 1);
+            const int pk = page_at(pos);
+            if (pk >= 0) {
+                tk[u] = *(const T *)((const unsigned char *)a.keys + (head_at(a, pk, h) + (size_t)sk * hd + dk) * EB);
+                if constexpr (TYPE == 2) wk[u] = a.ks[scales_at(a, pk, h) + ((size_t)(dk / 32) << a.shift) + sk];
+            }
+        }
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) turn[(j + e) * (hd + 4) + d] = y[e];
-        }
-        for (uint32_t i = tid; i < n * q; i += ST_WG) {
-            const uint32_t j = i / q, d = 4 * (i - j * q), pos = b.p0 + j, slot = pos & (P - 1);
-            const int pg = pos & 16 ? page[1] : page[0];
-            if (pg < 0) continue;
-            f4 y = decode<TYPE>(*(const T *)((const unsigned char *)a.keys + (head_at(a, pg, h) + (size_t)slot * hd + d) * EB));
-            if constexpr (TYPE == 2) {
-                const float w = a.ks[scales_at(a, pg, h) + ((size_t)(d / 32) << a.shift) + slot];
-                y *= w;
+        for (uint32_t u = 0; u < RD_PASSES; ++u) {
+            const uint32_t i = i0 + u * ST_WG;
+            if (i >= hd * (ST_POS / 4)) continue;
+            const uint32_t dv = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4));
+            if ((j & 16 ? page[1] : page[0]) >= 0) {
+                f4 y = decode<TYPE>(tv[u]);
+                if constexpr (TYPE == 2) y *= wv[u];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) turn[(j + e) * (hd + 4) + dv] = y[e];
             }
-            *(f4u *)(keys + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d) = y;
+            const uint32_t pos = base + i / q, dk = 4 * (i % q);
+            if (page_at(pos) >= 0) {
+                f4 y = decode<TYPE>(tk[u]);
+                if constexpr (TYPE == 2) y *= wk[u];
+                __builtin_nontemporal_store(y, (f4u *)(keys + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + dk));
+            }
         }
-        __syncthreads();
-        for (uint32_t i = tid; i < n * q; i += ST_WG) {
-            const uint32_t j = i / q, d = 4 * (i - j * q), pos = b.p0 + j;
-            if ((pos & 16 ? page[1] : page[0]) < 0) continue;
-            *(f4u *)(values + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d) = *(const f4 *)&turn[(pos - base) * (hd + 4) + d];
-        }
-        if (x + 1 < end) __syncthreads();
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) {
+        const uint32_t pos = base + i / q, d = 4 * (i % q);
+        if (page_at(pos) >= 0)
+            __builtin_nontemporal_store(*(const f4 *)&turn[(pos - base) * (hd + 4) + d],
+                                        (f4u *)(values + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d));
     }
 }
 
@@ -389,22 +412,23 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
 
 }  // namespace
 
-#define SMQ_PAGED(KERNEL, GRID, BLOCK, ...)                                                          \
+#define SMQ_PAGED(KERNEL, GRID, BLOCK, LDS, ...)                                                          \
     do {                                                                                             \
-        if (a.type == 0) hipLaunchKernelGGL((KERNEL<0>), GRID, BLOCK, 0, s, a, __VA_ARGS__);         \
-        else if (a.type == 1) hipLaunchKernelGGL((KERNEL<1>), GRID, BLOCK, 0, s, a, __VA_ARGS__);    \
-        else hipLaunchKernelGGL((KERNEL<2>), GRID, BLOCK, 0, s, a, __VA_ARGS__);                     \
+        if (a.type == 0) hipLaunchKernelGGL((KERNEL<0>), GRID, BLOCK, LDS, s, a, __VA_ARGS__);         \
+        else if (a.type == 1) hipLaunchKernelGGL((KERNEL<1>), GRID, BLOCK, LDS, s, a, __VA_ARGS__);    \
+        else hipLaunchKernelGGL((KERNEL<2>), GRID, BLOCK, LDS, s, a, __VA_ARGS__);                     \
     } while (0)
 
 hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out, const float *k, const float *v,
                                 const float *cs, const float *sn, hipStream_t s) {
-    SMQ_PAGED(k_paged_store, dim3((q ? a.tokens : 0) + most_blocks(a) * a.kv_heads), dim3(ST_WG), q, q_out, k, v, cs, sn);
+    const uint32_t kv_groups = 2 * most_blocks(a) * a.kv_heads;
+    SMQ_PAGED(k_paged_store, dim3((q ? a.tokens : 0) + kv_groups), dim3(ST_WG),
+              a.head_dim * (ST_POS * (4u >> a.type) + 4), q, q_out, k, v, cs, sn, kv_groups);
     return hipGetLastError();
 }
 
 hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s) {
-    const uint32_t blocks = most_blocks(a), run = (uint64_t)blocks * a.kv_heads >= 4096 ? 4 : 1;
-    SMQ_PAGED(k_paged_read, dim3((blocks + run - 1) / run * a.kv_heads), dim3(ST_WG), keys, values, run);
+    SMQ_PAGED(k_paged_read, dim3(most_blocks(a) * a.kv_heads), dim3(ST_WG), ST_POS * (a.head_dim + 4) * 4, keys, values);
     return hipGetLastError();
 }
 
