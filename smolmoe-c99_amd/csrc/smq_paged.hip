@@ -337,7 +337,7 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
     const i4 u = used[tile];
     const uint32_t parts = (uint32_t)u[0] & 0xffff, n = (uint32_t)u[0] >> 16, slot = (uint32_t)u[3];
     if (parts < 2 || r >= n || threadIdx.x / lanes >= per) return;
-    const f2 *pml = (const f2 *)(part + (size_t)2 * p.stream * a.kv_heads * p.tile_rows * hd);
+    const f2 *pml = (const f2 *)(part + (size_t)p.pieces * a.kv_heads * p.tile_rows * hd);
     float m = -FLT_MAX, l = 0.0f;
     f4 o = {};
     for (uint32_t i0 = 0; i0 < parts; i0 += JOIN_AT_ONCE) {
@@ -346,8 +346,7 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
         float top = m;
 #pragma unroll
         for (uint32_t i = 0; i < JOIN_AT_ONCE; ++i) {
-            const uint32_t k = min(i0 + i, parts - 1); /* the first one's slot, then slots 0 of the next workgroups */
-            const size_t y = ((size_t)(k ? (slot & ~1u) + 2 * k : slot) * a.kv_heads + kh) * p.tile_rows + r;
+            const size_t y = ((size_t)(slot + min(i0 + i, parts - 1)) * a.kv_heads + kh) * p.tile_rows + r;
             ml[i] = pml[y];
             x[i] = *(const f4 *)(part + y * hd + d);
         }
@@ -404,9 +403,14 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     const uint64_t tiles = seqs * ((rows / (seqs ? seqs : 1) + p.tile_rows - 1) >> p.row_shift) * a.kv_heads;
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
     if (tiles >= 1024 || (tiles < groups ? steps * (groups - tiles) / groups : 0) <= 24) p.stream = 0;
-    const size_t used = attend_used_bytes(a, p), each = attend_part_bytes(a, p.tile_rows);
+    const size_t used = attend_used_bytes(a, p), each = attend_piece_bytes(a, p.tile_rows);
     const uint64_t room = ws_bytes > used ? (ws_bytes - used) / each : 0;
-    if (room < p.stream) p.stream = room > p.tiles ? (uint32_t)room : 0;
+    auto pieces = [&](uint64_t aim) { return max(aim, (aim + 1) / 2 + p.tiles); }; /* at most: see by_piece */
+    const uint64_t longest = (uint64_t)p.tiles * p.cw / ((PA_LONG * 64 >> p.unit) + 1);
+    p.most = p.owns || longest <= p.stream ? p.stream : (uint32_t)min(longest, (uint64_t)3 * p.stream);
+    if (room < pieces(p.most)) p.most = p.stream;
+    if (room < pieces(p.stream)) p.most = p.stream = room > p.tiles ? (uint32_t)min(room, 2 * (room - p.tiles)) : 0;
+    p.pieces = p.stream ? (uint32_t)pieces(p.most) : 0;
     return p;
 }
 
@@ -434,7 +438,7 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
 
 size_t paged_attention_workspace(const PagedArgs &a) {
     const AttendPlan p = attend_plan(a, ~(size_t)0);
-    return p.stream ? attend_used_bytes(a, p) + p.stream * attend_part_bytes(a, p.tile_rows) : 0;
+    return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,

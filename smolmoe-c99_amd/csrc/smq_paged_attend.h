@@ -27,30 +27,30 @@ namespace smq {
 constexpr int PA_WAVES = 4; /* of a workgroup */
 constexpr uint32_t PA_STEP = 32;      /* positions */
 constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps are dealt out */
+constexpr uint32_t PA_LONG = 64;      /* of a piece, where there are more pieces than CUs hold at once */
 constexpr uint32_t PA_FIXED = 16;     /* steps that a tile costs beside its own */
 
 /* How a launch covers the rows: tiles of tile_rows rows of one sequence and KV head (`tiles`: as many as the batch can
  * need). owns: a wave owns 16 * RT of the tile's rows over all positions; else the tile has 16 rows and the waves share
  * the positions out.
  *
- * stream > 0: stream workgroups per KV head take equal runs of all tiles' steps laid end to end, so a run ends and the
- * next begins inside a tile, whose partial results k_paged_join joins. Lengths are known on the device only: each
- * workgroup finds its run there. A tile counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the
- * sequence: its steps nearly, with sums that need no loop, and PA_FIXED for what it costs beside its steps (the batch
- * looked at, queries, the first keys, the join). stream 0 (no workspace): a workgroup per tile. */
+ * stream > 0: tiles are cut into pieces, each with a workgroup of its own, so that about `stream` of them per KV head cost
+ * the same (up to `most`, of PA_LONG steps or more); k_paged_join joins a tile's. Lengths are known on the device only: each workgroup finds its piece there. A tile
+ * counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the sequence: its steps nearly, with sums
+ * that need no loop, and PA_FIXED for what it costs beside its steps (the batch looked at, queries, the first keys, the
+ * join). With all tiles' units laid end to end and cut every `each` units, a tile has a piece for each part of it, and
+ * these are made equal. There are at most `pieces` of them. stream 0 (no workspace): a workgroup per tile. */
 typedef int i4 __attribute__((ext_vector_type(4)));
 struct AttendPlan {
     bool owns;
-    uint32_t tile_rows, row_shift, tiles, stream;
+    uint32_t tile_rows, row_shift, tiles, stream, most, pieces;
     uint32_t unit, fixed, c1, cw, tile_tokens; /* units; tokens of a tile, at most */
 };
-/* The workspace: per tile and KV head four words (the workgroups that share it, its rows << 16; the sequence's first
- * token; the first row; the first one's slot), then per workgroup two slots of tile_rows rows: O, and behind all of them
- * the maxima and sums. A workgroup's first tile, if it shares that one, has slot 0, its last slot 1; the tiles between are
- * its own. */
+/* The workspace: per tile and KV head four words (its pieces, its rows << 16; the sequence's first token; the first row;
+ * the first piece's number), then per piece and KV head tile_rows rows: O, and behind all of them the maxima and sums. */
 inline size_t attend_used_bytes(const PagedArgs &a, const AttendPlan &p) { return (size_t)p.tiles * a.kv_heads * 16; }
-inline size_t attend_part_bytes(const PagedArgs &a, uint32_t tile_rows) { /* for a workgroup per KV head */
-    return (size_t)2 * a.kv_heads * tile_rows * (a.head_dim + 2) * 4;
+inline size_t attend_piece_bytes(const PagedArgs &a, uint32_t tile_rows) { /* of all KV heads */
+    return (size_t)a.kv_heads * tile_rows * (a.head_dim + 2) * 4;
 }
 
 template <uint32_t TYPE>
@@ -187,9 +187,10 @@ __device__ __forceinline__ Steps tile_steps(const PagedArgs &a, int pmin, int pm
     return s;
 }
 
-/* A tile: sequence, its number in it, its number in the batch, its first unit and its units. */
+/* A tile: sequence, its number in it, its number in the batch; its pieces, the number of the first one, which one is
+ * meant. */
 struct Tile {
-    uint32_t seq, j, t, first, units;
+    uint32_t seq, j, t, pieces, slot, piece;
     Seq sq;
 };
 template <int CTRL, int ROWS>
@@ -267,40 +268,67 @@ struct Tiles {
                 const uint32_t first = before + lane_of(tiles_upto, w) - lane_of(n, w);
                 take(t, w, x);
                 t.j = x - first;
+                t.pieces = 1;
+                t.piece = 0;
                 return true;
             }
             before += lane_of(tiles_upto, 63);
         }
         return false;
     }
-    /* The last tile whose first unit u and number t have key(u, t) <= x; key grows with both. False if x is behind all of
-     * them (key of the batch's end <= x). */
-    template <typename Key>
-    __device__ __forceinline__ bool last_with(uint32_t x, Key key, Tile &t) {
+    /* Pieces of the tiles that `units` of a sequence cover, `tiles` of them, where a piece has at most 1 / inv units. Grows
+     * with both; a rounding of the product moves a cut by a unit. */
+    static __device__ __forceinline__ uint32_t pieces(uint32_t units, uint32_t tiles, float inv) {
+        return (uint32_t)((float)units * inv) + tiles;
+    }
+    /* The tile that piece x is of, of `units` / `count` in all. False behind the last.
+     *
+     * Pieces of u units give units / u + tiles pieces at most: with u = units / (aim - tiles), the start of the search,
+     * there are `aim` or fewer; half of aim at least is kept for cuts. Every sequence's last part is rounded up, so a
+     * smaller u often has no more than aim either, down to units / aim: six halvings find it, where one look at the
+     * batch holds all sequences. */
+    __device__ __forceinline__ bool by_piece(uint32_t x, uint32_t units, uint32_t count, Tile &t) {
+        const float all = (float)units, least = (float)(PA_MIN_STEPS * 64 >> p.unit) + 1.0f;
+        const uint32_t aim = min(max(units / ((PA_LONG * 64 >> p.unit) + 1), p.stream), p.most);
+        const uint32_t cuts = max(aim > count ? aim - count : 0, (aim + 1) / 2);
+        float hi = 1.0f / fmaxf(all / (float)cuts * 1.0001f, least); /* hi, lo: pieces per unit */
+        if (a.seqs <= 64) {
+            float lo = hi;
+            hi = 1.0f / fmaxf(all / (float)aim, least);
+            for (int k = 0; k < 6; ++k) {
+                const float mid = 0.5f * (lo + hi);
+                const bool fits = lane_of(scan_wave(pieces(mine, n, mid)), 63) <= aim;
+                lo = fits ? mid : lo;
+                hi = fits ? hi : mid;
+            }
+            hi = lo;
+        }
         uint32_t before = 0, tiles = 0;
         for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
             if (s0 != at) look(s0);
-            const uint64_t past = __ballot(key(before + upto, tiles + tiles_upto) > x);
+            const uint32_t own = pieces(mine, n, hi), to = scan_wave(own);
+            const uint64_t past = __ballot(before + to > x);
             if (past) {
                 const int w = __ffsll((unsigned long long)past) - 1;
-                before += lane_of(upto, w) - lane_of(mine, w);
+                before += lane_of(to, w) - lane_of(own, w);
                 tiles += lane_of(tiles_upto, w) - lane_of(n, w);
                 const uint32_t N = lane_of(n, w), d0 = lane_of(c0, w), d1 = lane_of(c1, w), dw = lane_of(cw, w);
-                uint32_t lo = 0, span = N; /* the last j of [lo, lo + span) */
+                uint32_t j = 0, span = N; /* the last j of [j, j + span) whose first piece is x or before it */
                 while (span > 1) {
-                    const uint32_t step = (span + 63) / 64, j = lo + threadIdx.x % 64 * step;
-                    const uint64_t fit = __ballot(j < lo + span && key(before + sum(j, d0, d1, dw), tiles + j) <= x);
-                    const uint32_t k = 63 - (uint32_t)__builtin_clzll(fit); /* lane 0 fits */
-                    span = min(step, span - k * step);
-                    lo += k * step;
+                    const uint32_t step = (span + 63) / 64, k = j + threadIdx.x % 64 * step;
+                    const uint64_t fit = __ballot(k < j + span && before + pieces(sum(k, d0, d1, dw), k, hi) <= x);
+                    const uint32_t f = 63 - (uint32_t)__builtin_clzll(fit); /* lane 0 fits */
+                    span = min(step, span - f * step);
+                    j += f * step;
                 }
-                t.j = lo;
-                t.first = before + sum(lo, d0, d1, dw);
-                t.units = sum(lo + 1, d0, d1, dw) - sum(lo, d0, d1, dw);
-                take(t, w, tiles + lo);
+                take(t, w, tiles + j);
+                t.j = j;
+                t.slot = before + pieces(sum(j, d0, d1, dw), j, hi);
+                t.pieces = before + pieces(sum(j + 1, d0, d1, dw), j + 1, hi) - t.slot;
+                t.piece = x - t.slot;
                 return true;
             }
-            before += lane_of(upto, 63);
+            before += lane_of(to, 63);
             tiles += lane_of(tiles_upto, 63);
         }
         return false;
@@ -1075,31 +1103,23 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, c
     }
 }
 
-/* The units [v, e) of a tile, which belong to workgroup i's run [i each, (i + 1) each) of a KV head; each 0: all of the
- * tile, undivided. */
+/* A tile's piece. */
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
 __device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used,
-                                          float *part, uint32_t kh, const Tile &t, uint32_t i, uint32_t each, uint32_t v,
-                                          uint32_t e, unsigned char *lds) {
+                                          float *part, uint32_t kh, const Tile &t, unsigned char *lds) {
     const uint32_t G = a.heads / a.kv_heads, row0 = t.j * p.tile_rows, n = min(p.tile_rows, (uint32_t)t.sq.n * G - row0);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const Steps st = tile_steps(a, t.sq.first + (int)(row0 / G), t.sq.first + (int)((row0 + n - 1) / G));
     Out out = {a, t.sq, kh, row0, n, att, nullptr, nullptr};
     uint32_t u0 = 0, u1 = st.total;
-    if (each) {
-        const uint32_t i0 = t.first / each, parts = (t.first + t.units - 1) / each - i0 + 1;
-        const uint32_t slot = 2 * i + (v == i * each ? 0 : 1);
-        if (i == i0 && threadIdx.x == 0)
-            used[(size_t)t.t * a.kv_heads + kh] = i4{(int)(parts | n << 16), t.sq.begin, (int)row0, (int)slot};
-        if (parts > 1) {
-            const size_t r = ((size_t)slot * a.kv_heads + kh) * p.tile_rows;
-            out.po = part + r * a.head_dim;
-            out.pml = part + (size_t)2 * p.stream * a.kv_heads * p.tile_rows * a.head_dim + 2 * r;
-            /* both sides of a cut round it alike; the tile's ends are 0 and all */
-            const float f = (float)t.units, all = (float)st.total;
-            u0 = (uint32_t)((float)(v - t.first) / f * all);
-            u1 = (uint32_t)((float)(e - t.first) / f * all);
-        }
+    if (p.stream && t.piece == 0 && threadIdx.x == 0)
+        used[(size_t)t.t * a.kv_heads + kh] = i4{(int)(t.pieces | n << 16), t.sq.begin, (int)row0, (int)t.slot};
+    if (t.pieces > 1) {
+        const size_t r = ((size_t)(t.slot + t.piece) * a.kv_heads + kh) * p.tile_rows;
+        out.po = part + r * a.head_dim;
+        out.pml = part + (size_t)p.pieces * a.kv_heads * p.tile_rows * a.head_dim + 2 * r;
+        u0 = st.total * t.piece / t.pieces; /* 2^15 steps at most, pieces below 2^16 */
+        u1 = st.total * (t.piece + 1) / t.pieces;
     }
     if constexpr (OWNS) {
         if (n > 16) {
@@ -1111,59 +1131,30 @@ __device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &
 }
 
 /* Workgroups of one KV head follow each other at a distance of all heads, so where these are a multiple of the eight XCDs
- * the tiles of a sequence that read the same pages share an L2.
- *
- * A run's tiles are taken one after another by one workgroup while decoding: as many workgroups as CUs stream without a
- * pause, each its share. Where waves own rows every piece of a run is a workgroup of its own, in no loop: what a loop
- * carries costs the products their registers (heads of 128: 40 spilled), and pieces are long. */
+ * the tiles of a sequence that read the same pages share an L2. From the last tile to the first: the last rows of a chunk
+ * see the most. A piece has a workgroup of its own: a loop over several costs the products their registers (heads of 128:
+ * 40 spilled), and one that takes a second piece, however short, pays a tile's fixed cost twice. */
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
 __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_attend(PagedArgs a, const float *q, float *att,
                                                                                   AttendPlan p, i4 *used, float *part) {
     constexpr uint32_t OWN_LDS = OWNS ? 2 * InLds<TYPE, KS, SMALL>::BUFFER : 0;
     __shared__ __attribute__((aligned(16))) unsigned char lds[OWN_LDS > shared_lds(KS) ? OWN_LDS : shared_lds(KS)];
-    const uint32_t kh = blockIdx.x % a.kv_heads;
-    uint32_t i = blockIdx.x / a.kv_heads;
+    const uint32_t kh = blockIdx.x % a.kv_heads, i = blockIdx.x / a.kv_heads;
     if (blockIdx.x == 0) check_begin(a, threadIdx.x, 64 * PA_WAVES);
     Tile t;
-    if (!p.stream) { /* from the last tile to the first: the last rows of a chunk see the most */
-        Tiles tiles(a, p);
-        if (tiles.by_number(p.tiles - 1 - i, t))
-            tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, 0, 0, 0, lds);
-        return;
-    }
-    uint32_t units, count, each, v, e;
     {
         Tiles tiles(a, p);
-        tiles.total(units, count);
-        if (i == 0) /* tiles that the batch does not need */
-            for (uint32_t x = count + threadIdx.x; x < p.tiles; x += 64 * PA_WAVES) used[(size_t)x * a.kv_heads + kh] = i4{};
-        each = max((units + p.stream - 1) / p.stream, (PA_MIN_STEPS * 64 >> p.unit) + 1);
-        if constexpr (OWNS) { /* tile t's first piece has number t + its first unit / each, from the last to the first */
-            i = p.stream + p.tiles - 1 - i;
-            if (!tiles.last_with(i, [&](uint32_t u, uint32_t n) { return u / each + n; }, t)) return;
-            i -= t.t; /* the workgroup whose run it is */
-            v = max(t.first, i * each);
+        if (!p.stream) {
+            if (!tiles.by_number(p.tiles - 1 - i, t)) return;
         } else {
-            v = i * each; /* stream * each is below 2^31: see attend_plan */
-            if (v >= units) return;
-            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
+            uint32_t units, count;
+            tiles.total(units, count);
+            if (i == 0) /* tiles that the batch does not need */
+                for (uint32_t x = count + threadIdx.x; x < p.tiles; x += 64 * PA_WAVES) used[(size_t)x * a.kv_heads + kh] = i4{};
+            if (!tiles.by_piece(p.pieces - 1 - i, units, count, t)) return;
         }
     }
-    if constexpr (OWNS) {
-        e = min(t.first + t.units, (i + 1) * each);
-        if (v < e) tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
-    } else {
-        const uint32_t end = min(units, (i + 1) * each);
-        for (;;) {
-            e = min(end, t.first + t.units);
-            tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, i, each, v, e, lds);
-            v = e;
-            if (v >= end) break;
-            __syncthreads(); /* LDS is free */
-            Tiles tiles(a, p); /* again: carried along it took the products' registers */
-            tiles.last_with(v, [](uint32_t u, uint32_t) { return u; }, t);
-        }
-    }
+    tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, lds);
 }
 
 }  // namespace
@@ -1171,7 +1162,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
 template <uint32_t TYPE>
 hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
                          hipStream_t s) {
-    const dim3 grid(a.kv_heads * (!p.stream ? p.tiles : p.owns ? p.tiles + p.stream : p.stream));
+    const dim3 grid(a.kv_heads * (p.stream ? p.pieces : p.tiles));
 #define SMQ_ATTEND3(KS, RT, OWNS, SMALL)                                                                               \
     hipLaunchKernelGGL((k_paged_attend<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(64 * PA_WAVES), 0, s, a, q, att, p, used, \
                        part)
