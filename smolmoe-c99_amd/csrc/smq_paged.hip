@@ -370,13 +370,16 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
 /* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own
  * theirs.
  *
- * Workgroups that share the steps out: two a CU for products and for decoding heads of up to 64 (8 KiB of f16 a step and
- * wave: 64 sequences at 5000, 8 KV heads, 134 us with one a CU, 94 with two), one a CU for wider ones (16 x 12000, 8 KV
- * heads of 128: 145, 150; 32 x 3000 Q8, 2 KV heads: 31, 35).
+ * Pieces that the tiles are cut into: two a CU for products and for decoding heads of up to 64 (8 KiB of f16 a step and
+ * wave), one a CU for wider ones (one f16 sequence at 16384, 8 KV heads of 128: 22 us, two a CU 25); by_piece has what
+ * becomes of these numbers.
  *
- * Sharing them out costs a second launch, which joins: not where there are tiles for every CU four times over, and not
- * where a tile's steps at the longest length exceed an equal share by less than that (about 24 steps: 64 sequences at 700,
- * 2 KV heads of 64: 11.8 us with a workgroup per tile, 15.4 shared out). */
+ * Cutting costs partial results and a second launch, which joins them. No cuts
+ * - where the longest tile exceeds an equal share by about 24 steps or less (64 sequences at 700, 2 KV heads of 64: 11.8 us
+ *   whole, 15.4 cut; 8 with a window of 1024, 4 KV heads of 64: 22 whole, 13 cut);
+ * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
+ *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
+ *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). */
 AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     AttendPlan p;
     const uint32_t G = a.heads / a.kv_heads;
@@ -399,15 +402,21 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     while (((uint64_t)(p.tiles + 512) * ((most >> p.unit) + 1)) >= 1u << 30) ++p.unit;
     p.cw = (uint32_t)(most >> p.unit) + 1;
     p.c1 = 2 * p.tile_rows / G >> p.unit;
-    /* tiles of an even batch, and by how many steps the longest could exceed an equal share */
+    /* tiles of an even batch, the steps of the longest and of the mean */
     const uint64_t tiles = seqs * ((rows / (seqs ? seqs : 1) + p.tile_rows - 1) >> p.row_shift) * a.kv_heads;
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
-    if (tiles >= 1024 || (tiles < groups ? steps * (groups - tiles) / groups : 0) <= 24) p.stream = 0;
+    if (p.owns && tiles > 256) {
+        const uint64_t average = steps - (a.window ? 0 : min(rows / G / seqs / 64, steps / 2));
+        if (tiles >= 512 || average * (512 - tiles) / 256 <= 24) p.stream = 0;
+    } else if (tiles >= groups || steps * (groups - tiles) / groups <= 24) {
+        p.stream = 0;
+    }
     const size_t used = attend_used_bytes(a, p), each = attend_piece_bytes(a, p.tile_rows);
     const uint64_t room = ws_bytes > used ? (ws_bytes - used) / each : 0;
     auto pieces = [&](uint64_t aim) { return max(aim, (aim + 1) / 2 + p.tiles); }; /* at most: see by_piece */
-    const uint64_t longest = (uint64_t)p.tiles * p.cw / ((PA_LONG * 64 >> p.unit) + 1);
-    p.most = p.owns || longest <= p.stream ? p.stream : (uint32_t)min(longest, (uint64_t)3 * p.stream);
+    const uint64_t longest = p.owns ? 2 * p.tiles > p.stream ? p.stream + p.tiles : 0
+                                    : (uint64_t)p.tiles * p.cw / ((PA_LONG * 64 >> p.unit) + 1);
+    p.most = (uint32_t)max((uint64_t)p.stream, min(longest, (uint64_t)3 * p.stream));
     if (room < pieces(p.most)) p.most = p.stream;
     if (room < pieces(p.stream)) p.most = p.stream = room > p.tiles ? (uint32_t)min(room, 2 * (room - p.tiles)) : 0;
     p.pieces = p.stream ? (uint32_t)pieces(p.most) : 0;

@@ -27,7 +27,7 @@ namespace smq {
 constexpr int PA_WAVES = 4; /* of a workgroup */
 constexpr uint32_t PA_STEP = 32;      /* positions */
 constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps are dealt out */
-constexpr uint32_t PA_LONG = 64;      /* of a piece, where there are more pieces than CUs hold at once */
+constexpr uint32_t PA_LONG = 32;      /* of a piece, where there are more pieces than CUs hold at once */
 constexpr uint32_t PA_FIXED = 16;     /* steps that a tile costs beside its own */
 
 /* How a launch covers the rows: tiles of tile_rows rows of one sequence and KV head (`tiles`: as many as the batch can
@@ -289,7 +289,10 @@ struct Tiles {
      * batch holds all sequences. */
     __device__ __forceinline__ bool by_piece(uint32_t x, uint32_t units, uint32_t count, Tile &t) {
         const float all = (float)units, least = (float)(PA_MIN_STEPS * 64 >> p.unit) + 1.0f;
-        const uint32_t aim = min(max(units / ((PA_LONG * 64 >> p.unit) + 1), p.stream), p.most);
+        uint32_t aim = p.stream;
+        if (p.owns) aim += 2 * count > aim ? count : 0;
+        else aim *= max(units / ((PA_LONG * 64 >> p.unit) + 1) / aim, 1u);
+        aim = min(aim, p.most);
         const uint32_t cuts = max(aim > count ? aim - count : 0, (aim + 1) / 2);
         float hi = 1.0f / fmaxf(all / (float)cuts * 1.0001f, least); /* hi, lo: pieces per unit */
         if (a.seqs <= 64) {
