@@ -8,15 +8,20 @@
  *                 positions 8 (lane / 16) .. + 7 for row lane % 16, which is the B operand of
  *   O^T += V^T P^T  as it stands, no exchange between lanes: V^T is the A operand straight from the page, whose
  *                 values lie with positions innermost.
- * So neither product passes through LDS. One pass over the positions: the maximum m of a row is moved (and O and the sum
+ * So no score passes through LDS (keys and values do where waves own rows: InLds). One pass over the positions: the maximum m of a row is moved (and O and the sum
  * rescaled) only where a score exceeds it by 8, which costs a vote instead of a reduction across lanes in most steps;
  * the weights then reach 2^15, in f16's range, and what f16 subnormals drop is below 2^-32 of the row's largest weight.
  *
  * f32 accuracy on f16 MFMA: q (scaled by a power of two per row) and P are each two f16, value and remainder (22 bits);
  * f16 keys and values and Q8 codes are f16 exactly. Q8 key scales multiply the f32 product of their 32-wide block; value
  * scales multiply P before its split, divided by 2^E, E the exponent of the largest scale of the block so far (O is held
- * in units of 2^E). An f32 cache takes the f32 MFMA, a sixteenth of the rate: its steps are bound by that in chunks, by
- * memory while decoding. */
+ * in units of 2^E). An f32 cache takes the f32 MFMA, a sixteenth of the rate.
+ *
+ * What bounds it: chunks the matrix cores and the softmax's VALU beside them (f16 heads of 128 at 4096: 586 TFLOP/s of
+ * products without their remainders, twice that on the matrix cores; Q8 363, whose scales are VALU work; f32 127); decoding
+ * the bytes of the cache (16 f16 sequences at up to 16384, 815 MB: 154 us, 5.3 TB/s) once pieces are long, else the latency
+ * of a piece: batch, page ids, keys, products and the join one after another (32 Q8 sequences at up to 4090: 27 us for 58
+ * MB; one at 131: 8 us). */
 #ifndef SMQ_PAGED_ATTEND_H
 #define SMQ_PAGED_ATTEND_H
 
@@ -27,19 +32,20 @@ namespace smq {
 constexpr int PA_WAVES = 4; /* of a workgroup */
 constexpr uint32_t PA_STEP = 32;      /* positions */
 constexpr uint32_t PA_MIN_STEPS = 8;  /* of a workgroup, at least, where steps are dealt out */
-constexpr uint32_t PA_LONG = 32;      /* of a piece, where there are more pieces than CUs hold at once */
+constexpr uint32_t PA_LONG = 32;      /* of a piece, at least, where `stream` is exceeded */
 constexpr uint32_t PA_FIXED = 16;     /* steps that a tile costs beside its own */
 
 /* How a launch covers the rows: tiles of tile_rows rows of one sequence and KV head (`tiles`: as many as the batch can
  * need). owns: a wave owns 16 * RT of the tile's rows over all positions; else the tile has 16 rows and the waves share
  * the positions out.
  *
- * stream > 0: tiles are cut into pieces, each with a workgroup of its own, so that about `stream` of them per KV head cost
- * the same (up to `most`, of PA_LONG steps or more); k_paged_join joins a tile's. Lengths are known on the device only: each workgroup finds its piece there. A tile
- * counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the sequence: its steps nearly, with sums
- * that need no loop, and PA_FIXED for what it costs beside its steps (the batch looked at, queries, the first keys, the
- * join). With all tiles' units laid end to end and cut every `each` units, a tile has a piece for each part of it, and
- * these are made equal. There are at most `pieces` of them. stream 0 (no workspace): a workgroup per tile. */
+ * stream > 0: tiles are cut into pieces, each with a workgroup of its own, so that about `stream` of them per KV head (up
+ * to `most`: see by_piece) cost the same; k_paged_join joins a tile's. Lengths are known on the device only: each workgroup
+ * finds its piece there. A tile counts (c0 + c1 j, at most cw) units of 2^unit / 64 steps, j its number in the sequence:
+ * its steps nearly, with sums that need no loop, and PA_FIXED for what it costs beside its steps (the batch looked at,
+ * queries, the first keys, the join). A sequence's units laid end to end are cut into equal parts; a tile has a piece for
+ * each part that it meets, and these are made equal. There are at most `pieces` of them. stream 0 (no workspace, or nothing
+ * to gain): a workgroup per tile. */
 typedef int i4 __attribute__((ext_vector_type(4)));
 struct AttendPlan {
     bool owns;
@@ -283,10 +289,15 @@ struct Tiles {
     }
     /* The tile that piece x is of, of `units` / `count` in all. False behind the last.
      *
+     * aim: pieces at most. `stream` of them, two or three times as many where they stay long (decoding: uneven lengths
+     * even out; 24 f16 sequences at up to 4000, 8 KV heads of 128: 98 -> 70 us), or every tile's own beside these, where
+     * tiles fill half of the workgroups and equal shares would cut only some of them (4 chunks of 300 Q8 tokens at 2600, 8
+     * KV heads of 128: 263 -> 194 us).
+     *
      * Pieces of u units give units / u + tiles pieces at most: with u = units / (aim - tiles), the start of the search,
      * there are `aim` or fewer; half of aim at least is kept for cuts. Every sequence's last part is rounded up, so a
      * smaller u often has no more than aim either, down to units / aim: six halvings find it, where one look at the
-     * batch holds all sequences. */
+     * batch holds all sequences (16 f16 sequences at up to 16384: 215 -> 154 us). */
     __device__ __forceinline__ bool by_piece(uint32_t x, uint32_t units, uint32_t count, Tile &t) {
         const float all = (float)units, least = (float)(PA_MIN_STEPS * 64 >> p.unit) + 1.0f;
         uint32_t aim = p.stream;
