@@ -1454,8 +1454,11 @@ static bool paged_args(const smq_paged_batch *b, const smq_attn_shape *shape, co
                    shape->context, smq::MAX_PAGED_CONTEXT);
         return false;
     }
-    if (b->seqs > (1u << 20) || (uint64_t)b->tokens * shape->heads > (1u << 23) || (b->seqs && !b->table_stride) || b->table_stride > (1u << 20)) {
-        set_status(SMQ_ERR_RANGE, "%s: unsupported batch (%u sequences <= 2^20, %u tokens of %u heads <= 2^23, table stride %u of 1 .. 2^20)",
+    /* with these the largest grid (two workgroups per token and KV head and one per token) has less than 2^32 threads */
+    if (b->seqs > (1u << 20) || (uint64_t)b->tokens * shape->heads > (1u << 22) || (b->seqs && !b->table_stride) ||
+        b->table_stride > (1u << 20)) {
+        set_status(SMQ_ERR_RANGE,
+                   "%s: unsupported batch (%u sequences <= 2^20, %u tokens of %u heads <= 2^22, table stride %u of 1 .. 2^20)",
                    who, b->seqs, b->tokens, shape->heads, b->table_stride);
         return false;
     }
@@ -1501,6 +1504,10 @@ static bool paged_extents(const smq::PagedArgs &a, const char *who) {
     const size_t scales = a.type == SMQ_KV_Q8 ? positions * a.kv_heads * a.nb * 4 : 0;
     if (!a.pages) {
         set_status(SMQ_ERR_RANGE, "%s: a cache without pages", who);
+        return false;
+    }
+    if (positions > (size_t)-1 / 4 / kd) {
+        set_status(SMQ_ERR_RANGE, "%s: a cache of %u pages is past the address space", who, a.pages);
         return false;
     }
     if (((uintptr_t)a.keys | (uintptr_t)a.values | (scales ? (uintptr_t)a.ks | (uintptr_t)a.vs : 0)) & 15) {

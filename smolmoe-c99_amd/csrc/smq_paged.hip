@@ -51,10 +51,10 @@ __device__ __forceinline__ bool find_block(const PagedArgs &a, uint32_t x, Block
     }
     return false;
 }
-/* As many blocks as a batch can need. */
+/* As many blocks as a batch can need: n tokens touch (n - 1) / 32 + 2 at most, and n. */
 uint32_t most_blocks(const PagedArgs &a) {
-    const uint32_t seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
-    return a.tokens / ST_POS + 2 * seqs;
+    const uint64_t most = a.tokens / ST_POS + 2 * (uint64_t)a.seqs;
+    return most < a.tokens ? (uint32_t)most : a.tokens;
 }
 /* The block's page ids of 16 positions each, one per lane of 0 .. 1 (blocks of one page have the same one twice); -1, with
  * the flag, where a page that the block needs is none. */

@@ -248,12 +248,17 @@ struct Tiles {
         const uint32_t k = c1 ? min(j, (cw - c0 + c1 - 1) / c1) : j; /* those below cw */
         return k * c0 + (uint32_t)((uint64_t)k * (k - (k ? 1 : 0)) / 2 * c1) + (j - k) * cw;
     }
+    /* More tiles than a batch can have: its sequences overlap (begin does not ascend). None then, the units would not fit. */
     __device__ __forceinline__ void total(uint32_t &units, uint32_t &tiles) {
         units = tiles = 0;
         for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
             if (s0 != at) look(s0);
             units += lane_of(upto, 63);
             tiles += lane_of(tiles_upto, 63);
+            if (tiles > p.tiles) {
+                units = tiles = 0;
+                return;
+            }
         }
     }
     __device__ __forceinline__ void take(Tile &t, int w, uint32_t tiles_before) {
@@ -471,7 +476,7 @@ struct Rows {
             first[c] = a.window ? min(a.sinks, (uint32_t)(pc + 1)) : 0;
             lo = min(lo, pc);
             hi = max(hi, pc);
-            row[c] = in ? (int)(((uint32_t)sq.begin + tok) * a.heads + kh * G + g) : -1; /* below 2^23 */
+            row[c] = in ? (int)(((uint32_t)sq.begin + tok) * a.heads + kh * G + g) : -1; /* below 2^22 */
         }
 #pragma unroll
         for (int off = 1; off < 16; off *= 2) {
@@ -1165,7 +1170,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
             tiles.total(units, count);
             if (i == 0) /* tiles that the batch does not need */
                 for (uint32_t x = count + threadIdx.x; x < p.tiles; x += 64 * PA_WAVES) used[(size_t)x * a.kv_heads + kh] = i4{};
-            if (!tiles.by_piece(p.pieces - 1 - i, units, count, t)) return;
+            if (!count || !tiles.by_piece(p.pieces - 1 - i, units, count, t)) return;
         }
     }
     tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, lds);

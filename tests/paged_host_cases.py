@@ -116,6 +116,17 @@ def shapes():
             refused(f, words="unsupported batch")
     p.kv.pages = 0xFFFFFFFF
     refused(p.attend, words="unsupported cache")
+    # as many tokens times heads as fit, one more, and pools past the address space
+    p = Paged()
+    p.batch.tokens = (1 << 20) + 1
+    for f in (p.store, p.read, p.attend):
+        refused(f, words="unsupported batch")
+    p.batch.tokens = 1 << 20
+    refused(p.attend, words="q")
+    p = Paged(heads=65535, kv=65535, hd=256, pairs=0, type=0, page=16, pages=1, seqs=1, tokens=1, stride=1, context=16)
+    p.kv.pages, p.kv.page_size = 0x7FFFFFFF, 256
+    for f in (p.store, p.read, p.attend):
+        refused(f, words="past the address space")
 
 
 def buffers():

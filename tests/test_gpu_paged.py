@@ -340,6 +340,27 @@ def test_begins_that_do_not_ascend():
         assert np.isfinite(got).all() and flagged()
 
 
+def test_sequences_that_overlap():
+    """Sequences of the same rows, many more tiles than the batch's tokens can have, where tiles are cut: flagged, results
+    finite, rows behind left as they were, and the next call with the same workspace is right."""
+    heads, kv, hd, seqs = 4, 2, 64, 12
+    cache = Cache(F16, kv, hd, 64, [1300] * seqs).upload()
+    q = synth.normal(97, 6 * heads * hd).reshape(-1, heads, hd)
+    batch = Batch(cache, [1] * 6 + [0] * (seqs - 6))
+    assert smq.paged_attention_workspace(batch.desc, smq.attn_shape(heads, kv, hd, 0, 0, 1300)) > 0
+    want, tol = attend64(cache, batch, q, heads)
+    close(attend(cache, batch, q, heads, kv, hd), want, tol)
+    good = batch.begin.copy()
+    batch.bb.upload(np.array([0, 6] * (seqs // 2) + [0], np.int32))
+    assert np.isfinite(attend(cache, batch, q, heads, kv, hd)).all() and flagged()
+    z = dev(np.zeros(6 * kv * hd, np.float32))
+    smq.paged_read(batch.desc, smq.attn_shape(heads, kv, hd, 0, 0, 1300), cache.desc, z, z)
+    assert flagged()
+    batch.bb.upload(np.asarray(good, np.int32))
+    close(attend(cache, batch, q, heads, kv, hd), want, tol)
+    assert not flagged()
+
+
 @pytest.mark.parametrize("kv_type", [F32, F16, Q8])
 def test_replays(kv_type):
     """A captured decode step (store, attention) replayed at successive positions beside eager work, two graphs with
