@@ -377,12 +377,9 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
     *(f4u *)(att + row_at(a, u[1], kh, (uint32_t)u[2] + r) + d) = o * inv;
 }
 
-/* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own
- * theirs.
- *
- * Pieces that the tiles are cut into: two a CU for products and for decoding heads of up to 64 (8 KiB of f16 a step and
- * wave), one a CU for wider ones (one f16 sequence at 16384, 8 KV heads of 128: 22 us, two a CU 25); by_piece has what
- * becomes of these numbers.
+/* The pieces that tiles of so many rows are cut into: two a CU for products and for decoding heads of up to 64 (8 KiB of f16
+ * a step and wave), one a CU for wider ones (one f16 sequence at 16384, 8 KV heads of 128: 22 us, two a CU 25); by_piece has
+ * what becomes of these numbers.
  *
  * Cutting costs partial results and a second launch, which joins them. No cuts
  * - where the longest tile exceeds an equal share by about 24 steps or less (64 sequences at 700, 2 KV heads of 64: 11.8 us
@@ -390,12 +387,12 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
  * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
  *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
  *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). */
-AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
+AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
     AttendPlan p;
     const uint32_t G = a.heads / a.kv_heads;
     const uint64_t rows = (uint64_t)a.tokens * G, seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
-    p.owns = rows > 32 * seqs;
-    p.tile_rows = p.owns ? 64 * attend_rt(attend_ks(a.head_dim)) : 16;
+    p.owns = tile_rows > 16;
+    p.tile_rows = tile_rows;
     p.row_shift = p.tile_rows == 128 ? 7 : p.tile_rows == 64 ? 6 : 4;
     p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) >> p.row_shift);
     const uint32_t groups = p.owns || a.head_dim <= 64 ? 512 : 256;
@@ -431,6 +428,18 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
     if (room < pieces(p.stream)) p.most = p.stream = room > p.tiles ? (uint32_t)min(room, 2 * (room - p.tiles)) : 0;
     p.pieces = p.stream ? (uint32_t)pieces(p.most) : 0;
     return p;
+}
+
+/* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own theirs,
+ * 16 or 32 each. 32 where tiles are cut or many: a fragment read serves twice. Few whole tiles take as long as the longest
+ * one's chain of steps, and a step of half the rows is shorter (2048 tokens from an empty cache, f16, 8 KV heads of 64: 71
+ * us, 58; 1024 of 128: 51, 40; but 2048 of 128: 100, 104). */
+AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
+    const uint32_t ks = attend_ks(a.head_dim);
+    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
+    if (rows <= 32 * seqs) return plan_tiles(a, ws_bytes, 16);
+    const AttendPlan p = plan_tiles(a, ws_bytes, 64 * attend_rt(ks));
+    return p.stream || p.tile_rows == 64 || rows / 128 * a.kv_heads * ks >= 2048 ? p : plan_tiles(a, 0, 64);
 }
 
 }  // namespace

@@ -63,7 +63,7 @@ template <uint32_t TYPE>
 hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
                          hipStream_t s);
 
-/* RT of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles and two
+/* RT, at most, of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles and two
  * waves: each fragment read from LDS serves twice, the registers hold without spills, one wave's softmax runs beside the
  * other's products. Useful rate over 64 sequences of 128 tokens at 4096, 32 heads on 8 (RT 1 / 2 / 3 or 4): f16 heads of
  * 64 403 / 445 / 409 TFLOP/s, of 128 488 / 586 / 215; Q8 252 / 298 / 301, 301 / 363 / 195; f32 123 / 129 / 115, 99 / 127 /
@@ -1187,9 +1187,12 @@ hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q
                        part)
 #define SMQ_ATTEND(KS)                                                            \
     do {                                                                          \
-        constexpr int RT = attend_rt(KS);                                   \
-        if (p.owns && a.shift > 4) SMQ_ATTEND3(KS, RT, true, false);              \
-        else if (p.owns) SMQ_ATTEND3(KS, RT, true, true);                         \
+        constexpr int RT = attend_rt(KS);                                         \
+        const bool most = p.tile_rows == 64 * RT; /* else 64 */                   \
+        if (p.owns && most && a.shift > 4) SMQ_ATTEND3(KS, RT, true, false);      \
+        else if (p.owns && most) SMQ_ATTEND3(KS, RT, true, true);                 \
+        else if (p.owns && a.shift > 4) SMQ_ATTEND3(KS, 1, true, false);          \
+        else if (p.owns) SMQ_ATTEND3(KS, 1, true, true);                          \
         else if (a.shift > 4) SMQ_ATTEND3(KS, 1, false, false);                   \
         else SMQ_ATTEND3(KS, 1, false, true);                                     \
     } while (0)

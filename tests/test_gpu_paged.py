@@ -225,6 +225,28 @@ def test_attention_long(kv_type, lengths, new):
     smq.numeric_check()
 
 
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+def test_attention_of_many(kv_type):
+    """More sequences than a wave has lanes, cut into pieces; then so many tiles of chunks that none is."""
+    heads, kv, hd = 2, 1, 64
+    lengths = [1500, 1, 33] + [1300 + 3 * s for s in range(66)]
+    cache = Cache(kv_type, kv, hd, 64, lengths, stale="nan").upload()
+    batch = Batch(cache, [1, 0] + [1] * 67)
+    assert smq.paged_attention_workspace(batch.desc, smq.attn_shape(heads, kv, hd, 0, 0, 1500)) > 0
+    q = synth.normal(98, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    want, tol = attend64(cache, batch, q, heads)
+    close(attend(cache, batch, q, heads, kv, hd), want, tol)
+    heads, kv, hd = 32, 8, 128
+    lengths = [64 + s % 7 for s in range(34)]
+    cache = Cache(kv_type, kv, hd, 32, lengths, stale="nan").upload()
+    batch = Batch(cache, [64 - s % 5 for s in range(34)])
+    assert batch.tokens >= 2048  # 512 tiles of 128 rows of four 32-wide steps
+    q = synth.normal(99, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    want, tol = attend64(cache, batch, q, heads)
+    close(attend(cache, batch, q, heads, kv, hd), want, tol)
+    smq.numeric_check()
+
+
 def test_scores_of_every_size():
     """Rows whose softmax is one position, whose scores are all equal, tiny or past f16's range."""
     heads, kv, hd, n = 4, 2, 64, 90
