@@ -396,7 +396,10 @@ typedef struct smq_paged_kv {
  * shape->context or past the table (not stored, not read, its attention is
  * 0), a begin that does not ascend within 0 .. tokens (which rows are computed
  * is then unspecified). Rows in such pages are not stored and not read,
- * positions in them not seen. */
+ * positions in them not seen.
+ *
+ * Refused: more than 1,048,576 sequences or pages of a sequence, and tokens
+ * times shape->heads above 4,194,304. */
 typedef struct smq_paged_batch {
     const int32_t *begin;  /* device, seqs + 1 */
     const int32_t *length; /* device, seqs: positions including the new tokens */
@@ -426,8 +429,9 @@ smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *sh
  * shape->window w > 0 only those with j > p - w or j < sinks:
  *   att[h] = sum_j softmax_j(q[h] . k[j] / sqrt(head_dim)) v[j]
  * (KV head h / (heads / kv_heads)); f32 sums and statistics, each product of
- * f32 accuracy, no order of the sums promised beyond: the same call gives the
- * same bits. A row that sees nothing is 0. Keys and values at positions that a
+ * f32 accuracy (a Q8 value whose scale is far below the largest one of its 32
+ * dims so far is rounded relative to that one), no order of the sums promised
+ * beyond: the same call gives the same bits. A row that sees nothing is 0. Keys and values at positions that a
  * row does not see, and slots past a sequence's length, never matter, NaN and
  * infinities included; a visible one that is not finite leaves the row's result
  * unspecified. Pages that no row sees may have any id. att must not overlap q.
@@ -494,7 +498,10 @@ void smq_dequantize_q5_row(const unsigned char *w, uint32_t cols, float *out);
  * Work enqueued on the library stream between smq_capture_begin and
  * smq_capture_end is recorded, not run, and replayed by smq_graph_launch
  * (a HIP graph). Only asynchronous entry points may be captured: smq_gemm_*,
- * smq_dot_*_x4/_r4, smq_matmul, smq_quantize_q8_rows, smq_dequantize_*. */
+ * smq_dot_*_x4/_r4, smq_matmul, smq_quantize_q8_rows, smq_dequantize_*, the
+ * paged cache's and smq_logits_adjust (batches and rules are read on the
+ * device at each replay; what the host passed, tokens and context among it,
+ * stays). */
 smq_status smq_capture_begin(void);
 void *smq_capture_end(void);
 smq_status smq_graph_launch(void *graph);
