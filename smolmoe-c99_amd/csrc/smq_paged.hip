@@ -284,8 +284,24 @@ __global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, 
     if (!find_block(a, blockIdx.x / a.kv_heads, b)) return;
     int page[2];
     block_pages(a, b, page);
-    const uint32_t base = b.p0 / ST_POS * ST_POS;
-    auto page_at = [&](uint32_t pos) { return pos >= b.p0 && pos < b.p1 ? (pos & 16 ? page[1] : page[0]) : -1; };
+    const uint32_t base = b.p0 / ST_POS * ST_POS, first = base & (P - 1);
+    const float inv = 1.0f / (float)q;
+    auto row_of = [&](uint32_t i) { return (uint32_t)(((float)i + 0.5f) * inv); }; /* i / q: i is below 2^12, where this is exact */
+    auto holds = [&](uint32_t j) { return base + j >= b.p0 && base + j < b.p1 && page[j >> 4] >= 0; };
+    /* the block's two halves, from position 0 of the page on; in one page the second begins where the first ends */
+    const unsigned char *kp[2], *vp[2];
+    const float *kw[2], *vw[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int pg = max(page[x], 0);
+        const uint32_t slot = (first + 16 * x & (P - 1)) - 16 * x; /* of the half's position j, less j */
+        kp[x] = (const unsigned char *)a.keys + (head_at(a, pg, h) + (ptrdiff_t)(int)slot * hd) * EB;
+        vp[x] = (const unsigned char *)a.values + (head_at(a, pg, h) + (ptrdiff_t)(int)slot) * EB;
+        kw[x] = a.ks + scales_at(a, pg, h) + (ptrdiff_t)(int)slot;
+        vw[x] = a.vs + scales_at(a, pg, h) + (ptrdiff_t)(int)slot;
+    }
+    const ptrdiff_t row0 = ((ptrdiff_t)(b.row + (int)base) * a.kv_heads + h) * hd;
+    const uint32_t step = a.kv_heads * hd; /* of the rows */
     for (uint32_t i0 = tid; i0 < hd * (ST_POS / 4); i0 += RD_PASSES * ST_WG) {
         T tv[RD_PASSES], tk[RD_PASSES];
         f4 wv[RD_PASSES];
@@ -294,44 +310,39 @@ __global__ __launch_bounds__(ST_WG) void k_paged_read(PagedArgs a, float *keys, 
         for (uint32_t u = 0; u < RD_PASSES; ++u) {
             const uint32_t i = i0 + u * ST_WG;
             if (i >= hd * (ST_POS / 4)) continue;
-            const uint32_t dv = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4)), sv = (base + j) & (P - 1);
-            const int pv = j & 16 ? page[1] : page[0];
-            if (pv >= 0) {
-                tv[u] = *(const T *)((const unsigned char *)a.values + (head_at(a, pv, h) + ((size_t)dv << a.shift) + sv) * EB);
-                if constexpr (TYPE == 2) wv[u] = *(const f4 *)(a.vs + scales_at(a, pv, h) + ((size_t)(dv / 32) << a.shift) + sv);
+            const uint32_t dv = i / (ST_POS / 4), jv = 4 * (i % (ST_POS / 4)), jk = row_of(i), dk = 4 * (i - jk * q);
+            if (page[jv >> 4] >= 0) {
+                tv[u] = *(const T *)(vp[jv >> 4] + ((dv << a.shift) + jv) * EB);
+                if constexpr (TYPE == 2) wv[u] = *(const f4 *)(vw[jv >> 4] + (dv / 32 << a.shift) + jv);
             }
-            const uint32_t pos = base + i / q, dk = 4 * (i % q), sk = pos & (P - 1);
-            const int pk = page_at(pos);
-            if (pk >= 0) {
-                tk[u] = *(const T *)((const unsigned char *)a.keys + (head_at(a, pk, h) + (size_t)sk * hd + dk) * EB);
-                if constexpr (TYPE == 2) wk[u] = a.ks[scales_at(a, pk, h) + ((size_t)(dk / 32) << a.shift) + sk];
+            if (holds(jk)) {
+                tk[u] = *(const T *)(kp[jk >> 4] + (jk * hd + dk) * EB);
+                if constexpr (TYPE == 2) wk[u] = kw[jk >> 4][(dk / 32 << a.shift) + jk];
             }
         }
 #pragma unroll
         for (uint32_t u = 0; u < RD_PASSES; ++u) {
             const uint32_t i = i0 + u * ST_WG;
             if (i >= hd * (ST_POS / 4)) continue;
-            const uint32_t dv = i / (ST_POS / 4), j = 4 * (i % (ST_POS / 4));
-            if ((j & 16 ? page[1] : page[0]) >= 0) {
+            const uint32_t dv = i / (ST_POS / 4), jv = 4 * (i % (ST_POS / 4)), jk = row_of(i), dk = 4 * (i - jk * q);
+            if (page[jv >> 4] >= 0) {
                 f4 y = decode<TYPE>(tv[u]);
                 if constexpr (TYPE == 2) y *= wv[u];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) turn[(j + e) * (hd + 4) + dv] = y[e];
+                for (uint32_t e = 0; e < 4; ++e) turn[(jv + e) * (hd + 4) + dv] = y[e];
             }
-            const uint32_t pos = base + i / q, dk = 4 * (i % q);
-            if (page_at(pos) >= 0) {
+            if (holds(jk)) {
                 f4 y = decode<TYPE>(tk[u]);
                 if constexpr (TYPE == 2) y *= wk[u];
-                __builtin_nontemporal_store(y, (f4u *)(keys + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + dk));
+                __builtin_nontemporal_store(y, (f4u *)(keys + row0 + (ptrdiff_t)(jk * step + dk)));
             }
         }
     }
     __syncthreads();
     for (uint32_t i = tid; i < hd * (ST_POS / 4); i += ST_WG) {
-        const uint32_t pos = base + i / q, d = 4 * (i % q);
-        if (page_at(pos) >= 0)
-            __builtin_nontemporal_store(*(const f4 *)&turn[(pos - base) * (hd + 4) + d],
-                                        (f4u *)(values + ((size_t)(b.row + (int)pos) * a.kv_heads + h) * hd + d));
+        const uint32_t j = row_of(i), d = 4 * (i - j * q);
+        if (holds(j))
+            __builtin_nontemporal_store(*(const f4 *)&turn[j * (hd + 4) + d], (f4u *)(values + row0 + (ptrdiff_t)(j * step + d)));
     }
 }
 
