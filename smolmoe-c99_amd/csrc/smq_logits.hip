@@ -57,8 +57,8 @@ __device__ __forceinline__ void list_range(const int32_t *begin, uint32_t r, uin
  * integers (no order); the thread that counts an id first puts it on a list, and the ids of the list, few, are adjusted by
  * a thread each: in the pass over all ids some lane of almost every wave would divide.
  *
- * Bound by bytes for many rows: 64 of 151936, 79 MB, 31 us, 2.5 TB/s; the rest is the history, which every span's
- * workgroup counts (2000 entries), and the second launch (4 us). One row: 9 us, two launches. */
+ * 64 rows of 151936, 79 MB, 31 us, 2.5 TB/s with the second launch (4 us): bound by the latency of these trips in three
+ * rounds of workgroups; histories of 2000, biases and masks are 4 us of it. One row: 9 us, two launches. */
 template <uint32_t SPAN, bool WIDE>
 __global__ __launch_bounds__(LG_WG) void k_logits(LogitArgs a, Part *parts) {
     constexpr uint32_t U = SPAN / (4 * LG_WG), AHEAD = 2;

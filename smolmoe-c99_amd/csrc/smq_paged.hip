@@ -269,7 +269,7 @@ __device__ __forceinline__ f4 decode(typename Four<TYPE>::T t) {
  * have four: all at once took 182 us below, one after another 145). The results are stored past the caches, which they
  * would fill: the pages stay there.
  *
- * Bound by bytes: 8 Q8 sequences at up to 8100, 8 KV heads of 128, 553 MB, 142 us, 3.9 TB/s, where a large copy reaches 4.9;
+ * Bound by bytes: 8 Q8 sequences at up to 8100, 8 KV heads of 128, 553 MB, 140 us, 3.9 TB/s, where a large copy reaches 4.9;
  * a fifth of it is read and the rest written. A wave per position: 370 us. */
 constexpr uint32_t RD_PASSES = 2;
 template <uint32_t TYPE>

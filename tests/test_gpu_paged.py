@@ -247,6 +247,24 @@ def test_attention_of_many(kv_type):
     smq.numeric_check()
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 1, 400]])
+def test_the_longest_context(new):
+    """Tables and a context of 1,048,576 positions, lengths far below: the host plans for the first, the device cuts the
+    second. With windows, whose steps are few, too."""
+    heads, kv, hd = 6, 2, 64
+    cache = Cache(F16, kv, hd, 64, [3001, 1, 700], stale="nan", stride=1 << 14).upload()
+    batch = Batch(cache, new, padding=3)
+    q = synth.normal(100, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    n = int(batch.begin[-1])
+    for window, sinks in ((0, 0), (129, 5), (0xFFFFFFFF, 0xFFFFFFFF)):
+        want, tol = attend64(cache, batch, q, heads, window if window < 1 << 20 else 0, sinks if window < 1 << 20 else 0)
+        for split in (True, False):
+            got = attend(cache, batch, q, heads, kv, hd, window, sinks, context=1 << 20, split=split)
+            close(got, want, tol, slice(0, n))
+            assert (got[n:] == 9.0).all()
+    smq.numeric_check()
+
+
 def test_scores_of_every_size():
     """Rows whose softmax is one position, whose scores are all equal, tiny or past f16's range."""
     heads, kv, hd, n = 4, 2, 64, 90
