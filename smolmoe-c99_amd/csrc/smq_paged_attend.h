@@ -717,7 +717,9 @@ struct Rows {
             if (__any(up)) {
 #pragma unroll
                 for (int b = 0; b < KS; ++b) {
-                    const int e = max(-100, __builtin_amdgcn_frexp_expf(wave_max_quads(mx[b])));
+                    const float top = wave_max_quads(mx[b]);
+                    if (!(top > 0.0f)) continue; /* zeros: E stays, whichever block asked */
+                    const int e = max(-100, __builtin_amdgcn_frexp_expf(top));
                     const float n = fminf(__builtin_ldexpf(1.0f, -e), inv_e[b]), r = n / inv_e[b]; /* a power of two <= 1 */
                     inv_e[b] = n;
 #pragma unroll

@@ -568,3 +568,40 @@ def test_serving_together():
             assert token.download(np.uint32)[s] == pick
             history[s].append(pick)
     smq.numeric_check()
+
+
+def rows_in_bound(cache, new, heads, window=0, sinks=0, rows=None, padding=0, seed=110, size=1.0):
+    """Attention of the batch, cut into pieces and whole, within attend64's own bound in the rows of a mask (all)."""
+    batch = Batch(cache, new, padding=padding)
+    q = synth.normal(seed, batch.tokens * heads * cache.hd, size).reshape(-1, heads, cache.hd)
+    want, tol = attend64(cache, batch, q, heads, window, sinks)
+    rows = slice(0, int(batch.begin[-1])) if rows is None else rows
+    for split in (True, False):
+        got = attend(cache, batch, q, heads, cache.kv, cache.hd, window, sinks, split=split)
+        close(got, want, tol, rows, f"split {split}")
+    return batch, got, want, tol
+
+
+Q8_FORMS = [  # heads, kv, hd, page, new of 200 positions
+    (8, 2, 64, 32, 1),       # decode
+    (4, 2, 96, 16, 3),
+    (8, 2, 128, 64, 150),    # rows owned by waves
+    (2, 2, 64, 16, 150),
+    (6, 1, 160, 64, 40),
+]
+
+
+@pytest.mark.parametrize("heads,kv,hd,page,new", Q8_FORMS)
+@pytest.mark.parametrize("scale", [1e-6, 1e-8, 1e-10, 1e-20])
+def test_q8_values_after_a_block_of_zeros(heads, kv, hd, page, new, scale):
+    """A step whose values are all zero in one block of 32 dims says nothing of that block's size: neither before its first
+    values nor between them, while the other blocks have ordinary ones."""
+    say("q8 zeros", heads, kv, hd, page, new, scale)
+    for zeros in (slice(0, 32), slice(0, 64), slice(64, 96)):
+        cache = Cache(Q8, kv, hd, page, [200], stale="nan")
+        pg, sl = cache.slots(0, np.arange(200))
+        cache.vs[pg, :, 1, sl] *= np.float32(scale)
+        pg, sl = cache.slots(0, np.arange(200)[zeros])
+        cache.vs[pg, :, 1, sl] = 0.0
+        rows_in_bound(cache.upload(), [new], heads)
+    smq.numeric_check()
