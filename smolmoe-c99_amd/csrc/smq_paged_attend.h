@@ -14,8 +14,8 @@
  *
  * f32 accuracy on f16 MFMA: q (scaled by a power of two per row) and P are each two f16, value and remainder (22 bits);
  * f16 keys and values and Q8 codes are f16 exactly. Q8 key scales multiply the f32 product of their 32-wide block; value
- * scales multiply P before its split, divided by 2^E, E the exponent of the largest scale of the block so far (O is held
- * in units of 2^E). An f32 cache takes the f32 MFMA, a sixteenth of the rate.
+ * scales multiply P before its split, divided by 2^E, E the exponent of the largest scale that the row has seen of the
+ * block (O is held in units of 2^E). An f32 cache takes the f32 MFMA, a sixteenth of the rate.
  *
  * What bounds it: chunks the matrix cores and the softmax's VALU beside them (f16 heads of 128 at 4096: 586 TFLOP/s of
  * products without their remainders, twice that on the matrix cores; Q8 363, whose scales are VALU work; f32 127); decoding
@@ -450,7 +450,8 @@ struct Rows {
     uint32_t low_last; /* where the last row's window begins */
     f4 o[RT][DT];
     float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
-    float inv_e[TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values */
+    float inv_e[RT][TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values, of this lane's columns */
+    bool alike = true;                   /* every lane's columns have the same E each */
 
     /* `count` rows of the sequence from row0 on; columns past them see what the first one sees and are not stored. First
      * what they see, then (queries) their values, so that loads of keys can run beside those. */
@@ -488,7 +489,9 @@ struct Rows {
         span = span_of(a, pmin, pmax);
         low_last = span_of(a, pmax, pmax).low;
 #pragma unroll
-        for (int b = 0; b < (TYPE == 2 ? KS : 1); ++b) inv_e[b] = __builtin_ldexpf(1.0f, 100);
+        for (int c = 0; c < RT; ++c)
+#pragma unroll
+            for (int b = 0; b < (TYPE == 2 ? KS : 1); ++b) inv_e[c][b] = __builtin_ldexpf(1.0f, 112);
     }
     __device__ __forceinline__ void queries(const float *q) {
         const uint32_t hd = a.head_dim;
@@ -667,8 +670,12 @@ struct Rows {
     }
 
     /* O += V^T P^T. In a step that not every row sees whole, a value that is not finite would reach rows that do not see
-     * it, as 0 times it: it counts as 0, and the sums of the rows that see it become NaN. Slots that no row sees hold
-     * anything; a Q8 scale there must not set E either. */
+     * it, as 0 times it: it counts as 0, and the sums of the rows that see it become NaN.
+     *
+     * Q8 scales belong to the weights: a row takes those that it sees, and E comes of them alone, so that no other position
+     * coarsens its weights (with one E for the wave, one of 1e6 times the size that only later rows saw left 1e-4). A
+     * column is a row, so E is a lane's own. Where all rows see the step and a lane's columns have the same E, the scales are
+     * divided by 2^E once for both (64 chunks of 128 tokens at 4096, 8 KV heads of 128: 1.23 ms; always apart 1.28). */
     template <typename Src>
     __device__ __forceinline__ void product(uint32_t p0, uint32_t ok, bool full, const Src &src, const float (&x)[RT][8]) {
         const bool have = ok >> (quad >> 1) & 1;
@@ -679,67 +686,79 @@ struct Rows {
                 w[b][0] = src.vscale(b, 0);
                 w[b][1] = src.vscale(b, 1);
             }
-            if (!full) {
-                float r = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t in = have && span.holds(p0 + quad * 8 + j) ? 0xffffffffu : 0u;
-#pragma unroll
-                    for (int b = 0; b < KS; ++b) {
-                        float &y = ((float *)&w[b][j >> 2])[j & 3];
-                        y = __uint_as_float(__float_as_uint(y) & in);
-                        r = __builtin_fmaf(y, 0.0f, r);
-                    }
-                }
-                if (__any(!(r == 0.0f))) {
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int b = 0; b < KS; ++b)
-                            if (odd(w[b][j >> 2][j & 3])) {
-                                w[b][j >> 2][j & 3] = 0.0f;
-                                bits |= 1u << j;
-                            }
-                    spoil(p0, bits);
-                }
-            }
-            float mx[KS];
-            bool up = false;
-#pragma unroll
-            for (int b = 0; b < KS; ++b) {
+            auto largest = [](const float(&y)[8]) {
                 float z[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z[j] = fabsf(w[b][j >> 2][j & 3]);
-                mx[b] = max8(z);
-                up = up || mx[b] * inv_e[b] > 1.0f;
+                for (int j = 0; j < 8; ++j) z[j] = fabsf(y[j]);
+                return max8(z);
+            };
+            /* of the scales what column c sees: elsewhere its weight is 0 */
+            auto seen = [&](int c, const float(&y)[8], float(&z)[8]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = x[c][j] > 0.0f ? y[j] : 0.0f;
+            };
+            typedef float(&F8)[8];
+            const bool same = RT == 1 || (full && alike); /* one set of scales in units of 2^E serves all columns */
+            if (RT == 1 && !full) {
+#pragma unroll
+                for (int b = 0; b < KS; ++b) seen(0, (F8)w[b], (F8)w[b]);
             }
-            if (__any(up)) {
+            float mx[RT][KS];
+            if (same) {
 #pragma unroll
                 for (int b = 0; b < KS; ++b) {
-                    const float top = wave_max_quads(mx[b]);
-                    if (!(top > 0.0f)) continue; /* zeros: E stays, whichever block asked */
-                    const int e = max(-100, __builtin_amdgcn_frexp_expf(top));
-                    const float n = fminf(__builtin_ldexpf(1.0f, -e), inv_e[b]), r = n / inv_e[b]; /* a power of two <= 1 */
-                    inv_e[b] = n;
+                    mx[0][b] = largest((F8)w[b]);
 #pragma unroll
-                    for (int c = 0; c < RT; ++c) {
+                    for (int c = 1; c < RT; ++c) mx[c][b] = mx[0][b];
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < RT; ++c)
+#pragma unroll
+                    for (int b = 0; b < KS; ++b) {
+                        float z[8];
+                        seen(c, (F8)w[b], z);
+                        mx[c][b] = largest(z);
+                    }
+            }
+            bool up = false;
+#pragma unroll
+            for (int c = 0; c < RT; ++c)
+#pragma unroll
+                for (int b = 0; b < KS; ++b) up = up || mx[c][b] * inv_e[c][b] > 1.0f;
+            if (__any(up)) {
+                bool other = false;
+#pragma unroll
+                for (int c = 0; c < RT; ++c)
+#pragma unroll
+                    for (int b = 0; b < KS; ++b) {
+                        const float top = wave_max_quads(mx[c][b]), old = inv_e[c][b];
+                        const int e = max(-112, __builtin_amdgcn_frexp_expf(top));
+                        /* zeros: E stays, whichever block asked */
+                        inv_e[c][b] = top > 0.0f ? fminf(__builtin_ldexpf(1.0f, -e), old) : old;
+                        const float r = __builtin_ldexpf(1.0f, __builtin_amdgcn_frexp_expf(inv_e[c][b]) -
+                                                                   __builtin_amdgcn_frexp_expf(old)); /* <= 1 */
                         o[c][2 * b] *= r;
                         o[c][2 * b + 1] *= r;
+                        other = other || inv_e[c][b] != inv_e[0][b];
                     }
-                }
+                alike = RT == 1 || !__any(other);
             }
 #pragma unroll
             for (int b = 0; b < KS; ++b) {
-                w[b][0] *= inv_e[b];
-                w[b][1] *= inv_e[b];
                 const h8 v0 = codes8(src.v(2 * b)), v1 = codes8(src.v(2 * b + 1));
+                float u[8]; /* the scales in units of 2^E */
 #pragma unroll
                 for (int c = 0; c < RT; ++c) {
+                    if (c == 0 || !same) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) u[j] = w[b][j >> 2][j & 3] * inv_e[c][b];
+                        if (!same) seen(c, u, u);
+                    }
                     float y[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        y[j] = x[c][j] * w[b][j >> 2][j & 3];
+                        y[j] = x[c][j] * u[j];
                         asm("" : "+v"(y[j])); /* rounded to f32, for both halves of the split */
                     }
                     h8 hi, lo;
@@ -802,7 +821,7 @@ struct Rows {
             if constexpr (TYPE == 2) {
 #pragma unroll
                 for (int b = 0; b < KS; ++b) {
-                    const float r = 1.0f / inv_e[b];
+                    const float r = 1.0f / inv_e[c][b];
                     o[c][2 * b] *= r;
                     o[c][2 * b + 1] *= r;
                 }

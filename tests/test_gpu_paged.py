@@ -6,6 +6,7 @@ import torch
 
 from checks import assert_same_f32, say
 from paged_ref import F16, F32, Q8, Batch, Cache, attend64, rotate, tables
+from paged_ref import visible
 from smq_pkg import smq, synth
 
 pytestmark = pytest.mark.gpu
@@ -604,4 +605,29 @@ def test_q8_values_after_a_block_of_zeros(heads, kv, hd, page, new, scale):
         pg, sl = cache.slots(0, np.arange(200)[zeros])
         cache.vs[pg, :, 1, sl] = 0.0
         rows_in_bound(cache.upload(), [new], heads)
+    smq.numeric_check()
+
+
+@pytest.mark.parametrize("heads,kv,hd,page,new", Q8_FORMS[2:] + [(16, 1, 32, 128, 2), (3, 1, 256, 32, 50)])
+@pytest.mark.parametrize("ratio", [1e6, 2.0 ** 40, 1e30, 3e38])
+def test_q8_scales_that_a_row_does_not_see(heads, kv, hd, page, new, ratio):
+    """Values of a chunk's last token, and of a position that the window has left, far larger than all others: the rows
+    that do not see them keep their own accuracy, and the rows that do are off by no more than the documented rounding."""
+    say("q8 unseen scales", heads, kv, hd, page, new, ratio)
+    n, first = 200, 200 - new
+    for window, sinks, large in ((0, 0, [n - 1]), (0, 0, [n - 2, n - 1]), (20, 0, [first - 10]), (20, 3, [first - 19, n - 1]),
+                                 (40, 2, [first - 5, first + new // 2])):
+        cache = Cache(Q8, kv, hd, page, [n], stale="nan")
+        pg, sl = cache.slots(0, large)
+        cache.vs[pg, 0, 1 % cache.nb, sl] = np.float32(min(ratio * 0.01, 3e38))
+        cache.upload()
+        pos = np.arange(first, n)
+        sees = np.array([np.isin(large, visible(p, window, sinks)).any() for p in pos])
+        batch, got, want, tol = rows_in_bound(cache, [new], heads, window, sinks, ~sees)
+        if ratio > 1e38:  # a code of 2 is past f32 there
+            continue
+        # half a step of f16's subnormals, 2^-25, per weight of at most twice the largest scale's power of two; 127 is the
+        # largest code but one, the row's largest weight at least 2^6
+        v = float(cache.vs[pg, 0, 1 % cache.nb, sl].max())
+        close(got, want, tol + n * 2.0 ** -25 * 2 * v * 128 / 2 ** 6, sees)
     smq.numeric_check()
