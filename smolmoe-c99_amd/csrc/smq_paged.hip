@@ -360,6 +360,7 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
     if (parts < 2 || r >= n || threadIdx.x / lanes >= per) return;
     const f2 *pml = (const f2 *)(part + (size_t)p.pieces * a.kv_heads * p.tile_rows * hd);
     float m = -FLT_MAX, l = 0.0f;
+    const float share = (float)(32 - __builtin_clz(parts)); /* of 2^-share each: their sum stays below the values */
     f4 o = {};
     for (uint32_t i0 = 0; i0 < parts; i0 += JOIN_AT_ONCE) {
         f2 ml[JOIN_AT_ONCE];
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
         m = top;
 #pragma unroll
         for (uint32_t i = 0; i < JOIN_AT_ONCE; ++i) {
-            const float e = i0 + i < parts ? __builtin_amdgcn_exp2f(ml[i][0] - m) : 0.0f;
+            const float e = i0 + i < parts ? __builtin_amdgcn_exp2f(ml[i][0] - m - share) : 0.0f;
             l += e * ml[i][1];
             o += e * x[i];
         }

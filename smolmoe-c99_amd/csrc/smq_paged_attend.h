@@ -4,7 +4,7 @@
  * A wave takes 16 rows (RT times 16 where it owns rows) as the columns of its products and 32 positions a step:
  *   S^T = K Q^T   two 16 x 16 tiles of positions x rows, K as the A operand straight from the page (its rows are
  *                 positions), position 8 u + i of the step in tile i / 4, row 4 u + i % 4;
- *   P   = 2^(S' - m + 7), S' the score in units of log2 e: by this order a lane holds the scores of 8 consecutive
+ *   P   = 2^(S' - m + 7) (f32 caches: Rows::lift), S' the score in units of log2 e: by this order a lane holds the scores of 8 consecutive
  *                 positions 8 (lane / 16) .. + 7 for row lane % 16, which is the B operand of
  *   O^T += V^T P^T  as it stands, no exchange between lanes: V^T is the A operand straight from the page, whose
  *                 values lie with positions innermost.
@@ -448,6 +448,11 @@ struct Rows {
     int pmin;
     Span span;
     uint32_t low_last; /* where the last row's window begins */
+    /* Weights are 2^(S' - m + lift), and m moves where a score exceeds it by more than SLACK. An f32 cache needs no f16
+     * range: there a row's weights, one for each position up to the wave's last, sum to less than 1, so that O stays below
+     * the values (with weights of 2^15 those of 5e36 made it infinite). The same in every piece: one join takes them. */
+    static constexpr float SLACK = TYPE == 0 ? 0.0f : 8.0f;
+    float lift;
     f4 o[RT][DT];
     float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
     float inv_e[RT][TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values, of this lane's columns */
@@ -488,6 +493,7 @@ struct Rows {
         const int pmax = __builtin_amdgcn_readfirstlane(hi);
         span = span_of(a, pmin, pmax);
         low_last = span_of(a, pmax, pmax).low;
+        lift = TYPE == 0 ? (float)(pmax > 0 ? __builtin_clz((uint32_t)pmax) - 33 : -1) : 7.0f;
 #pragma unroll
         for (int c = 0; c < RT; ++c)
 #pragma unroll
@@ -595,7 +601,7 @@ struct Rows {
         }
     }
 
-    /* Products to weights 2^(S' - m + 7), and their sums. */
+    /* Products to weights, and their sums. */
     __device__ __forceinline__ void weights(uint32_t p0, uint32_t ok, bool full, float (&x)[RT][8]) {
         if (!full) {
             /* positions of a page that is none: past every row */
@@ -610,12 +616,12 @@ struct Rows {
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
             mx[c] = max8(x[c]) * factor[c];
-            up = up || mx[c] > m[c] + 8.0f;
+            up = up || mx[c] > m[c] + SLACK;
         }
         if (__any(up)) {
 #pragma unroll
             for (int c = 0; c < RT; ++c) {
-                /* a whole number: 7 - m and the rescaling are exact */
+                /* a whole number: lift - m and the rescaling are exact */
                 const float n = fmaxf(m[c], ceilf(wave_max_quads(mx[c]))), alpha = __builtin_amdgcn_exp2f(m[c] - n);
                 m[c] = n;
                 l[c] *= alpha;
@@ -625,7 +631,7 @@ struct Rows {
         }
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
-            const float off = 7.0f - m[c];
+            const float off = lift - m[c];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 x[c][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j], factor[c], off));
@@ -813,17 +819,21 @@ struct Rows {
         }
     }
 
-    /* O in units of 1 and the sum over the lanes of a column. */
+    /* O in units of 1 and the sum over the lanes of a column; both times the power of two that brings the sum into
+     * [1/2, 1), with m for it, so that O is no larger than the values (f16 ones cannot leave f32's range). */
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
             l[c] = wave_sum_quads(l[c]);
-            if constexpr (TYPE == 2) {
+            if constexpr (TYPE != 1) {
+                const int k = __builtin_amdgcn_frexp_expf(l[c]); /* 0 where the sum is 0 */
+                l[c] = __builtin_ldexpf(l[c], -k);
+                m[c] += (float)k;
 #pragma unroll
-                for (int b = 0; b < KS; ++b) {
-                    const float r = 1.0f / inv_e[c][b];
-                    o[c][2 * b] *= r;
-                    o[c][2 * b + 1] *= r;
+                for (int t = 0; t < DT; ++t) {
+                    const int e = TYPE == 2 ? 1 - __builtin_amdgcn_frexp_expf(inv_e[c][TYPE == 2 ? t / 2 : 0]) : 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[c][t][j] = __builtin_ldexpf(o[c][t][j], e - k);
                 }
             }
         }
@@ -1075,6 +1085,7 @@ __device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, 
         float m = sml[0][r][0], l = 0.0f;
 #pragma unroll
         for (int x = 1; x < PA_WAVES; ++x) m = fmaxf(m, sml[x][r][0]);
+        m += 2.0f; /* a quarter of each of the four: O stays below the values, however large */
         f4 o = {};
 #pragma unroll
         for (int x = 0; x < PA_WAVES; ++x) {

@@ -631,3 +631,43 @@ def test_q8_scales_that_a_row_does_not_see(heads, kv, hd, page, new, ratio):
         v = float(cache.vs[pg, 0, 1 % cache.nb, sl].max())
         close(got, want, tol + n * 2.0 ** -25 * 2 * v * 128 / 2 ** 6, sees)
     smq.numeric_check()
+
+
+LARGE = [  # heads, kv, hd, page, lengths, new, window, sinks
+    (4, 2, 64, 32, [1, 2, 40], [1, 1, 1], 0, 0),
+    (8, 2, 64, 64, [5000, 3001, 64], [1, 1, 1], 0, 0),       # cut into pieces
+    (4, 2, 128, 16, [150], [150], 0, 0),                     # rows owned by waves
+    (4, 1, 48, 64, [1500, 90], [1, 90], 33, 2),
+    (2, 1, 256, 32, [100], [60], 0, 0),
+]
+
+
+@pytest.mark.parametrize("kv_type", [F32, Q8])
+@pytest.mark.parametrize("size", [3e38, 1e36, 1e33, 1e-30])
+@pytest.mark.parametrize("heads,kv,hd,page,lengths,new,window,sinks", LARGE)
+def test_values_near_the_ends_of_f32(kv_type, size, heads, kv, hd, page, lengths, new, window, sinks):
+    """Finite values give finite results: averages of values up to f32's largest, and of tiny ones."""
+    say("paged values", TYPES[kv_type], size, heads, kv, hd, page, lengths, new, window, sinks)
+    cache = Cache(kv_type, kv, hd, page, lengths, stale=None)
+    rng = np.random.default_rng(7)
+    if kv_type == Q8:
+        cache.v = np.clip(cache.v, -127, 127)
+        cache.vs = (size / 127 * rng.uniform(0.25, 1, cache.vs.shape)).astype(np.float32)
+    else:
+        cache.v = (size * rng.uniform(-1, 1, cache.v.shape)).astype(np.float32)
+    rows_in_bound(cache.upload(), new, heads, window, sinks, seed=111, size=0.3)
+    smq.numeric_check()
+
+
+@pytest.mark.parametrize("kv_type", [F32, Q8])
+def test_values_of_one_sign_near_the_largest(kv_type):
+    """All values alike: the average is the value, however many positions and pieces."""
+    heads, kv, hd = 8, 2, 64
+    for lengths, new in (([4000, 1, 130], [1, 1, 1]), ([300], [150])):
+        cache = Cache(kv_type, kv, hd, 64, lengths, stale=None)
+        if kv_type == Q8:
+            cache.v[:] = 127
+            cache.vs[:] = np.float32(3.3e38 / 127)
+        else:
+            cache.v[:] = np.float32(-3.3e38)
+        rows_in_bound(cache.upload(), new, heads, seed=112, size=0.3)
