@@ -437,11 +437,12 @@ smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *sh
  * a visible one that is not finite leaves the row's result unspecified. Pages that no row sees may have any id. att must not overlap q.
  * workspace (device, 16-byte aligned, may be NULL): where the call splits long
  * sequences over workgroups, their partial results;
- * smq_paged_attention_workspace gives the bytes that allow the widest split,
- * fewer bytes split less. Whether to split at all the host decides by
- * shape->context (and the table's width): a value near the longest length
- * saves short batches a launch. Calls that may overlap in time, replays of different
- * graphs among them, must not share one. Asynchronous, capturable. */
+ * smq_paged_attention_workspace gives the bytes that allow the widest split
+ * with any number of sinks, fewer bytes split less. Whether to split at all the
+ * host decides by shape->context, the table's width, the window and the sinks: a
+ * context near the longest length saves short batches a launch. Calls that may
+ * overlap in time, replays of different graphs among them, must not share one.
+ * Asynchronous, capturable. */
 size_t smq_paged_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape);
 smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                uint32_t sinks, const smq_paged_kv *kv, void *workspace, size_t workspace_bytes);

@@ -434,7 +434,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
     const uint64_t room = ws_bytes > used ? (ws_bytes - used) / each : 0;
     auto pieces = [&](uint64_t aim) { return max(aim, (aim + 1) / 2 + p.tiles); }; /* at most: see by_piece */
     const uint64_t longest = p.owns ? 2 * p.tiles > p.stream ? p.stream + p.tiles : 0
-                                    : (uint64_t)p.tiles * p.cw / ((PA_LONG * 64 >> p.unit) + 1);
+                                    : p.tiles * most / (PA_LONG * 64); /* no fewer than by_piece has, growing with `most` */
     p.most = (uint32_t)max((uint64_t)p.stream, min(longest, (uint64_t)3 * p.stream));
     if (room < pieces(p.most)) p.most = p.stream;
     if (room < pieces(p.stream)) p.most = p.stream = room > p.tiles ? (uint32_t)min(room, 2 * (room - p.tiles)) : 0;
@@ -476,7 +476,9 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
     return hipGetLastError();
 }
 
-size_t paged_attention_workspace(const PagedArgs &a) {
+size_t paged_attention_workspace(const PagedArgs &given) {
+    PagedArgs a = given;
+    a.sinks = a.limit; /* the call brings them: a plan of more positions needs no fewer bytes, up to all of the context's */
     const AttendPlan p = attend_plan(a, ~(size_t)0);
     return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
 }

@@ -224,6 +224,40 @@ def logits():
 
 CASES = [f for f in (valid_calls, empty_batches, shapes, buffers, captures, logits)]
 
+
+def grids():
+    g = [line.split(" grid ")[1].split()[0] for line in fake.fake_log().decode().splitlines()]
+    fake.fake_clear()
+    return g
+
+
+def widest_split():
+    """The bytes that the workspace query gives make the launches that boundless ones would, whatever sinks and table the call
+    brings: the query knows neither."""
+    cut = 0
+    for heads, kv, hd, seqs, new, window, context in (
+            (32, 4, 64, 8, 1, 64, 5000), (32, 8, 128, 1, 1, 512, 131072), (14, 2, 64, 3, 1, 1000, 32768),
+            (4, 1, 64, 1, 1, 16, 1 << 20), (8, 2, 128, 2, 300, 200, 9000), (32, 8, 128, 6, 64, 33, 60000),
+            (8, 2, 256, 1, 100, 0, 4000), (4, 1, 64, 1, 1, 0, 1 << 20)):
+        p = Paged(heads=heads, kv=kv, hd=hd, pairs=0, type=1, page=64, pages=1, seqs=seqs, tokens=seqs * new,
+                  stride=-(-context // 64), window=window, context=context)
+        need = smq.load().smq_paged_attention_workspace(p.batch, p.shape)
+        large = smq.DeviceBuffer(max(4 * need, 1 << 28))
+        for sinks in (0, 1, 100, 4000, context - 500, context, 0xFFFFFFFF):
+            for stride in (p.o["stride"], p.o["stride"] - 1, p.o["stride"] // 2 + 1):
+                p.batch.table_stride = stride
+                got = []
+                for n in (large.nbytes, need):
+                    fake.fake_clear()
+                    smq.paged_attention(p.b["q"], p.b["att"], p.batch, p.shape, sinks, p.kv, large.at(0), n)
+                    got.append(grids())
+                assert got[0] == got[1], (heads, kv, hd, seqs, new, window, context, sinks, stride, need, got)
+                cut += len(got[0]) == 2
+    assert cut > 50
+
+
+CASES += [widest_split]
+
 if __name__ == "__main__":
     load(sys.argv[1])
     {f.__name__: f for f in CASES}[sys.argv[2]]()
