@@ -1591,6 +1591,9 @@ smq_status smq_logits_adjust(const float *logits, size_t stride, uint32_t rows, 
     if (!rows) return SMQ_OK;
     if (rows > 1 && (stride < vocab || (out && out_stride < vocab)))
         return set_status(SMQ_ERR_RANGE, "logits_adjust: row strides %zu, %zu below the vocabulary", stride, out_stride);
+    const size_t most = rows > 1 ? ((size_t)-1 / 4 - vocab) / (rows - 1) : (size_t)-1;
+    if (stride > most || (out && out_stride > most))
+        return set_status(SMQ_ERR_RANGE, "logits_adjust: row strides %zu, %zu are past the address space", stride, out_stride);
     if (out == logits && rows > 1 && out_stride != stride)
         return set_status(SMQ_ERR_RANGE, "logits_adjust: in place with another stride");
     smq::LogitArgs a;

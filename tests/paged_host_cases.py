@@ -256,7 +256,29 @@ def widest_split():
     assert cut > 50
 
 
-CASES += [widest_split]
+def logits_past_the_address_space():
+    """Row strides whose product with the rows wraps around: refused, not taken for a few bytes."""
+    rows, vocab = 3, 1000
+    logits, out, token, ws = (smq.DeviceBuffer(n) for n in (rows * vocab * 4, rows * vocab * 4, rows * 4,
+                                                            smq.logits_workspace(rows, vocab)))
+
+    def call(stride, out_stride, to=out):
+        smq.logits_adjust(logits, rows, vocab, None, to, token, ws, ws.nbytes, stride, out_stride)
+
+    call(vocab, vocab)
+    for stride in (1 << 61, (1 << 61) + vocab, 1 << 62, (1 << 63) + 1, (1 << 64) - 1):
+        refused(lambda: call(stride, vocab), words="address space")
+        refused(lambda: call(vocab, stride), words="address space")
+        refused(lambda: call(stride, vocab, None), words="address space")
+        refused(lambda: call(stride, stride, logits), words="address space")
+    refused(lambda: call(1 << 60, vocab), words="exceed its allocation")
+    # of one row the stride is not looked at
+    fake.fake_clear()
+    smq.logits_adjust(logits, 1, vocab, None, out, token, ws, ws.nbytes, (1 << 64) - 1, 1 << 62)
+    assert launches() >= 1
+
+
+CASES += [widest_split, logits_past_the_address_space]
 
 if __name__ == "__main__":
     load(sys.argv[1])
