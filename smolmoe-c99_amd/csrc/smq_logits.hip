@@ -260,9 +260,11 @@ uint32_t span_of(uint32_t rows, uint32_t vocab) {
 
 }  // namespace
 
+/* Enough for fewer rows or ids too, which may have more spans: below the line they are of half the size, 2046 at most. */
 size_t logits_workspace(uint32_t rows, uint32_t vocab) {
     const uint32_t span = span_of(rows, vocab);
-    return (size_t)rows * ((vocab + span - 1) / span) * sizeof(Part);
+    const size_t parts = (size_t)rows * ((vocab + span - 1) / span);
+    return (span == WIDE_SPAN && parts < 2046 ? 2046 : parts) * sizeof(Part);
 }
 
 hipError_t launch_logits(const LogitArgs &a, uint32_t *token, void *ws, hipStream_t s) {

@@ -278,7 +278,19 @@ def logits_past_the_address_space():
     assert launches() >= 1
 
 
-CASES += [widest_split, logits_past_the_address_space]
+def logits_workspace_of_the_largest_batch():
+    """A workspace for the most rows and ids serves every call of fewer: a batch that shrinks is not refused."""
+    for rows, vocab in ((64, 151936), (16, 151936), (14, 151936), (13, 151936), (342, 4099), (341, 4099), (1, 3_000_000)):
+        have = smq.logits_workspace(rows, vocab)
+        b, token = smq.DeviceBuffer(rows * vocab * 4), smq.DeviceBuffer(rows * 4)
+        ws = smq.DeviceBuffer(have)
+        for n in sorted({1, rows // 2, rows - 3, rows - 1, rows, 13, 14} & set(range(1, rows + 1))):
+            for v in sorted({vocab, vocab - 1, vocab * 9 // 10, vocab // 2, 2049, 1024, 5} & set(range(1, vocab + 1))):
+                assert smq.logits_workspace(n, v) <= have, (rows, vocab, n, v)
+                smq.logits_adjust(b, n, v, None, b, token, ws, have)
+
+
+CASES += [widest_split, logits_past_the_address_space, logits_workspace_of_the_largest_batch]
 
 if __name__ == "__main__":
     load(sys.argv[1])
