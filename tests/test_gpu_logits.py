@@ -196,3 +196,36 @@ def test_replays_and_streams():
             assert list(b[2].download(np.uint32)) == [t for _, t in want]
     for g in graphs:
         g.destroy()
+
+
+@pytest.mark.parametrize("rows,vocab", [(341, 4099), (342, 4099), (64, 32769), (512, 2049), (1030, 5)])
+def test_all_rules_on_both_sides_of_the_span_rule(rows, vocab):
+    """Spans of 2048 ids from 1024 workgroups on, of 1024 below (341 x 3 spans are 1023, and the largest batch of
+    test_all_rules has 780): rows of several spans, of one and a bit, and of less than one, aligned, at 4-byte addresses
+    and in place."""
+    say("logits, spans", rows, vocab)
+    test_all_rules(rows, vocab)
+
+
+def test_special_values_and_long_lists_in_spans_of_2048():
+    """Ties over threads, waves and spans, NaN and infinities, thousands of entries on few ids, in 352 rows of three spans."""
+    vocab, rows = 5000, 352
+    logits = np.zeros((rows, vocab), np.float32)
+    logits[0::8, 4500] = logits[0::8, 2100] = logits[0::8, 2047] = 5.0
+    logits[1::8, 0] = np.nan
+    logits[2::8, 1] = logits[2::8, 4999] = np.nan
+    logits[3::8] = -np.inf
+    logits[4::8] = np.nan
+    logits[5::8, 4097] = np.inf
+    logits[6::8] = -0.0
+    logits[6::8, 3000] = 0.0
+    logits[7::8] = -np.inf
+    logits[7::8, :3000] = np.nan
+    masks = [np.arange(vocab) >= 2500 if r % 8 == 7 else None for r in range(rows)]
+    plain = [logits_rules(logits[r], masks=masks[r]) for r in range(8)]
+    check(logits, Rules(vocab, masks=masks), [plain[r % 8] for r in range(rows)])
+    rng = np.random.default_rng(5)
+    ids, vals = rng.integers(0, 5, 900) * 1020, rng.standard_normal(900).astype(np.float32)
+    h, p = np.concatenate([np.full(6000, 2047), np.full(5, 2048), [0, 1, 4999]]), (1.3, 0.2, 0.001)
+    want = [logits_rules(logits[r], h, p, (ids, vals), masks[r]) for r in range(8)]
+    check(logits, Rules(vocab, [h] * rows, [p] * rows, [(ids, vals)] * rows, masks), [want[r % 8] for r in range(rows)])
