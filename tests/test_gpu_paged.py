@@ -671,3 +671,41 @@ def test_values_of_one_sign_near_the_largest(kv_type):
         else:
             cache.v[:] = np.float32(-3.3e38)
         rows_in_bound(cache.upload(), new, heads, seed=112, size=0.3)
+
+
+WIDE_CHUNKS = [  # heads, kv, hd, page, lengths, new, window, sinks
+    (4, 2, 256, 16, [90, 64], [90, 33], 0, 0),
+    (4, 1, 256, 64, [300], [70], 0, 0),
+    (8, 2, 144, 16, [100, 40], [64, 40], 0, 0),
+    (8, 2, 144, 128, [150], [100], 31, 2),
+    (2, 2, 192, 32, [130, 77], [130, 50], 0, 0),
+    (6, 2, 208, 16, [200], [90], 50, 3),
+    (3, 1, 240, 256, [280], [40], 0, 0),
+    (4, 4, 256, 32, [5000, 40], [40, 40], 0, 0),             # cut into pieces
+]
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("heads,kv,hd,page,lengths,new,window,sinks", WIDE_CHUNKS)
+def test_chunks_of_wide_heads(kv_type, heads, kv, hd, page, lengths, new, window, sinks):
+    """Heads above 128 where waves own rows (more than 32 rows a sequence and KV head), over pages of 16 and larger ones."""
+    say("paged attention, wide heads", TYPES[kv_type], heads, kv, hd, page, lengths, new, window, sinks)
+    assert sum(new) * heads // kv > 32 * len(new)
+    cache = Cache(kv_type, kv, hd, page, lengths, stale="nan")
+    for s, (m, n) in enumerate(zip(lengths, new)):
+        if window:
+            low = m - n + 1 - window
+            cache.spoil_positions(s, np.arange(min(sinks, low), low) if low > sinks else np.zeros(0, int))
+    batch, got, _, _ = rows_in_bound(cache.upload(), new, heads, window, sinks, padding=2, seed=113, size=1.5)
+    assert (got[int(batch.begin[-1]):] == 9.0).all()
+    smq.numeric_check()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("hd", [144, 176, 208, 240])
+def test_decode_of_wide_heads(kv_type, hd):
+    """Head sizes between 128 and 256 whose last block or last 32 dims are not whole."""
+    for page in (16, 64):
+        cache = Cache(kv_type, 2, hd, page, [700, 33, 1], stale="nan").upload()
+        rows_in_bound(cache, [1, 3, 1], 6, seed=114, size=1.5)
+    smq.numeric_check()
