@@ -4,7 +4,7 @@
  * A wave takes 16 rows (RT times 16 where it owns rows) as the columns of its products and 32 positions a step:
  *   S^T = K Q^T   two 16 x 16 tiles of positions x rows, K as the A operand straight from the page (its rows are
  *                 positions), position 8 u + i of the step in tile i / 4, row 4 u + i % 4;
- *   P   = 2^(S' - m + 7) (f32 caches: Rows::lift), S' the score in units of log2 e: by this order a lane holds the scores of 8 consecutive
+ *   P   = 2^(S' - m + 7) (f32 caches: Rows::unit), S' the score in units of log2 e: by this order a lane holds the scores of 8 consecutive
  *                 positions 8 (lane / 16) .. + 7 for row lane % 16, which is the B operand of
  *   O^T += V^T P^T  as it stands, no exchange between lanes: V^T is the A operand straight from the page, whose
  *                 values lie with positions innermost.
@@ -448,11 +448,12 @@ struct Rows {
     int pmin;
     Span span;
     uint32_t low_last; /* where the last row's window begins */
-    /* Weights are 2^(S' - m + lift), and m moves where a score exceeds it by more than SLACK. An f32 cache needs no f16
-     * range: there a row's weights, one for each position up to the wave's last, sum to less than 1, so that O stays below
-     * the values (with weights of 2^15 those of 5e36 made it infinite). The same in every piece: one join takes them. */
-    static constexpr float SLACK = TYPE == 0 ? 0.0f : 8.0f;
-    float lift;
+    /* Weights are 2^(S' - m + LIFT) * unit, and m moves where a score exceeds it by more than SLACK. An f32 cache needs no
+     * f16 range: there a row's weights, one for each position up to the wave's last, sum to less than 1, so that O stays
+     * below the values (with weights of 2^15 those of 5e36 made it infinite). The same in every piece: one join takes them.
+     * A factor, not part of LIFT: an exponent rounds relative to its size (one sequence at 131: 4.0e-7 off, 4.3e-7). */
+    static constexpr float SLACK = TYPE == 0 ? 0.0f : 8.0f, LIFT = TYPE == 0 ? 0.0f : 7.0f;
+    float unit;
     f4 o[RT][DT];
     float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
     float inv_e[RT][TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values, of this lane's columns */
@@ -493,7 +494,7 @@ struct Rows {
         const int pmax = __builtin_amdgcn_readfirstlane(hi);
         span = span_of(a, pmin, pmax);
         low_last = span_of(a, pmax, pmax).low;
-        lift = TYPE == 0 ? (float)(pmax > 0 ? __builtin_clz((uint32_t)pmax) - 33 : -1) : 7.0f;
+        unit = TYPE == 0 ? __builtin_ldexpf(1.0f, pmax > 0 ? __builtin_clz((uint32_t)pmax) - 33 : -1) : 1.0f;
 #pragma unroll
         for (int c = 0; c < RT; ++c)
 #pragma unroll
@@ -621,7 +622,7 @@ struct Rows {
         if (__any(up)) {
 #pragma unroll
             for (int c = 0; c < RT; ++c) {
-                /* a whole number: lift - m and the rescaling are exact */
+                /* a whole number: LIFT - m and the rescaling are exact */
                 const float n = fmaxf(m[c], ceilf(wave_max_quads(mx[c]))), alpha = __builtin_amdgcn_exp2f(m[c] - n);
                 m[c] = n;
                 l[c] *= alpha;
@@ -631,10 +632,11 @@ struct Rows {
         }
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
-            const float off = lift - m[c];
+            const float off = LIFT - m[c];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 x[c][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][j], factor[c], off));
+                if constexpr (TYPE == 0) x[c][j] *= unit;
                 l[c] += x[c][j];
             }
         }
