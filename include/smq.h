@@ -431,10 +431,12 @@ smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *sh
  * (KV head h / (heads / kv_heads)); f32 sums and statistics, each product of
  * f32 accuracy (a Q8 value whose scale is far below the largest one that the
  * row sees of its 32 dims, or below 2^-112, is rounded relative to that), no
- * order of the sums promised beyond: the same call gives the same bits. A row
- * that sees nothing is 0. Keys and values at positions that a row does not see,
- * and slots past a sequence's length, never matter, NaN and infinities included;
- * a visible one that is not finite leaves the row's result unspecified. Pages that no row sees may have any id. att must not overlap q.
+ * order of the sums promised beyond: the same call gives the same bits. Values
+ * of up to 3.3e38 give finite results. A row that sees nothing is 0. Keys and
+ * values at positions that a row does not see, and slots past a sequence's
+ * length, never matter, NaN and infinities included; a visible one that is not
+ * finite leaves the row's result unspecified. Pages that no row sees may have
+ * any id. att must not overlap q.
  * workspace (device, 16-byte aligned, may be NULL): where the call splits long
  * sequences over workgroups, their partial results;
  * smq_paged_attention_workspace gives the bytes that allow the widest split
@@ -473,8 +475,8 @@ typedef struct smq_logit_rules {
                                    * An index at or past allowed_rows raises the numeric flag and allows nothing. */
 } smq_logit_rules;
 /* Row r of logits at logits + r * stride, of out at out + r * out_stride (out
- * may be logits with the same stride; NULL: only the tokens); token (rows, may
- * be NULL when out is not). rules NULL: only the choice. workspace (device,
+ * may be logits with the same stride, must not overlap it otherwise; NULL: only
+ * the tokens); token (rows, may be NULL when out is not). rules NULL: only the choice. workspace (device,
  * 16-byte aligned, smq_logits_workspace bytes, which suffice for fewer rows or
  * ids too) is needed with token; calls that may overlap in time must not share
  * one. Asynchronous, capturable. */

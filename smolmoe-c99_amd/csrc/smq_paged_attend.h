@@ -4,24 +4,26 @@
  * A wave takes 16 rows (RT times 16 where it owns rows) as the columns of its products and 32 positions a step:
  *   S^T = K Q^T   two 16 x 16 tiles of positions x rows, K as the A operand straight from the page (its rows are
  *                 positions), position 8 u + i of the step in tile i / 4, row 4 u + i % 4;
- *   P   = 2^(S' - m + 7) (f32 caches: Rows::unit), S' the score in units of log2 e: by this order a lane holds the scores of 8 consecutive
- *                 positions 8 (lane / 16) .. + 7 for row lane % 16, which is the B operand of
+ *   P   = 2^(S' - m + 7), S' the score in units of log2 e (f32 caches: Rows::unit): by this order a lane holds the
+ *                 scores of 8 consecutive positions 8 (lane / 16) .. + 7 for row lane % 16, which is the B operand of
  *   O^T += V^T P^T  as it stands, no exchange between lanes: V^T is the A operand straight from the page, whose
  *                 values lie with positions innermost.
- * So no score passes through LDS (keys and values do where waves own rows: InLds). One pass over the positions: the maximum m of a row is moved (and O and the sum
- * rescaled) only where a score exceeds it by 8, which costs a vote instead of a reduction across lanes in most steps;
- * the weights then reach 2^15, in f16's range, and what f16 subnormals drop is below 2^-32 of the row's largest weight.
+ * So no score passes through LDS (keys and values do where waves own rows: InLds). One pass over the positions: the
+ * maximum m of a row is moved (and O and the sum rescaled) only where a score exceeds it by 8, which costs a vote instead
+ * of a reduction across lanes in most steps; the weights then reach 2^15, in f16's range, and what f16 subnormals round
+ * off is at most 2^-25, 2^-31 of the row's largest weight, which is above 2^6.
  *
  * f32 accuracy on f16 MFMA: q (scaled by a power of two per row) and P are each two f16, value and remainder (22 bits);
  * f16 keys and values and Q8 codes are f16 exactly. Q8 key scales multiply the f32 product of their 32-wide block; value
  * scales multiply P before its split, divided by 2^E, E the exponent of the largest scale that the row has seen of the
- * block (O is held in units of 2^E). An f32 cache takes the f32 MFMA, a sixteenth of the rate.
+ * block (O is held in units of 2^E): the 2^-25 is then of that scale. An f32 cache takes the f32 MFMA, a sixteenth of the
+ * rate.
  *
- * What bounds it: chunks the matrix cores and the softmax's VALU beside them (f16 heads of 128 at 4096: 586 TFLOP/s of
- * products without their remainders, twice that on the matrix cores; Q8 363, whose scales are VALU work; f32 127); decoding
- * the bytes of the cache (16 f16 sequences at up to 16384, 815 MB: 154 us, 5.3 TB/s) once pieces are long, else the latency
- * of a piece: batch, page ids, keys, products and the join one after another (32 Q8 sequences at up to 4090: 27 us for 58
- * MB; one at 131: 8 us). */
+ * What bounds it: chunks the matrix cores and the softmax's VALU beside them (64 chunks of 128 tokens at 4096, 32 heads on 8
+ * of 128: f16 543 TFLOP/s of products without their remainders, twice that on the matrix cores; Q8 353, whose scales are
+ * VALU work; f32 123); decoding the bytes of the cache (16 f16 sequences at up to 16384, 815 MB: 152 us, 5.4 TB/s) once
+ * pieces are long, else the latency of a piece: batch, page ids, keys, products and the join one after another (32 Q8
+ * sequences at up to 4090: 27 us for 58 MB; one at 131: 8 us). */
 #ifndef SMQ_PAGED_ATTEND_H
 #define SMQ_PAGED_ATTEND_H
 
@@ -63,11 +65,13 @@ template <uint32_t TYPE>
 hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
                          hipStream_t s);
 
-/* RT, at most, of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles and two
- * waves: each fragment read from LDS serves twice, the registers hold without spills, one wave's softmax runs beside the
- * other's products. Useful rate over 64 sequences of 128 tokens at 4096, 32 heads on 8 (RT 1 / 2 / 3 or 4): f16 heads of
- * 64 403 / 445 / 409 TFLOP/s, of 128 488 / 586 / 215; Q8 252 / 298 / 301, 301 / 363 / 195; f32 123 / 129 / 115, 99 / 127 /
- * 114. Three waves of RT 2: the same or spills. */
+/* RT, at most, of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles
+ * and two waves: each fragment read from LDS serves twice, one wave's softmax runs beside the other's products, and the
+ * registers hold (f32 heads of 128: 15 spilled). Useful rate over 64 sequences of 128 tokens at 4096, 32 heads on 8 (RT 1 / 2
+ * / 3 or 4), before a column had its own E: f16 heads of 64 403 / 445 / 409 TFLOP/s, of 128 488 / 586 / 215; Q8 252 / 298 /
+ * 301, 301 / 363 / 195; f32 123 / 129 / 115, 99 / 127 / 114. Three waves of RT 2: the same or spills. Heads above 128 have one
+ * step count (8) and one column tile of one wave a SIMD, whose O and queries fill the registers: 192 dims cost what 256 do (4
+ * chunks of 500 at 3000, 32 heads on 8: f16 0.42 and 0.41 ms, Q8 0.74 and 0.75). */
 constexpr uint32_t attend_rt(uint32_t ks) { return ks <= 4 ? 2 : 1; }
 constexpr int attend_waves(uint32_t ks) { return ks == 8 ? 1 : 2; }
 constexpr uint32_t attend_ks(uint32_t hd) { return hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : hd <= 128 ? 4 : 8; }
@@ -455,7 +459,7 @@ struct Rows {
     static constexpr float SLACK = TYPE == 0 ? 0.0f : 8.0f, LIFT = TYPE == 0 ? 0.0f : 7.0f;
     float unit;
     f4 o[RT][DT];
-    float m[RT], l[RT]; /* l: this lane's positions; f16: of the whole column, a product of P with ones */
+    float m[RT], l[RT]; /* l: of this lane's positions, until finish() */
     float inv_e[RT][TYPE == 2 ? KS : 1]; /* 2^-E of each block of the values, of this lane's columns */
     bool alike = true;                   /* every lane's columns have the same E each */
 
