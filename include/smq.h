@@ -476,10 +476,10 @@ typedef struct smq_logit_rules {
 } smq_logit_rules;
 /* Row r of logits at logits + r * stride, of out at out + r * out_stride (out
  * may be logits with the same stride, must not overlap it otherwise; NULL: only
- * the tokens); token (rows, may be NULL when out is not). rules NULL: only the choice. workspace (device,
- * 16-byte aligned, smq_logits_workspace bytes, which suffice for fewer rows or
- * ids too) is needed with token; calls that may overlap in time must not share
- * one. Asynchronous, capturable. */
+ * the tokens); token (rows, may be NULL when out is not). rules NULL: only the
+ * choice. workspace (device, 16-byte aligned, smq_logits_workspace bytes, which
+ * suffice for fewer rows or ids too) is needed with token; calls that may
+ * overlap in time must not share one. Asynchronous, capturable. */
 size_t smq_logits_workspace(uint32_t rows, uint32_t vocab);
 smq_status smq_logits_adjust(const float *logits, size_t stride, uint32_t rows, uint32_t vocab,
                              const smq_logit_rules *rules, float *out, size_t out_stride, uint32_t *token,
