@@ -429,14 +429,14 @@ smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *sh
  * shape->window w > 0 only those with j > p - w or j < sinks:
  *   att[h] = sum_j softmax_j(q[h] . k[j] / sqrt(head_dim)) v[j]
  * (KV head h / (heads / kv_heads)); f32 sums and statistics, each product of
- * f32 accuracy (a Q8 value whose scale is far below the largest one that the
- * row sees of its 32 dims, or below 2^-112, is rounded relative to that), no
- * order of the sums promised beyond: the same call gives the same bits. Values
- * of up to 3.3e38 give finite results. A row that sees nothing is 0. Keys and
- * values at positions that a row does not see, and slots past a sequence's
- * length, never matter, NaN and infinities included; a visible one that is not
- * finite leaves the row's result unspecified. Pages that no row sees may have
- * any id. att must not overlap q.
+ * f32 accuracy, where the cache is not f32 down to 2^-31 of the row's largest
+ * weight (Q8: of that times the largest scale that the row sees of the value's
+ * 32 dims, 2^-112 at least), no order of the sums promised beyond: the same call
+ * gives the same bits. Values of up to 3.3e38 give finite results. A row that
+ * sees nothing is 0. Keys and values at positions that a row does not see, and
+ * slots past a sequence's length, never matter, NaN and infinities included; a
+ * visible one that is not finite leaves the row's result unspecified. Pages that
+ * no row sees may have any id. att must not overlap q.
  * workspace (device, 16-byte aligned, may be NULL): where the call splits long
  * sequences over workgroups, their partial results;
  * smq_paged_attention_workspace gives the bytes that allow the widest split

@@ -709,3 +709,36 @@ def test_decode_of_wide_heads(kv_type, hd):
         cache = Cache(kv_type, 2, hd, page, [700, 33, 1], stale="nan").upload()
         rows_in_bound(cache, [1, 3, 1], 6, seed=114, size=1.5)
     smq.numeric_check()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("heads,kv,hd,page,new", Q8_FORMS)
+def test_weights_far_below_the_largest(kv_type, heads, kv, hd, page, new):
+    """A first position that takes nearly the whole weight and whose values are 0: what the others leave is off by f32's
+    rounding and, where the cache is not f32, by 2^-31 of the largest weight for each of them (half a step of f16, 2^-25, in
+    units where the largest is above 2^6)."""
+    say("weights far apart", TYPES[kv_type], heads, kv, hd, page, new)
+    n = 200
+    for power in (4.0, 9.0, 14.0):  # the others' weights, about 2^-power of the first one's
+        cache = Cache(kv_type, kv, hd, page, [n], stale="nan")
+        pg, sl = cache.slots(0, [0])
+        cache.k[pg, :, sl] = 127 if kv_type == Q8 else 1
+        cache.v[pg, :, sl] = 0
+        if kv_type == Q8:
+            cache.ks[pg, :, :, sl] = 1 / 127
+        cache.upload()
+        batch = Batch(cache, [new])
+        q = synth.normal(115, new * heads * hd, 0.3).reshape(-1, heads, hd)
+        q += np.float32(power * np.log(2) / np.sqrt(hd))  # q . 1 / sqrt(hd): power in units of log 2, beside the rest
+        want, tol = attend64(cache, batch, q, heads)
+        if kv_type != F32:
+            for i, p in enumerate(range(n - new, n)):
+                _, v = cache.rows(0, np.arange(p + 1), np.float64)
+                big = np.abs(v).max(0)
+                if kv_type == Q8:  # 127 codes of the block's largest scale
+                    pg, sl = cache.slots(0, np.arange(p + 1))
+                    big = np.repeat(cache.vs[pg, :, :, sl].max(0).astype(np.float64), 32, -1)[:, :hd] * 128
+                tol[i] += (p + 1) * 2.0 ** -31 * np.repeat(big, heads // kv, 0)
+        for split in (True, False):
+            close(attend(cache, batch, q, heads, kv, hd, split=split), want, tol, what=f"2^-{power}")
+    smq.numeric_check()
