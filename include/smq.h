@@ -449,6 +449,168 @@ size_t smq_paged_attention_workspace(const smq_paged_batch *batch, const smq_att
 smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                uint32_t sinks, const smq_paged_kv *kv, void *workspace, size_t workspace_bytes);
 
+/* ---- drafted tokens and beams over the paged cache --------------------------
+ * No reference counterpart (the reference decodes one sequence, one token at a
+ * time): what goes on top of the paged cache where a step brings a tree of
+ * drafted tokens for each sequence, or where sequences are the beams of a
+ * search and share pages. */
+/* The rows of smq_paged_norm_rope_kv. A stride is the floats from one token's
+ * row to the next one's, 0 for rows one after another: q, k and v may be parts
+ * of one wider row. */
+typedef struct smq_paged_rows {
+    const float *q;            /* heads * head_dim floats a row; NULL with q_out: none */
+    float *q_out;              /* q itself with the same stride: in place */
+    const float *k, *v;        /* kv_heads * head_dim floats a row */
+    size_t q_stride, q_out_stride, k_stride, v_stride;
+    const float *q_norm, *k_norm; /* head_dim floats each, device; NULL: no norm */
+    float eps;                 /* finite, not negative */
+    const int32_t *depth;      /* device, one per token: its rotary position is depth positions behind the sequence's
+                                * last one that is not new (a draft's children of one token share a position); NULL: the
+                                * rotary position is the position in the cache */
+} smq_paged_rows;
+/* smq_paged_rope_kv with an RMSNorm of each head of q and k before the rotation
+ * and with rotary positions of the tokens' own:
+ *   y = (x * (1 / sqrt(mean(x^2) + eps))) * norm
+ * mean, root and quotient in 64 bits, the quotient and both products rounded to
+ * f32 each (no order of the mean's sum shows in the result), then the rotation
+ * and the cache's rounding as smq_paged_rope_kv has them. Keys and values go to
+ * the tokens' own places whatever their depth. A row whose rotary position is
+ * outside [0, context) raises the numeric flag: its k is not stored and its q
+ * not written. q_out must not overlap k, v or, but for in place, q.
+ * Asynchronous, capturable. */
+smq_status smq_paged_norm_rope_kv(const smq_paged_rows *rows, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                                  const float *cos_table, const float *sin_table, const smq_paged_kv *kv);
+/* Trees of drafted tokens: parent[r], for row r of the batch, is the index
+ * among its sequence's new tokens of the token that r continues, below its
+ * own index; negative where that is the last token of the context. depth[r]: 0
+ * there, else its parent's + 1. mask, mask_stride words a row: bit t % 32 of
+ * word t / 32 is set where t is the token itself or an ancestor; the other bits
+ * of the row's words are cleared. A parent that is none of these raises the numeric flag
+ * and counts as negative; so does a sequence of more than 32 * mask_stride new
+ * tokens, whose rows are left as they are, and rows of padding are too.
+ * mask_stride: 1 .. 128. One call serves the attention of all layers.
+ * Asynchronous, capturable. */
+smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, int32_t *depth, uint32_t *mask,
+                           uint32_t mask_stride);
+/* smq_paged_attention where a mask says which of its sequence's new tokens a
+ * row sees: of the positions before them (the context) all, with shape->window
+ * w > 0 those with j > p - w or j < sinks, p = the context's positions +
+ * depth[r] (depth may be NULL where there is no window); of the new tokens
+ * those whose bit is set, whatever the window, later ones too. mask as smq_draft_masks writes it,
+ * or any other: bits behind the last new token do not matter. A row that sees
+ * nothing is 0. Numbers, errors, workspace and what does not matter as
+ * smq_paged_attention's; a depth below 0 or where p is not below the context's size raises the
+ * numeric flag, its row is 0, and so are those of a sequence of more
+ * than 32 * mask_stride new tokens. All pages of the new tokens must be pages.
+ * mask_stride: 1 .. 128. The workspace has a query of its own. Asynchronous,
+ * capturable. */
+size_t smq_paged_tree_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape);
+smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                                    uint32_t sinks, const int32_t *depth, const uint32_t *mask, uint32_t mask_stride,
+                                    const smq_paged_kv *kv, void *workspace, size_t workspace_bytes);
+/* The accepted path of each sequence's draft to the front of its new tokens, in
+ * every pool (the layers' caches: same type, page_size and pages): for k below
+ * count[s] the keys and values of new token accepted[s * accepted_stride + k]
+ * go to the place of new token k, as the cache holds them. length_out[s] (may
+ * be `length` itself) = the positions before the new tokens + count[s]. A list that does not ascend strictly within the
+ * sequence's new tokens, or is longer than accepted_stride, raises the numeric
+ * flag: the sequence stays as it is, its length too. Positions without a place
+ * or page raise the flag and are not moved. Sequences must not share a page that the call writes to. At most
+ * SMQ_MAX_POOLS pools. Asynchronous, capturable. */
+#define SMQ_MAX_POOLS 1024u
+smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,
+                             uint32_t accepted_stride, const int32_t *count, const smq_paged_kv *pools, uint32_t n_pools,
+                             int32_t *length_out);
+/* The next page tables of a set of sequences: rows of the new table that go on
+ * from rows of the old one. New row d keeps the first keep[d] positions of old
+ * row parent[d] (-1: none, and nothing is kept) and gets pages for room[d]
+ * positions in all (at least keep[d]):
+ *  - pages that keep[d] fills are shared with every row that names them;
+ *  - a page that it fills in part stays where nothing else holds it then (of
+ *    several rows that take it in part the first one keeps it), else its
+ *    positions are to be copied to a page of the row's own: copies[d];
+ *  - further pages are free ones, the lowest ids in the order of rows and
+ *    entries.
+ * So one call forks sequences (a parent named twice), ends them (a parent not
+ * named), begins them (-1), gives back what drafts have taken (keep below the
+ * length) and makes room for the next tokens (room above it). Old arrays are
+ * left as they are and must not overlap the new ones.
+ *
+ * refs counts, for each page, the entries of the old table (of the first held[s] ones of each row) that name it and other
+ * holders (a store of prompts), which stay counted; 0: free. refs_out: the same
+ * for the new table. held_out[d] = ceil(room[d] / page_size); entries behind it
+ * are -1. copies: three words a row, the page copied from and to and its
+ * positions; -1, -1, 0 where nothing is to be copied. free_out: the pages free
+ * afterwards; negative where so many were missing: then the numeric flag is
+ * raised, entries without a page are -1, and the old arrays still hold.
+ *
+ * Raise the flag as well: held, keep or room outside the table's row (cut), a
+ * keep above the parent's pages (cut) or above room (room is raised), a parent outside the old rows
+ * (-1), an entry that is no page (it stays none), refs below the old table's
+ * entries (such a page may be given twice). workspace: device, 16-byte aligned.
+ * At most 65535 rows and 2^24 pages. Asynchronous, capturable. */
+typedef struct smq_page_fork {
+    const int32_t *table; /* old_seqs * table_stride page ids */
+    const int32_t *held;  /* old_seqs: entries that hold pages */
+    const int32_t *refs;  /* pages */
+    uint32_t old_seqs, seqs, table_stride;
+    uint32_t page_size, pages; /* as smq_paged_kv's */
+    const int32_t *parent, *keep, *room; /* seqs */
+    int32_t *table_out;   /* seqs * table_stride */
+    int32_t *held_out;    /* seqs */
+    int32_t *refs_out;    /* pages */
+    int32_t *copies;      /* seqs * 3 */
+    int32_t *free_out;    /* one word */
+} smq_page_fork;
+size_t smq_paged_fork_workspace(const smq_page_fork *fork);
+smq_status smq_paged_fork(const smq_page_fork *fork, void *workspace, size_t workspace_bytes);
+/* The copies of smq_paged_fork in every pool: of row i the first copies[3 i + 2]
+ * positions of page copies[3 i] into page copies[3 i + 1], nothing else of that
+ * page. No page may be written twice or be read and written. Ids that are no page, or more positions than page_size, raise the numeric
+ * flag, and the row is skipped; so is one of no positions, without the flag.
+ * shape: kv_heads and head_dim. Pools as
+ * smq_paged_compact's. Asynchronous, capturable. */
+smq_status smq_paged_copy(const int32_t *copies, uint32_t rows, const smq_attn_shape *shape, const smq_paged_kv *pools,
+                          uint32_t n_pools);
+/* A step of a beam search: `groups` of `beams` rows of logits each (row r at
+ * logits + r * stride), and of each group the `select` best continuations, best
+ * first. A continuation of row r by id v is worth
+ *   score[r] + (l[v] - log sum_u exp(l[u]))
+ * in 64 bits, sum and logarithm included; the results are rounded to f32. Equal ones: the
+ * lower row first; of one row, the larger logit, then the lower id. A row that is done has one continuation, by `pad`, worth
+ * score[r]. Continuations worth -inf (masked ids) are none. Where a group has
+ * fewer than `select`, the rest gets parent -1, token UINT32_MAX, score -inf
+ * and counts as done. A row that is not done with a NaN or +inf among its logits, or any with a score that is
+ * NaN or +inf, raises the numeric flag and has no continuation.
+ *
+ * parent[i] is the row in 0 .. groups * beams - 1, as smq_paged_fork takes it. done_out[i]: the
+ * parent was done or the token is eos. History rows (history_stride ids each,
+ * as many as `length` says): row i of history_out has the parent's ids and,
+ * unless the parent was done, the token behind them (a row that is full raises the numeric flag and stays as
+ * it is); the rest of the row is UINT32_MAX, which smq_logits_adjust skips, so
+ * that history_begin may be multiples of history_stride. Lengths outside [0, history_stride] raise the flag and are cut.
+ * New arrays must not overlap old ones. select: 1 .. 64, beams 1 .. 64, at most 65535 rows of logits or results. workspace: device, 16-byte
+ * aligned; calls that may overlap in time must not share one. Asynchronous, capturable. */
+typedef struct smq_beam_step {
+    const float *logits;
+    size_t stride;
+    uint32_t groups, beams, vocab, select;
+    const float *score;         /* device, a row's own so far */
+    const uint8_t *done;        /* device, a row's own; NULL: none is */
+    uint32_t pad, eos;          /* eos UINT32_MAX: none */
+    int32_t *parent;            /* groups * select each */
+    uint32_t *token;
+    float *score_out;
+    uint8_t *done_out;          /* NULL: not wanted */
+    const uint32_t *history;    /* groups * beams rows; NULL: no histories */
+    uint32_t *history_out;      /* groups * select rows */
+    uint32_t history_stride;
+    const int32_t *length;      /* ids in each row */
+    int32_t *length_out;
+} smq_beam_step;
+size_t smq_beam_select_workspace(const smq_beam_step *step);
+smq_status smq_beam_select(const smq_beam_step *step, void *workspace, size_t workspace_bytes);
+
 /* ---- logits of several rows before the choice of a token -------------------
  * No reference counterpart (sampler.c:57-63 only skips banned ids). For each
  * row, with c the times id v stands in the row's history:
@@ -505,9 +667,9 @@ void smq_dequantize_q5_row(const unsigned char *w, uint32_t cols, float *out);
  * smq_capture_end is recorded, not run, and replayed by smq_graph_launch
  * (a HIP graph). Only asynchronous entry points may be captured: smq_gemm_*,
  * smq_dot_*_x4/_r4, smq_matmul, smq_quantize_q8_rows, smq_dequantize_*, the
- * paged cache's and smq_logits_adjust (batches and rules are read on the
- * device at each replay; what the host passed, tokens and context among it,
- * stays). */
+ * paged cache's, smq_logits_adjust and those of drafts and beams (batches,
+ * rules, trees, parents and scores are read on the device at each replay; what
+ * the host passed, tokens and context among it, stays). */
 smq_status smq_capture_begin(void);
 void *smq_capture_end(void);
 smq_status smq_graph_launch(void *graph);

@@ -82,6 +82,25 @@ class _LogitRules(ctypes.Structure):
                 ("allowed_rows", _u32), ("mask_row", _vp)]
 
 
+class _PagedRows(ctypes.Structure):
+    _fields_ = [("q", _vp), ("q_out", _vp), ("k", _vp), ("v", _vp), ("q_stride", _sz), ("q_out_stride", _sz),
+                ("k_stride", _sz), ("v_stride", _sz), ("q_norm", _vp), ("k_norm", _vp), ("eps", ctypes.c_float),
+                ("depth", _vp)]
+
+
+class _PageFork(ctypes.Structure):
+    _fields_ = [("table", _vp), ("held", _vp), ("refs", _vp), ("old_seqs", _u32), ("seqs", _u32), ("table_stride", _u32),
+                ("page_size", _u32), ("pages", _u32), ("parent", _vp), ("keep", _vp), ("room", _vp), ("table_out", _vp),
+                ("held_out", _vp), ("refs_out", _vp), ("copies", _vp), ("free_out", _vp)]
+
+
+class _BeamStep(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("stride", _sz), ("groups", _u32), ("beams", _u32), ("vocab", _u32), ("select", _u32),
+                ("score", _vp), ("done", _vp), ("pad", _u32), ("eos", _u32), ("parent", _vp), ("token", _vp),
+                ("score_out", _vp), ("done_out", _vp), ("history", _vp), ("history_out", _vp), ("history_stride", _u32),
+                ("length", _vp), ("length_out", _vp)]
+
+
 _SIGS = {
     "smq_last_status": (ctypes.c_int, []),
     "smq_last_error": (ctypes.c_char_p, []),
@@ -148,6 +167,19 @@ _SIGS = {
     "smq_paged_attention_workspace": (_sz, [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape)]),
     "smq_paged_attention": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape), _u32,
                                            ctypes.POINTER(_PagedKv), _vp, _sz]),
+    "smq_paged_norm_rope_kv": (ctypes.c_int, [ctypes.POINTER(_PagedRows), ctypes.POINTER(_PagedBatch),
+                                              ctypes.POINTER(_AttnShape), _vp, _vp, ctypes.POINTER(_PagedKv)]),
+    "smq_draft_masks": (ctypes.c_int, [_vp, ctypes.POINTER(_PagedBatch), _vp, _vp, _u32]),
+    "smq_paged_tree_attention_workspace": (_sz, [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape)]),
+    "smq_paged_tree_attention": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape), _u32, _vp,
+                                                _vp, _u32, ctypes.POINTER(_PagedKv), _vp, _sz]),
+    "smq_paged_compact": (ctypes.c_int, [ctypes.POINTER(_PagedBatch), ctypes.POINTER(_AttnShape), _vp, _u32, _vp,
+                                         ctypes.POINTER(_PagedKv), _u32, _vp]),
+    "smq_paged_fork_workspace": (_sz, [ctypes.POINTER(_PageFork)]),
+    "smq_paged_fork": (ctypes.c_int, [ctypes.POINTER(_PageFork), _vp, _sz]),
+    "smq_paged_copy": (ctypes.c_int, [_vp, _u32, ctypes.POINTER(_AttnShape), ctypes.POINTER(_PagedKv), _u32]),
+    "smq_beam_select_workspace": (_sz, [ctypes.POINTER(_BeamStep)]),
+    "smq_beam_select": (ctypes.c_int, [ctypes.POINTER(_BeamStep), _vp, _sz]),
     "smq_logits_workspace": (_sz, [_u32, _u32]),
     "smq_logits_adjust": (ctypes.c_int, [_vp, _sz, _u32, _u32, ctypes.POINTER(_LogitRules), _vp, _sz, _vp, _vp, _sz]),
     "smq_quantize_q5_row": (None, [_vp, _u32, _vp]),
@@ -621,6 +653,109 @@ def paged_attention(q, att, batch, shape, sinks, kv, workspace=None, workspace_b
     if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
         workspace_bytes = workspace.nbytes
     _check(load().smq_paged_attention(_p(q), _p(att), batch, shape, sinks, kv, _p(workspace), workspace_bytes))
+
+
+# ---- drafted tokens and beams over the paged cache
+def paged_rows(q, q_out, k, v, q_norm=None, k_norm=None, eps=1e-6, depth=None, q_stride=0, q_out_stride=0, k_stride=0,
+               v_stride=0):
+    """The new tokens' rows, norms and depths (smq_paged_rows), strides in floats (0: rows one after another); holds its
+    buffers."""
+    r = _PagedRows(_p(q), _p(q_out), _p(k), _p(v), q_stride, q_out_stride, k_stride, v_stride, _p(q_norm), _p(k_norm), eps,
+                   _p(depth))
+    r._keep = (q, q_out, k, v, q_norm, k_norm, depth)
+    return r
+
+
+def paged_norm_rope_kv(rows, batch, shape, cos_table, sin_table, kv):
+    """smq_paged_norm_rope_kv: RMSNorm of each head of q and k, RoPE by the tokens' own positions, keys and values into
+    their pages."""
+    _check(load().smq_paged_norm_rope_kv(rows, batch, shape, _p(cos_table), _p(sin_table), kv))
+
+
+def draft_masks(parent, batch, depth, mask, mask_stride):
+    """smq_draft_masks: depths of the batch's new tokens, and which of them each one sees, from their parents."""
+    _check(load().smq_draft_masks(_p(parent), batch, _p(depth), _p(mask), mask_stride))
+
+
+def paged_tree_attention_workspace(batch, shape):
+    """Bytes of workspace that allow paged_tree_attention its widest split."""
+    n = load().smq_paged_tree_attention_workspace(batch, shape)
+    if not n:
+        _check()
+    return n
+
+
+def paged_tree_attention(q, att, batch, shape, sinks, depth, mask, mask_stride, kv, workspace=None, workspace_bytes=0):
+    """smq_paged_tree_attention: the new tokens over their sequences' contexts and the new tokens of their masks."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+        workspace_bytes = workspace.nbytes
+    _check(load().smq_paged_tree_attention(_p(q), _p(att), batch, shape, sinks, _p(depth), _p(mask), mask_stride, kv,
+                                           _p(workspace), workspace_bytes))
+
+
+def paged_pools(kvs):
+    """The pools of several layers (paged_kv's) as one array; holds them."""
+    pools = (_PagedKv * len(kvs))(*kvs)
+    pools._keep = list(kvs)
+    return pools
+
+
+def paged_compact(batch, shape, accepted, accepted_stride, count, pools, length_out):
+    """smq_paged_compact: each sequence's accepted path to the front of its new tokens, in every pool."""
+    _check(load().smq_paged_compact(batch, shape, _p(accepted), accepted_stride, _p(count), pools, len(pools),
+                                    _p(length_out)))
+
+
+def page_fork(table, held, refs, old_seqs, seqs, table_stride, page_size, pages, parent, keep, room, table_out, held_out,
+              refs_out, copies, free_out):
+    """The old tables, what becomes of them, and the new ones (smq_page_fork); holds its buffers."""
+    f = _PageFork(_p(table), _p(held), _p(refs), old_seqs, seqs, table_stride, page_size, pages, _p(parent), _p(keep),
+                  _p(room), _p(table_out), _p(held_out), _p(refs_out), _p(copies), _p(free_out))
+    f._keep = (table, held, refs, parent, keep, room, table_out, held_out, refs_out, copies, free_out)
+    return f
+
+
+def paged_fork_workspace(fork):
+    n = load().smq_paged_fork_workspace(fork)
+    if not n:
+        _check()
+    return n
+
+
+def paged_fork(fork, workspace, workspace_bytes=0):
+    """smq_paged_fork: the sequences' next tables; pages shared, to be copied, fresh and freed."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+        workspace_bytes = workspace.nbytes
+    _check(load().smq_paged_fork(fork, _p(workspace), workspace_bytes))
+
+
+def paged_copy(copies, rows, shape, pools):
+    """smq_paged_copy: the copies that paged_fork asks for, in every pool."""
+    _check(load().smq_paged_copy(_p(copies), rows, shape, pools, len(pools)))
+
+
+def beam_step(logits, stride, groups, beams, vocab, select, score, parent, token, score_out, done=None, pad=0,
+              eos=0xFFFFFFFF, done_out=None, history=None, history_out=None, history_stride=0, length=None,
+              length_out=None):
+    """A step of a beam search (smq_beam_step); holds its buffers."""
+    b = _BeamStep(_p(logits), stride, groups, beams, vocab, select, _p(score), _p(done), pad, eos, _p(parent), _p(token),
+                  _p(score_out), _p(done_out), _p(history), _p(history_out), history_stride, _p(length), _p(length_out))
+    b._keep = (logits, score, done, parent, token, score_out, done_out, history, history_out, length, length_out)
+    return b
+
+
+def beam_select_workspace(step):
+    n = load().smq_beam_select_workspace(step)
+    if not n:
+        _check()
+    return n
+
+
+def beam_select(step, workspace, workspace_bytes=0):
+    """smq_beam_select: each group's best continuations, and the histories that go on from them."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+        workspace_bytes = workspace.nbytes
+    _check(load().smq_beam_select(step, _p(workspace), workspace_bytes))
 
 
 # ---- logits of several rows before the choice of a token

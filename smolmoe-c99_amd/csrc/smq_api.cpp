@@ -1497,8 +1497,8 @@ static bool paged_args(const smq_paged_batch *b, const smq_attn_shape *shape, co
     return true;
 }
 
-/* The descriptors' arrays, of a batch that is not empty. */
-static bool paged_extents(const smq::PagedArgs &a, const char *who) {
+/* A pool's arrays. */
+static bool pool_extents(const smq::PagedArgs &a, const char *who) {
     static const size_t bytes[3] = {4, 2, 1};
     const size_t positions = (size_t)a.pages << a.shift, kd = (size_t)a.kv_heads * a.head_dim;
     const size_t scales = a.type == SMQ_KV_Q8 ? positions * a.kv_heads * a.nb * 4 : 0;
@@ -1514,11 +1514,14 @@ static bool paged_extents(const smq::PagedArgs &a, const char *who) {
         set_status(SMQ_ERR_RANGE, "%s: the pools must be 16-byte aligned", who);
         return false;
     }
-    return extent_ok(a.begin, ((size_t)a.seqs + 1) * 4, "begin") && extent_ok(a.length, (size_t)a.seqs * 4, "length") &&
-           extent_ok(a.table, (size_t)a.seqs * a.table_stride * 4, "table") &&
-           extent_ok(a.keys, positions * kd * bytes[a.type], "keys") &&
+    return extent_ok(a.keys, positions * kd * bytes[a.type], "keys") &&
            extent_ok(a.values, positions * kd * bytes[a.type], "values") && extent_ok(a.ks, scales, "key scales") &&
            extent_ok(a.vs, scales, "value scales");
+}
+/* The descriptors' arrays, of a batch that is not empty. */
+static bool paged_extents(const smq::PagedArgs &a, const char *who) {
+    return extent_ok(a.begin, ((size_t)a.seqs + 1) * 4, "begin") && extent_ok(a.length, (size_t)a.seqs * 4, "length") &&
+           extent_ok(a.table, (size_t)a.seqs * a.table_stride * 4, "table") && pool_extents(a, who);
 }
 
 smq_status smq_paged_rope_kv(const float *q, float *q_out, const float *k, const float *v,
@@ -1577,6 +1580,292 @@ smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch
     return hip_ok(smq::launch_paged_attention(a, q, att, workspace, workspace_bytes, g.cur), "paged_attention")
                ? SMQ_OK
                : t_status;
+}
+
+/* Whether [p, p + n) and [q, q + m) share a byte. */
+static bool overlap(const void *p, size_t n, const void *q, size_t m) {
+    return n && m && (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n;
+}
+
+/* Bytes of `rows` rows of `width` floats, `stride` apart (0: width); 0 with an error where they are none. */
+static size_t row_bytes_of(uint32_t rows, size_t width, size_t *stride, const char *who, const char *what) {
+    if (!*stride) *stride = width;
+    if ((rows > 1 && *stride < width) || *stride > ((size_t)-1 / 4 - width) / rows) {
+        set_status(SMQ_ERR_RANGE, "%s: %s: a row stride of %zu for rows of %zu", who, what, *stride, width);
+        return 0;
+    }
+    return ((rows - 1) * *stride + width) * 4;
+}
+
+smq_status smq_paged_norm_rope_kv(const smq_paged_rows *rows, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                                  const float *cos_table, const float *sin_table, const smq_paged_kv *kv) {
+    static const char who[] = "paged_norm_rope_kv";
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!rows) return set_status(SMQ_ERR_RANGE, "%s: the rows are NULL", who);
+    if (!kv) return set_status(SMQ_ERR_RANGE, "%s: the cache is NULL", who);
+    if (!paged_args(batch, shape, kv, who, &a)) return t_status;
+    if (!rows->q != !rows->q_out) return set_status(SMQ_ERR_RANGE, "%s: q without q_out, or q_out without q", who);
+    if (!(rows->eps >= 0.0f && rows->eps < INFINITY)) return set_status(SMQ_ERR_RANGE, "%s: eps %g", who, (double)rows->eps);
+    if (!a.seqs || !a.tokens) return SMQ_OK;
+    smq::RowArgs r = {rows->q,        rows->q_out,    rows->k,      rows->v,      rows->q_stride, rows->q_out_stride,
+                      rows->k_stride, rows->v_stride, rows->q_norm, rows->k_norm, rows->eps,      rows->depth};
+    const size_t table = (size_t)a.context * a.pairs * 4, qd = (size_t)a.heads * a.head_dim,
+                 kd = (size_t)a.kv_heads * a.head_dim, norm = (size_t)a.head_dim * 4;
+    const size_t kn = row_bytes_of(a.tokens, kd, &r.k_stride, who, "k"), vn = row_bytes_of(a.tokens, kd, &r.v_stride, who, "v");
+    if (!kn || !vn) return t_status;
+    size_t qn = 0, on = 0;
+    if (r.q) {
+        qn = row_bytes_of(a.tokens, qd, &r.q_stride, who, "q");
+        on = row_bytes_of(a.tokens, qd, &r.q_out_stride, who, "q_out");
+        if (!qn || !on) return t_status;
+        if (r.q == r.q_out && r.q_stride != r.q_out_stride)
+            return set_status(SMQ_ERR_RANGE, "%s: in place with another stride", who);
+    }
+    if (!paged_extents(a, who) || !extent_ok(r.q, qn, "q") || !extent_ok(r.q_out, on, "q_out") || !extent_ok(r.k, kn, "k") ||
+        !extent_ok(r.v, vn, "v") || !extent_ok(r.q_norm, r.q_norm ? norm : 0, "q_norm") ||
+        !extent_ok(r.k_norm, r.k_norm ? norm : 0, "k_norm") ||
+        !extent_ok(r.depth, r.depth ? (size_t)a.tokens * 4 : 0, "depth") || !extent_ok(cos_table, table, "cos table") ||
+        !extent_ok(sin_table, table, "sin table"))
+        return t_status;
+    return hip_ok(smq::launch_paged_norm_rope_kv(a, r, cos_table, sin_table, g.cur), who) ? SMQ_OK : t_status;
+}
+
+static bool mask_words_ok(uint32_t words, const char *who) {
+    if (words && words <= smq::MAX_MASK_WORDS) return true;
+    set_status(SMQ_ERR_RANGE, "%s: mask rows of %u words of 1 .. %u", who, words, smq::MAX_MASK_WORDS);
+    return false;
+}
+
+smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, int32_t *depth, uint32_t *mask,
+                           uint32_t mask_stride) {
+    static const char who[] = "draft_masks";
+    if (!ready()) return t_status;
+    if (!batch) return set_status(SMQ_ERR_RANGE, "%s: NULL argument", who);
+    if (!mask_words_ok(mask_stride, who)) return t_status;
+    if (batch->seqs > (1u << 20) || batch->tokens > (1u << 22))
+        return set_status(SMQ_ERR_RANGE, "%s: unsupported batch (%u sequences <= 2^20, %u tokens <= 2^22)", who, batch->seqs,
+                          batch->tokens);
+    if (!batch->seqs || !batch->tokens) return SMQ_OK;
+    smq::PagedArgs a;
+    memset(&a, 0, sizeof(a));
+    a.begin = batch->begin;
+    a.seqs = batch->seqs;
+    a.tokens = batch->tokens;
+    a.flag = g.flag;
+    const size_t n = (size_t)a.tokens * 4;
+    if (!extent_ok(a.begin, ((size_t)a.seqs + 1) * 4, "begin") || !extent_ok(parent, n, "parent") ||
+        !extent_ok(depth, n, "depth") || !extent_ok(mask, n * mask_stride, "mask"))
+        return t_status;
+    if (overlap(parent, n, depth, n) || overlap(parent, n, mask, n * mask_stride) || overlap(depth, n, mask, n * mask_stride))
+        return set_status(SMQ_ERR_RANGE, "%s: parent, depth and mask overlap", who);
+    return hip_ok(smq::launch_draft_masks(a, parent, depth, mask, mask_stride, g.cur), who) ? SMQ_OK : t_status;
+}
+
+size_t smq_paged_tree_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape) {
+    smq::PagedArgs a;
+    return paged_args(batch, shape, nullptr, "paged_tree_attention_workspace", &a) ? smq::paged_tree_workspace(a) : 0;
+}
+
+smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
+                                    uint32_t sinks, const int32_t *depth, const uint32_t *mask, uint32_t mask_stride,
+                                    const smq_paged_kv *kv, void *workspace, size_t workspace_bytes) {
+    static const char who[] = "paged_tree_attention";
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!kv) return set_status(SMQ_ERR_RANGE, "%s: the cache is NULL", who);
+    if (!paged_args(batch, shape, kv, who, &a) || !mask_words_ok(mask_stride, who)) return t_status;
+    if (a.window && !depth) return set_status(SMQ_ERR_RANGE, "%s: a window without depths", who);
+    if (!a.seqs || !a.tokens) return SMQ_OK;
+    a.sinks = sinks;
+    const smq::TreeArgs t = {depth, mask, mask_stride};
+    const size_t rows = (size_t)a.tokens * a.heads * a.head_dim * 4;
+    if (!workspace) workspace_bytes = 0;
+    if ((uintptr_t)workspace & 15) return set_status(SMQ_ERR_RANGE, "%s: the workspace must be 16-byte aligned", who);
+    if (!paged_extents(a, who) || !extent_ok(q, rows, "q") || !extent_ok(att, rows, "att") ||
+        !extent_ok(depth, depth ? (size_t)a.tokens * 4 : 0, "depth") ||
+        !extent_ok(mask, (size_t)a.tokens * mask_stride * 4, "mask") || !extent_ok(workspace, workspace_bytes, "workspace"))
+        return t_status;
+    return hip_ok(smq::launch_paged_tree(a, t, q, att, workspace, workspace_bytes, g.cur), who) ? SMQ_OK : t_status;
+}
+
+/* The pools of a call that goes over all layers: alike, and of a's shape. */
+static bool pool_args(const smq_paged_kv *pools, uint32_t n, const char *who, const smq::PagedArgs *a, smq::Pool *out) {
+    if (n > SMQ_MAX_POOLS) {
+        set_status(SMQ_ERR_RANGE, "%s: %u pools of at most %u", who, n, SMQ_MAX_POOLS);
+        return false;
+    }
+    for (uint32_t i = 0; i < n; ++i) {
+        const smq_paged_kv &p = pools[i];
+        if (p.type != pools->type || p.page_size != pools->page_size || p.pages != pools->pages) {
+            set_status(SMQ_ERR_RANGE, "%s: pool %u has another type, page size or number of pages than the first", who, i);
+            return false;
+        }
+        smq::PagedArgs one = *a;
+        one.keys = p.keys;
+        one.values = p.values;
+        one.ks = p.key_scales;
+        one.vs = p.value_scales;
+        if (!pool_extents(one, who)) return false;
+        out[i] = {p.keys, p.values, p.key_scales, p.value_scales};
+    }
+    return true;
+}
+
+smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,
+                             uint32_t accepted_stride, const int32_t *count, const smq_paged_kv *pools, uint32_t n_pools,
+                             int32_t *length_out) {
+    static const char who[] = "paged_compact";
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    if (!pools || !n_pools) return set_status(SMQ_ERR_RANGE, "%s: no pools", who);
+    if (!paged_args(batch, shape, pools, who, &a)) return t_status;
+    if (!a.seqs) return SMQ_OK;
+    if ((uint64_t)a.seqs * a.kv_heads > smq::MAX_POOL_ROWS)
+        return set_status(SMQ_ERR_RANGE, "%s: %u sequences of %u KV heads exceed %u", who, a.seqs, a.kv_heads, smq::MAX_POOL_ROWS);
+    if (!accepted_stride || accepted_stride > (1u << 22))
+        return set_status(SMQ_ERR_RANGE, "%s: an accepted_stride of %u of 1 .. 2^22", who, accepted_stride);
+    const size_t n = (size_t)a.seqs * 4;
+    if (!extent_ok(a.begin, n + 4, "begin") || !extent_ok(a.length, n, "length") ||
+        !extent_ok(a.table, n * a.table_stride, "table") || !extent_ok(accepted, n * accepted_stride, "accepted") ||
+        !extent_ok(count, n, "count") || !extent_ok(length_out, n, "length_out"))
+        return t_status;
+    if (overlap(length_out, n, a.length, n) || overlap(length_out, n, count, n) || overlap(length_out, n, accepted, n * accepted_stride))
+        return set_status(SMQ_ERR_RANGE, "%s: length_out overlaps length, accepted or count", who);
+    smq::Pool p[SMQ_MAX_POOLS];
+    if (!pool_args(pools, n_pools, who, &a, p)) return t_status;
+    return hip_ok(smq::launch_paged_compact(a, p, n_pools, accepted, accepted_stride, count, length_out, g.cur), who)
+               ? SMQ_OK
+               : t_status;
+}
+
+smq_status smq_paged_copy(const int32_t *copies, uint32_t rows, const smq_attn_shape *shape, const smq_paged_kv *pools,
+                          uint32_t n_pools) {
+    static const char who[] = "paged_copy";
+    if (!ready()) return t_status;
+    smq::PagedArgs a;
+    const smq_paged_batch none = {nullptr, nullptr, nullptr, 0, 0, 0};
+    if (!pools || !n_pools) return set_status(SMQ_ERR_RANGE, "%s: no pools", who);
+    if (!paged_args(&none, shape, pools, who, &a)) return t_status;
+    if (!rows) return SMQ_OK;
+    if ((uint64_t)rows * a.kv_heads > smq::MAX_POOL_ROWS)
+        return set_status(SMQ_ERR_RANGE, "%s: %u rows of %u KV heads exceed %u", who, rows, a.kv_heads, smq::MAX_POOL_ROWS);
+    smq::Pool p[SMQ_MAX_POOLS];
+    if (!extent_ok(copies, (size_t)rows * 12, "copies") || !pool_args(pools, n_pools, who, &a, p)) return t_status;
+    return hip_ok(smq::launch_paged_copy(a, p, n_pools, copies, rows, g.cur), who) ? SMQ_OK : t_status;
+}
+
+static bool fork_args(const smq_page_fork *f, const char *who, smq::ForkArgs *out) {
+    if (!f) {
+        set_status(SMQ_ERR_RANGE, "%s: NULL argument", who);
+        return false;
+    }
+    if (f->old_seqs > smq::MAX_FORK_ROWS || f->seqs > smq::MAX_FORK_ROWS || !f->table_stride || f->table_stride > (1u << 20) ||
+        f->page_size < 16 || f->page_size > 256 || (f->page_size & (f->page_size - 1)) || !f->pages ||
+        f->pages > smq::MAX_FORK_PAGES) {
+        set_status(SMQ_ERR_RANGE,
+                   "%s: unsupported tables (%u and %u rows <= %u, table stride %u of 1 .. 2^20, page size %u of 16, 32, 64, "
+                   "128 or 256, %u pages of 1 .. %u)",
+                   who, f->old_seqs, f->seqs, smq::MAX_FORK_ROWS, f->table_stride, f->page_size, f->pages, smq::MAX_FORK_PAGES);
+        return false;
+    }
+    smq::ForkArgs a = {f->table, f->held, f->refs, f->parent, f->keep, f->room, f->table_out, f->held_out, f->refs_out,
+                       f->copies, f->free_out, f->old_seqs, f->seqs, f->table_stride, 0, f->pages, g.flag};
+    while ((1u << a.shift) < f->page_size) ++a.shift;
+    *out = a;
+    return true;
+}
+
+size_t smq_paged_fork_workspace(const smq_page_fork *fork) {
+    smq::ForkArgs a;
+    return fork_args(fork, "paged_fork_workspace", &a) ? smq::fork_workspace(a.pages, a.seqs) : 0;
+}
+
+smq_status smq_paged_fork(const smq_page_fork *fork, void *workspace, size_t workspace_bytes) {
+    static const char who[] = "paged_fork";
+    if (!ready()) return t_status;
+    smq::ForkArgs a;
+    if (!fork_args(fork, who, &a)) return t_status;
+    const size_t old = (size_t)a.old_seqs * 4, now = (size_t)a.seqs * 4, pages = (size_t)a.pages * 4;
+    const struct {
+        const void *p;
+        size_t bytes;
+        const char *what;
+    } in[6] = {{a.table, old * a.table_stride, "table"}, {a.held, old, "held"}, {a.refs, pages, "refs"},
+               {a.parent, now, "parent"}, {a.keep, now, "keep"}, {a.room, now, "room"}},
+      to[5] = {{a.table_out, now * a.table_stride, "table_out"}, {a.held_out, now, "held_out"},
+               {a.refs_out, pages, "refs_out"}, {a.copies, now * 3, "copies"}, {a.free_out, 4, "free_out"}};
+    for (const auto &x : in)
+        if (!extent_ok(x.p, x.bytes, x.what)) return t_status;
+    const size_t need = smq::fork_workspace(a.pages, a.seqs);
+    if (workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return set_status(SMQ_ERR_RANGE, "%s: the workspace has %zu bytes of %zu, 16-byte aligned", who, workspace_bytes, need);
+    if (!extent_ok(workspace, need, "workspace")) return t_status;
+    for (const auto &y : to) {
+        if (!extent_ok(y.p, y.bytes, y.what)) return t_status;
+        for (const auto &x : in)
+            if (overlap(x.p, x.bytes, y.p, y.bytes)) return set_status(SMQ_ERR_RANGE, "%s: %s overlaps %s", who, y.what, x.what);
+    }
+    return hip_ok(smq::launch_fork(a, workspace, g.cur), who) ? SMQ_OK : t_status;
+}
+
+static bool beam_args(const smq_beam_step *b, const char *who, smq::BeamArgs *out) {
+    if (!b) {
+        set_status(SMQ_ERR_RANGE, "%s: NULL argument", who);
+        return false;
+    }
+    if (!b->beams || b->beams > smq::MAX_BEAMS || !b->select || b->select > smq::MAX_SELECT || !b->vocab ||
+        b->vocab > (1u << 30) || (uint64_t)b->groups * b->beams > smq::MAX_BEAM_ROWS ||
+        (uint64_t)b->groups * b->select > smq::MAX_BEAM_ROWS) {
+        set_status(SMQ_ERR_RANGE,
+                   "%s: unsupported step (%u groups of %u beams of 1 .. %u, %u selected of 1 .. %u, at most %u rows, "
+                   "a vocabulary of %u ids)",
+                   who, b->groups, b->beams, smq::MAX_BEAMS, b->select, smq::MAX_SELECT, smq::MAX_BEAM_ROWS, b->vocab);
+        return false;
+    }
+    *out = {b->logits, b->stride, b->groups, b->beams, b->vocab, b->select, b->score, b->done, b->pad, b->eos, b->parent,
+            b->token, b->score_out, b->done_out, b->history, b->history_out, b->history_stride, b->length, b->length_out, g.flag};
+    return true;
+}
+
+size_t smq_beam_select_workspace(const smq_beam_step *step) {
+    smq::BeamArgs a;
+    return beam_args(step, "beam_select_workspace", &a) ? smq::beam_workspace(a) : 0;
+}
+
+smq_status smq_beam_select(const smq_beam_step *step, void *workspace, size_t workspace_bytes) {
+    static const char who[] = "beam_select";
+    if (!ready()) return t_status;
+    smq::BeamArgs a;
+    if (!beam_args(step, who, &a)) return t_status;
+    if (!a.groups) return SMQ_OK;
+    const size_t rows = (size_t)a.groups * a.beams, now = (size_t)a.groups * a.select;
+    if ((rows > 1 && a.stride < a.vocab) || (rows > 1 && a.stride > ((size_t)-1 / 4 - a.vocab) / (rows - 1)))
+        return set_status(SMQ_ERR_RANGE, "%s: a row stride of %zu for %u ids", who, a.stride, a.vocab);
+    if (a.history && (!a.history_stride || a.history_stride > 0x7fffffffu))
+        return set_status(SMQ_ERR_RANGE, "%s: a history_stride of %u", who, a.history_stride);
+    const size_t hs = a.history ? a.history_stride : 0, h = a.history ? 4 : 0;
+    const struct {
+        const void *p;
+        size_t bytes;
+        const char *what;
+    } in[5] = {{a.logits, ((rows - 1) * a.stride + a.vocab) * 4, "logits"}, {a.score, rows * 4, "score"},
+               {a.done, a.done ? rows : 0, "done"}, {a.history, rows * hs * 4, "history"}, {a.length, rows * h, "length"}},
+      to[6] = {{a.parent, now * 4, "parent"}, {a.token, now * 4, "token"}, {a.score_out, now * 4, "score_out"},
+               {a.done_out, a.done_out ? now : 0, "done_out"}, {a.history_out, now * hs * 4, "history_out"},
+               {a.length_out, now * h, "length_out"}};
+    for (const auto &x : in)
+        if (!extent_ok(x.p, x.bytes, x.what)) return t_status;
+    for (const auto &y : to) {
+        if (!extent_ok(y.p, y.bytes, y.what)) return t_status;
+        for (const auto &x : in)
+            if (overlap(x.p, x.bytes, y.p, y.bytes)) return set_status(SMQ_ERR_RANGE, "%s: %s overlaps %s", who, y.what, x.what);
+    }
+    const size_t need = smq::beam_workspace(a);
+    if (workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return set_status(SMQ_ERR_RANGE, "%s: the workspace has %zu bytes of %zu, 16-byte aligned", who, workspace_bytes, need);
+    if (!extent_ok(workspace, need, "workspace")) return t_status;
+    return hip_ok(smq::launch_beam(a, workspace, g.cur), who) ? SMQ_OK : t_status;
 }
 
 size_t smq_logits_workspace(uint32_t rows, uint32_t vocab) { return smq::logits_workspace(rows, vocab); }

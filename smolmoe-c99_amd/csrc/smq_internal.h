@@ -281,13 +281,84 @@ struct PagedArgs {
     uint32_t heads, kv_heads, head_dim, nb, pairs, window, sinks, context, limit;
     int *flag;
 };
+/* New tokens' rows: strides in floats; norms, depth: null where there is none. */
+struct RowArgs {
+    const float *q;
+    float *q_out;
+    const float *k, *v;
+    size_t q_stride, q_out_stride, k_stride, v_stride;
+    const float *q_norm, *k_norm;
+    float eps;
+    const int32_t *depth;
+};
 hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out, const float *k, const float *v,
                                 const float *cs, const float *sn, hipStream_t s);
+hipError_t launch_paged_norm_rope_kv(const PagedArgs &a, const RowArgs &r, const float *cs, const float *sn, hipStream_t s);
 hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s);
 /* The workspace of the widest split that the kernel would take. */
 size_t paged_attention_workspace(const PagedArgs &a);
 hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
                                   hipStream_t s);
+
+/* Trees of drafted tokens (csrc/smq_drafts.hip). words: of a row of the mask. */
+constexpr uint32_t MAX_MASK_WORDS = 128;
+struct TreeArgs {
+    const int32_t *depth;
+    const uint32_t *mask;
+    uint32_t words;
+};
+hipError_t launch_draft_masks(const PagedArgs &a, const int32_t *parent, int32_t *depth, uint32_t *mask, uint32_t words,
+                              hipStream_t s);
+size_t paged_tree_workspace(const PagedArgs &a);
+hipError_t launch_paged_tree(const PagedArgs &a, const TreeArgs &t, const float *q, float *att, void *ws, size_t ws_bytes,
+                             hipStream_t s);
+
+/* Pages: next tables, copies, accepted drafts (csrc/smq_pages.hip). Rows times KV heads of a call on pools are at most
+ * MAX_POOL_ROWS, so that a launch over one pool has less than 2^32 threads. */
+constexpr uint32_t MAX_FORK_ROWS = 65535, MAX_FORK_PAGES = 1u << 24, MAX_POOL_ROWS = 1u << 22, POOLS_AT_ONCE = 48;
+struct ForkArgs {
+    const int32_t *table, *held, *refs, *parent, *keep, *room;
+    int32_t *table_out, *held_out, *refs_out, *copies, *free_out;
+    uint32_t old_seqs, seqs, table_stride, shift, pages;
+    int *flag;
+};
+struct Pool {
+    void *keys, *values;
+    float *ks, *vs;
+};
+struct Pools { /* of a launch */
+    uint32_t n;
+    Pool p[POOLS_AT_ONCE];
+};
+size_t fork_workspace(uint32_t pages, uint32_t rows);
+hipError_t launch_fork(const ForkArgs &a, void *ws, hipStream_t s);
+hipError_t launch_paged_copy(const PagedArgs &a, const Pool *pools, uint32_t n, const int32_t *copies, uint32_t rows,
+                             hipStream_t s);
+hipError_t launch_paged_compact(const PagedArgs &a, const Pool *pools, uint32_t n, const int32_t *accepted, uint32_t stride,
+                                const int32_t *count, int32_t *length_out, hipStream_t s);
+
+/* A step of a beam search (csrc/smq_beam.hip). */
+constexpr uint32_t MAX_BEAMS = 64, MAX_SELECT = 64, MAX_BEAM_ROWS = 65535;
+struct BeamArgs {
+    const float *logits;
+    size_t stride;
+    uint32_t groups, beams, vocab, select;
+    const float *score;
+    const uint8_t *done;
+    uint32_t pad, eos;
+    int32_t *parent;
+    uint32_t *token;
+    float *score_out;
+    uint8_t *done_out;
+    const uint32_t *history;
+    uint32_t *history_out;
+    uint32_t history_stride;
+    const int32_t *length;
+    int32_t *length_out;
+    int *flag;
+};
+size_t beam_workspace(const BeamArgs &a);
+hipError_t launch_beam(const BeamArgs &a, void *ws, hipStream_t s);
 
 /* Penalties, biases, masks and the greedy choice on rows of logits (csrc/smq_logits.hip). */
 struct LogitArgs {

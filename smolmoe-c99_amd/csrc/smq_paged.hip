@@ -87,6 +87,39 @@ __device__ __forceinline__ f4 rotated(f4 x, uint32_t d, uint32_t pairs, const fl
     return x;
 }
 
+/* The lanes of a head's RMSNorm, four dims each: a power of two, so that they lie in one wave. */
+__device__ __forceinline__ uint32_t norm_lanes(const PagedArgs &a) {
+    return a.head_dim <= 32 ? 8 : a.head_dim <= 64 ? 16 : a.head_dim <= 128 ? 32 : 64;
+}
+/* Dims d .. d + 3 (0 past the head) of a head that `lanes` lanes hold, normed. The sum of squares, whose products are exact,
+ * the root and the quotient in 64 bits: no order of the sum shows in the f32 quotient, and the bits are the same whichever
+ * lanes hold the head; the two products round to f32 as the formula has them. */
+__device__ __forceinline__ f4 normed(f4 x, const float *norm, uint32_t d, const PagedArgs &a, uint32_t lanes, float eps) {
+    if (!norm) return x;
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += (double)x[e] * (double)x[e];
+    for (uint32_t off = 1; off < lanes; off *= 2) sum += __shfl_xor(sum, (int)off);
+    const float inv = (float)(1.0 / sqrt(sum / (double)a.head_dim + (double)eps));
+    const f4u g = *(const f4u *)(norm + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = x[e] * inv;
+        x[e] = y * g[e];
+    }
+    return x;
+}
+/* The rotary position of a token whose sequence's new tokens begin at position first; false, with the flag, where the tables have none. */
+__device__ __forceinline__ bool own_turn(const PagedArgs &a, int first, int depth, uint32_t &at) {
+    const int64_t p = (int64_t)first + depth;
+    if (p < 0 || p >= (int64_t)a.context) {
+        *a.flag = 1;
+        return false;
+    }
+    at = (uint32_t)p;
+    return true;
+}
+
 template <uint32_t TYPE>
 struct Four; /* four elements as the cache holds them */
 template <>
@@ -155,9 +188,9 @@ __device__ __forceinline__ typename Four<TYPE>::T encode(f4 x, float &scale, boo
  * 64; by bytes for chunks: 4 prompts of up to 700 tokens, 12 heads on 2 of 128, f16, 10.4 us (keys and values in one
  * workgroup, one pass after another: 5 us longer). */
 constexpr uint32_t ST_PASSES = 4;
-template <uint32_t TYPE>
-__global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float *q, float *q_out, const float *k,
-                                                       const float *v, const float *cs, const float *sn, uint32_t kv_groups) {
+template <uint32_t TYPE, bool NORM>
+__global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, const float *cs, const float *sn,
+                                                       uint32_t kv_groups) {
     typedef typename Four<TYPE>::T T;
     constexpr uint32_t EB = sizeof(T) / 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char turn[]; /* [head_dim][ST_POS * EB + 4] */
@@ -167,11 +200,26 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float 
         uint32_t s, pos;
         const uint32_t r = blockIdx.x - kv_groups;
         if (!place_of(a, r, s, pos)) return;
+        if constexpr (NORM) {
+            uint32_t turn_at = pos;
+            if (w.depth && !own_turn(a, (int)pos - (int)(r - (uint32_t)a.begin[s]), w.depth[r], turn_at)) return;
+            const float *c = cs + (size_t)turn_at * a.pairs, *sr = sn + (size_t)turn_at * a.pairs;
+            const uint32_t lanes = norm_lanes(a), d = 4 * (tid % lanes);
+            for (uint32_t h0 = 0; h0 < a.heads; h0 += ST_WG / lanes) { /* uniform: the norm's sums shuffle */
+                const uint32_t h = h0 + tid / lanes;
+                const bool in = h < a.heads && d < hd;
+                f4 x = {};
+                if (in) x = *(const f4u *)(w.q + r * w.q_stride + h * hd + d);
+                x = normed(x, w.q_norm, in ? d : 0, a, lanes, w.eps);
+                if (in) *(f4u *)(w.q_out + r * w.q_out_stride + h * hd + d) = rotated(x, d, a.pairs, c, sr);
+            }
+            return;
+        }
         const float *c = cs + (size_t)pos * a.pairs, *sr = sn + (size_t)pos * a.pairs;
         const size_t row = (size_t)r * a.heads * hd;
 #pragma unroll 2
         for (uint32_t i = tid; i < a.heads * hd / 4; i += ST_WG)
-            *(f4u *)(q_out + row + 4 * i) = rotated(*(const f4u *)(q + row + 4 * i), 4 * i % hd, a.pairs, c, sr);
+            *(f4u *)(w.q_out + row + 4 * i) = rotated(*(const f4u *)(w.q + row + 4 * i), 4 * i % hd, a.pairs, c, sr);
         return;
     }
     const uint32_t kind = blockIdx.x & 1, x = blockIdx.x >> 1, h = x % a.kv_heads; /* kind 0: keys, 1: values */
@@ -179,23 +227,36 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, const float 
     if (!find_block(a, x / a.kv_heads, b)) return;
     int page[2];
     block_pages(a, b, page);
-    const uint32_t P = 1u << a.shift, lanes = a.nb * 8, n = b.p1 - b.p0; /* lanes of a row: whole 32-wide blocks */
+    /* lanes of a row: whole 32-wide blocks */
+    const uint32_t P = 1u << a.shift, lanes = NORM ? norm_lanes(a) : a.nb * 8, n = b.p1 - b.p0;
     const bool few = n <= 2;
-    const float *from = kind ? v : k;
+    const float *from = kind ? w.v : w.k;
+    const size_t stride = NORM ? kind ? w.v_stride : w.k_stride : (size_t)a.kv_heads * hd;
+    const int first = NORM && w.depth ? a.begin[b.seq] - b.row : 0;
     for (uint32_t i0 = tid; i0 < (n * lanes + ST_WG - 1) / ST_WG * ST_WG; i0 += ST_PASSES * ST_WG) { /* whole waves: encode shuffles */
         f4 y[ST_PASSES];
 #pragma unroll
         for (uint32_t u = 0; u < ST_PASSES; ++u) {
             const uint32_t i = i0 + u * ST_WG, j = i / lanes, d = 4 * (i - j * lanes);
             y[u] = f4{};
-            if (j < n && d < hd) y[u] = *(const f4u *)(from + ((size_t)(b.row + (int)(b.p0 + j)) * a.kv_heads + h) * hd + d);
+            if (j < n && d < hd) y[u] = *(const f4u *)(from + (size_t)(b.row + (int)(b.p0 + j)) * stride + h * hd + d);
         }
 #pragma unroll
         for (uint32_t u = 0; u < ST_PASSES; ++u) {
             const uint32_t i = i0 + u * ST_WG, j = i / lanes, d = 4 * (i - j * lanes), pos = b.p0 + j, slot = pos & (P - 1);
             const int pg = pos & 16 ? page[1] : page[0];
-            const bool in = j < n && d < hd;
-            if (!kind && in) y[u] = rotated(y[u], d, a.pairs, cs + (size_t)pos * a.pairs, sn + (size_t)pos * a.pairs);
+            bool in = j < n && d < hd;
+            uint32_t at = pos;
+            if constexpr (NORM) {
+                if (!kind) {
+                    y[u] = normed(y[u], w.k_norm, in ? d : 0, a, lanes, w.eps);
+                    if (in && w.depth && !own_turn(a, first, w.depth[b.row + (int)pos], at)) {
+                        in = false;
+                        y[u] = f4{};
+                    }
+                }
+            }
+            if (!kind && in) y[u] = rotated(y[u], d, a.pairs, cs + (size_t)at * a.pairs, sn + (size_t)at * a.pairs);
             float scale;
             bool bad = false;
             const T t = encode<TYPE>(y[u], scale, bad);
@@ -463,12 +524,28 @@ AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
         else hipLaunchKernelGGL((KERNEL<2>), GRID, BLOCK, LDS, s, a, __VA_ARGS__);                     \
     } while (0)
 
+template <bool NORM>
+hipError_t launch_store(const PagedArgs &a, const RowArgs &r, const float *cs, const float *sn, hipStream_t s) {
+    const uint32_t kv_groups = 2 * most_blocks(a) * a.kv_heads, lds = a.head_dim * (ST_POS * (4u >> a.type) + 4);
+    const dim3 grid((r.q ? a.tokens : 0) + kv_groups);
+    if (a.type == 0) hipLaunchKernelGGL((k_paged_store<0, NORM>), grid, dim3(ST_WG), lds, s, a, r, cs, sn, kv_groups);
+    else if (a.type == 1) hipLaunchKernelGGL((k_paged_store<1, NORM>), grid, dim3(ST_WG), lds, s, a, r, cs, sn, kv_groups);
+    else hipLaunchKernelGGL((k_paged_store<2, NORM>), grid, dim3(ST_WG), lds, s, a, r, cs, sn, kv_groups);
+    return hipGetLastError();
+}
+
 hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out, const float *k, const float *v,
                                 const float *cs, const float *sn, hipStream_t s) {
-    const uint32_t kv_groups = 2 * most_blocks(a) * a.kv_heads;
-    SMQ_PAGED(k_paged_store, dim3((q ? a.tokens : 0) + kv_groups), dim3(ST_WG),
-              a.head_dim * (ST_POS * (4u >> a.type) + 4), q, q_out, k, v, cs, sn, kv_groups);
-    return hipGetLastError();
+    RowArgs r = {};
+    r.q = q;
+    r.q_out = q_out;
+    r.k = k;
+    r.v = v;
+    return launch_store<false>(a, r, cs, sn, s);
+}
+
+hipError_t launch_paged_norm_rope_kv(const PagedArgs &a, const RowArgs &r, const float *cs, const float *sn, hipStream_t s) {
+    return launch_store<true>(a, r, cs, sn, s);
 }
 
 hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s) {
