@@ -495,7 +495,7 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
 /* smq_paged_attention where a mask says which of its sequence's new tokens a
  * row sees: of the positions before them (the context) all, with shape->window
  * w > 0 those with j > p - w or j < sinks, p = the context's positions +
- * depth[r] (depth may be NULL where there is no window); of the new tokens
+ * depth[r] (not read where there is no window); of the new tokens
  * those whose bit is set, whatever the window, later ones too. mask as smq_draft_masks writes it,
  * or any other: bits behind the last new token do not matter. A row that sees
  * nothing is 0. Numbers, errors, workspace and what does not matter as

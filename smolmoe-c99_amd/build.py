@@ -17,7 +17,7 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libsmq_gfx950.so")
 SOURCES = [os.path.join(HERE, "csrc", f) for f in ("smq_kernels.hip", "smq_gemv.hip", "smq_decode.hip", "smq_mfma.hip", "smq_fused.hip", "smq_convert.hip", "smq_attend.hip",
                                                      "smq_paged.hip", "smq_paged_f32.hip", "smq_paged_f16.hip",
-                                                     "smq_paged_q8.hip", "smq_drafts.hip", "smq_pages.hip", "smq_beam.hip", "smq_logits.hip", "smq_anchor.hip", "smq_api.cpp")]
+                                                     "smq_paged_q8.hip", "smq_tree_f32.hip", "smq_tree_f16.hip", "smq_tree_q8.hip", "smq_drafts.hip", "smq_pages.hip", "smq_beam.hip", "smq_logits.hip", "smq_anchor.hip", "smq_api.cpp")]
 HEADERS = [os.path.join(HERE, "csrc", "smq_internal.h"), os.path.join(HERE, "csrc", "smq_device.h"),
            os.path.join(HERE, "csrc", "smq_paged.h"), os.path.join(HERE, "csrc", "smq_paged_attend.h"),
            os.path.join(ROOT, "include", "smq.h")]

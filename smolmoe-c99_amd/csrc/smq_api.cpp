@@ -1559,7 +1559,7 @@ smq_status smq_paged_read(const smq_paged_batch *batch, const smq_attn_shape *sh
 
 size_t smq_paged_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape) {
     smq::PagedArgs a;
-    return paged_args(batch, shape, nullptr, "paged_attention_workspace", &a) ? smq::paged_attention_workspace(a) : 0;
+    return paged_args(batch, shape, nullptr, "paged_attention_workspace", &a) ? smq::paged_attention_workspace(a, false) : 0;
 }
 
 smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
@@ -1577,7 +1577,7 @@ smq_status smq_paged_attention(const float *q, float *att, const smq_paged_batch
     if (!paged_extents(a, "paged_attention") || !extent_ok(q, rows, "q") || !extent_ok(att, rows, "att") ||
         !extent_ok(workspace, workspace_bytes, "workspace"))
         return t_status;
-    return hip_ok(smq::launch_paged_attention(a, q, att, workspace, workspace_bytes, g.cur), "paged_attention")
+    return hip_ok(smq::launch_paged_attention(a, nullptr, q, att, workspace, workspace_bytes, g.cur), "paged_attention")
                ? SMQ_OK
                : t_status;
 }
@@ -1664,7 +1664,7 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
 
 size_t smq_paged_tree_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape) {
     smq::PagedArgs a;
-    return paged_args(batch, shape, nullptr, "paged_tree_attention_workspace", &a) ? smq::paged_tree_workspace(a) : 0;
+    return paged_args(batch, shape, nullptr, "paged_tree_attention_workspace", &a) ? smq::paged_attention_workspace(a, true) : 0;
 }
 
 smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
@@ -1686,7 +1686,7 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
         !extent_ok(depth, depth ? (size_t)a.tokens * 4 : 0, "depth") ||
         !extent_ok(mask, (size_t)a.tokens * mask_stride * 4, "mask") || !extent_ok(workspace, workspace_bytes, "workspace"))
         return t_status;
-    return hip_ok(smq::launch_paged_tree(a, t, q, att, workspace, workspace_bytes, g.cur), who) ? SMQ_OK : t_status;
+    return hip_ok(smq::launch_paged_attention(a, &t, q, att, workspace, workspace_bytes, g.cur), who) ? SMQ_OK : t_status;
 }
 
 /* The pools of a call that goes over all layers: alike, and of a's shape. */

@@ -295,11 +295,6 @@ hipError_t launch_paged_rope_kv(const PagedArgs &a, const float *q, float *q_out
                                 const float *cs, const float *sn, hipStream_t s);
 hipError_t launch_paged_norm_rope_kv(const PagedArgs &a, const RowArgs &r, const float *cs, const float *sn, hipStream_t s);
 hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hipStream_t s);
-/* The workspace of the widest split that the kernel would take. */
-size_t paged_attention_workspace(const PagedArgs &a);
-hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
-                                  hipStream_t s);
-
 /* Trees of drafted tokens (csrc/smq_drafts.hip). words: of a row of the mask. */
 constexpr uint32_t MAX_MASK_WORDS = 128;
 struct TreeArgs {
@@ -309,9 +304,10 @@ struct TreeArgs {
 };
 hipError_t launch_draft_masks(const PagedArgs &a, const int32_t *parent, int32_t *depth, uint32_t *mask, uint32_t words,
                               hipStream_t s);
-size_t paged_tree_workspace(const PagedArgs &a);
-hipError_t launch_paged_tree(const PagedArgs &a, const TreeArgs &t, const float *q, float *att, void *ws, size_t ws_bytes,
-                             hipStream_t s);
+/* Attention over the pages, causal or (tree) by the mask; the workspace of the widest split that the kernel would take. */
+size_t paged_attention_workspace(const PagedArgs &a, bool tree);
+hipError_t launch_paged_attention(const PagedArgs &a, const TreeArgs *tree, const float *q, float *att, void *ws,
+                                  size_t ws_bytes, hipStream_t s);
 
 /* Pages: next tables, copies, accepted drafts (csrc/smq_pages.hip). Rows times KV heads of a call on pools are at most
  * MAX_POOL_ROWS, so that a launch over one pool has less than 2^32 threads. */

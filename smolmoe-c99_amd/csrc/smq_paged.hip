@@ -460,7 +460,7 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
  * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
  *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
  *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). */
-AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
+AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, bool tree) {
     AttendPlan p;
     const uint32_t G = a.heads / a.kv_heads;
     const uint64_t rows = (uint64_t)a.tokens * G, seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
@@ -470,7 +470,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
     p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) >> p.row_shift);
     const uint32_t groups = p.owns || a.head_dim <= 64 ? 512 : 256;
     p.stream = (groups + a.kv_heads - 1) / a.kv_heads;
-    p.tile_tokens = p.tile_rows / G + 1;
+    p.tile_tokens = tree ? a.tokens : p.tile_rows / G + 1; /* a tree's tile goes over all new tokens of its sequence */
     p.fixed = 64 * (PA_FIXED + 1);
     uint64_t most = a.limit + PA_STEP; /* positions of a tile's steps */
     if (a.window) {
@@ -481,12 +481,12 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
     p.unit = 0; /* all units and the last workgroup's end below 2^31 */
     while (((uint64_t)(p.tiles + 512) * ((most >> p.unit) + 1)) >= 1u << 30) ++p.unit;
     p.cw = (uint32_t)(most >> p.unit) + 1;
-    p.c1 = 2 * p.tile_rows / G >> p.unit;
+    p.c1 = tree ? 0 : 2 * p.tile_rows / G >> p.unit;
     /* tiles of an even batch, the steps of the longest and of the mean */
     const uint64_t tiles = seqs * ((rows / (seqs ? seqs : 1) + p.tile_rows - 1) >> p.row_shift) * a.kv_heads;
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
     if (p.owns && tiles > 256) {
-        const uint64_t average = steps - (a.window ? 0 : min(rows / G / seqs / 64, steps / 2));
+        const uint64_t average = steps - (a.window || tree ? 0 : min(rows / G / seqs / 64, steps / 2));
         if (tiles >= 512 || average * (512 - tiles) / 256 <= 24) p.stream = 0;
     } else if (tiles >= groups || steps * (groups - tiles) / groups <= 24) {
         p.stream = 0;
@@ -507,12 +507,12 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows) {
  * 16 or 32 each. 32 where tiles are cut or many: a fragment read serves twice. Few whole tiles take as long as the longest
  * one's chain of steps, and a step of half the rows is shorter (2048 tokens from an empty cache, f16, 8 KV heads of 64: 71
  * us, 58; 1024 of 128: 51, 40; but 2048 of 128: 100, 104). */
-AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes) {
+AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes, bool tree) {
     const uint32_t ks = attend_ks(a.head_dim);
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
-    if (rows <= 32 * seqs) return plan_tiles(a, ws_bytes, 16);
-    const AttendPlan p = plan_tiles(a, ws_bytes, 64 * attend_rt(ks));
-    return p.stream || p.tile_rows == 64 || rows / 128 * a.kv_heads * ks >= 2048 ? p : plan_tiles(a, 0, 64);
+    if (rows <= 32 * seqs) return plan_tiles(a, ws_bytes, 16, tree);
+    const AttendPlan p = plan_tiles(a, ws_bytes, 64 * attend_rt(ks), tree);
+    return p.stream || p.tile_rows == 64 || rows / 128 * a.kv_heads * ks >= 2048 ? p : plan_tiles(a, 0, 64, tree);
 }
 
 }  // namespace
@@ -553,21 +553,28 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
     return hipGetLastError();
 }
 
-size_t paged_attention_workspace(const PagedArgs &given) {
+size_t paged_attention_workspace(const PagedArgs &given, bool tree) {
     PagedArgs a = given;
     a.sinks = a.limit; /* the call brings them: a plan of more positions needs no fewer bytes, up to all of the context's */
-    const AttendPlan p = attend_plan(a, ~(size_t)0);
+    const AttendPlan p = attend_plan(a, ~(size_t)0, tree);
     return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
 }
 
-hipError_t launch_paged_attention(const PagedArgs &a, const float *q, float *att, void *ws, size_t ws_bytes,
-                                  hipStream_t s) {
-    const AttendPlan p = attend_plan(a, ws_bytes);
+hipError_t launch_paged_attention(const PagedArgs &a, const TreeArgs *tree, const float *q, float *att, void *ws,
+                                  size_t ws_bytes, hipStream_t s) {
+    const AttendPlan p = attend_plan(a, ws_bytes, tree != nullptr);
     i4 *used = p.stream ? (i4 *)ws : nullptr;
     float *part = p.stream ? (float *)((char *)ws + attend_used_bytes(a, p)) : nullptr;
-    hipError_t e = a.type == 0 ? launch_attend<0>(a, p, q, att, used, part, s)
-                 : a.type == 1 ? launch_attend<1>(a, p, q, att, used, part, s)
-                               : launch_attend<2>(a, p, q, att, used, part, s);
+    const TreeArgs t = tree ? *tree : TreeArgs{};
+    hipError_t e;
+    if (tree)
+        e = a.type == 0 ? launch_attend<0, true>(a, t, p, q, att, used, part, s)
+          : a.type == 1 ? launch_attend<1, true>(a, t, p, q, att, used, part, s)
+                        : launch_attend<2, true>(a, t, p, q, att, used, part, s);
+    else
+        e = a.type == 0 ? launch_attend<0, false>(a, t, p, q, att, used, part, s)
+          : a.type == 1 ? launch_attend<1, false>(a, t, p, q, att, used, part, s)
+                        : launch_attend<2, false>(a, t, p, q, att, used, part, s);
     if (e != hipSuccess || !p.stream) return e;
     const uint32_t per = JOIN_WG / (a.head_dim / 4), groups = (p.tile_rows + per - 1) / per;
     hipLaunchKernelGGL(k_paged_join, dim3(a.kv_heads * p.tiles * groups), dim3(JOIN_WG), 0, s, a, att, p, used, part);

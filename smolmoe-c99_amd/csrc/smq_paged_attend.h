@@ -52,7 +52,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 struct AttendPlan {
     bool owns;
     uint32_t tile_rows, row_shift, tiles, stream, most, pieces;
-    uint32_t unit, fixed, c1, cw, tile_tokens; /* units; tokens of a tile, at most */
+    uint32_t unit, fixed, c1, cw, tile_tokens; /* units; new tokens whose positions a tile goes over, at most */
 };
 /* The workspace: per tile and KV head four words (its pieces, its rows << 16; the sequence's first token; the first row;
  * the first piece's number), then per piece and KV head tile_rows rows: O, and behind all of them the maxima and sums. */
@@ -61,9 +61,10 @@ inline size_t attend_piece_bytes(const PagedArgs &a, uint32_t tile_rows) { /* of
     return (size_t)a.kv_heads * tile_rows * (a.head_dim + 2) * 4;
 }
 
-template <uint32_t TYPE>
-hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
-                         hipStream_t s);
+/* TREE: the mask's rows say which of its sequence's new tokens a token sees (t is not read otherwise). */
+template <uint32_t TYPE, bool TREE>
+hipError_t launch_attend(const PagedArgs &a, const TreeArgs &t, const AttendPlan &p, const float *q, float *att, i4 *used,
+                         float *part, hipStream_t s);
 
 /* RT, at most, of the kernels whose waves own rows, by the head size's 32-wide steps, and waves per SIMD. Two column tiles
  * and two waves: each fragment read from LDS serves twice, one wave's softmax runs beside the other's products, and the
@@ -375,6 +376,16 @@ __device__ __forceinline__ Span span_of(const PagedArgs &a, int pmin, int pmax) 
     return s;
 }
 
+/* What some token of a tree may see, depths aside: the context of a token that stands right behind it, and all new tokens. */
+__device__ __forceinline__ Span tree_span(const PagedArgs &a, const Seq &sq) {
+    const uint32_t ctx = (uint32_t)max(sq.first, 0);
+    Span s;
+    s.high = min(sq.first + sq.n, (int)a.limit) - 1;
+    s.low = a.window && ctx + 1 > a.window ? ctx + 1 - a.window : 0;
+    s.sinks = a.window ? min(a.sinks, ctx) : 0;
+    return s;
+}
+
 /* A sequence's pages for one KV head. SMALL: pages of 16 positions, so that a step of 32 lies in two; else in one. The
  * page ids are read 64 at a time, one per lane. */
 template <uint32_t TYPE, bool SMALL>
@@ -437,16 +448,22 @@ struct Pages {
 };
 
 /* A wave's rows: queries, positions, and the running maximum, sum and O. */
-template <uint32_t TYPE, int KS, int RT>
+template <uint32_t TYPE, int KS, int RT, bool TREE>
 struct Rows {
     static constexpr int DT = 2 * KS;
     typedef typename Elem<TYPE>::Frag Frag;
 
     const PagedArgs &a;
+    const TreeArgs &tree;
     uint32_t lane, col, quad;
     /* What this lane's column sees: positions of [from, from + reach] and below first. */
     uint32_t from[RT], reach[RT], first[RT];
     int row[RT]; /* of q and att; -1: none */
+    /* TREE: from, reach and first are of the context (its size: ctx, negative where rows have no place); mrow is the row's
+     * token in the mask, -1: sees nothing; vis: which of the lane's 8 positions of the step each column sees (of a step that
+     * not every row sees whole). */
+    int ctx, count_new, mrow[TREE ? RT : 1];
+    uint32_t vis[TREE ? RT : 1];
     float factor[RT];   /* of a product: the score's scale, log2 e, the row's power of two */
     QFrag<TYPE> qf[RT][KS];
     int pmin;
@@ -465,7 +482,8 @@ struct Rows {
 
     /* `count` rows of the sequence from row0 on; columns past them see what the first one sees and are not stored. First
      * what they see, then (queries) their values, so that loads of keys can run beside those. */
-    __device__ __forceinline__ Rows(const PagedArgs &a_, const Seq &sq, uint32_t kh, uint32_t row0, int count) : a(a_) {
+    __device__ __forceinline__ Rows(const PagedArgs &a_, const TreeArgs &t_, const Seq &sq, uint32_t kh, uint32_t row0, int count)
+        : a(a_), tree(t_) {
         lane = threadIdx.x % 64;
         col = lane % 16;
         quad = lane / 16;
@@ -479,14 +497,33 @@ struct Rows {
             const uint32_t up = (uint32_t)(((float)r + 0.5f) * inv); /* r / G: r is below 2^17, where this is exact */
             const uint32_t tok = tok0 + up, g = r - up * G;
             const uint32_t p = (uint32_t)(sq.first + (int)tok);
-            const bool place = p < a.limit;
-            if (in && !place) *a.flag = 1;
-            const int pc = place ? (int)p : -1;
-            from[c] = !place ? 0xffffffffu : a.window && p + 1 > a.window ? p + 1 - a.window : 0;
-            reach[c] = place ? p - from[c] : 0;
-            first[c] = a.window ? min(a.sinks, (uint32_t)(pc + 1)) : 0;
-            lo = min(lo, pc);
-            hi = max(hi, pc);
+            bool place = p < a.limit;
+            if constexpr (TREE) {
+                const uint32_t end = (uint32_t)max(sq.first, 0);
+                uint32_t low = 0;
+                place = place && (uint32_t)sq.n <= 32 * tree.words;
+                if (a.window) { /* from the token's own position, behind the context by its depth */
+                    const uint32_t d = (uint32_t)tree.depth[sq.begin + (int)tok], at = end + min(d, a.context);
+                    place = place && at < a.context;
+                    low = at + 1 > a.window ? at + 1 - a.window : 0;
+                }
+                if (in && !place) *a.flag = 1;
+                const bool some = place && low < end;
+                from[c] = some ? low : 0xffffffffu;
+                reach[c] = some ? end - 1 - low : 0;
+                first[c] = place && a.window ? min(a.sinks, end) : 0;
+                mrow[c] = place ? sq.begin + (int)tok : -1;
+                lo = min(lo, place ? (int)end - 1 : -1); /* of what every row sees: the last position and the first */
+                hi = max(hi, place ? (int)low : 0);
+            } else {
+                if (in && !place) *a.flag = 1;
+                const int pc = place ? (int)p : -1;
+                from[c] = !place ? 0xffffffffu : a.window && p + 1 > a.window ? p + 1 - a.window : 0;
+                reach[c] = place ? p - from[c] : 0;
+                first[c] = a.window ? min(a.sinks, (uint32_t)(pc + 1)) : 0;
+                lo = min(lo, pc);
+                hi = max(hi, pc);
+            }
             row[c] = in ? (int)(((uint32_t)sq.begin + tok) * a.heads + kh * G + g) : -1; /* below 2^22 */
         }
 #pragma unroll
@@ -495,9 +532,17 @@ struct Rows {
             hi = max(hi, __shfl_xor(hi, off));
         }
         pmin = __builtin_amdgcn_readfirstlane(lo);
-        const int pmax = __builtin_amdgcn_readfirstlane(hi);
-        span = span_of(a, pmin, pmax);
-        low_last = span_of(a, pmax, pmax).low;
+        int pmax = __builtin_amdgcn_readfirstlane(hi);
+        if constexpr (TREE) {
+            ctx = sq.first;
+            count_new = sq.n;
+            low_last = (uint32_t)pmax;
+            span = tree_span(a, sq);
+            pmax = span.high;
+        } else {
+            span = span_of(a, pmin, pmax);
+            low_last = span_of(a, pmax, pmax).low;
+        }
         unit = TYPE == 0 ? __builtin_ldexpf(1.0f, pmax > 0 ? __builtin_clz((uint32_t)pmax) - 33 : -1) : 1.0f;
 #pragma unroll
         for (int c = 0; c < RT; ++c)
@@ -550,6 +595,19 @@ struct Rows {
     }
 
     __device__ __forceinline__ bool sees(uint32_t pos, int c) const { return pos - from[c] <= reach[c] || pos < first[c]; }
+    /* TREE: the lane's 8 positions from p on that column c sees, a bit each. The bits of new tokens come out of two words of
+     * the mask, whichever they are: position p is new token i, before the first one the words are 0. */
+    __device__ __forceinline__ uint32_t seen8(uint32_t p, int c) const {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bits |= sees(p + j, c) ? 1u << j : 0;
+        const int i = (int)p - ctx, w = i >> 5, left = count_new - i;
+        if (mrow[c] < 0 || i <= -8 || left <= 0) return bits;
+        const uint32_t *m = tree.mask + (size_t)mrow[c] * tree.words;
+        const uint64_t lo = w >= 0 ? m[w] : 0, hi = w + 1 < (int)tree.words ? m[w + 1] : 0;
+        const uint32_t x = (uint32_t)((lo | hi << 32) >> (i & 31)) & 255;
+        return bits | (left < 8 ? x & ((1u << left) - 1) : x);
+    }
     /* Whether every row sees all of the step at p0 (rows without a place: pmin -1, never). */
     __device__ __forceinline__ bool full(uint32_t p0, uint32_t ok) const {
         const uint32_t last = p0 + PA_STEP - 1;
@@ -612,9 +670,11 @@ struct Rows {
             /* positions of a page that is none: past every row */
             const uint32_t p = ok >> (quad >> 1) & 1 ? p0 + quad * 8 : 0xfffffff0u;
 #pragma unroll
-            for (int c = 0; c < RT; ++c)
+            for (int c = 0; c < RT; ++c) {
+                if constexpr (TREE) vis[c] = seen8(p, c);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[c][j] = sees(p + j, c) ? x[c][j] : -INFINITY;
+                for (int j = 0; j < 8; ++j) x[c][j] = (TREE ? vis[c] >> j & 1 : sees(p + j, c)) ? x[c][j] : -INFINITY;
+            }
         }
         bool up = false;
         float mx[RT];
@@ -678,7 +738,7 @@ struct Rows {
         for (int c = 0; c < RT; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if ((bits >> j & 1) && sees(p0 + quad * 8 + j, c)) l[c] = __builtin_nanf("");
+                if ((bits >> j & 1) && (TREE ? vis[c] >> j & 1 : sees(p0 + quad * 8 + j, c))) l[c] = __builtin_nanf("");
     }
 
     /* O += V^T P^T. In a step that not every row sees whole, a value that is not finite would reach rows that do not see
@@ -1047,13 +1107,13 @@ struct Out {
 /* 16 rows or fewer: the waves take the steps [u0, u1) in turn, each with its steps' keys and values in registers, and
  * join their results in LDS. In turn, not in runs: a step's values are 64 bytes (f16) of each dim's row in the page, and
  * the cache lines' other halves are the next steps'; with runs half of every line was fetched twice. The keys of a wave's next step are requested as soon as this step's are used. */
-template <uint32_t TYPE, int KS, bool SMALL>
-__device__ __forceinline__ void tile_shared(const PagedArgs &a, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
+template <uint32_t TYPE, int KS, bool SMALL, bool TREE>
+__device__ __forceinline__ void tile_shared(const PagedArgs &a, const TreeArgs &tree, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
                                             uint32_t u0, uint32_t u1, uint32_t wave, const Out &out, unsigned char *lds) {
     constexpr int LD = 32 * KS + 4;
     float(*so)[16][LD] = (float(*)[16][LD])lds;
     float(*sml)[16][2] = (float(*)[16][2])(lds + PA_WAVES * 16 * LD * 4);
-    Rows<TYPE, KS, 1> w(a, sq, out.kh, out.row0, (int)out.n);
+    Rows<TYPE, KS, 1, TREE> w(a, tree, sq, out.kh, out.row0, (int)out.n);
     u0 += wave;
     if (u0 >= u1) {
         w.queries(q);
@@ -1106,17 +1166,17 @@ constexpr uint32_t shared_lds(int ks) { return PA_WAVES * 16 * (32 * ks + 4) * 4
 
 /* Each wave has 16 * RT rows of the tile over the steps [u0, u1), whose keys and values the workgroup brings to LDS, the
  * next step's while this one is computed. A wave without rows (or whose rows do not see a step) only loads. */
-template <uint32_t TYPE, int KS, int RT, bool SMALL>
-__device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
+template <uint32_t TYPE, int KS, int RT, bool SMALL, bool TREE>
+__device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &tree, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
                                            uint32_t u0, uint32_t u1, uint32_t wave, const Out &out, unsigned char *lds) {
     typedef InLds<TYPE, KS, SMALL> Src;
     const uint32_t first = wave * 16 * RT, G = a.heads / a.kv_heads;
     const bool mine = first < out.n;
     /* the last wave's rows again where there are none: never stored */
-    Rows<TYPE, KS, RT> w(a, sq, out.kh, out.row0 + (mine ? first : 0), mine ? (int)min(16u * RT, out.n - first) : 1);
+    Rows<TYPE, KS, RT, TREE> w(a, tree, sq, out.kh, out.row0 + (mine ? first : 0), mine ? (int)min(16u * RT, out.n - first) : 1);
     /* what the tile sees: the pages that the workgroup needs */
     const int tmin = sq.first + (int)(out.row0 / G), tmax = min(sq.first + (int)((out.row0 + out.n - 1) / G), (int)a.limit - 1);
-    const Span span = span_of(a, max(-1, tmin), max(-1, tmax));
+    const Span span = TREE ? tree_span(a, sq) : span_of(a, max(-1, tmin), max(-1, tmax));
     if (u0 >= u1) {
         w.queries(q);
     } else {
@@ -1161,12 +1221,14 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const float *q, c
 }
 
 /* A tile's piece. */
-template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
-__device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used,
+template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL, bool TREE>
+__device__ __forceinline__ void tile_part(const PagedArgs &a, const TreeArgs &tree, const AttendPlan &p, const float *q, float *att, i4 *used,
                                           float *part, uint32_t kh, const Tile &t, unsigned char *lds) {
     const uint32_t G = a.heads / a.kv_heads, row0 = t.j * p.tile_rows, n = min(p.tile_rows, (uint32_t)t.sq.n * G - row0);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Steps st = tile_steps(a, t.sq.first + (int)(row0 / G), t.sq.first + (int)((row0 + n - 1) / G));
+    /* a tree's rows may see any of the new tokens, and the context that the first position behind it sees */
+    const Steps st = TREE ? tile_steps(a, t.sq.first, t.sq.first + t.sq.n - 1)
+                          : tile_steps(a, t.sq.first + (int)(row0 / G), t.sq.first + (int)((row0 + n - 1) / G));
     Out out = {a, t.sq, kh, row0, n, att, nullptr, nullptr};
     uint32_t u0 = 0, u1 = st.total;
     if (p.stream && t.piece == 0 && threadIdx.x == 0)
@@ -1180,20 +1242,20 @@ __device__ __forceinline__ void tile_part(const PagedArgs &a, const AttendPlan &
     }
     if constexpr (OWNS) {
         if (n > 16) {
-            tile_owned<TYPE, KS, RT, SMALL>(a, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
+            tile_owned<TYPE, KS, RT, SMALL, TREE>(a, tree, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
             return;
         }
     }
-    tile_shared<TYPE, KS, SMALL>(a, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
+    tile_shared<TYPE, KS, SMALL, TREE>(a, tree, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
 }
 
 /* Workgroups of one KV head follow each other at a distance of all heads, so where these are a multiple of the eight XCDs
  * the tiles of a sequence that read the same pages share an L2. From the last tile to the first: the last rows of a chunk
  * see the most. A piece has a workgroup of its own: a loop over several costs the products their registers (heads of 128:
  * 40 spilled), and one that takes a second piece, however short, pays a tile's fixed cost twice. */
-template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
-__global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_attend(PagedArgs a, const float *q, float *att,
-                                                                                  AttendPlan p, i4 *used, float *part) {
+template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL, bool TREE>
+__device__ __forceinline__ void attend_piece(const PagedArgs &a, const TreeArgs &tree, const float *q, float *att,
+                                             const AttendPlan &p, i4 *used, float *part) {
     constexpr uint32_t OWN_LDS = OWNS ? 2 * InLds<TYPE, KS, SMALL>::BUFFER : 0;
     __shared__ __attribute__((aligned(16))) unsigned char lds[OWN_LDS > shared_lds(KS) ? OWN_LDS : shared_lds(KS)];
     const uint32_t kh = blockIdx.x % a.kv_heads, i = blockIdx.x / a.kv_heads;
@@ -1211,18 +1273,34 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
             if (!count || !tiles.by_piece(p.pieces - 1 - i, units, count, t)) return;
         }
     }
-    tile_part<TYPE, KS, RT, OWNS, SMALL>(a, p, q, att, used, part, kh, t, lds);
+    tile_part<TYPE, KS, RT, OWNS, SMALL, TREE>(a, tree, p, q, att, used, part, kh, t, lds);
+}
+template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
+__global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_attend(PagedArgs a, const float *q, float *att,
+                                                                                  AttendPlan p, i4 *used, float *part) {
+    attend_piece<TYPE, KS, RT, OWNS, SMALL, false>(a, TreeArgs{}, q, att, p, used, part);
+}
+template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
+__global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_tree(PagedArgs a, TreeArgs tree, const float *q,
+                                                                                float *att, AttendPlan p, i4 *used, float *part) {
+    attend_piece<TYPE, KS, RT, OWNS, SMALL, true>(a, tree, q, att, p, used, part);
 }
 
 }  // namespace
 
-template <uint32_t TYPE>
-hipError_t launch_attend(const PagedArgs &a, const AttendPlan &p, const float *q, float *att, i4 *used, float *part,
-                         hipStream_t s) {
+template <uint32_t TYPE, bool TREE>
+hipError_t launch_attend(const PagedArgs &a, const TreeArgs &t, const AttendPlan &p, const float *q, float *att, i4 *used,
+                         float *part, hipStream_t s) {
     const dim3 grid(a.kv_heads * (p.stream ? p.pieces : p.tiles));
-#define SMQ_ATTEND3(KS, RT, OWNS, SMALL)                                                                               \
-    hipLaunchKernelGGL((k_paged_attend<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(64 * PA_WAVES), 0, s, a, q, att, p, used, \
-                       part)
+#define SMQ_ATTEND3(KS, RT, OWNS, SMALL)                                                                                 \
+    do {                                                                                                                 \
+        if constexpr (TREE)                                                                                              \
+            hipLaunchKernelGGL((k_paged_tree<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(64 * PA_WAVES), 0, s, a, t, q, att, \
+                               p, used, part);                                                                           \
+        else                                                                                                             \
+            hipLaunchKernelGGL((k_paged_attend<TYPE, KS, RT, OWNS, SMALL>), grid, dim3(64 * PA_WAVES), 0, s, a, q, att,  \
+                               p, used, part);                                                                           \
+    } while (0)
 #define SMQ_ATTEND(KS)                                                            \
     do {                                                                          \
         constexpr int RT = attend_rt(KS);                                         \

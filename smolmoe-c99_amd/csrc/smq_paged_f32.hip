@@ -3,6 +3,6 @@
 #include "smq_paged_attend.h"
 
 namespace smq {
-template hipError_t launch_attend<0>(const PagedArgs &, const AttendPlan &, const float *, float *, i4 *, float *,
-                                       hipStream_t);
+template hipError_t launch_attend<0, false>(const PagedArgs &, const TreeArgs &, const AttendPlan &, const float *, float *,
+                                              i4 *, float *, hipStream_t);
 }  // namespace smq

@@ -429,8 +429,9 @@ def test_tree_rows_that_are_refused_on_the_device(kv_type):
     keep = trees.depth.copy()
     for d in (-1, 10, 2 ** 31 - 1, -2 ** 31):  # 70 + 10 is the context
         trees.depth[3] = d
-        check([3])
-        check([3], split=False)
+        check([3], window=1000)
+        check([3], window=1000, split=False)
+        check([])  # without a window depths are not read
     trees.depth = keep
     trees.words, trees.stride = trees.words[:, :1].copy(), 1
     check(list(range(10, 50)))
