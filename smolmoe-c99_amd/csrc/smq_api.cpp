@@ -1815,12 +1815,13 @@ static bool beam_args(const smq_beam_step *b, const char *who, smq::BeamArgs *ou
         return false;
     }
     if (!b->beams || b->beams > smq::MAX_BEAMS || !b->select || b->select > smq::MAX_SELECT || !b->vocab ||
-        b->vocab > (1u << 30) || (uint64_t)b->groups * b->beams > smq::MAX_BEAM_ROWS ||
+        b->vocab > smq::MAX_BEAM_VOCAB || (uint64_t)b->groups * b->beams > smq::MAX_BEAM_ROWS ||
         (uint64_t)b->groups * b->select > smq::MAX_BEAM_ROWS) {
         set_status(SMQ_ERR_RANGE,
                    "%s: unsupported step (%u groups of %u beams of 1 .. %u, %u selected of 1 .. %u, at most %u rows, "
-                   "a vocabulary of %u ids)",
-                   who, b->groups, b->beams, smq::MAX_BEAMS, b->select, smq::MAX_SELECT, smq::MAX_BEAM_ROWS, b->vocab);
+                   "a vocabulary of %u ids of 1 .. %u)",
+                   who, b->groups, b->beams, smq::MAX_BEAMS, b->select, smq::MAX_SELECT, smq::MAX_BEAM_ROWS, b->vocab,
+                   smq::MAX_BEAM_VOCAB);
         return false;
     }
     *out = {b->logits, b->stride, b->groups, b->beams, b->vocab, b->select, b->score, b->done, b->pad, b->eos, b->parent,

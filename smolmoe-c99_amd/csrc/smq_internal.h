@@ -334,7 +334,7 @@ hipError_t launch_paged_compact(const PagedArgs &a, const Pool *pools, uint32_t 
                                 const int32_t *count, int32_t *length_out, hipStream_t s);
 
 /* A step of a beam search (csrc/smq_beam.hip). */
-constexpr uint32_t MAX_BEAMS = 64, MAX_SELECT = 64, MAX_BEAM_ROWS = 65535;
+constexpr uint32_t MAX_BEAMS = 64, MAX_SELECT = 64, MAX_BEAM_ROWS = 65535, MAX_BEAM_VOCAB = 1u << 20;
 struct BeamArgs {
     const float *logits;
     size_t stride;
