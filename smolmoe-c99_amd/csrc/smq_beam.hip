@@ -14,7 +14,7 @@ namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t BM_WG = 256, BM_WAVES = BM_WG / 64, NONE = 0xffffffffu;
-constexpr uint32_t BM_BLOCK = 64, BM_LANES = BM_BLOCK / 4; /* ids of a block, lanes that have four each */
+constexpr uint32_t BM_BLOCK = 64, BM_LANES = 16; /* ids of a block, lanes that have four each */
 
 /* Keys of one row: the larger logit, then the lower id, is the larger key. 0: no candidate. */
 __device__ __forceinline__ uint64_t key_of(float l, uint32_t id) {
@@ -40,10 +40,13 @@ __device__ __forceinline__ uint64_t order_of(double x) { /* as key_of; not 0 */
 }
 __device__ __forceinline__ double value_of(uint64_t v) { return __longlong_as_double(v >> 63 ? v & ~(1ull << 63) : ~v); }
 
-/* 2^(x log2 e), x <= 0: the polynomial of 2^f on [-1/2, 1/2] with the least relative error of its degree, 1.4e-14. 16
- * instructions on 64 bits, which run at the rate of those on 32; the library's exp takes over twice as many. */
+/* e^x, x <= 0 (below -700, -infinity too, as at -700: nothing beside the largest term, 1): x log2 e to a whole number, which
+ * the sum with 1.5 * 2^52 leaves in its low bits, and f in [-1/2, 1/2], whose 2^f is the polynomial with the least relative
+ * error of its degree, 1.4e-14. 15 instructions on 64 bits, which run at the rate of those on 32. */
 __device__ __forceinline__ double exp_of(double x) {
-    const double t = fmax(x * 0x1.71547652b82fep+0, -1100.0), n = __builtin_rint(t), f = t - n;
+    x = fmax(x, -700.0);
+    const double log2e = 0x1.71547652b82fep+0, magic = 0x1.8p+52;
+    const double r = __builtin_fma(x, log2e, magic), f = __builtin_fma(x, log2e, -(r - magic));
     double p = 0x1.b4014c1ff3fbep-24;
     p = __builtin_fma(p, f, 0x1.63ee359dfa9f3p-20);
     p = __builtin_fma(p, f, 0x1.ffce18ebcfb6cp-17);
@@ -54,18 +57,35 @@ __device__ __forceinline__ double exp_of(double x) {
     p = __builtin_fma(p, f, 0x1.ebfbdff81568ap-3);
     p = __builtin_fma(p, f, 0x1.62e42fefa374fp-1);
     p = __builtin_fma(p, f, 0x1.0000000000039p+0);
-    return __builtin_ldexp(p, (int)n);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ T reduce(T x, T *lds, F f) { /* over the workgroup */
-    for (int off = 1; off < 64; off *= 2) x = f(x, __shfl_xor(x, off));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
-    __syncthreads();
-    x = lds[0];
-    for (uint32_t w = 1; w < BM_WAVES; ++w) x = f(x, lds[w]);
-    return x;
+/* x with its neighbour's by a rotation in rows of 16 lanes. */
+template <int N>
+__device__ __forceinline__ int turned(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, false);
+}
+template <int N>
+__device__ __forceinline__ float turned(float x) {
+    return __int_as_float(turned<N>(__float_as_int(x)));
+}
+template <int N>
+__device__ __forceinline__ double turned(double x) {
+    return __hiloint2double(turned<N>(__double2hiint(x)), turned<N>(__double2loint(x)));
+}
+__device__ __forceinline__ float max_row(float x) { /* of 16 lanes */
+    x = fmaxf(x, turned<8>(x));
+    x = fmaxf(x, turned<4>(x));
+    x = fmaxf(x, turned<2>(x));
+    return fmaxf(x, turned<1>(x));
+}
+__device__ __forceinline__ double sum_wave(double x) {
+    x += turned<8>(x);
+    x += turned<4>(x);
+    x += turned<2>(x);
+    x += turned<1>(x);
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
 }
 
 /* What the first launch leaves of a row: block maxima (NaN where an id's logit is NaN or +inf), and of each wave of its
@@ -101,8 +121,7 @@ __global__ __launch_bounds__(BM_WG) void k_beam_sums(BeamArgs a, Sums s) {
         bool bad = false;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) bad = bad || !(l[u][e] < INFINITY);
-#pragma unroll
-        for (int off = 1; off < (int)BM_LANES; off *= 2) m = fmaxf(m, __shfl_xor(m, off));
+        m = max_row(m);
         const uint64_t those = __ballot(bad);
         const uint32_t block = (wave * U + u) * (64 / BM_LANES) + lane / BM_LANES;
         if (lane % BM_LANES == 0 && block < s.blocks) s.top[(size_t)r * s.blocks + block] = those ? __builtin_nanf("") : m;
@@ -116,86 +135,110 @@ __global__ __launch_bounds__(BM_WG) void k_beam_sums(BeamArgs a, Sums s) {
     for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) sum += exp_of((double)l[u][e] - off);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    sum = sum_wave(sum);
     if (lane == 0) s.sum[(size_t)r * s.sums + wave] = sum;
 }
 
-/* The `most` largest keys of list[0 .. m), descending, into best; returns their number. Until a list has 256 keys: of each
+/* The `most`-th largest of some keys of which no two are equal but zeros: of keys[0 .. n), which all threads have written; 0 if
+ * there are fewer. Every wave finds it for itself: no barrier. */
+template <typename K>
+__device__ __forceinline__ K kth_of(const K *keys, uint32_t n, uint32_t most) {
+    K found = {};
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const K mine = keys[i0 + threadIdx.x % 64];
+        uint32_t rank = 0;
+#pragma unroll 16
+        for (uint32_t i = 0; i < n; ++i) rank += keys[i] > mine;
+        const uint64_t hit = __ballot(rank == most - 1 && some(mine));
+        if (hit) found = keys[i0 + __ffsll((unsigned long long)hit) - 1];
+    }
+    return found;
+}
+
+/* The `most` largest keys of list[0 .. m), descending, into best; returns their number. Until a list has BM_WG keys: of each
  * thread's keys the largest, of these the most-th largest, and only keys that are no smaller go on: those of `most` threads
- * at most, to the other of two lists (list, other) in turn. Then each key is put where its rank says. */
+ * at most, to the other of two lists (list, other) in turn. Then each key is put where its rank says. Begins with a
+ * barrier, and ends with one. */
 template <typename K>
 __device__ __forceinline__ uint32_t best_of(K *list, K *other, uint32_t m, uint32_t most, K *keys, K *best, uint32_t *count) {
     const uint32_t tid = threadIdx.x;
     const K zero = {};
+    __syncthreads();
     while (m > BM_WG) {
         K mine = zero;
         for (uint32_t i = tid; i < m; i += BM_WG) mine = list[i] > mine ? list[i] : mine;
-        __syncthreads();
         keys[tid] = mine;
-        if (tid == 0) {
-            *count = 0;
-            best[0] = zero;
-        }
+        if (tid == 0) *count = 0;
         __syncthreads();
-        uint32_t rank = 0;
-#pragma unroll 8
-        for (uint32_t i = 0; i < BM_WG; ++i) rank += keys[i] > mine;
-        if (rank == most - 1 && some(mine)) best[0] = mine;
-        __syncthreads();
-        const K least = best[0];
+        const K least = kth_of(keys, BM_WG, most);
         for (uint32_t i = tid; i < m; i += BM_WG)
-            if (some(list[i]) && !(least > list[i])) other[atomicAdd(count, 1u)] = list[i];
+            if (!(least > list[i])) other[atomicAdd(count, 1u)] = list[i];
         __syncthreads();
         m = *count;
         K *x = list;
         list = other;
         other = x;
+        __syncthreads();
+    }
+    if (tid < m) {
+        const K mine = list[tid];
+        uint32_t rank = 0;
+#pragma unroll 16
+        for (uint32_t i = 0; i < m; ++i) rank += list[i] > mine;
+        if (rank < most) best[rank] = mine;
     }
     __syncthreads();
-    keys[tid] = tid < m ? list[tid] : zero;
-    if (tid == 0) *count = 0;
-    __syncthreads();
-    const K mine = keys[tid];
-    uint32_t rank = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < BM_WG; ++i) rank += keys[i] > mine;
-    if (some(mine) && rank < most) {
-        best[rank] = mine;
-        atomicMax(count, rank + 1);
-    }
-    __syncthreads();
-    return *count;
+    return min(m, most);
 }
 /* LDS of the lists: the first one's keys, and what of it can go on. */
 __host__ __device__ inline uint32_t list_next(uint32_t first, uint32_t most) { return most * ((first + BM_WG - 1) / BM_WG); }
+/* Columns that a row's blocks are dealt to, and of whose maxima the select-th largest bounds the list: 64, one per lane, where
+ * that keeps lists short. */
+__host__ __device__ inline uint32_t columns_of(uint32_t blocks, uint32_t select) { return select <= 32 && blocks <= 4096 ? 64 : BM_WG; }
 
-/* A workgroup per row: its `select` best ids and their values. */
+/* A workgroup per row: its `select` best ids and their values. What the row's blocks have is requested at once; the best
+ * blocks' logits are on their way while the sums are joined. */
 __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double *value, uint32_t *id) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ double sums[BM_WAVES];
-    __shared__ float tops[BM_WAVES];
-    __shared__ int bads[BM_WAVES];
     __shared__ uint64_t keys[BM_WG], best[MAX_SELECT], blocks[MAX_SELECT];
-    __shared__ uint32_t count;
+    __shared__ uint32_t counts[3];
     uint64_t *list = (uint64_t *)lds, *other = list + a.select * BM_BLOCK;
-    const uint32_t r = blockIdx.x, tid = threadIdx.x;
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, columns = columns_of(s.blocks, a.select);
     const float *row = a.logits + (size_t)r * a.stride, *bt = s.top + (size_t)r * s.blocks;
     const float score = a.score[r];
     value += (size_t)r * a.select;
     id += (size_t)r * a.select;
     const bool done = a.done && a.done[r];
-    float top = -INFINITY;
     int bad = !(score < INFINITY);
-    if (!done)
+    auto block_key = [&](uint32_t i) { return bt[i] == -INFINITY ? 0 : key_of(bt[i], i); };
+    uint64_t mine = 0;
+    if (!done) {
+#pragma unroll 4
         for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
             bad |= !(bt[i] < INFINITY);
-            top = fmaxf(top, bt[i]);
+            const uint64_t k = block_key(i);
+            mine = k > mine ? k : mine;
         }
-    bad = reduce(bad, bads, [](int x, int y) { return x | y; });
-    top = reduce(top, tops, [](float x, float y) { return fmaxf(x, y); });
+    }
+    keys[tid] = mine;
+    if (tid < 3) counts[tid] = 0;
+    bad = __syncthreads_or(bad);
+    if (columns == 64 && tid < 64) {
+#pragma unroll
+        for (uint32_t w = 1; w < BM_WAVES; ++w) mine = keys[w * 64 + tid] > mine ? keys[w * 64 + tid] : mine;
+        keys[tid] = mine;
+    }
+    __syncthreads();
+    uint64_t most = 0;
+    for (uint32_t i = tid % 64; i < columns; i += 64) most = keys[i] > most ? keys[i] : most;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+        const uint64_t o = __shfl_xor(most, off);
+        most = o > most ? o : most;
+    }
     if (bad && tid == 0) *a.flag = 1;
-    const bool none = bad || score == -INFINITY || (!done && top == -INFINITY);
+    const bool none = bad || score == -INFINITY || (!done && !most);
     if (none || done) {
         for (uint32_t k = tid; k < a.select; k += BM_WG) {
             value[k] = !none && k == 0 ? (double)score : -INFINITY;
@@ -203,58 +246,50 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
         }
         return;
     }
+    const double top = (double)logit_of(most);
+    /* the blocks that are no smaller than the select-th of the columns' maxima, and the best of them */
+    const uint64_t least = max(kth_of(keys, columns, a.select), (uint64_t)1);
+#pragma unroll 4
+    for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
+        const uint64_t k = block_key(i);
+        if (k >= least) list[atomicAdd(&counts[0], 1u)] = k;
+    }
+    __syncthreads();
+    const uint32_t listed = counts[0], nb = best_of(list, other, listed, a.select, keys, blocks, &counts[2]);
+    /* their ids, BM_WG / BM_LANES blocks at a time, a lane four */
+    const float low = nb == a.select ? logit_of(blocks[nb - 1]) : -FLT_MAX;
+    auto load = [&](uint32_t b, float(&l)[4]) {
+        const uint32_t i = b < nb ? id_of(blocks[b]) * BM_BLOCK + 4 * (tid % BM_LANES) : a.vocab;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) l[e] = i + e < a.vocab ? row[i + e] : -INFINITY;
+        return i;
+    };
+    float l[4];
+    uint32_t i = load(tid / BM_LANES, l);
     double sum = 0.0;
     for (uint32_t i = tid; i < s.sums; i += BM_WG) {
         float m = -INFINITY;
         for (uint32_t k = 0; k < s.per; ++k)
             if (i * s.per + k < s.blocks) m = fmaxf(m, bt[i * s.per + k]);
-        if (m > -INFINITY) sum += s.sum[(size_t)r * s.sums + i] * exp_of((double)m - (double)top);
+        if (m > -INFINITY) sum += s.sum[(size_t)r * s.sums + i] * exp_of((double)m - top);
     }
-    sum = reduce(sum, sums, [](double x, double y) { return x + y; });
-    const double lse = (double)top + log(sum);
-    /* the blocks: of each thread's the largest, and those that are no smaller than the select-th of these */
-    uint64_t mine = 0;
-    for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
-        const uint64_t k = bt[i] == -INFINITY ? 0 : key_of(bt[i], i);
-        mine = k > mine ? k : mine;
-    }
-    keys[tid] = mine;
-    if (tid == 0) {
-        count = 0;
-        best[0] = 1;
-    }
-    __syncthreads();
-    uint32_t rank = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < BM_WG; ++i) rank += keys[i] > mine;
-    if (rank == a.select - 1 && mine) best[0] = mine;
-    __syncthreads();
-    const uint64_t least = best[0];
-    for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
-        const uint64_t k = bt[i] == -INFINITY ? 0 : key_of(bt[i], i);
-        if (k >= least) list[atomicAdd(&count, 1u)] = k;
-    }
-    __syncthreads();
-    const uint32_t nb = best_of(list, other, count, a.select, keys, blocks, &count);
-    /* their ids */
-    __syncthreads();
-    if (tid == 0) count = 0;
-    const float low = nb == a.select ? logit_of(blocks[nb - 1]) : -FLT_MAX;
-    __syncthreads();
+    sum = sum_wave(sum);
+    if (tid % 64 == 0) sums[tid / 64] = sum;
     for (uint32_t b = tid / BM_LANES; b < nb; b += BM_WG / BM_LANES) {
-        const uint32_t i = id_of(blocks[b]) * BM_BLOCK + 4 * (tid % BM_LANES);
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-            const float l = i + e < a.vocab ? row[i + e] : -INFINITY;
-            if (l >= low) list[atomicAdd(&count, 1u)] = key_of(l, i + e);
-        }
+        for (uint32_t e = 0; e < 4; ++e)
+            if (l[e] >= low) list[atomicAdd(&counts[1], 1u)] = key_of(l[e], i + e);
+        i = load(b + BM_WG / BM_LANES, l);
     }
     __syncthreads();
-    const uint32_t n = best_of(list, other, count, a.select, keys, best, &count);
-    for (uint32_t k = tid; k < a.select; k += BM_WG) {
-        const uint64_t b = k < n ? best[k] : 0;
-        value[k] = b ? (double)score + ((double)logit_of(b) - lse) : -INFINITY;
-        id[k] = id_of(b);
+    sum = sums[0];
+#pragma unroll
+    for (uint32_t w = 1; w < BM_WAVES; ++w) sum += sums[w];
+    const uint32_t n = best_of(list, other, counts[1], a.select, keys, best, &counts[2]);
+    if (tid < a.select) {
+        const uint64_t b = tid < n ? best[tid] : 0;
+        value[tid] = b ? (double)score + ((double)logit_of(b) - (top + log(sum))) : -INFINITY;
+        id[tid] = id_of(b);
     }
 }
 
@@ -266,7 +301,7 @@ __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *v
     const uint32_t g = blockIdx.x / per, tid = threadIdx.x, n = a.beams * a.select;
     const size_t at = (size_t)g * n;
     Cand *list = (Cand *)lds, *other = list + (n > BM_WG ? list_next(n, a.select) : BM_WG);
-    auto cand = [&](uint32_t i) {
+    const auto cand = [&](uint32_t i) {
         const double v = value[at + i];
         return v > -INFINITY ? Cand{order_of(v), ~(uint64_t)i} : Cand{0, 0};
     };
@@ -278,27 +313,23 @@ __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *v
             mine = c > mine ? c : mine;
         }
         keys[tid] = mine;
-        if (tid == 0) {
-            count = 0;
-            best[0] = Cand{1, 0};
-        }
+        if (tid == 0) count = 0;
         __syncthreads();
-        uint32_t rank = 0;
-#pragma unroll 8
-        for (uint32_t i = 0; i < BM_WG; ++i) rank += keys[i] > mine;
-        if (rank == a.select - 1 && some(mine)) best[0] = mine;
-        __syncthreads();
-        const Cand least = best[0];
+        const Cand kth = kth_of(keys, BM_WG, a.select), least = some(kth) ? kth : Cand{1, 0};
         for (uint32_t i = tid; i < n; i += BM_WG) {
             const Cand c = cand(i);
             if (!(least > c)) list[atomicAdd(&count, 1u)] = c;
         }
         __syncthreads();
         m = count;
-    } else if (tid < n) {
-        list[tid] = cand(tid);
+    } else {
+        if (tid == 0) count = 0;
+        __syncthreads();
+        const Cand c = tid < n ? cand(tid) : Cand{0, 0};
+        if (some(c)) list[atomicAdd(&count, 1u)] = c;
+        __syncthreads();
+        m = count;
     }
-    __syncthreads();
     const uint32_t found = best_of(list, other, m, a.select, keys, best, &count);
     for (uint32_t k = blockIdx.x % per; k < a.select; k += per) {
         const uint32_t o = g * a.select + k, w = k < found ? (uint32_t)~best[k].i : 0;
