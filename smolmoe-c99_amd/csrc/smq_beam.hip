@@ -42,28 +42,34 @@ __device__ __forceinline__ double value_of(uint64_t v) { return __longlong_as_do
 
 /* e^x, x <= 0 (below -700, -infinity too, as at -700: nothing beside the largest term, 1): x log2 e to a whole number, which
  * the sum with 1.5 * 2^52 leaves in its low bits, and f in [-1/2, 1/2], whose 2^f is the polynomial with the least relative
- * error of its degree, 1.4e-14. 15 instructions on 64 bits, which run at the rate of those on 32. */
-__device__ __forceinline__ double exp_of(double x) {
+ * error of its degree, 7.8e-13. 14 instructions on 64 bits, which run at the rate of those on 32. lead: the polynomial's first
+ * coefficient, in vector registers (an instruction takes one scalar operand). */
+constexpr double EXP_LEAD = 0x1.61af6ea7cb2d7p-20;
+__device__ __forceinline__ double exp_of(double x, double lead) {
     x = fmax(x, -700.0);
     const double log2e = 0x1.71547652b82fep+0, magic = 0x1.8p+52;
     const double r = __builtin_fma(x, log2e, magic), f = __builtin_fma(x, log2e, -(r - magic));
-    double p = 0x1.b4014c1ff3fbep-24;
-    p = __builtin_fma(p, f, 0x1.63ee359dfa9f3p-20);
-    p = __builtin_fma(p, f, 0x1.ffce18ebcfb6cp-17);
-    p = __builtin_fma(p, f, 0x1.43088f9609f89p-13);
-    p = __builtin_fma(p, f, 0x1.5d87fd93161f0p-10);
-    p = __builtin_fma(p, f, 0x1.3b2ab72a268b1p-7);
-    p = __builtin_fma(p, f, 0x1.c6b08d70d1248p-5);
-    p = __builtin_fma(p, f, 0x1.ebfbdff81568ap-3);
-    p = __builtin_fma(p, f, 0x1.62e42fefa374fp-1);
-    p = __builtin_fma(p, f, 0x1.0000000000039p+0);
+    double p = __builtin_fma(lead, f, 0x1.00dad0d6f5ff9p-16);
+    p = __builtin_fma(p, f, 0x1.430accf559f5cp-13);
+    p = __builtin_fma(p, f, 0x1.5d87483a5a42cp-10);
+    p = __builtin_fma(p, f, 0x1.3b2ab5c4fcf88p-7);
+    p = __builtin_fma(p, f, 0x1.c6b08dd46bc16p-5);
+    p = __builtin_fma(p, f, 0x1.ebfbdff931c07p-3);
+    p = __builtin_fma(p, f, 0x1.62e42fef8615ep-1);
+    p = __builtin_fma(p, f, 0x1.ffffffffff7a6p-1);
     return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));
+}
+/* The largest of three in one instruction (the compiler's fmaxf makes every input canonical first). A NaN loses. */
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
 }
 
 /* x with its neighbour's by a rotation in rows of 16 lanes. */
 template <int N>
 __device__ __forceinline__ int turned(int x) {
-    return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, false);
+    return __builtin_amdgcn_mov_dpp(x, 0x120 + N, 0xf, 0xf, false);
 }
 template <int N>
 __device__ __forceinline__ float turned(float x) {
@@ -74,10 +80,10 @@ __device__ __forceinline__ double turned(double x) {
     return __hiloint2double(turned<N>(__double2hiint(x)), turned<N>(__double2loint(x)));
 }
 __device__ __forceinline__ float max_row(float x) { /* of 16 lanes */
-    x = fmaxf(x, turned<8>(x));
-    x = fmaxf(x, turned<4>(x));
-    x = fmaxf(x, turned<2>(x));
-    return fmaxf(x, turned<1>(x));
+    x = max3(x, turned<8>(x), x);
+    x = max3(x, turned<4>(x), x);
+    x = max3(x, turned<2>(x), x);
+    return max3(x, turned<1>(x), x);
 }
 __device__ __forceinline__ double sum_wave(double x) {
     x += turned<8>(x);
@@ -88,12 +94,15 @@ __device__ __forceinline__ double sum_wave(double x) {
     return x + __shfl_xor(x, 32);
 }
 
-/* What the first launch leaves of a row: block maxima (NaN where an id's logit is NaN or +inf), and of each wave of its
- * spans the sum of exp(l - the largest of the wave's blocks). */
+/* What the first launch leaves of a row: block maxima (NaN where an id's logit is NaN or +inf), and of each wave the largest
+ * logit and the sum of exp(l - that one). */
+struct WaveSum {
+    double sum, top;
+};
 struct Sums {
     float *top;
-    double *sum;
-    uint32_t blocks, sums, per; /* of a row; blocks a wave */
+    WaveSum *sum;
+    uint32_t blocks, sums; /* of a row */
 };
 
 /* A wave takes U times 256 ids of the span: no exchange with the others. */
@@ -117,7 +126,7 @@ __global__ __launch_bounds__(BM_WG) void k_beam_sums(BeamArgs a, Sums s) {
     float top = -INFINITY;
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-        float m = fmaxf(fmaxf(l[u][0], l[u][1]), fmaxf(l[u][2], l[u][3]));
+        float m = max3(max3(l[u][0], l[u][1], l[u][2]), l[u][3], l[u][3]);
         bool bad = false;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) bad = bad || !(l[u][e] < INFINITY);
@@ -129,14 +138,15 @@ __global__ __launch_bounds__(BM_WG) void k_beam_sums(BeamArgs a, Sums s) {
     }
 #pragma unroll
     for (int off = BM_LANES; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-    const double off = top == -INFINITY ? 0.0 : (double)top;
-    double sum = 0.0;
+    const double off = top == -INFINITY ? 0.0 : (double)top; /* all masked: as at -700 each, and next to nothing in the row */
+    double sum = 0.0, lead = EXP_LEAD;
+    asm("" : "+v"(lead));
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) sum += exp_of((double)l[u][e] - off);
+        for (uint32_t e = 0; e < 4; ++e) sum += exp_of((double)l[u][e] - off, lead);
     sum = sum_wave(sum);
-    if (lane == 0) s.sum[(size_t)r * s.sums + wave] = sum;
+    if (lane == 0) s.sum[(size_t)r * s.sums + wave] = WaveSum{sum, (double)top};
 }
 
 /* The `most`-th largest of some keys of which no two are equal but zeros: of keys[0 .. n), which all threads have written; 0 if
@@ -211,16 +221,26 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     id += (size_t)r * a.select;
     const bool done = a.done && a.done[r];
     int bad = !(score < INFINITY);
-    auto block_key = [&](uint32_t i) { return bt[i] == -INFINITY ? 0 : key_of(bt[i], i); };
+    /* the thread's blocks, BT of them in registers, and sums: one trip to memory for vocabularies of up to 262144 ids */
+    constexpr uint32_t BT = 16, ST = 3;
+    float t[BT];
+    WaveSum ws[ST];
+    const WaveSum *sum_row = s.sum + (size_t)r * s.sums;
+#pragma unroll
+    for (uint32_t k = 0; k < BT; ++k) t[k] = !done && tid + k * BM_WG < s.blocks ? bt[tid + k * BM_WG] : -INFINITY;
+#pragma unroll
+    for (uint32_t k = 0; k < ST; ++k) ws[k] = !done && tid + k * BM_WG < s.sums ? sum_row[tid + k * BM_WG] : WaveSum{0.0, -INFINITY};
+    auto block_key = [](float x, uint32_t i) { return x == -INFINITY ? 0 : key_of(x, i); };
     uint64_t mine = 0;
-    if (!done) {
-#pragma unroll 4
-        for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
-            bad |= !(bt[i] < INFINITY);
-            const uint64_t k = block_key(i);
-            mine = k > mine ? k : mine;
-        }
-    }
+    auto look = [&](float x, uint32_t i) {
+        bad |= !(x < INFINITY);
+        const uint64_t k = block_key(x, i);
+        mine = k > mine ? k : mine;
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < BT; ++k) look(t[k], tid + k * BM_WG);
+    if (!done)
+        for (uint32_t i = tid + BT * BM_WG; i < s.blocks; i += BM_WG) look(bt[i], i);
     keys[tid] = mine;
     if (tid < 3) counts[tid] = 0;
     bad = __syncthreads_or(bad);
@@ -249,11 +269,13 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     const double top = (double)logit_of(most);
     /* the blocks that are no smaller than the select-th of the columns' maxima, and the best of them */
     const uint64_t least = max(kth_of(keys, columns, a.select), (uint64_t)1);
-#pragma unroll 4
-    for (uint32_t i = tid; i < s.blocks; i += BM_WG) {
-        const uint64_t k = block_key(i);
+    auto put = [&](float x, uint32_t i) {
+        const uint64_t k = block_key(x, i);
         if (k >= least) list[atomicAdd(&counts[0], 1u)] = k;
-    }
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < BT; ++k) put(t[k], tid + k * BM_WG);
+    for (uint32_t i = tid + BT * BM_WG; i < s.blocks; i += BM_WG) put(bt[i], i);
     __syncthreads();
     const uint32_t listed = counts[0], nb = best_of(list, other, listed, a.select, keys, blocks, &counts[2]);
     /* their ids, BM_WG / BM_LANES blocks at a time, a lane four */
@@ -267,12 +289,10 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     float l[4];
     uint32_t i = load(tid / BM_LANES, l);
     double sum = 0.0;
-    for (uint32_t i = tid; i < s.sums; i += BM_WG) {
-        float m = -INFINITY;
-        for (uint32_t k = 0; k < s.per; ++k)
-            if (i * s.per + k < s.blocks) m = fmaxf(m, bt[i * s.per + k]);
-        if (m > -INFINITY) sum += s.sum[(size_t)r * s.sums + i] * exp_of((double)m - top);
-    }
+    auto add = [&](const WaveSum &w) { sum += w.sum * exp_of(w.top - top, EXP_LEAD); };
+#pragma unroll
+    for (uint32_t k = 0; k < ST; ++k) add(ws[k]);
+    for (uint32_t i = tid + ST * BM_WG; i < s.sums; i += BM_WG) add(sum_row[i]);
     sum = sum_wave(sum);
     if (tid % 64 == 0) sums[tid / 64] = sum;
     for (uint32_t b = tid / BM_LANES; b < nb; b += BM_WG / BM_LANES) {
@@ -356,34 +376,30 @@ __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *v
     }
 }
 
-/* Blocks a wave of the first launch: eight where the rows fill the card with them. */
-uint32_t wave_loads(const BeamArgs &a) {
-    const uint64_t ids = (uint64_t)a.groups * a.beams * a.vocab;
-    return ids >= (uint64_t)1024 * 4096 ? 4 : ids >= (uint64_t)1024 * 2048 ? 2 : 1;
-}
+/* Loads of four ids a lane in the first launch. 128 rows of 151936: 1 24.6 us, 2 21.2, 4 21.0; 4 rows: 3.2, 3.3, 3.7. */
+uint32_t wave_loads(const BeamArgs &a) { return (uint64_t)a.groups * a.beams * a.vocab >= (1u << 21) ? 2 : 1; }
 Sums sums_of(const BeamArgs &a) {
     Sums s;
     s.top = nullptr;
     s.sum = nullptr;
-    s.per = 64 / BM_LANES * wave_loads(a);
+    const uint32_t per = 256 * wave_loads(a);
     s.blocks = (a.vocab + BM_BLOCK - 1) / BM_BLOCK;
-    s.sums = (s.blocks + s.per - 1) / s.per;
+    s.sums = (a.vocab + per - 1) / per;
     return s;
 }
 
 }  // namespace
 
 size_t beam_workspace(const BeamArgs &a) {
-    const Sums s = sums_of(a);
-    const size_t rows = (size_t)a.groups * a.beams;
-    return rows * ((size_t)a.select * 12 + s.sums * 8 + s.blocks * 4);
+    const size_t rows = (size_t)a.groups * a.beams; /* sums of one load each: enough for fewer rows or ids too */
+    return rows * ((size_t)a.select * 12 + (a.vocab + 255) / 256 * sizeof(WaveSum) + sums_of(a).blocks * 4);
 }
 
 hipError_t launch_beam(const BeamArgs &a, void *ws, hipStream_t st) {
     const uint32_t rows = a.groups * a.beams, U = wave_loads(a);
     Sums s = sums_of(a);
     double *value = (double *)ws;
-    s.sum = value + (size_t)rows * a.select;
+    s.sum = (WaveSum *)(value + (size_t)rows * a.select);
     s.top = (float *)(s.sum + (size_t)rows * s.sums);
     uint32_t *id = (uint32_t *)(s.top + (size_t)rows * s.blocks);
     const bool wide = !(((uintptr_t)a.logits | (rows > 1 ? a.stride * 4 : 0)) & 15);
@@ -393,8 +409,7 @@ hipError_t launch_beam(const BeamArgs &a, void *ws, hipStream_t st) {
         if (wide) hipLaunchKernelGGL((k_beam_sums<U, true>), grid, dim3(BM_WG), 0, st, a, s);              \
         else hipLaunchKernelGGL((k_beam_sums<U, false>), grid, dim3(BM_WG), 0, st, a, s);                  \
     } while (0)
-    if (U == 4) SMQ_BEAM(4);
-    else if (U == 2) SMQ_BEAM(2);
+    if (U == 2) SMQ_BEAM(2);
     else SMQ_BEAM(1);
 #undef SMQ_BEAM
     const uint32_t first = a.select * BM_BLOCK, n = a.beams * a.select;

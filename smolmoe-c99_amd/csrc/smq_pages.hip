@@ -6,26 +6,6 @@ namespace smq {
 namespace {
 
 constexpr uint32_t PG_WG = 256, PG_CHUNK = 1024; /* pages of a chunk */
-constexpr uint32_t PART = 1u << 31;              /* of a page's claims: some new row takes it in part */
-
-/* The workspace: per page the old table's entries and the new one's claims; per chunk its free pages; per new row the page
- * that it takes in part (-1: none), its first entry that needs a page and how many do. */
-struct ForkSpace {
-    uint32_t *gone, *claims, *chunk, *need;
-    int32_t *last;
-    uint32_t *from;
-};
-__host__ __device__ inline ForkSpace fork_space(void *ws, uint32_t pages, uint32_t rows) {
-    const uint32_t chunks = (pages + PG_CHUNK - 1) / PG_CHUNK;
-    ForkSpace s;
-    s.gone = (uint32_t *)ws;
-    s.claims = s.gone + pages;
-    s.chunk = s.claims + pages;
-    s.need = s.chunk + chunks;
-    s.last = (int32_t *)(s.need + rows);
-    s.from = (uint32_t *)(s.last + rows);
-    return s;
-}
 
 /* New row d, cut to what the tables hold. */
 struct NewRow {
@@ -54,75 +34,275 @@ __device__ __forceinline__ NewRow new_row(const ForkArgs &a, uint32_t d, bool fl
     if (bad && flag) *a.flag = 1;
     return r;
 }
+/* Entries of old row s. */
+__device__ __forceinline__ uint32_t old_held(const ForkArgs &a, uint32_t s, bool flag) {
+    const int held = a.held[s];
+    if (flag && (held < 0 || held > (int)a.table_stride)) *a.flag = 1;
+    return (uint32_t)min(max(held, 0), (int)a.table_stride);
+}
+template <uint32_t WAVES>
 __device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t *lds) {
+#pragma unroll
     for (int off = 1; off < 64; off *= 2) x += __shfl_xor(x, off);
     __syncthreads();
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
     __syncthreads();
     uint32_t t = 0;
-    for (uint32_t w = 0; w < blockDim.x / 64; ++w) t += lds[w];
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) t += lds[w];
     return t;
 }
-
-__global__ __launch_bounds__(PG_WG) void k_fork_clear(ForkArgs a, ForkSpace w) {
-    const uint32_t i = blockIdx.x * PG_WG + threadIdx.x;
-    if (i < a.pages) {
-        w.gone[i] = 0;
-        w.claims[i] = 0;
+/* The sum of x over the threads before this one; all: over all. */
+template <uint32_t WAVES>
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *lds, uint32_t &all) {
+    uint32_t upto = x;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+        const uint32_t y = __shfl_up(upto, off);
+        upto += (int)(threadIdx.x % 64) >= off ? y : 0;
     }
+    __syncthreads();
+    if (threadIdx.x % 64 == 63) lds[threadIdx.x / 64] = upto;
+    __syncthreads();
+    uint32_t before = upto - x;
+    all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        before += w < threadIdx.x / 64 ? lds[w] : 0;
+        all += lds[w];
+    }
+    return before;
 }
 
-/* A workgroup per old row, then one per new row: how often each page was named, and is. */
+/* Few rows and pages: one workgroup, the pages' holders in LDS. Three trips to memory (row arrays and holders, old entries, the
+ * parents' entries) and ten barriers: the launch and 4 us, where the four launches below take 11. */
+constexpr uint32_t SMALL_WG = 1024, SMALL_WAVES = SMALL_WG / 64, SMALL_PAGES = 8192, SMALL_ROWS = 256, SMALL_ENTRIES = 16384;
+__global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
+    __shared__ int holders[SMALL_PAGES];
+    __shared__ uint32_t in_part[SMALL_PAGES / 32], free_words[SMALL_PAGES / 32], word_rank[SMALL_PAGES / 32];
+    __shared__ int parents[SMALL_ROWS], last[SMALL_ROWS];
+    __shared__ uint32_t olds[SMALL_ROWS], full[SMALL_ROWS], held[SMALL_ROWS], from[SMALL_ROWS], rank[SMALL_ROWS + 1];
+    __shared__ uint32_t lds[SMALL_WAVES];
+    const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
+    NewRow row = {};
+    if (tid < a.old_seqs) olds[tid] = old_held(a, tid, true);
+    if (tid < a.seqs) {
+        row = new_row(a, tid, true);
+        parents[tid] = row.parent;
+        full[tid] = row.full;
+        held[tid] = row.held;
+        last[tid] = -1;
+    }
+    for (uint32_t i = tid; i < a.pages; i += SMALL_WG) {
+        const int n = a.refs[i];
+        holders[i] = n;
+        if (n < 0) *a.flag = 1;
+    }
+    if (tid < words) in_part[tid] = 0;
+    __syncthreads();
+    const float inv = 1.0f / (float)a.table_stride;
+    auto row_of = [&](uint32_t i) { return (uint32_t)(((float)i + 0.5f) * inv); }; /* i / stride: below 2^15, where this is exact */
+#pragma unroll 4
+    for (uint32_t i = tid; i < a.old_seqs * a.table_stride; i += SMALL_WG) {
+        const uint32_t s = row_of(i), x = i - s * a.table_stride;
+        const uint32_t id = (uint32_t)a.table[i];
+        if (x >= olds[s]) continue;
+        if (id < a.pages) atomicSub(&holders[id], 1);
+        else *a.flag = 1;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < a.pages; i += SMALL_WG)
+        if (holders[i] < 0) {
+            *a.flag = 1;
+            holders[i] = 0;
+        }
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = tid; i < a.seqs * a.table_stride; i += SMALL_WG) {
+        const uint32_t d = row_of(i), x = i - d * a.table_stride;
+        const uint32_t id = x < full[d] ? (uint32_t)a.table[(size_t)parents[d] * a.table_stride + x] : a.pages;
+        if (id < a.pages) atomicAdd(&holders[id], 1);
+        if (x < full[d] || x >= held[d]) a.table_out[i] = id < a.pages ? (int)id : -1;
+    }
+    if (tid < a.seqs && row.part) {
+        const uint32_t id = (uint32_t)a.table[(size_t)row.parent * a.table_stride + row.full];
+        if (id < a.pages) {
+            last[tid] = (int)id;
+            atomicOr(&in_part[id / 32], 1u << (id % 32));
+        }
+    }
+    __syncthreads();
+    /* rows: the first one that takes a page in part keeps it, if nothing else holds it */
+    uint32_t need = 0;
+    bool mine = false;
+    if (tid < a.seqs) {
+        mine = last[tid] >= 0 && holders[last[tid]] == 0;
+        if (mine)
+            for (uint32_t i = 0; i < tid; ++i) mine = mine & (last[i] != last[tid]);
+        from[tid] = row.full + mine;
+        need = row.held - from[tid]; /* a page in part is one of them */
+    }
+    uint32_t wanted, spare, count = 0;
+    /* pages, a word of 32 a thread */
+    if (tid < words) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            const uint32_t k = (i + tid) % 32, id = tid * 32 + k; /* 32 banks a step */
+            bits |= id < a.pages && holders[id] == 0 ? 1u << k : 0;
+        }
+        bits &= ~in_part[tid];
+        free_words[tid] = bits;
+        count = (uint32_t)__popc(bits);
+    }
+    const uint32_t before = block_scan<SMALL_WAVES>(need, lds, wanted), below = block_scan<SMALL_WAVES>(count, lds, spare);
+    if (tid < a.seqs) rank[tid] = before;
+    if (tid < words) word_rank[tid] = below;
+    __syncthreads();
+    if (mine) {
+        holders[last[tid]] = 1;
+        a.table_out[(size_t)tid * a.table_stride + row.full] = last[tid];
+    }
+    if (tid < a.seqs) {
+        a.held_out[tid] = (int)row.held;
+        if (!(last[tid] >= 0 && !mine && before < spare)) { /* else with the page below */
+            a.copies[3 * tid] = a.copies[3 * tid + 1] = -1;
+            a.copies[3 * tid + 2] = 0;
+        }
+    }
+    if (tid == 0) {
+        *a.free_out = (int)(spare - wanted);
+        if (wanted > spare) *a.flag = 1;
+    }
+    /* number k of the wanted pages: the last row that begins at k or before, the last word */
+    auto last_of = [](const uint32_t *x, uint32_t n, uint32_t k) {
+        uint32_t at = 0;
+        for (uint32_t step = n > 1 ? 1u << (31 - __builtin_clz(n - 1)) : 0; step; step /= 2)
+            if (at + step < n && x[at + step] <= k) at += step;
+        return at;
+    };
+    for (uint32_t k = tid; k < wanted; k += SMALL_WG) {
+        const uint32_t d = last_of(rank, a.seqs, k), x = from[d] + k - rank[d];
+        int id = -1;
+        if (k < spare) {
+            const uint32_t w = last_of(word_rank, words, k);
+            uint32_t bits = free_words[w];
+            for (uint32_t i = word_rank[w]; i < k; ++i) bits &= bits - 1;
+            id = (int)(w * 32) + __ffs(bits) - 1;
+            holders[id] = 1;
+            if (x == full[d] && last[d] >= 0) {
+                a.copies[3 * d] = last[d];
+                a.copies[3 * d + 1] = id;
+                a.copies[3 * d + 2] = a.keep[d] & ((1 << a.shift) - 1);
+            }
+        }
+        a.table_out[(size_t)d * a.table_stride + x] = id;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < a.pages; i += SMALL_WG) a.refs_out[i] = holders[i];
+}
+
+/* The workspace: per page what its holders change by; as bits, which pages new rows take in part and which are free; the
+ * free ones counted by chunks; per new row the page that it takes in part (-1: none), its first entry that needs a page and
+ * how many do. */
+struct ForkSpace {
+    int *change;
+    uint32_t *part, *bits, *chunk, *need, *from;
+    int32_t *last;
+};
+inline uint32_t chunks_of(uint32_t pages) { return (pages + PG_CHUNK - 1) / PG_CHUNK; }
+inline ForkSpace fork_space(void *ws, uint32_t pages, uint32_t rows) {
+    const size_t chunks = chunks_of(pages), words = chunks * (PG_CHUNK / 32);
+    ForkSpace s;
+    s.change = (int *)ws;
+    s.part = (uint32_t *)(s.change + chunks * PG_CHUNK);
+    s.bits = s.part + words;
+    s.chunk = s.bits + words;
+    s.need = s.chunk + chunks;
+    s.from = s.need + rows;
+    s.last = (int32_t *)(s.from + rows);
+    return s;
+}
+
+/* change and part, which follow it. */
+__global__ __launch_bounds__(PG_WG) void k_fork_clear(uint4 *p, uint32_t n) {
+    const uint32_t i = blockIdx.x * PG_WG + threadIdx.x;
+    if (i < n) p[i] = uint4{0, 0, 0, 0};
+}
+
+/* A workgroup per old row: its first new row (the first one that names it as its parent) takes its holders over, so that only
+ * entries behind that one's are given up: a change costs an atomic across the XCDs' L2s, of 256 rows of 2000 pages 29 us when
+ * each entry was counted out and in. Then a workgroup per new row: those that are not the first add themselves. */
 __global__ __launch_bounds__(PG_WG) void k_fork_count(ForkArgs a, ForkSpace w) {
+    __shared__ uint32_t lds[PG_WG / 64], least;
     const uint32_t tid = threadIdx.x;
-    if (blockIdx.x < a.old_seqs) {
-        const int held = a.held[blockIdx.x];
-        if ((held < 0 || held > (int)a.table_stride) && tid == 0) *a.flag = 1;
-        const uint32_t n = (uint32_t)min(max(held, 0), (int)a.table_stride);
+    const bool old = blockIdx.x < a.old_seqs;
+    const uint32_t d = blockIdx.x - a.old_seqs;
+    NewRow r = {};
+    if (!old) r = new_row(a, d, tid == 0);
+    const int s = old ? (int)blockIdx.x : r.parent;
+    if (tid == 0) least = a.seqs;
+    __syncthreads();
+    uint32_t first = a.seqs;
+    for (uint32_t i = tid; i < (old ? a.seqs : d); i += PG_WG)
+        if (a.parent[i] == s) {
+            first = i;
+            break;
+        }
+    if (first < a.seqs) atomicMin(&least, first);
+    __syncthreads();
+    first = least;
+    const int32_t *row = a.table + (size_t)max(s, 0) * a.table_stride;
+    if (old) {
+        const uint32_t n = old_held(a, (uint32_t)s, tid == 0), kept = first < a.seqs ? new_row(a, first, false).full : 0;
         for (uint32_t x = tid; x < n; x += PG_WG) {
-            const uint32_t id = (uint32_t)a.table[(size_t)blockIdx.x * a.table_stride + x];
-            if (id < a.pages) atomicAdd(&w.gone[id], 1u);
-            else *a.flag = 1;
+            const uint32_t id = (uint32_t)row[x];
+            if (id >= a.pages || a.refs[id] < 1) *a.flag = 1;
+            else if (x >= kept) atomicSub(&w.change[id], 1);
         }
         return;
     }
-    const uint32_t d = blockIdx.x - a.old_seqs;
-    const NewRow r = new_row(a, d, tid == 0);
-    const int32_t *row = a.table + (size_t)max(r.parent, 0) * a.table_stride;
-    for (uint32_t x = tid; x < r.full; x += PG_WG) {
-        const uint32_t id = (uint32_t)row[x];
-        if (id < a.pages) atomicAdd(&w.claims[id], 1u);
-    }
+    if (first < a.seqs) /* a lower row has the same parent */
+        for (uint32_t x = tid; x < r.full; x += PG_WG) {
+            const uint32_t id = (uint32_t)row[x];
+            if (id < a.pages && a.refs[id] >= 1) atomicAdd(&w.change[id], 1);
+        }
     if (tid == 0) {
         const uint32_t id = r.part ? (uint32_t)row[r.full] : a.pages;
-        if (id < a.pages) atomicOr(&w.claims[id], PART);
+        if (id < a.pages) atomicOr(&w.part[id / 32], 1u << (id % 32));
         w.last[d] = id < a.pages ? (int)id : -1;
     }
 }
 
-/* What holds page id beside the old table's rows and the rows that take it in part. */
-__device__ __forceinline__ uint32_t others(const ForkArgs &a, const ForkSpace &w, uint32_t id, bool flag) {
-    const int refs = a.refs[id];
-    const uint32_t gone = w.gone[id];
-    if (flag && (refs < 0 || (uint32_t)refs < gone)) *a.flag = 1;
-    return (refs > 0 && (uint32_t)refs > gone ? (uint32_t)refs - gone : 0) + (w.claims[id] & ~PART);
+/* Holders of a page beside the rows that take it in part. */
+__device__ __forceinline__ int holders_of(const ForkArgs &a, const ForkSpace &w, uint32_t id, bool flag) {
+    const int refs = a.refs[id], n = refs + w.change[id];
+    if (flag && (n < 0 || refs < 0)) *a.flag = 1;
+    return max(n, 0);
 }
 
-/* Chunks of pages: their holders but for fresh ones, and the free ones counted. Then a workgroup per new row: whether it
- * keeps the page that it takes in part, and the pages it needs. */
+/* Chunks of pages: their holders but for fresh ones, and the free ones. Then a workgroup per new row: whether it keeps the page
+ * that it takes in part, and the pages that it needs. */
 __global__ __launch_bounds__(PG_WG) void k_fork_rows(ForkArgs a, ForkSpace w, uint32_t chunks) {
     __shared__ uint32_t lds[PG_WG / 64];
     const uint32_t tid = threadIdx.x;
     if (blockIdx.x < chunks) {
         uint32_t free = 0;
+#pragma unroll
         for (uint32_t k = 0; k < PG_CHUNK / PG_WG; ++k) {
             const uint32_t id = blockIdx.x * PG_CHUNK + k * PG_WG + tid;
-            if (id >= a.pages) break;
-            const uint32_t n = others(a, w, id, true), kept = n == 0 && (w.claims[id] & PART);
-            a.refs_out[id] = (int)(n + kept);
-            free += n + kept == 0;
+            bool none = false;
+            if (id < a.pages) {
+                const int n = holders_of(a, w, id, true);
+                const bool kept = n == 0 && (w.part[id / 32] >> (id % 32) & 1);
+                none = n == 0 && !kept;
+                a.refs_out[id] = n + kept;
+            }
+            const uint64_t those = __ballot(none);
+            if (tid % 64 < 2) w.bits[id / 64 * 2 + tid % 64] = (uint32_t)(those >> (32 * (tid % 64)));
+            free += none;
         }
-        free = block_sum(free, lds);
+        free = block_sum<PG_WG / 64>(free, lds);
         if (tid == 0) w.chunk[blockIdx.x] = free;
         return;
     }
@@ -132,83 +312,85 @@ __global__ __launch_bounds__(PG_WG) void k_fork_rows(ForkArgs a, ForkSpace w, ui
     bool lower = false;
     if (last >= 0)
         for (uint32_t i = tid; i < d; i += PG_WG) lower = lower || w.last[i] == last;
-    const uint32_t any = block_sum(lower, lds);
+    const uint32_t any = block_sum<PG_WG / 64>(lower, lds);
     if (tid == 0) {
-        const bool mine = last >= 0 && !any && others(a, w, (uint32_t)last, false) == 0;
+        const bool mine = last >= 0 && !any && holders_of(a, w, (uint32_t)last, false) == 0;
         w.from[d] = r.full + mine;
-        w.need[d] = r.held - min(r.held, r.full + mine);
+        w.need[d] = r.held - (r.full + mine); /* a page in part is one of them */
     }
 }
 
-/* Chunks of pages: each free one to the row and entry whose number it has. Then a workgroup per new row: the other
- * entries. */
+/* A workgroup per new row: its entries. Its fresh pages are the free ones of the numbers that the rows before it leave off at:
+ * the chunk where they begin, then the words of eight chunks at a time. */
 __global__ __launch_bounds__(PG_WG) void k_fork_assign(ForkArgs a, ForkSpace w, uint32_t chunks) {
-    __shared__ uint32_t lds[PG_WG / 64], scan[PG_WG];
-    const uint32_t tid = threadIdx.x;
-    uint32_t need = 0, free = 0, mine = 0;
-    const uint32_t d = blockIdx.x - chunks;
-    for (uint32_t i = tid; i < a.seqs; i += PG_WG) {
-        need += w.need[i];
-        if (blockIdx.x >= chunks && i < d) mine += w.need[i];
-    }
-    for (uint32_t i = tid; i < chunks; i += PG_WG) {
-        free += w.chunk[i];
-        if (blockIdx.x < chunks && i < blockIdx.x) mine += w.chunk[i];
-    }
-    need = block_sum(need, lds);
-    free = block_sum(free, lds);
-    mine = block_sum(mine, lds);
-    if (blockIdx.x == 0 && tid == 0) {
-        *a.free_out = (int)(free - need);
-        if (need > free) *a.flag = 1;
-    }
-    if (blockIdx.x < chunks) {
-        for (uint32_t k = 0; k < PG_CHUNK / PG_WG; ++k) {
-            const uint32_t id = blockIdx.x * PG_CHUNK + k * PG_WG + tid;
-            const bool ok = id < a.pages && a.refs_out[id] == 0 && w.claims[id] == 0;
-            scan[tid] = ok;
-            __syncthreads();
-            uint32_t at = mine, all = 0;
-            for (uint32_t i = 0; i < PG_WG; ++i) {
-                at += i < tid ? scan[i] : 0;
-                all += scan[i];
-            }
-            __syncthreads();
-            if (ok && at < need) {
-                uint32_t row = 0;
-                while (at >= w.need[row]) at -= w.need[row++];
-                const uint32_t x = w.from[row] + at;
-                a.table_out[(size_t)row * a.table_stride + x] = (int)id;
-                a.refs_out[id] = 1;
-                const NewRow r = new_row(a, row, false);
-                if (r.part && w.last[row] >= 0 && x == r.full) {
-                    a.copies[3 * row] = w.last[row];
-                    a.copies[3 * row + 1] = (int)id;
-                    a.copies[3 * row + 2] = (int)r.part;
-                }
-            }
-            mine += all;
-        }
-        return;
-    }
-    const NewRow r = new_row(a, d, false);
-    const uint32_t from = w.from[d], end = from + w.need[d], have = mine < free ? min(w.need[d], free - mine) : 0;
+    __shared__ uint32_t lds[PG_WG / 64], begin[2];
+    const uint32_t tid = threadIdx.x, d = blockIdx.x;
+    const bool row_there = d < a.seqs;
+    const NewRow r = row_there ? new_row(a, d, false) : NewRow{-1, 0, 0, 0};
+    const uint32_t from = row_there ? w.from[d] : 0, need = row_there ? w.need[d] : 0;
+    const int last = row_there ? w.last[d] : -1;
     const int32_t *row = a.table + (size_t)max(r.parent, 0) * a.table_stride;
     int32_t *out = a.table_out + (size_t)d * a.table_stride;
-    for (uint32_t x = tid; x < a.table_stride; x += PG_WG) {
-        if (x < from) {
-            const int id = row[x];
-            out[x] = (uint32_t)id < a.pages ? id : -1;
-        } else if (x >= from + have || x >= end) {
-            out[x] = -1;
+    if (row_there) {
+#pragma unroll 4
+        for (uint32_t x = tid; x < a.table_stride; x += PG_WG) {
+            if (x < from) {
+                const int id = row[x];
+                out[x] = (uint32_t)id < a.pages ? id : -1;
+            } else if (x >= from + need) {
+                out[x] = -1;
+            }
         }
+        if (tid == 0) a.held_out[d] = (int)r.held;
     }
-    if (tid == 0) {
-        a.held_out[d] = (int)r.held;
-        if (!(r.part && w.last[d] >= 0 && from == r.full && have)) {
-            a.copies[3 * d] = a.copies[3 * d + 1] = -1;
-            a.copies[3 * d + 2] = 0;
+    const bool copies = last >= 0 && from == r.full;
+    bool copied = false;
+    if (need || d == 0) {
+        uint32_t before = 0, sum = 0;
+        for (uint32_t i = tid; i < (d == 0 ? a.seqs : d); i += PG_WG) before += w.need[i];
+        before = block_sum<PG_WG / 64>(before, lds);
+        const uint32_t all = before;
+        if (d == 0) before = 0;
+        const uint32_t each = (chunks + PG_WG - 1) / PG_WG, c0 = tid * each, c1 = min(c0 + each, chunks);
+        for (uint32_t c = c0; c < c1; ++c) sum += w.chunk[c];
+        uint32_t spare, at = block_scan<PG_WG / 64>(sum, lds, spare);
+        if (before >= at && before < at + sum) /* one thread, if any */
+            for (uint32_t c = c0; c < c1; at += w.chunk[c++])
+                if (before < at + w.chunk[c]) {
+                    begin[0] = c;
+                    begin[1] = at;
+                    break;
+                }
+        if (d == 0 && tid == 0) {
+            *a.free_out = (int)(spare - all);
+            if (all > spare) *a.flag = 1;
         }
+        __syncthreads();
+        const uint32_t end = min(before + need, spare), words = chunks * (PG_CHUNK / 32);
+        copied = copies && before < spare;
+        if (before < end) {
+            uint32_t number = begin[1], total;
+            for (uint32_t w0 = begin[0] * (PG_CHUNK / 32); number < end && w0 < words; w0 += PG_WG, number += total) {
+                uint32_t bits = w0 + tid < words ? w.bits[w0 + tid] : 0;
+                uint32_t k = number + block_scan<PG_WG / 64>((uint32_t)__popc(bits), lds, total);
+                for (; bits && k < end; bits &= bits - 1, ++k) {
+                    if (k < before) continue;
+                    const int id = (int)((w0 + tid) * 32) + __ffs(bits) - 1;
+                    out[from + k - before] = id;
+                    a.refs_out[id] = 1;
+                    if (k == before && copies) {
+                        a.copies[3 * d] = last;
+                        a.copies[3 * d + 1] = id;
+                        a.copies[3 * d + 2] = (int)r.part;
+                    }
+                }
+            }
+        }
+        for (uint32_t k = max(before, spare) + tid; k < before + need; k += PG_WG) out[from + k - before] = -1;
+    }
+    if (row_there && !copied && tid == 0) {
+        a.copies[3 * d] = a.copies[3 * d + 1] = -1;
+        a.copies[3 * d + 2] = 0;
     }
 }
 
@@ -343,16 +525,22 @@ __global__ __launch_bounds__(PG_WG) void k_paged_compact(PagedArgs a, Pools pool
 
 size_t fork_workspace(uint32_t pages, uint32_t rows) {
     const ForkSpace s = fork_space(nullptr, pages, rows);
-    return (size_t)((char *)(s.from + rows) - (char *)nullptr);
+    return (size_t)((char *)(s.last + rows) - (char *)nullptr);
 }
 
 hipError_t launch_fork(const ForkArgs &a, void *ws, hipStream_t s) {
+    const uint64_t rows = max(a.old_seqs, a.seqs);
+    if (a.pages <= SMALL_PAGES && rows <= SMALL_ROWS && rows * a.table_stride <= SMALL_ENTRIES) {
+        hipLaunchKernelGGL(k_fork_small, dim3(1), dim3(SMALL_WG), 0, s, a);
+        return hipGetLastError();
+    }
     const ForkSpace w = fork_space(ws, a.pages, a.seqs);
-    const uint32_t chunks = (a.pages + PG_CHUNK - 1) / PG_CHUNK;
-    hipLaunchKernelGGL(k_fork_clear, dim3((a.pages + PG_WG - 1) / PG_WG), dim3(PG_WG), 0, s, a, w);
-    hipLaunchKernelGGL(k_fork_count, dim3(a.old_seqs + a.seqs), dim3(PG_WG), 0, s, a, w);
+    const uint32_t chunks = chunks_of(a.pages), clear = chunks * (PG_CHUNK / 4 + PG_CHUNK / 128);
+    hipLaunchKernelGGL(k_fork_clear, dim3((clear + PG_WG - 1) / PG_WG), dim3(PG_WG), 0, s, (uint4 *)ws, clear);
+    if (a.old_seqs + a.seqs)
+        hipLaunchKernelGGL(k_fork_count, dim3(a.old_seqs + a.seqs), dim3(PG_WG), 0, s, a, w);
     hipLaunchKernelGGL(k_fork_rows, dim3(chunks + a.seqs), dim3(PG_WG), 0, s, a, w, chunks);
-    hipLaunchKernelGGL(k_fork_assign, dim3(chunks + a.seqs), dim3(PG_WG), 0, s, a, w, chunks);
+    hipLaunchKernelGGL(k_fork_assign, dim3(a.seqs ? a.seqs : 1), dim3(PG_WG), 0, s, a, w, chunks);
     return hipGetLastError();
 }
 
