@@ -396,15 +396,71 @@ __global__ __launch_bounds__(PG_WG) void k_fork_assign(ForkArgs a, ForkSpace w, 
 
 /* ---- copies and moves in every pool --------------------------------------------- */
 
-template <typename T>
-__device__ __forceinline__ void copy_run(T *to, const T *from, uint32_t n) {
-    for (uint32_t i = threadIdx.x; i < n; i += PG_WG) to[i] = from[i];
-}
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+/* i / n of numbers below 2^20 with a quotient below 2^12. */
+struct Divide {
+    uint32_t n;
+    float inv;
+    __device__ __forceinline__ Divide(uint32_t n_) : n(n_), inv(1.0f / (float)n_) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t i, uint32_t &rest) const {
+        uint32_t q = (uint32_t)((float)i * inv);
+        int r = (int)i - (int)(q * n);
+        if (r < 0) { /* the estimate is off by one at most */
+            --q;
+            r += (int)n;
+        } else if (r >= (int)n) {
+            ++q;
+            r -= (int)n;
+        }
+        rest = (uint32_t)r;
+        return q;
+    }
+};
 
-/* A workgroup per row of `copies`, pool and KV head. */
+/* A workgroup per row of `copies`, pool, KV head and kind (keys, values). Keys are one run of bytes; of a value dim's row the
+ * first positions, 16 bytes at a time and a shorter end. Scales go with their codes. CP_BATCH pieces a thread are requested
+ * before the first is written. Bound by three trips to memory where pages are few; 64 rows of 12 f16 layers of 2 KV heads of
+ * 128 in pages of 128, 29 of them copied, 15 MB. */
+constexpr uint32_t CP_BATCH = 4;
+template <typename T, typename At>
+__device__ __forceinline__ void copy_pieces(uint32_t n, const void *from, void *to, At at) {
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += CP_BATCH * PG_WG) {
+        T x[CP_BATCH];
+#pragma unroll
+        for (uint32_t u = 0; u < CP_BATCH; ++u)
+            if (i0 + u * PG_WG < n) x[u] = *(const T *)((const char *)from + at(i0 + u * PG_WG));
+#pragma unroll
+        for (uint32_t u = 0; u < CP_BATCH; ++u)
+            if (i0 + u * PG_WG < n) *(T *)((char *)to + at(i0 + u * PG_WG)) = x[u];
+    }
+}
+/* Of each of `rows` rows, `stride` bytes apart, the first `bytes`, which are whole elements of `unit` bytes. */
+__device__ __forceinline__ void copy_rows(const void *from, void *to, uint32_t rows, uint32_t stride, uint32_t bytes, uint32_t unit) {
+    const uint32_t whole = bytes / 16, rest = bytes % 16;
+    if (whole) {
+        const Divide by(whole);
+        copy_pieces<u4>(rows * whole, from, to, [&](uint32_t i) {
+            uint32_t x;
+            const uint32_t r = by(i, x);
+            return (size_t)r * stride + 16 * x;
+        });
+    }
+    if (rest) {
+        const uint32_t n = rest / unit;
+        const Divide by(n);
+        auto at = [&](uint32_t i) {
+            uint32_t x;
+            const uint32_t r = by(i, x);
+            return (size_t)r * stride + 16 * whole + x * unit;
+        };
+        if (unit == 4) copy_pieces<uint32_t>(rows * n, from, to, at);
+        else if (unit == 2) copy_pieces<uint16_t>(rows * n, from, to, at);
+        else copy_pieces<uint8_t>(rows * n, from, to, at);
+    }
+}
 __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, const int32_t *copies) {
-    const uint32_t h = blockIdx.x % a.kv_heads, l = blockIdx.x / a.kv_heads % pools.n;
-    const int32_t *c = copies + 3 * (size_t)(blockIdx.x / a.kv_heads / pools.n);
+    const uint32_t kind = blockIdx.x & 1, y = blockIdx.x >> 1, h = y % a.kv_heads, l = y / a.kv_heads % pools.n;
+    const int32_t *c = copies + 3 * (size_t)(y / a.kv_heads / pools.n);
     const int from = c[0], to = c[1], n = c[2];
     if (n == 0) return;
     if ((uint32_t)from >= a.pages || (uint32_t)to >= a.pages || n < 0 || n > 1 << a.shift) {
@@ -413,111 +469,119 @@ __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, 
     }
     const uint32_t EB = 4 >> a.type;
     const Pool &p = pools.p[l];
-    const size_t head = (size_t)a.head_dim << a.shift, f = ((size_t)from * a.kv_heads + h) * head * EB,
-                 t = ((size_t)to * a.kv_heads + h) * head * EB;
-    copy_run((uint32_t *)((char *)p.keys + t), (const uint32_t *)((const char *)p.keys + f), (uint32_t)n * a.head_dim * EB / 4);
-    for (uint32_t i = threadIdx.x; i < a.head_dim * (uint32_t)n * EB; i += PG_WG) {
-        const uint32_t d = i / (n * EB), x = i % (n * EB);
-        ((char *)p.values)[t + ((size_t)d * EB << a.shift) + x] = ((const char *)p.values)[f + ((size_t)d * EB << a.shift) + x];
-    }
-    if (a.type == 2)
-        for (uint32_t i = threadIdx.x; i < a.nb * (uint32_t)n; i += PG_WG) {
-            const uint32_t b = i / n, x = i % n;
-            const size_t sf = ((((size_t)from * a.kv_heads + h) * a.nb + b) << a.shift) + x,
-                         st = ((((size_t)to * a.kv_heads + h) * a.nb + b) << a.shift) + x;
-            p.ks[st] = p.ks[sf];
-            p.vs[st] = p.vs[sf];
-        }
+    const size_t f = (size_t)from * a.kv_heads + h, t = (size_t)to * a.kv_heads + h;
+    char *x = (char *)(kind ? p.values : p.keys), *w = (char *)(kind ? p.vs : p.ks);
+    const size_t head = ((size_t)a.head_dim << a.shift) * EB, scales = ((size_t)a.nb << a.shift) * 4;
+    if (a.type == 2) copy_rows(w + f * scales, w + t * scales, a.nb, 4u << a.shift, (uint32_t)n * 4, 4);
+    if (kind) copy_rows(x + f * head, x + t * head, a.head_dim, EB << a.shift, (uint32_t)n * EB, EB);
+    else copy_pieces<u4>((uint32_t)n * a.head_dim * EB / 16, x + f * head, x + t * head, [](uint32_t i) { return (size_t)i * 16; });
 }
 
-/* A workgroup per sequence, pool and KV head: 16 of the path's tokens at a time into LDS, then to their places. The places
- * of one round lie before the next rounds' tokens, since the path ascends. */
-constexpr uint32_t CP_AT_ONCE = 16;
+/* A workgroup per sequence, pool, KV head and kind: some of the path's tokens at a time into registers, then to their places. The
+ * places of one round lie before the next rounds' tokens, since the path ascends. Keys 16 bytes a piece, values an element: of
+ * a dim's row the path's positions lie next to each other, in the same lines of memory.
+ *
+ * Bound by four trips to memory (batch, path, page ids, tokens). */
+constexpr uint32_t CM_TOKENS = 64, CM_PIECES = 8;
+template <uint32_t EB>
+struct Element;
+template <>
+struct Element<4> {
+    typedef uint32_t T;
+};
+template <>
+struct Element<2> {
+    typedef uint16_t T;
+};
+template <>
+struct Element<1> {
+    typedef uint8_t T;
+};
+struct Moves {
+    size_t from[CM_TOKENS], to[CM_TOKENS]; /* page times KV heads plus head, << 8 | slot; NONE: stays */
+};
+constexpr size_t NONE = ~(size_t)0;
+/* n pieces of each of the tokens, `each` of them a thread at most: piece x of token k at at(place of k, x). */
+template <typename T, bool INNER, typename At>
+__device__ __forceinline__ void move_pieces(const Moves &m, uint32_t tokens, uint32_t n, void *p, At at) {
+    const Divide by(INNER ? tokens : n); /* INNER: tokens innermost */
+    T x[CM_PIECES];
+    size_t to[CM_PIECES];
+#pragma unroll
+    for (uint32_t u = 0; u < CM_PIECES; ++u) {
+        const uint32_t i = u * PG_WG + threadIdx.x;
+        to[u] = NONE;
+        if (i >= tokens * n) continue;
+        uint32_t rest;
+        const uint32_t q = by(i, rest), k = INNER ? rest : q, y = INNER ? q : rest;
+        if (m.from[k] == NONE) continue;
+        x[u] = *(const T *)((const char *)p + at(m.from[k], y));
+        to[u] = at(m.to[k], y);
+    }
+    __syncthreads(); /* what is read here may be another's place */
+#pragma unroll
+    for (uint32_t u = 0; u < CM_PIECES; ++u)
+        if (to[u] != NONE) *(T *)((char *)p + to[u]) = x[u];
+}
+template <uint32_t EB>
+__device__ __forceinline__ void move_tokens(const PagedArgs &a, const Pool &p, uint32_t kind, const Moves &m, uint32_t tokens) {
+    typedef typename Element<EB>::T T;
+    const uint32_t hd = a.head_dim, shift = a.shift, nb = a.nb;
+    if (kind)
+        move_pieces<T, true>(m, tokens, hd, p.values, [=](size_t w, uint32_t d) { return (((w >> 8) * hd + d << shift) + (w & 255)) * EB; });
+    else
+        move_pieces<u4, false>(m, tokens, hd * EB / 16, p.keys, [=](size_t w, uint32_t i) { return (((w >> 8) << shift) + (w & 255)) * hd * EB + 16 * i; });
+    if constexpr (EB == 1)
+        move_pieces<uint32_t, true>(m, tokens, nb, kind ? p.vs : p.ks, [=](size_t w, uint32_t b) { return (((w >> 8) * nb + b << shift) + (w & 255)) * 4; });
+}
 __global__ __launch_bounds__(PG_WG) void k_paged_compact(PagedArgs a, Pools pools, const int32_t *accepted, uint32_t stride,
                                                          const int32_t *count, int32_t *length_out) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ int from_page[CP_AT_ONCE], to_page[CP_AT_ONCE];
-    __shared__ uint32_t from_slot[CP_AT_ONCE], to_slot[CP_AT_ONCE];
-    const uint32_t tid = threadIdx.x, h = blockIdx.x % a.kv_heads, l = blockIdx.x / a.kv_heads % pools.n;
-    const uint32_t s = blockIdx.x / a.kv_heads / pools.n;
-    const Pool &p = pools.p[l];
-    const bool first_one = h == 0 && l == 0 && length_out;
-    Seq sq;
-    const int m = count[s];
+    __shared__ Moves moves;
+    const uint32_t tid = threadIdx.x, kind = blockIdx.x & 1, y = blockIdx.x >> 1, h = y % a.kv_heads;
+    const uint32_t l = y / a.kv_heads % pools.n, s = y / a.kv_heads / pools.n;
     const int32_t *path = accepted + (size_t)s * stride;
-    bool ok = sequence(a, s, sq);
-    bool good = ok && m >= 0 && m <= sq.n && (uint32_t)m <= stride;
+    const int mine = tid < stride ? path[tid] : 0, m = count[s]; /* the first entries with the count */
+    const bool tells = h == 0 && l == 0 && kind == 0 && length_out && tid == 0;
+    Seq sq;
+    const bool ok = sequence(a, s, sq);
+    bool good = ok && m >= 0 && m <= sq.n && (uint32_t)m <= stride, moved = false;
     if (good)
-        for (uint32_t k = tid; k < (uint32_t)m; k += PG_WG)
-            if (path[k] < 0 || path[k] >= sq.n || (k && path[k] <= path[k - 1])) good = false;
+        for (uint32_t k = tid; k < (uint32_t)m; k += PG_WG) {
+            const int at = k == tid ? mine : path[k];
+            if (at < 0 || at >= sq.n || (k && at <= path[k - 1])) good = false;
+            moved = moved || at != (int)k;
+        }
     good = __syncthreads_and(good);
-    if (!good) {
-        if (tid == 0) *a.flag = 1;
-        if (tid == 0 && first_one) length_out[s] = a.length[s];
-        return;
-    }
-    if (tid == 0 && first_one) length_out[s] = sq.first + m;
-    const uint32_t EB = 4 >> a.type, hd = a.head_dim, P = 1u << a.shift, words = hd * EB / 4;
-    uint32_t *keys = (uint32_t *)lds;
-    unsigned char *values = lds + CP_AT_ONCE * hd * EB;
-    float *scales = (float *)(values + CP_AT_ONCE * hd * EB);
-    for (uint32_t k0 = 0; k0 < (uint32_t)m; k0 += CP_AT_ONCE) {
-        const uint32_t n = min(CP_AT_ONCE, (uint32_t)m - k0);
-        __syncthreads();
+    if (tid == 0 && !good) *a.flag = 1;
+    if (tells) length_out[s] = good ? sq.first + m : a.length[s];
+    if (!good || !__syncthreads_or(moved)) return;
+    const uint32_t EB = 4 >> a.type, P = 1u << a.shift;
+    /* tokens a round: their pieces (of 16 bytes, or elements) are CM_PIECES a thread at most */
+    const uint32_t round = min(CM_TOKENS, CM_PIECES * PG_WG / (kind ? a.head_dim : a.head_dim * EB / 16));
+    for (uint32_t k0 = 0; k0 < (uint32_t)m; k0 += round) {
+        const uint32_t n = min(round, (uint32_t)m - k0);
         if (tid < n) {
-            const int f = sq.first + path[k0 + tid], t = sq.first + (int)(k0 + tid);
-            from_page[tid] = to_page[tid] = -1;
+            const int x = k0 ? path[k0 + tid] : mine, f = sq.first + x, t = sq.first + (int)(k0 + tid);
+            size_t from = NONE, to = NONE;
             if (f != t) {
-                if ((uint32_t)f < a.limit && (uint32_t)t < a.limit && f >= 0 && t >= 0) {
+                if (f >= 0 && t >= 0 && (uint32_t)f < a.limit) {
                     const int fp = page_of(a, s, (uint32_t)f), tp = page_of(a, s, (uint32_t)t);
-                    from_page[tid] = fp;
-                    to_page[tid] = fp < 0 ? -1 : tp;
-                    from_slot[tid] = (uint32_t)f & (P - 1);
-                    to_slot[tid] = (uint32_t)t & (P - 1);
+                    if (fp >= 0 && tp >= 0) {
+                        from = ((size_t)fp * a.kv_heads + h) << 8 | ((uint32_t)f & (P - 1));
+                        to = ((size_t)tp * a.kv_heads + h) << 8 | ((uint32_t)t & (P - 1));
+                    }
                 } else {
                     *a.flag = 1;
                 }
             }
+            moves.from[tid] = from;
+            moves.to[tid] = to;
         }
         __syncthreads();
-        for (int store = 0; store < 2; ++store) {
-            auto place = [&](uint32_t k, size_t &page, uint32_t &slot) {
-                const int pg = store ? to_page[k] : from_page[k];
-                page = (size_t)max(pg, 0) * a.kv_heads + h;
-                slot = store ? to_slot[k] : from_slot[k];
-                return to_page[k] >= 0;
-            };
-            size_t page;
-            uint32_t slot;
-            for (uint32_t i = tid; i < n * words; i += PG_WG) {
-                if (!place(i / words, page, slot)) continue;
-                uint32_t *x = (uint32_t *)p.keys + ((page << a.shift) + slot) * words + i % words;
-                if (store) *x = keys[i];
-                else keys[i] = *x;
-            }
-            for (uint32_t i = tid; i < n * hd; i += PG_WG) {
-                if (!place(i / hd, page, slot)) continue;
-                const size_t at = ((page * hd + i % hd) << a.shift) + slot;
-                unsigned char *x = (unsigned char *)p.values + at * EB, *y = values + (size_t)i * EB;
-                unsigned char *to = store ? x : y, *from = store ? y : x;
-                if (a.type == 0) *(uint32_t *)to = *(const uint32_t *)from;
-                else if (a.type == 1) *(uint16_t *)to = *(const uint16_t *)from;
-                else *to = *from;
-            }
-            if (a.type == 2)
-                for (uint32_t i = tid; i < n * a.nb; i += PG_WG) {
-                    if (!place(i / a.nb, page, slot)) continue;
-                    const size_t at = ((page * a.nb + i % a.nb) << a.shift) + slot;
-                    if (store) {
-                        p.ks[at] = scales[2 * i];
-                        p.vs[at] = scales[2 * i + 1];
-                    } else {
-                        scales[2 * i] = p.ks[at];
-                        scales[2 * i + 1] = p.vs[at];
-                    }
-                }
-            __syncthreads();
-        }
+        if (a.type == 0) move_tokens<4>(a, pools.p[l], kind, moves, n);
+        else if (a.type == 1) move_tokens<2>(a, pools.p[l], kind, moves, n);
+        else move_tokens<1>(a, pools.p[l], kind, moves, n);
+        __syncthreads();
     }
 }
 
@@ -546,7 +610,7 @@ hipError_t launch_fork(const ForkArgs &a, void *ws, hipStream_t s) {
 
 /* As many pools a launch as its arguments hold and its grid's threads allow. */
 uint32_t pools_at_once(const PagedArgs &a, uint32_t rows) {
-    const uint64_t most = (1u << 23) / ((uint64_t)rows * a.kv_heads);
+    const uint64_t most = (1u << 22) / ((uint64_t)rows * a.kv_heads);
     return most < POOLS_AT_ONCE ? (most ? (uint32_t)most : 1) : POOLS_AT_ONCE;
 }
 template <typename F>
@@ -566,15 +630,14 @@ hipError_t each_pools(const PagedArgs &a, const Pool *pools, uint32_t n, uint32_
 hipError_t launch_paged_copy(const PagedArgs &a, const Pool *pools, uint32_t n, const int32_t *copies, uint32_t rows,
                              hipStream_t s) {
     return each_pools(a, pools, n, rows, [&](const Pools &p, bool) {
-        hipLaunchKernelGGL(k_paged_copy, dim3(rows * p.n * a.kv_heads), dim3(PG_WG), 0, s, a, p, copies);
+        hipLaunchKernelGGL(k_paged_copy, dim3(2 * rows * p.n * a.kv_heads), dim3(PG_WG), 0, s, a, p, copies);
     });
 }
 
 hipError_t launch_paged_compact(const PagedArgs &a, const Pool *pools, uint32_t n, const int32_t *accepted, uint32_t stride,
                                 const int32_t *count, int32_t *length_out, hipStream_t s) {
-    const uint32_t EB = 4 >> a.type, lds = CP_AT_ONCE * (2 * a.head_dim * EB + 8 * a.nb);
     return each_pools(a, pools, n, a.seqs, [&](const Pools &p, bool first) {
-        hipLaunchKernelGGL(k_paged_compact, dim3(a.seqs * p.n * a.kv_heads), dim3(PG_WG), lds, s, a, p, accepted, stride, count,
+        hipLaunchKernelGGL(k_paged_compact, dim3(2 * a.seqs * p.n * a.kv_heads), dim3(PG_WG), 0, s, a, p, accepted, stride, count,
                            first ? length_out : nullptr);
     });
 }
