@@ -477,12 +477,12 @@ __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, 
     else copy_pieces<u4>((uint32_t)n * a.head_dim * EB / 16, x + f * head, x + t * head, [](uint32_t i) { return (size_t)i * 16; });
 }
 
-/* A workgroup per sequence, pool, KV head and kind: some of the path's tokens at a time into registers, then to their places. The
- * places of one round lie before the next rounds' tokens, since the path ascends. Keys 16 bytes a piece, values an element: of
- * a dim's row the path's positions lie next to each other, in the same lines of memory.
+/* A workgroup per sequence, pool and KV head: 16 of the path's tokens at a time into registers, then to their places. The places of one round lie before the next rounds' tokens, since the path ascends. A thread has one token: of its
+ * key every 16th piece of 16 bytes, of its value every 16th dim (lanes next to each other have the path's tokens of one dim,
+ * which lie in the same lines of memory).
  *
  * Bound by four trips to memory (batch, path, page ids, tokens). */
-constexpr uint32_t CM_TOKENS = 64, CM_PIECES = 8;
+constexpr uint32_t CM_TOKENS = 16;
 template <uint32_t EB>
 struct Element;
 template <>
@@ -497,91 +497,97 @@ template <>
 struct Element<1> {
     typedef uint8_t T;
 };
-struct Moves {
-    size_t from[CM_TOKENS], to[CM_TOKENS]; /* page times KV heads plus head, << 8 | slot; NONE: stays */
-};
-constexpr size_t NONE = ~(size_t)0;
-/* n pieces of each of the tokens, `each` of them a thread at most: piece x of token k at at(place of k, x). */
-template <typename T, bool INNER, typename At>
-__device__ __forceinline__ void move_pieces(const Moves &m, uint32_t tokens, uint32_t n, void *p, At at) {
-    const Divide by(INNER ? tokens : n); /* INNER: tokens innermost */
-    T x[CM_PIECES];
-    size_t to[CM_PIECES];
+/* n pieces of `step` bytes, N at most, of a token: requested, then written. */
+template <typename T, uint32_t N>
+struct Piece {
+    T x[N];
+    __device__ __forceinline__ void load(const char *from, uint32_t n, uint32_t step) {
 #pragma unroll
-    for (uint32_t u = 0; u < CM_PIECES; ++u) {
-        const uint32_t i = u * PG_WG + threadIdx.x;
-        to[u] = NONE;
-        if (i >= tokens * n) continue;
-        uint32_t rest;
-        const uint32_t q = by(i, rest), k = INNER ? rest : q, y = INNER ? q : rest;
-        if (m.from[k] == NONE) continue;
-        x[u] = *(const T *)((const char *)p + at(m.from[k], y));
-        to[u] = at(m.to[k], y);
+        for (uint32_t j = 0; j < N; ++j)
+            if (j < n) x[j] = *(const T *)(from + j * step);
     }
-    __syncthreads(); /* what is read here may be another's place */
+    __device__ __forceinline__ void store(char *to, uint32_t n, uint32_t step) const {
 #pragma unroll
-    for (uint32_t u = 0; u < CM_PIECES; ++u)
-        if (to[u] != NONE) *(T *)((char *)p + to[u]) = x[u];
+        for (uint32_t j = 0; j < N; ++j)
+            if (j < n) *(T *)(to + j * step) = x[j];
+    }
+};
+/* A token's move: its page and slot before and after. in: it does move. */
+struct Move {
+    bool in;
+    int fp, tp;
+    uint32_t fs, ts;
+};
+__device__ __forceinline__ Move move_of(const PagedArgs &a, uint32_t s, const Seq &sq, int x, uint32_t k, bool there) {
+    const int f = sq.first + x, t = sq.first + (int)k;
+    const uint32_t P = 1u << a.shift;
+    Move m = {false, -1, -1, (uint32_t)f & (P - 1), (uint32_t)t & (P - 1)};
+    if (!there || f == t) return m;
+    if (f < 0 || t < 0 || (uint32_t)f >= a.limit) {
+        *a.flag = 1;
+        return m;
+    }
+    m.fp = page_of(a, s, (uint32_t)f);
+    m.tp = page_of(a, s, (uint32_t)t);
+    m.in = m.fp >= 0 && m.tp >= 0;
+    return m;
 }
 template <uint32_t EB>
-__device__ __forceinline__ void move_tokens(const PagedArgs &a, const Pool &p, uint32_t kind, const Moves &m, uint32_t tokens) {
-    typedef typename Element<EB>::T T;
-    const uint32_t hd = a.head_dim, shift = a.shift, nb = a.nb;
-    if (kind)
-        move_pieces<T, true>(m, tokens, hd, p.values, [=](size_t w, uint32_t d) { return (((w >> 8) * hd + d << shift) + (w & 255)) * EB; });
-    else
-        move_pieces<u4, false>(m, tokens, hd * EB / 16, p.keys, [=](size_t w, uint32_t i) { return (((w >> 8) << shift) + (w & 255)) * hd * EB + 16 * i; });
-    if constexpr (EB == 1)
-        move_pieces<uint32_t, true>(m, tokens, nb, kind ? p.vs : p.ks, [=](size_t w, uint32_t b) { return (((w >> 8) * nb + b << shift) + (w & 255)) * 4; });
-}
 __global__ __launch_bounds__(PG_WG) void k_paged_compact(PagedArgs a, Pools pools, const int32_t *accepted, uint32_t stride,
                                                          const int32_t *count, int32_t *length_out) {
-    __shared__ Moves moves;
-    const uint32_t tid = threadIdx.x, kind = blockIdx.x & 1, y = blockIdx.x >> 1, h = y % a.kv_heads;
-    const uint32_t l = y / a.kv_heads % pools.n, s = y / a.kv_heads / pools.n;
+    typedef typename Element<EB>::T T;
+    const uint32_t tid = threadIdx.x, h = blockIdx.x % a.kv_heads, y = blockIdx.x / a.kv_heads, s = y / pools.n;
+    const Pool &p = pools.p[y % pools.n];
+    const uint32_t kt = tid / 16, kx = tid % 16, vt = tid % 16, vx = tid / 16; /* token and part, of keys and of values */
     const int32_t *path = accepted + (size_t)s * stride;
-    const int mine = tid < stride ? path[tid] : 0, m = count[s]; /* the first entries with the count */
-    const bool tells = h == 0 && l == 0 && kind == 0 && length_out && tid == 0;
+    /* of the first round, requested with the count */
+    const int entry = tid < stride ? path[tid] : 0, m = count[s];
+    int k_at = kt < stride ? path[kt] : 0, v_at = vt < stride ? path[vt] : 0;
     Seq sq;
     const bool ok = sequence(a, s, sq);
     bool good = ok && m >= 0 && m <= sq.n && (uint32_t)m <= stride, moved = false;
     if (good)
         for (uint32_t k = tid; k < (uint32_t)m; k += PG_WG) {
-            const int at = k == tid ? mine : path[k];
+            const int at = k == tid ? entry : path[k];
             if (at < 0 || at >= sq.n || (k && at <= path[k - 1])) good = false;
             moved = moved || at != (int)k;
         }
     good = __syncthreads_and(good);
     if (tid == 0 && !good) *a.flag = 1;
-    if (tells) length_out[s] = good ? sq.first + m : a.length[s];
+    if (length_out && y % pools.n == 0 && h == 0 && tid == 0) length_out[s] = good ? sq.first + m : a.length[s];
     if (!good || !__syncthreads_or(moved)) return;
-    const uint32_t EB = 4 >> a.type, P = 1u << a.shift;
-    /* tokens a round: their pieces (of 16 bytes, or elements) are CM_PIECES a thread at most */
-    const uint32_t round = min(CM_TOKENS, CM_PIECES * PG_WG / (kind ? a.head_dim : a.head_dim * EB / 16));
-    for (uint32_t k0 = 0; k0 < (uint32_t)m; k0 += round) {
-        const uint32_t n = min(round, (uint32_t)m - k0);
-        if (tid < n) {
-            const int x = k0 ? path[k0 + tid] : mine, f = sq.first + x, t = sq.first + (int)(k0 + tid);
-            size_t from = NONE, to = NONE;
-            if (f != t) {
-                if (f >= 0 && t >= 0 && (uint32_t)f < a.limit) {
-                    const int fp = page_of(a, s, (uint32_t)f), tp = page_of(a, s, (uint32_t)t);
-                    if (fp >= 0 && tp >= 0) {
-                        from = ((size_t)fp * a.kv_heads + h) << 8 | ((uint32_t)f & (P - 1));
-                        to = ((size_t)tp * a.kv_heads + h) << 8 | ((uint32_t)t & (P - 1));
-                    }
-                } else {
-                    *a.flag = 1;
-                }
-            }
-            moves.from[tid] = from;
-            moves.to[tid] = to;
+    const uint32_t hd = a.head_dim, shift = a.shift, nb = a.nb, pieces = hd * EB / 16;
+    const uint32_t kn = pieces > kx ? (pieces - kx + 15) / 16 : 0, vn = hd / 16, vstep = 16 * EB << shift;
+    for (uint32_t k0 = 0; k0 < (uint32_t)m; k0 += CM_TOKENS) {
+        if (k0) {
+            k_at = k0 + kt < (uint32_t)m ? path[k0 + kt] : 0;
+            v_at = k0 + vt < (uint32_t)m ? path[k0 + vt] : 0;
         }
-        __syncthreads();
-        if (a.type == 0) move_tokens<4>(a, pools.p[l], kind, moves, n);
-        else if (a.type == 1) move_tokens<2>(a, pools.p[l], kind, moves, n);
-        else move_tokens<1>(a, pools.p[l], kind, moves, n);
-        __syncthreads();
+        const Move km = move_of(a, s, sq, k_at, k0 + kt, k0 + kt < (uint32_t)m), vm = move_of(a, s, sq, v_at, k0 + vt, k0 + vt < (uint32_t)m);
+        auto head = [&](int page) { return (size_t)page * a.kv_heads + h; };
+        auto key = [&](int page, uint32_t slot) { return (char *)p.keys + ((head(page) << shift) + slot) * hd * EB + 16 * kx; };
+        auto value = [&](int page, uint32_t slot) { return (char *)p.values + (((head(page) * hd + vx) << shift) + slot) * EB; };
+        auto scale = [&](float *w, int page, uint32_t slot) { return w + ((head(page) * nb + vx) << shift) + slot; };
+        Piece<u4, 4> kp;
+        Piece<T, 16> vp;
+        float ks = 0.0f, vs = 0.0f;
+        if (km.in) kp.load(key(km.fp, km.fs), kn, 256);
+        if (vm.in) {
+            vp.load(value(vm.fp, vm.fs), vn, vstep);
+            if (EB == 1 && vx < nb) {
+                ks = *scale(p.ks, vm.fp, vm.fs);
+                vs = *scale(p.vs, vm.fp, vm.fs);
+            }
+        }
+        __syncthreads(); /* what is read here may be another's place */
+        if (km.in) kp.store(key(km.tp, km.ts), kn, 256);
+        if (vm.in) {
+            vp.store(value(vm.tp, vm.ts), vn, vstep);
+            if (EB == 1 && vx < nb) {
+                *scale(p.ks, vm.tp, vm.ts) = ks;
+                *scale(p.vs, vm.tp, vm.ts) = vs;
+            }
+        }
     }
 }
 
@@ -637,8 +643,11 @@ hipError_t launch_paged_copy(const PagedArgs &a, const Pool *pools, uint32_t n, 
 hipError_t launch_paged_compact(const PagedArgs &a, const Pool *pools, uint32_t n, const int32_t *accepted, uint32_t stride,
                                 const int32_t *count, int32_t *length_out, hipStream_t s) {
     return each_pools(a, pools, n, a.seqs, [&](const Pools &p, bool first) {
-        hipLaunchKernelGGL(k_paged_compact, dim3(2 * a.seqs * p.n * a.kv_heads), dim3(PG_WG), 0, s, a, p, accepted, stride, count,
-                           first ? length_out : nullptr);
+        const dim3 grid(a.seqs * p.n * a.kv_heads);
+        int32_t *const tells = first ? length_out : nullptr;
+        if (a.type == 0) hipLaunchKernelGGL((k_paged_compact<4>), grid, dim3(PG_WG), 0, s, a, p, accepted, stride, count, tells);
+        else if (a.type == 1) hipLaunchKernelGGL((k_paged_compact<2>), grid, dim3(PG_WG), 0, s, a, p, accepted, stride, count, tells);
+        else hipLaunchKernelGGL((k_paged_compact<1>), grid, dim3(PG_WG), 0, s, a, p, accepted, stride, count, tells);
     });
 }
 
