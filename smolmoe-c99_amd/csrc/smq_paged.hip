@@ -73,16 +73,22 @@ __device__ __forceinline__ size_t scales_at(const PagedArgs &a, int page, uint32
     return (((size_t)page * a.kv_heads + h) * a.nb) << a.shift;
 }
 
-/* Dims d .. d + 3 of a head row, rotated (smq_rope_kv's products and order). */
+/* Two dims rotated by a cosine and a sine (smq_rope_kv's products and order). */
+__device__ __forceinline__ void turn_pair(float &p, float &q, float c, float s) {
+    const float pc = p * c, qs = q * s, ps = p * s, qc = q * c;
+    p = pc - qs;
+    q = ps + qc;
+}
+/* Dims d .. d + 3 of a head row, rotated. */
 __device__ __forceinline__ f4 rotated(f4 x, uint32_t d, uint32_t pairs, const float *c, const float *s) {
 #pragma unroll
     for (uint32_t e = 0; e < 4; e += 2) {
         const uint32_t i = (d + e) / 2;
         if (i >= pairs) continue;
-        const float p = x[e], q = x[e + 1];
-        const float pc = p * c[i], qs = q * s[i], ps = p * s[i], qc = q * c[i];
-        x[e] = pc - qs;
-        x[e + 1] = ps + qc;
+        float p = x[e], q = x[e + 1];
+        turn_pair(p, q, c[i], s[i]);
+        x[e] = p;
+        x[e + 1] = q;
     }
     return x;
 }
@@ -91,23 +97,45 @@ __device__ __forceinline__ f4 rotated(f4 x, uint32_t d, uint32_t pairs, const fl
 __device__ __forceinline__ uint32_t norm_lanes(const PagedArgs &a) {
     return a.head_dim <= 32 ? 8 : a.head_dim <= 64 ? 16 : a.head_dim <= 128 ? 32 : 64;
 }
-/* Dims d .. d + 3 (0 past the head) of a head that `lanes` lanes hold, normed. The sum of squares, whose products are exact,
- * the root and the quotient in 64 bits: no order of the sum shows in the f32 quotient, and the bits are the same whichever
- * lanes hold the head; the two products round to f32 as the formula has them. */
-__device__ __forceinline__ f4 normed(f4 x, const float *norm, uint32_t d, const PagedArgs &a, uint32_t lanes, float eps) {
-    if (!norm) return x;
-    double sum = 0.0;
+template <int CTRL>
+__device__ __forceinline__ double lane_add(double x) { /* x and the lane's that CTRL names */
+    const int lo = __builtin_amdgcn_mov_dpp(__double2loint(x), CTRL, 0xf, 0xf, false),
+              hi = __builtin_amdgcn_mov_dpp(__double2hiint(x), CTRL, 0xf, 0xf, false);
+    return x + __hiloint2double(hi, lo);
+}
+template <int CTRL>
+__device__ __forceinline__ float lane_of_four(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+/* Four heads' dims d .. d + 3 (0 past the head), each head in `lanes` lanes, normed by g, their part of the norm. The sum of
+ * squares, whose products are exact, the root and the quotient in 64 bits: no order of the sum shows in the f32 quotient, and the
+ * bits are the same whichever lanes hold the head; the two products round to f32 as the formula has them. Roots and quotients,
+ * about 40 instructions on 64 bits, one for the four heads: a lane of four does that of one. */
+__device__ __forceinline__ void normed(f4 (&x)[4], f4 g, const PagedArgs &a, uint32_t lanes, float eps) {
+    double sum[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum += (double)x[e] * (double)x[e];
-    for (uint32_t off = 1; off < lanes; off *= 2) sum += __shfl_xor(sum, (int)off);
-    const float inv = (float)(1.0 / sqrt(sum / (double)a.head_dim + (double)eps));
-    const f4u g = *(const f4u *)(norm + d);
+    for (int u = 0; u < 4; ++u) {
+        sum[u] = 0.0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float y = x[e] * inv;
-        x[e] = y * g[e];
+        for (int e = 0; e < 4; ++e) sum[u] = __builtin_fma((double)x[u][e], (double)x[u][e], sum[u]);
+        sum[u] = lane_add<0xB1>(sum[u]); /* the other of two, the other two of four, four of eight (mirrored, they are alike) */
+        sum[u] = lane_add<0x4E>(sum[u]);
+        sum[u] = lane_add<0x141>(sum[u]);
+        if (lanes > 8) sum[u] = lane_add<0x140>(sum[u]);
+        if (lanes > 16) sum[u] += __shfl_xor(sum[u], 16);
+        if (lanes > 32) sum[u] += __shfl_xor(sum[u], 32);
     }
-    return x;
+    const uint32_t k = threadIdx.x & 3;
+    const double mean = (k & 2 ? k & 1 ? sum[3] : sum[2] : k & 1 ? sum[1] : sum[0]) / (double)a.head_dim;
+    const float own = (float)(1.0 / sqrt(mean + (double)eps));
+    const float inv[4] = {lane_of_four<0x00>(own), lane_of_four<0x55>(own), lane_of_four<0xAA>(own), lane_of_four<0xFF>(own)};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float y = x[u][e] * inv[u];
+            x[u][e] = y * g[e];
+        }
 }
 /* The rotary position of a token whose sequence's new tokens begin at position first; false, with the flag, where the tables have none. */
 __device__ __forceinline__ bool own_turn(const PagedArgs &a, int first, int depth, uint32_t &at) {
@@ -187,7 +215,7 @@ __device__ __forceinline__ typename Four<TYPE>::T encode(f4 x, float &scale, boo
  * Bound by the launch and three round trips (batch, page ids, rows) for a decode step: 4.7 us for 48 tokens of 2 KV heads of
  * 64; by bytes for chunks: 4 prompts of up to 700 tokens, 12 heads on 2 of 128, f16, 10.4 us (keys and values in one
  * workgroup, one pass after another: 5 us longer). */
-constexpr uint32_t ST_PASSES = 4;
+constexpr uint32_t ST_PASSES = 4, ST_HEADS = 4;
 template <uint32_t TYPE, bool NORM>
 __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, const float *cs, const float *sn,
                                                        uint32_t kv_groups) {
@@ -203,15 +231,39 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, c
         if constexpr (NORM) {
             uint32_t turn_at = pos;
             if (w.depth && !own_turn(a, (int)pos - (int)(r - (uint32_t)a.begin[s]), w.depth[r], turn_at)) return;
-            const float *c = cs + (size_t)turn_at * a.pairs, *sr = sn + (size_t)turn_at * a.pairs;
-            const uint32_t lanes = norm_lanes(a), d = 4 * (tid % lanes);
-            for (uint32_t h0 = 0; h0 < a.heads; h0 += ST_WG / lanes) { /* uniform: the norm's sums shuffle */
-                const uint32_t h = h0 + tid / lanes;
-                const bool in = h < a.heads && d < hd;
-                f4 x = {};
-                if (in) x = *(const f4u *)(w.q + r * w.q_stride + h * hd + d);
-                x = normed(x, w.q_norm, in ? d : 0, a, lanes, w.eps);
-                if (in) *(f4u *)(w.q_out + r * w.q_out_stride + h * hd + d) = rotated(x, d, a.pairs, c, sr);
+            /* a thread has the same dims of several heads: their norm, cosines and sines once, the heads requested together */
+            const uint32_t lanes = norm_lanes(a), d = 4 * (tid % lanes), per = ST_WG / lanes;
+            const size_t at = (size_t)turn_at * a.pairs;
+            f4 g = {};
+            f2 c = {}, sr = {};
+            if (w.q_norm && d < hd) g = *(const f4u *)(w.q_norm + d);
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e)
+                if (d / 2 + e < a.pairs) {
+                    c[e] = cs[at + d / 2 + e];
+                    sr[e] = sn[at + d / 2 + e];
+                }
+            const float *from = w.q + r * w.q_stride + d;
+            float *to = w.q_out + r * w.q_out_stride + d;
+            for (uint32_t h0 = tid / lanes; h0 < a.heads + tid / lanes; h0 += ST_HEADS * per) { /* uniform: the norm's sums shuffle */
+                f4 x[ST_HEADS];
+#pragma unroll
+                for (uint32_t u = 0; u < ST_HEADS; ++u) {
+                    x[u] = f4{};
+                    if (h0 + u * per < a.heads && d < hd) x[u] = *(const f4u *)(from + (h0 + u * per) * hd);
+                }
+                if (w.q_norm) normed(x, g, a, lanes, w.eps);
+#pragma unroll
+                for (uint32_t u = 0; u < ST_HEADS; ++u) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        float y = x[u][2 * e], z = x[u][2 * e + 1];
+                        if (d / 2 + e < a.pairs) turn_pair(y, z, c[e], sr[e]);
+                        x[u][2 * e] = y;
+                        x[u][2 * e + 1] = z;
+                    }
+                    if (h0 + u * per < a.heads && d < hd) *(f4u *)(to + (h0 + u * per) * hd) = x[u];
+                }
             }
             return;
         }
@@ -233,6 +285,8 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, c
     const float *from = kind ? w.v : w.k;
     const size_t stride = NORM ? kind ? w.v_stride : w.k_stride : (size_t)a.kv_heads * hd;
     const int first = NORM && w.depth ? a.begin[b.seq] - b.row : 0;
+    f4 g = {}; /* a thread's dims are the same in every pass */
+    if (NORM && !kind && w.k_norm && 4 * (tid % lanes) < hd) g = *(const f4u *)(w.k_norm + 4 * (tid % lanes));
     for (uint32_t i0 = tid; i0 < (n * lanes + ST_WG - 1) / ST_WG * ST_WG; i0 += ST_PASSES * ST_WG) { /* whole waves: encode shuffles */
         f4 y[ST_PASSES];
 #pragma unroll
@@ -240,6 +294,9 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, c
             const uint32_t i = i0 + u * ST_WG, j = i / lanes, d = 4 * (i - j * lanes);
             y[u] = f4{};
             if (j < n && d < hd) y[u] = *(const f4u *)(from + (size_t)(b.row + (int)(b.p0 + j)) * stride + h * hd + d);
+        }
+        if constexpr (NORM) {
+            if (!kind && w.k_norm) normed(y, g, a, lanes, w.eps);
         }
 #pragma unroll
         for (uint32_t u = 0; u < ST_PASSES; ++u) {
@@ -249,7 +306,6 @@ __global__ __launch_bounds__(ST_WG) void k_paged_store(PagedArgs a, RowArgs w, c
             uint32_t at = pos;
             if constexpr (NORM) {
                 if (!kind) {
-                    y[u] = normed(y[u], w.k_norm, in ? d : 0, a, lanes, w.eps);
                     if (in && w.depth && !own_turn(a, first, w.depth[b.row + (int)pos], at)) {
                         in = false;
                         y[u] = f4{};
