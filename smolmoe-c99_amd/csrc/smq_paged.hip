@@ -559,11 +559,26 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     return p;
 }
 
+/* A tile's rows for trees, whose tiles all go over the whole context. 16, whose waves share the positions out, while their steps
+ * are few in all: 13 drafts at 613 and 3000 (f16, 14 heads on 2 of 64) 12.1 and 15.2 us, 64 rows 15.3 and 17.4; 8 Q8
+ * sequences of 16 at 1500 17.9, 20.6; 8064 steps (two f32 ones of 30 at 2000, 32 on 8 of 64) 28.8, 29.7; but 32000 (4 f16 ones of
+ * 16 at 8000, 32 on 8 of 128) 73, 35. Else 64 where a sequence has no more (that one 35.3 us, 128 rows 44.3), 128 above (8 f16
+ * sequences of 63 at 16384 252, 64 rows 401). */
+uint32_t tree_rows(const PagedArgs &a) {
+    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
+    uint64_t reach = a.limit;
+    if (a.window && (uint64_t)a.window + a.sinks + a.tokens < reach) reach = (uint64_t)a.window + a.sinks + a.tokens;
+    const uint64_t tiles = (rows + seqs * 15) / 16 * a.kv_heads;
+    if (rows <= 32 * seqs || tiles * (reach / PA_STEP + 1) <= 8192) return 16;
+    return rows <= 64 * seqs ? 64 : 64 * attend_rt(attend_ks(a.head_dim));
+}
+
 /* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own theirs,
  * 16 or 32 each. 32 where tiles are cut or many: a fragment read serves twice. Few whole tiles take as long as the longest
  * one's chain of steps, and a step of half the rows is shorter (2048 tokens from an empty cache, f16, 8 KV heads of 64: 71
  * us, 58; 1024 of 128: 51, 40; but 2048 of 128: 100, 104). */
 AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes, bool tree) {
+    if (tree) return plan_tiles(a, ws_bytes, tree_rows(a), true);
     const uint32_t ks = attend_ks(a.head_dim);
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
     if (rows <= 32 * seqs) return plan_tiles(a, ws_bytes, 16, tree);
@@ -611,9 +626,16 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
 
 size_t paged_attention_workspace(const PagedArgs &given, bool tree) {
     PagedArgs a = given;
+    auto bytes = [&](const AttendPlan &p) {
+        return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
+    };
     a.sinks = a.limit; /* the call brings them: a plan of more positions needs no fewer bytes, up to all of the context's */
-    const AttendPlan p = attend_plan(a, ~(size_t)0, tree);
-    return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
+    const size_t most = bytes(attend_plan(a, ~(size_t)0, tree));
+    if (!tree) return most;
+    a.sinks = 0; /* with fewer the tiles may have other rows */
+    const uint32_t rows = tree_rows(a);
+    a.sinks = a.limit;
+    return max(most, bytes(plan_tiles(a, ~(size_t)0, rows, true)));
 }
 
 hipError_t launch_paged_attention(const PagedArgs &a, const TreeArgs *tree, const float *q, float *att, void *ws,
