@@ -2,6 +2,7 @@
 attention against 64 bits within the bound beside tree64, scores of beams against 64 bits."""
 import numpy as np
 import pytest
+import torch
 
 import drafts_ref as ref
 from checks import assert_same_f32, say
@@ -858,3 +859,358 @@ def test_beam_histories_that_are_full():
         for parent, token, h, m in zip(got[0], got[1], got[4], got[5]):
             want = list(history[parent]) if length[0] > 0 else [token] + [NONE] * 9
             assert list(h) == want and m == (10 if length[0] > 0 else 1)
+
+
+# ---- together -----------------------------------------------------------------
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+def test_drafts_together(kv_type):
+    """Drafting on a shared pool: trees stored, attended, an accepted path kept, the rest given back, new pages, for several
+    steps. Another cache gets the accepted tokens one after another: its rows are the same bits, and causal attention over it
+    gives the accepted tokens' results."""
+    heads, kv, hd, page, context = 6, 2, 64, 16, 256
+    rng = np.random.default_rng(8)
+    lengths = np.array([70, 33, 16], np.int32)
+    cache = Cache(kv_type, kv, hd, page, list(lengths), spare=60, stride=16).upload()
+    plain = Cache(kv_type, kv, hd, page, [context - 16] * 3, spare=0, stride=16, stale="nan")
+    for s, m in enumerate(lengths):
+        for a, b in zip(ref.pool_parts(plain), ref.pool_parts(cache)):
+            pg, sl = plain.slots(s, np.arange(m))
+            cg, cl = cache.slots(s, np.arange(m))
+            if a[1] == 2:
+                a[0][pg, :, sl] = b[0][cg, :, cl]
+            else:
+                a[0][pg, :, :, sl] = b[0][cg, :, :, cl]
+    plain.upload()
+    shape = smq.attn_shape(heads, kv, hd, hd // 2, 0, context)
+    cb, sb = (dev(x) for x in tables(context, hd // 2))
+    w = [dev((1 + 0.2 * synth.normal(300 + i, hd)).astype(np.float32)) for i in range(2)]
+    held = np.array([-(-m // page) for m in lengths], np.int32)
+    refs = np.zeros(cache.pages, np.int32)
+    for s in range(3):
+        refs[cache.table[s, :held[s]]] += 1
+    words = 1
+    for step in range(4):
+        new = [int(rng.integers(1, 20)), 12, 1 if step % 2 else 9]
+        # room for the drafts: every row goes on
+        grown = lengths + np.array(new, np.int32)
+        bufs = [dev(x) for x in (cache.table, held, refs, np.arange(3, dtype=np.int32), lengths, grown)]
+        outs = [smq.DeviceBuffer(4 * n) for n in (3 * 16, 3, cache.pages, 9, 1)]
+        f = smq.page_fork(*bufs[:3], 3, 3, 16, page, cache.pages, *bufs[3:], *outs)
+        smq.paged_fork(f, smq.DeviceBuffer(smq.paged_fork_workspace(f)))
+        assert (outs[3].download(np.int32).reshape(3, 3)[:, 2] == 0).all()  # alone in its last page
+        cache.table, held, refs = outs[0].download(np.int32).reshape(3, 16), outs[1].download(np.int32), outs[2].download(np.int32)
+        assert (held == -(-grown // page)).all() and refs.sum() == held.sum() and refs.max() == 1
+        cache.tb = outs[0]
+        batch = Batch(cache, new, lengths=grown)
+        n = batch.tokens
+        trees = Trees(batch, seed=step, stride=words).upload()
+        q, k, v = (synth.normal(310 + 3 * step + i, n * x * hd, 2.0).reshape(n, x, hd) for i, x in enumerate((heads, kv, kv)))
+        d, m, rot, att, out = (smq.DeviceBuffer(x) for x in (4 * n, 4 * n * words, q.nbytes, q.nbytes, 12))
+        smq.draft_masks(trees.pb, batch.desc, d, m, words)
+        smq.paged_norm_rope_kv(smq.paged_rows(dev(q), rot, dev(k), dev(v), *w, 1e-6, d), batch.desc, shape, cb, sb, cache.desc)
+        ws = smq.DeviceBuffer(max(16, smq.paged_tree_attention_workspace(batch.desc, shape)))
+        smq.paged_tree_attention(rot, att, batch.desc, shape, 0, d, m, words, cache.desc, ws)
+        # the path of each sequence's deepest token
+        paths = []
+        for s in range(3):
+            t = int(np.argmax(trees.depth[batch.begin[s]:batch.begin[s + 1]]))
+            paths.append([int(x) for x in np.nonzero(trees.seen[s][t])[0]])
+        stride = max(map(len, paths))
+        acc = np.array([p + [0] * (stride - len(p)) for p in paths], np.int32)
+        count = np.array([len(p) for p in paths], np.int32)
+        smq.paged_compact(batch.desc, shape, dev(acc), stride, dev(count), smq.paged_pools([cache.desc]), out)
+        first, lengths = lengths, out.download(np.int32)
+        same(lengths, first + count)
+        # the same tokens, one path each
+        at = np.concatenate([batch.begin[s] + np.array(paths[s], int) for s in range(3)])
+        one = Batch(plain, list(count), lengths=lengths)
+        prot, patt = (smq.DeviceBuffer(4 * len(at) * heads * hd) for _ in range(2))
+        smq.paged_norm_rope_kv(smq.paged_rows(dev(q[at]), prot, dev(k[at]), dev(v[at]), *w), one.desc, shape, cb, sb, plain.desc)
+        smq.paged_attention(prot, patt, one.desc, shape, 0, plain.desc)
+        same(rot.download(np.float32).reshape(q.shape)[at], prot.download(np.float32).reshape(-1, heads, hd))
+        both = []
+        for c in (cache, plain):
+            whole = Batch(c, list(lengths), lengths=lengths)
+            rk, rv = (smq.DeviceBuffer(4 * whole.tokens * kv * hd) for _ in range(2))
+            smq.paged_read(whole.desc, smq.attn_shape(heads, kv, hd, 0, 0, context), c.desc, rk, rv)
+            both.append((rk.download(np.float32), rv.download(np.float32)))
+        for a, b in zip(*both):
+            same(a, b)
+        got, want = att.download(np.float32).reshape(q.shape)[at], patt.download(np.float32).reshape(-1, heads, hd)
+        top = np.abs(both[1][1]).max()
+        # both within an f32 calculation's error of the same value: scores off by (hd + 8) 2^-24 of sum |q k| each, see tree64
+        size = max(np.abs(both[1][0]).max() * np.abs(prot.download(np.float32)).max() * np.sqrt(hd), 1.0)
+        limit = 2 * top * (4 * size * (hd + 8) + 4 * (size + 2) + lengths.max() / 8 + 64) * 2.0 ** -24
+        assert np.abs(got - want).max() <= limit
+        assert not flagged()
+
+
+def test_beams_together():
+    """A beam search of three prompts' beams over one pool: choice, fork, copy, store and attention of every step against a
+    search that keeps each beam's tokens and works its attention out from them in 64 bits."""
+    heads, kv, hd, page, beams, groups, vocab, layers = 4, 2, 32, 16, 4, 3, 300, 2
+    rng = np.random.default_rng(9)
+    rows, stride, context = groups * beams, 8, 128
+    pages = rows * 6
+    embed = [(rng.standard_normal((vocab, x * hd))).astype(np.float32) for x in (heads, kv, kv)]
+    head = rng.standard_normal((heads * hd, vocab)) * 0.5
+    shape = smq.attn_shape(heads, kv, hd, hd // 2, 0, context)
+    cos, sin = tables(context, hd // 2)
+    cb, sb = dev(cos), dev(sin)
+    pools = [Cache(F32, kv, hd, page, [page * pages], spare=0).upload() for _ in range(layers)]
+    descs = smq.paged_pools([p.desc for p in pools])
+    prompts = [list(rng.integers(3, vocab, n)) for n in (37, 16, 5)]
+
+    def logits_of(tokens):
+        pos = np.arange(len(tokens))
+        q = rotate(embed[0][tokens[-1:]].reshape(1, heads, hd), cos[pos[-1:]], sin[pos[-1:]], hd // 2)[0].astype(np.float64)
+        k = rotate(embed[1][tokens].reshape(-1, kv, hd), cos[pos], sin[pos], hd // 2).astype(np.float64)
+        v = embed[2][tokens].reshape(-1, kv, hd).astype(np.float64)
+        out = []
+        for h in range(heads):
+            x = k[:, h // 2] @ q[h] / np.sqrt(hd)
+            p = np.exp(x - x.max())
+            out.append(p @ v[:, h // 2] / p.sum())
+        return (np.concatenate(out) @ head).astype(np.float32)
+
+    # old rows: one per prompt, its pages shared by the beams from the first fork on
+    table = np.full((groups, stride), -1, np.int32)
+    order, at = rng.permutation(pages).astype(np.int32), 0
+    held = np.array([-(-len(p) // page) for p in prompts], np.int32)
+    for g, n in enumerate(held):
+        table[g, :n] = order[at:at + n]
+        at += n
+    refs = np.bincount(table[table >= 0], minlength=pages).astype(np.int32)
+    tb, hb, rb = dev(table), dev(held), dev(refs)
+
+    def store(tb, n_rows, new, lengths, tokens):
+        begin = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        total = int(begin[-1])
+        batch = smq.paged_batch(dev(begin), dev(np.asarray(lengths, np.int32)), tb, n_rows, total, stride)
+        q, k, v = (dev(np.ascontiguousarray(e[tokens])) for e in embed)
+        rot, att = smq.DeviceBuffer(4 * total * heads * hd), smq.DeviceBuffer(4 * total * heads * hd)
+        for p in pools:
+            smq.paged_norm_rope_kv(smq.paged_rows(q, rot, k, v), batch, shape, cb, sb, p.desc)
+        ws = smq.DeviceBuffer(max(16, smq.paged_attention_workspace(batch, shape)))
+        smq.paged_attention(rot, att, batch, shape, 0, pools[-1].desc, ws)
+        return att.download(np.float32).reshape(total, -1)[begin[1:] - 1] @ head
+
+    first = store(tb, groups, [len(p) for p in prompts], [len(p) for p in prompts], [t for p in prompts for t in p])
+    live = [[(list(p), 0.0, False)] for p in prompts]
+    logits, score, done = first.astype(np.float32), np.zeros(groups, np.float32), np.zeros(groups, np.uint8)
+    width, ends, eos = 1, 0, NONE
+    history = np.full((groups, 64), NONE, np.uint32)
+    for g, p in enumerate(prompts):
+        history[g, :len(p)] = p
+    hist, length = dev(history), dev(np.array([len(p) for p in prompts], np.int32))
+    old = groups
+    for step in range(9):
+        n = groups * beams
+        # the search on tokens
+        nxt = []
+        for g in range(groups):
+            cand = []
+            for i, (tokens, s, over) in enumerate(live[g]):
+                if over:
+                    cand.append((-s, i, 0, tokens, True))
+                    continue
+                l = logits_of(tokens).astype(np.float64)
+                l -= l.max() + np.log(np.exp(l - l.max()).sum())
+                cand += [(-(s + l[v]), i, int(v), tokens + [int(v)], False) for v in np.argsort(-l, kind="stable")[:beams]]
+            cand.sort(key=lambda c: c[:3])
+            nxt.append([(c[3], -c[0], c[4]) for c in cand[:beams]])
+        if step == 2:
+            eos = nxt[0][1][0][-1]  # one that some beam ends with
+        nxt = [[(tokens, s, over or tokens[-1] == eos) for tokens, s, over in x] for x in nxt]
+        lb, sc, dn = dev(np.ascontiguousarray(logits, np.float32)), dev(score), dev(done)
+        outs = [smq.DeviceBuffer(4 * n) for _ in range(3)] + [smq.DeviceBuffer(n), smq.DeviceBuffer(4 * n * 64), smq.DeviceBuffer(4 * n)]
+        b = smq.beam_step(lb, vocab, groups, width, vocab, beams, sc, *outs[:3], done=dn, pad=0, eos=eos, done_out=outs[3],
+                          history=hist, history_out=outs[4], history_stride=64, length=length, length_out=outs[5])
+        smq.beam_select(b, smq.DeviceBuffer(smq.beam_select_workspace(b)))
+        parent, token, score, done = (o.download(t) for o, t in zip(outs, (np.int32, np.uint32, np.float32, np.uint8)))
+        live = nxt
+        hist, length, lens = outs[4], outs[5], outs[5].download(np.int32)
+        rows_of = hist.download(np.uint32).reshape(n, 64)
+        for i in range(n):
+            tokens, s, over = live[i // beams][i % beams]
+            assert list(rows_of[i, :lens[i]]) == tokens and bool(done[i]) == over, (step, i)
+            assert abs(score[i] - s) < 1e-4 * max(1.0, abs(s))  # of nine steps' f32 attention and logits
+            ends += over
+        # pages: each beam keeps its parent's positions and gets room for its last token (done ones: the same as before)
+        kept = (lens - 1).astype(np.int32)
+        no = [smq.DeviceBuffer(4 * x) for x in (n * stride, n, pages, n * 3, 1)]
+        f = smq.page_fork(tb, hb, rb, old, n, stride, page, pages, outs[0], dev(kept), dev(lens.astype(np.int32)), *no)
+        smq.paged_fork(f, smq.DeviceBuffer(smq.paged_fork_workspace(f)))
+        smq.paged_copy(no[3], n, shape, descs)
+        tb, hb, rb, old, width = no[0], no[1], no[2], n, beams
+        assert no[4].download(np.int32)[0] >= 0
+        now, counts = tb.download(np.int32).reshape(n, stride), rb.download(np.int32)
+        same(np.bincount(now[now >= 0], minlength=pages).astype(np.int32), counts)
+        logits = store(tb, n, [1] * n, lens, [int(r[m - 1]) for r, m in zip(rows_of, lens)])
+        assert not flagged()
+    assert ends
+    now, lens = tb.download(np.int32).reshape(n, stride), length.download(np.int32)
+    keys = [p.kb.download(np.float32).reshape(pages, kv, page, hd) for p in pools]
+    for row in range(n):  # every layer went the same way
+        for pos in range(lens[row]):
+            pg, sl = now[row, pos // page], pos % page
+            a, b = (x[pg, :, sl] for x in keys)
+            same(a, b)
+            same(a[0], rotate(embed[1][rows_of[row, pos]].reshape(1, kv, hd), cos[pos:pos + 1], sin[pos:pos + 1], hd // 2)[0, 0])
+
+
+def test_replays_of_all():
+    """Each operator captured into one graph and replayed with other contents beside eager work on buffers of its own, and on
+    another stream; two graphs at the same time have workspaces of their own."""
+    heads, kv, hd, page, words = 8, 2, 64, 32, 2
+    lengths, new = [700, 190, 64], [20, 33, 1]
+    cos, sin = (dev(x) for x in tables(800, hd // 2))
+    shape = smq.attn_shape(heads, kv, hd, hd // 2, 0, 800)
+    n, groups, beams, select, vocab = sum(new), 3, 2, 3, 3000
+
+    class Side:
+        """The same calls on buffers of its own."""
+
+        def __init__(self):
+            self.cache = Cache(Q8, kv, hd, page, lengths, seed=12, spare=20).upload()
+            c = self.cache
+            self.batch = Batch(c, new)
+            buf = smq.DeviceBuffer
+            self.q, self.k, self.v = (buf(4 * n * x * hd) for x in (heads, kv, kv))
+            self.norm, self.parent, self.depth, self.mask = buf(4 * hd), buf(4 * n), buf(4 * n), buf(4 * n * words)
+            self.rot, self.att, self.acc, self.count, self.out = buf(4 * n * heads * hd), buf(4 * n * heads * hd), buf(36), buf(12), buf(12)
+            self.rows = smq.paged_rows(self.q, self.rot, self.k, self.v, self.norm, self.norm, 1e-6, self.depth)
+            self.pools = smq.paged_pools([c.desc])
+            held = np.array([-(-m // page) for m in lengths], np.int32)
+            refs = np.bincount(c.table[c.table >= 0], minlength=c.pages).astype(np.int32)
+            self.old = [dev(x) for x in (held, refs)]
+            self.plan = [buf(12) for _ in range(3)]
+            self.no = [buf(4 * x) for x in (3 * c.stride, 3, c.pages, 9, 1)]
+            self.fork = smq.page_fork(c.tb, *self.old, 3, 3, c.stride, page, c.pages, *self.plan, *self.no)
+            self.logits, self.score = buf(4 * groups * beams * vocab), buf(4 * groups * beams)
+            self.res = [buf(4 * groups * select) for _ in range(3)]
+            self.step = smq.beam_step(self.logits, vocab, groups, beams, vocab, select, self.score, *self.res)
+            self.ws = [buf(max(16, x)) for x in (smq.paged_tree_attention_workspace(self.batch.desc, shape),
+                                                 smq.paged_fork_workspace(self.fork), smq.beam_select_workspace(self.step))]
+
+        def run(self):
+            c = self.cache.desc
+            smq.draft_masks(self.parent, self.batch.desc, self.depth, self.mask, words)
+            smq.paged_norm_rope_kv(self.rows, self.batch.desc, shape, cos, sin, c)
+            smq.paged_tree_attention(self.rot, self.att, self.batch.desc, shape, 0, self.depth, self.mask, words, c, self.ws[0])
+            smq.paged_compact(self.batch.desc, shape, self.acc, 3, self.count, self.pools, self.out)
+            smq.paged_fork(self.fork, self.ws[1])
+            smq.paged_copy(self.no[3], 3, shape, self.pools)
+            smq.beam_select(self.step, self.ws[2])
+
+        def fill(self, t):
+            rng = np.random.default_rng(500 + t)
+            f32 = lambda m: rng.standard_normal(m).astype(np.float32)  # noqa: E731
+            for b in (self.q, self.k, self.v, self.norm, self.score):
+                b.upload(f32(b.nbytes // 4))
+            self.logits.upload(3 * f32(groups * beams * vocab))
+            self.parent.upload(np.concatenate([ref.random_tree(rng, m) for m in new]).astype(np.int32))
+            self.acc.upload(np.array([sorted(rng.choice(m, 3, replace=False)) if m > 3 else [0, 0, 0] for m in new], np.int32))
+            self.count.upload(np.array([3, 2, 1], np.int32))
+            keep = [int(rng.integers(0, m)) for m in lengths]
+            for b, x in zip(self.plan, ([0, 0, 2], [keep[0], keep[0], keep[2]], [keep[0] + 9, keep[0] + 40, keep[2]])):
+                b.upload(np.array(x, np.int32))
+
+        def results(self):
+            bufs = [self.depth, self.mask, self.rot, self.att, self.out, *self.no, *self.res]
+            return [b.download(np.uint32) for b in bufs] + [x.view(np.uint8) for x in map(np.ascontiguousarray, self.cache.download())]
+
+    sides = [Side() for _ in range(3)]
+    graphs = [smq.capture(s.run) for s in sides[:2]]
+    side = torch.cuda.Stream()
+    for t in range(4):
+        for s in sides:
+            s.fill(t)
+        smq.synchronize()
+        smq.load().smq_set_stream(side.cuda_stream)
+        try:
+            graphs[1].launch()
+        finally:
+            smq.load().smq_set_stream(None)
+        graphs[0].launch()
+        sides[2].run()
+        smq.synchronize()
+        side.synchronize()
+        assert not flagged()
+        want = sides[2].results()
+        for s in sides[:2]:
+            for a, b in zip(s.results(), want):
+                assert np.array_equal(a, b)
+    for g in graphs:
+        g.destroy()
+
+
+def test_offsets_past_32_bits_of_all():
+    """A Q8 pool of more than 2^32 codes, pages at its end: stored, attended, copied and moved there."""
+    heads, kv, hd, page = 4, 4, 128, 256
+    pages = (1 << 32) // (kv * hd * page) + 12
+    shape = smq.attn_shape(heads, kv, hd, 0, 0, 600)
+    small = Cache(Q8, kv, hd, page, [600], spare=5, seed=2)  # the same pages at the end of a large pool
+    k, v = (smq.DeviceBuffer(pages * kv * hd * page) for _ in range(2))
+    ks, vs = (smq.DeviceBuffer(pages * kv * 4 * page * 4) for _ in range(2))
+    low = pages - small.pages
+    for b, x, one in ((k, small.k, kv * hd * page), (v, small.values_layout(small.v), kv * hd * page),
+                      (ks, small.ks, kv * 16 * page), (vs, small.vs, kv * 16 * page)):
+        b.upload(x, low * one)
+    small.upload()
+    big = smq.paged_kv(k, v, ks, vs, Q8, page, pages)
+    small.tb.upload(np.where(small.table >= 0, small.table + low, -1).astype(np.int32))
+    pools = smq.paged_pools([big])
+    batch = Batch(small, [40])
+    trees = Trees(batch).upload()
+    rows = [synth.normal(97 + i, 40 * kv * hd).reshape(40, kv, hd) for i in range(2)]
+    q = synth.normal(99, 40 * heads * hd).reshape(40, heads, hd)
+    w = (1 + 0.2 * synth.normal(31, hd)).astype(np.float32)
+    z = dev(np.zeros(1, np.float32))
+    rot, att, out = smq.DeviceBuffer(q.nbytes), smq.DeviceBuffer(q.nbytes), smq.DeviceBuffer(4)
+    smq.paged_norm_rope_kv(smq.paged_rows(dev(q), rot, dev(rows[0]), dev(rows[1]), dev(w), dev(w)), batch.desc, shape, z, z, big)
+    small.put(0, np.arange(560, 600), ref.normed(rows[0], w, 1e-6), rows[1])
+    want, tol = ref.tree64(small, batch, ref.normed(q, w, 1e-6), heads, trees.depth, trees.seen)
+    smq.paged_tree_attention(rot, att, batch.desc, shape, 0, trees.db, trees.wb, trees.stride, big)
+    close(att.download(np.float32).reshape(q.shape), want, tol)
+    path = [1, 2, 9, 30, 39]
+    smq.paged_compact(batch.desc, shape, dev(np.array(path, np.int32)), 5, dev(np.array([5], np.int32)), pools, out)
+    ref.compact(small, 0, 560, path)
+    free = [p for p in range(small.pages) if p not in small.table]
+    copies = np.array([[small.table[0, 1], free[0], 200], [small.table[0, 2], free[1], 53]], np.int32)
+    smq.paged_copy(dev((copies + [low, low, 0]).astype(np.int32)), 2, shape, pools)
+    ref.copy(small, copies)
+    for b, x, one, t in ((k, small.k, kv * hd * page, np.int8), (v, small.values_layout(small.v), kv * hd * page, np.int8),
+                         (ks, small.ks, kv * 4 * page, np.float32), (vs, small.vs, kv * 4 * page, np.float32)):
+        same(b.download(t, x.size, low * one * x.itemsize).reshape(x.shape), x)
+    assert not flagged()
+
+
+def test_unaligned_rows_of_drafts():
+    """q, k, v, norms and outputs at 4-byte addresses."""
+    heads, kv, hd, n = 6, 2, 64, 21
+    cache = Cache(F16, kv, hd, 32, [70], stale="nan").upload()
+    batch = Batch(cache, [n])
+    trees = Trees(batch).upload()
+    shape = smq.attn_shape(heads, kv, hd, 32, 0, 70)
+    cos, sin = tables(70, 32)
+    q, k, v = (synth.normal(101 + i, n * w).reshape(n, -1, hd) for i, w in enumerate((heads * hd, kv * hd, kv * hd)))
+    w = (1 + 0.2 * synth.normal(31, hd)).astype(np.float32)
+
+    def off(x):
+        b = smq.DeviceBuffer(x.nbytes + 4)
+        b.upload(x, 4)
+        return b
+
+    qb, kb, vb, wb, cb, sb = (off(x) for x in (q, k, v, w, cos, sin))
+    att = smq.DeviceBuffer(q.nbytes + 4)
+    r = smq.paged_rows(qb.at(4), qb.at(4), kb.at(4), vb.at(4), wb.at(4), wb.at(4), 1e-6, trees.db)
+    smq.paged_norm_rope_kv(r, batch.desc, shape, cb.at(4), sb.at(4), cache.desc)
+    smq.paged_tree_attention(qb.at(4), att.at(4), batch.desc, shape, 0, trees.db, trees.wb, trees.stride, cache.desc)
+    turn = 49 + trees.depth
+    cache.put(0, np.arange(49, 70), rotate(ref.normed(k, w, 1e-6), cos[turn], sin[turn], 32), v)
+    qr = rotate(ref.normed(q, w, 1e-6), cos[turn], sin[turn], 32)
+    same(qb.download(np.float32, offset=4).reshape(q.shape), qr)
+    want, tol = ref.tree64(cache, batch, qr, heads, trees.depth, trees.seen)
+    close(att.download(np.float32, offset=4).reshape(q.shape), want, tol)
