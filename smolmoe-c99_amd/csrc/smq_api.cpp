@@ -223,8 +223,14 @@ float *take_scores(hipStream_t s) {
     return free_slot->p;
 }
 
+/* The allocation that a call has looked up last: its next range often lies there too (layers of one buffer). */
+struct Allocation {
+    uintptr_t base = 0;
+    size_t size = 0;
+    bool holds(uintptr_t q, size_t bytes) const { return q >= base && q - base <= size && bytes <= size - (q - base); }
+};
 /* The byte range [p, p + bytes) must lie inside one device allocation. */
-bool extent_ok(const void *p, size_t bytes, const char *what) {
+bool extent_ok(const void *p, size_t bytes, const char *what, Allocation *known_to = nullptr) {
     if (!bytes) return true;
     if (!p) {
         set_status(SMQ_ERR_RANGE, "%s is NULL", what);
@@ -232,6 +238,7 @@ bool extent_ok(const void *p, size_t bytes, const char *what) {
     }
     if (!g.checks) return true;
     const uintptr_t q = (uintptr_t)p;
+    if (known_to && known_to->size && known_to->holds(q, bytes)) return true;
     uintptr_t rb = 0;
     size_t rsize = 0;
     const int known = registry_extent(q, bytes, rb, rsize);
@@ -256,6 +263,10 @@ bool extent_ok(const void *p, size_t bytes, const char *what) {
         set_status(SMQ_ERR_RANGE, "%s: %zu bytes at offset %zu exceed its allocation of %zu bytes", what, bytes,
                    (size_t)(q - b), size);
         return false;
+    }
+    if (known_to) {
+        known_to->base = b;
+        known_to->size = size;
     }
     return true;
 }
@@ -1498,7 +1509,7 @@ static bool paged_args(const smq_paged_batch *b, const smq_attn_shape *shape, co
 }
 
 /* A pool's arrays. */
-static bool pool_extents(const smq::PagedArgs &a, const char *who) {
+static bool pool_extents(const smq::PagedArgs &a, const char *who, Allocation *in = nullptr) {
     static const size_t bytes[3] = {4, 2, 1};
     const size_t positions = (size_t)a.pages << a.shift, kd = (size_t)a.kv_heads * a.head_dim;
     const size_t scales = a.type == SMQ_KV_Q8 ? positions * a.kv_heads * a.nb * 4 : 0;
@@ -1514,9 +1525,11 @@ static bool pool_extents(const smq::PagedArgs &a, const char *who) {
         set_status(SMQ_ERR_RANGE, "%s: the pools must be 16-byte aligned", who);
         return false;
     }
-    return extent_ok(a.keys, positions * kd * bytes[a.type], "keys") &&
-           extent_ok(a.values, positions * kd * bytes[a.type], "values") && extent_ok(a.ks, scales, "key scales") &&
-           extent_ok(a.vs, scales, "value scales");
+    /* one allocation each for a kind's layers: in[0 .. 3] */
+    return extent_ok(a.keys, positions * kd * bytes[a.type], "keys", in) &&
+           extent_ok(a.values, positions * kd * bytes[a.type], "values", in ? in + 1 : nullptr) &&
+           extent_ok(a.ks, scales, "key scales", in ? in + 2 : nullptr) &&
+           extent_ok(a.vs, scales, "value scales", in ? in + 3 : nullptr);
 }
 /* The descriptors' arrays, of a batch that is not empty. */
 static bool paged_extents(const smq::PagedArgs &a, const char *who) {
@@ -1695,6 +1708,7 @@ static bool pool_args(const smq_paged_kv *pools, uint32_t n, const char *who, co
         set_status(SMQ_ERR_RANGE, "%s: %u pools of at most %u", who, n, SMQ_MAX_POOLS);
         return false;
     }
+    Allocation in[4];
     for (uint32_t i = 0; i < n; ++i) {
         const smq_paged_kv &p = pools[i];
         if (p.type != pools->type || p.page_size != pools->page_size || p.pages != pools->pages) {
@@ -1706,7 +1720,7 @@ static bool pool_args(const smq_paged_kv *pools, uint32_t n, const char *who, co
         one.values = p.values;
         one.ks = p.key_scales;
         one.vs = p.value_scales;
-        if (!pool_extents(one, who)) return false;
+        if (!pool_extents(one, who, in)) return false;
         out[i] = {p.keys, p.values, p.key_scales, p.value_scales};
     }
     return true;
