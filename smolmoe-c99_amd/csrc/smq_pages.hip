@@ -83,7 +83,11 @@ __global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
     __shared__ int parents[SMALL_ROWS], last[SMALL_ROWS];
     __shared__ uint32_t olds[SMALL_ROWS], full[SMALL_ROWS], held[SMALL_ROWS], from[SMALL_ROWS], rank[SMALL_ROWS + 1];
     __shared__ uint32_t lds[SMALL_WAVES];
-    const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32;
+    const uint32_t tid = threadIdx.x, words = (a.pages + 31) / 32, entries = a.old_seqs * a.table_stride;
+    constexpr uint32_t EARLY = 4; /* old entries of a thread that are requested with the row arrays */
+    uint32_t early[EARLY];
+#pragma unroll
+    for (uint32_t k = 0; k < EARLY; ++k) early[k] = tid + k * SMALL_WG < entries ? (uint32_t)a.table[tid + k * SMALL_WG] : 0;
     NewRow row = {};
     if (tid < a.old_seqs) olds[tid] = old_held(a, tid, true);
     if (tid < a.seqs) {
@@ -102,14 +106,16 @@ __global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
     __syncthreads();
     const float inv = 1.0f / (float)a.table_stride;
     auto row_of = [&](uint32_t i) { return (uint32_t)(((float)i + 0.5f) * inv); }; /* i / stride: below 2^15, where this is exact */
-#pragma unroll 4
-    for (uint32_t i = tid; i < a.old_seqs * a.table_stride; i += SMALL_WG) {
+    auto give_up = [&](uint32_t i, uint32_t id) {
         const uint32_t s = row_of(i), x = i - s * a.table_stride;
-        const uint32_t id = (uint32_t)a.table[i];
-        if (x >= olds[s]) continue;
+        if (x >= olds[s]) return;
         if (id < a.pages) atomicSub(&holders[id], 1);
         else *a.flag = 1;
-    }
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < EARLY; ++k)
+        if (tid + k * SMALL_WG < entries) give_up(tid + k * SMALL_WG, early[k]);
+    for (uint32_t i = tid + EARLY * SMALL_WG; i < entries; i += SMALL_WG) give_up(i, (uint32_t)a.table[i]);
     __syncthreads();
     for (uint32_t i = tid; i < a.pages; i += SMALL_WG)
         if (holders[i] < 0) {
@@ -132,13 +138,14 @@ __global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
         }
     }
     __syncthreads();
-    /* rows: the first one that takes a page in part keeps it, if nothing else holds it */
+    /* rows: the first one that takes a page in part keeps it, if nothing else holds it (the most of SMALL_ROWS - row there) */
     uint32_t need = 0;
-    bool mine = false;
+    bool mine = tid < a.seqs && last[tid] >= 0 && holders[last[tid]] == 0;
+    __syncthreads();
+    if (mine) atomicMax(&holders[last[tid]], (int)(SMALL_ROWS - tid));
+    __syncthreads();
+    mine = mine && holders[last[tid]] == (int)(SMALL_ROWS - tid);
     if (tid < a.seqs) {
-        mine = last[tid] >= 0 && holders[last[tid]] == 0;
-        if (mine)
-            for (uint32_t i = 0; i < tid; ++i) mine = mine & (last[i] != last[tid]);
         from[tid] = row.full + mine;
         need = row.held - from[tid]; /* a page in part is one of them */
     }
