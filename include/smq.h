@@ -464,59 +464,61 @@ typedef struct smq_paged_rows {
     size_t q_stride, q_out_stride, k_stride, v_stride;
     const float *q_norm, *k_norm; /* head_dim floats each, device; NULL: no norm */
     float eps;                 /* finite, not negative */
-    const int32_t *depth;      /* device, one per token: its rotary position is depth positions behind the sequence's
-                                * last one that is not new (a draft's children of one token share a position); NULL: the
-                                * rotary position is the position in the cache */
+    const int32_t *depth;      /* device, one per token: its rotary position is the number of positions before its
+                                * sequence's new tokens + depth (drafts that continue the same token share a position);
+                                * NULL: the position in the cache */
 } smq_paged_rows;
-/* smq_paged_rope_kv with an RMSNorm of each head of q and k before the rotation
- * and with rotary positions of the tokens' own:
+/* smq_paged_rope_kv with an RMSNorm of each head of q and k before the
+ * rotation and with rotary positions of the tokens' own:
  *   y = (x * (1 / sqrt(mean(x^2) + eps))) * norm
- * mean, root and quotient in 64 bits, the quotient and both products rounded to
- * f32 each (no order of the mean's sum shows in the result), then the rotation
- * and the cache's rounding as smq_paged_rope_kv has them. Keys and values go to
- * the tokens' own places whatever their depth. A row whose rotary position is
- * outside [0, context) raises the numeric flag: its k is not stored and its q
- * not written. q_out must not overlap k, v or, but for in place, q.
- * Asynchronous, capturable. */
+ * mean, root and quotient in 64 bits, the quotient and both products rounded
+ * to f32 each (no order of the mean's sum shows in the result), then the
+ * rotation and the cache's rounding as smq_paged_rope_kv has them. Keys and
+ * values go to the tokens' own places whatever their depth. A row whose rotary
+ * position is outside [0, context) raises the numeric flag: its k is not
+ * stored and its q not written. q_out must not overlap k, v or, but for in
+ * place, q. Asynchronous, capturable. */
 smq_status smq_paged_norm_rope_kv(const smq_paged_rows *rows, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                   const float *cos_table, const float *sin_table, const smq_paged_kv *kv);
 /* Trees of drafted tokens: parent[r], for row r of the batch, is the index
- * among its sequence's new tokens of the token that r continues, below its
- * own index; negative where that is the last token of the context. depth[r]: 0
+ * among its sequence's new tokens of the token that r continues, below its own
+ * index; negative where that is the last token of the context. depth[r]: 0
  * there, else its parent's + 1. mask, mask_stride words a row: bit t % 32 of
- * word t / 32 is set where t is the token itself or an ancestor; the other bits
- * of the row's words are cleared. A parent that is none of these raises the numeric flag
- * and counts as negative; so does a sequence of more than 32 * mask_stride new
- * tokens, whose rows are left as they are, and rows of padding are too.
- * mask_stride: 1 .. 128. One call serves the attention of all layers.
- * Asynchronous, capturable. */
+ * word t / 32 is set where t is the token itself or an ancestor; the other
+ * bits of the row's words are cleared. A parent at or past its own index
+ * raises the numeric flag and counts as negative. A sequence of more than
+ * 32 * mask_stride new tokens raises the flag; its rows are left as they are,
+ * as those of padding. mask_stride: 1 .. 128. One call serves the attention of
+ * all layers. depth, mask and parent must not overlap. Asynchronous,
+ * capturable. */
 smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, int32_t *depth, uint32_t *mask,
                            uint32_t mask_stride);
 /* smq_paged_attention where a mask says which of its sequence's new tokens a
  * row sees: of the positions before them (the context) all, with shape->window
  * w > 0 those with j > p - w or j < sinks, p = the context's positions +
- * depth[r] (not read where there is no window); of the new tokens
- * those whose bit is set, whatever the window, later ones too. mask as smq_draft_masks writes it,
- * or any other: bits behind the last new token do not matter. A row that sees
- * nothing is 0. Numbers, errors, workspace and what does not matter as
- * smq_paged_attention's; a depth below 0 or where p is not below the context's size raises the
- * numeric flag, its row is 0, and so are those of a sequence of more
- * than 32 * mask_stride new tokens. All pages of the new tokens must be pages.
- * mask_stride: 1 .. 128. The workspace has a query of its own. Asynchronous,
- * capturable. */
+ * depth[r] (not read where there is no window); of the new tokens those whose
+ * bit is set, whatever the window, later ones too. mask as smq_draft_masks
+ * writes it, or any other: bits behind the last new token do not matter. A row
+ * that sees nothing is 0. Numbers, errors, workspace and what does not matter
+ * as smq_paged_attention's; a depth below 0 or where p is not below the
+ * context's size raises the numeric flag, its row is 0, and so are those of a
+ * sequence of more than 32 * mask_stride new tokens. All pages of the new
+ * tokens must be pages. mask_stride: 1 .. 128. The workspace has a query of
+ * its own. Asynchronous, capturable. */
 size_t smq_paged_tree_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape);
 smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                     uint32_t sinks, const int32_t *depth, const uint32_t *mask, uint32_t mask_stride,
                                     const smq_paged_kv *kv, void *workspace, size_t workspace_bytes);
-/* The accepted path of each sequence's draft to the front of its new tokens, in
- * every pool (the layers' caches: same type, page_size and pages): for k below
- * count[s] the keys and values of new token accepted[s * accepted_stride + k]
- * go to the place of new token k, as the cache holds them. length_out[s] (may
- * be `length` itself) = the positions before the new tokens + count[s]. A list that does not ascend strictly within the
- * sequence's new tokens, or is longer than accepted_stride, raises the numeric
- * flag: the sequence stays as it is, its length too. Positions without a place
- * or page raise the flag and are not moved. Sequences must not share a page that the call writes to. At most
- * SMQ_MAX_POOLS pools. Asynchronous, capturable. */
+/* The accepted path of each sequence's draft to the front of its new tokens,
+ * in every pool (the layers' caches: same type, page_size and pages): for k
+ * below count[s] the keys and values of new token accepted[s * accepted_stride
+ * + k] go to the place of new token k, as the cache holds them. length_out[s]
+ * = the positions before the new tokens + count[s]; it must not overlap
+ * length, accepted or count. A list that does not ascend strictly within the sequence's new tokens, or is
+ * longer than accepted_stride, raises the numeric flag: the sequence stays as
+ * it is, its length too. Positions without a place or page raise the flag and
+ * are not moved. Sequences must not share a page that the call writes to. At
+ * most SMQ_MAX_POOLS pools. Asynchronous, capturable. */
 #define SMQ_MAX_POOLS 1024u
 smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,
                              uint32_t accepted_stride, const int32_t *count, const smq_paged_kv *pools, uint32_t n_pools,
@@ -534,21 +536,23 @@ smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape 
  * So one call forks sequences (a parent named twice), ends them (a parent not
  * named), begins them (-1), gives back what drafts have taken (keep below the
  * length) and makes room for the next tokens (room above it). Old arrays are
- * left as they are and must not overlap the new ones.
+ * left as they are; no new one may overlap another array.
  *
- * refs counts, for each page, the entries of the old table (of the first held[s] ones of each row) that name it and other
- * holders (a store of prompts), which stay counted; 0: free. refs_out: the same
- * for the new table. held_out[d] = ceil(room[d] / page_size); entries behind it
- * are -1. copies: three words a row, the page copied from and to and its
- * positions; -1, -1, 0 where nothing is to be copied. free_out: the pages free
- * afterwards; negative where so many were missing: then the numeric flag is
- * raised, entries without a page are -1, and the old arrays still hold.
+ * refs counts, for each page, the entries of the old table (of the first
+ * held[s] ones of each row) that name it and other holders (a store of
+ * prompts), which stay counted; 0: free. refs_out: the same for the new table.
+ * held_out[d] = ceil(room[d] / page_size); entries behind it are -1. copies:
+ * three words a row, the page copied from and to and its positions; -1, -1, 0
+ * where nothing is to be copied. free_out: the pages free afterwards; negative
+ * where so many were missing: then the numeric flag is raised, entries without
+ * a page are -1, and the old arrays still hold.
  *
  * Raise the flag as well: held, keep or room outside the table's row (cut), a
- * keep above the parent's pages (cut) or above room (room is raised), a parent outside the old rows
- * (-1), an entry that is no page (it stays none), refs below the old table's
- * entries (such a page may be given twice). workspace: device, 16-byte aligned.
- * At most 65535 rows and 2^24 pages. Asynchronous, capturable. */
+ * keep above the parent's pages (cut) or above room (room is raised), a parent
+ * outside the old rows (-1), an entry that is no page (it stays none), refs
+ * seen to be below the old table's entries (such a page may be given twice).
+ * workspace: device, 16-byte aligned; calls that may overlap in time must not
+ * share one. At most 65535 rows and 2^24 pages. Asynchronous, capturable. */
 typedef struct smq_page_fork {
     const int32_t *table; /* old_seqs * table_stride page ids */
     const int32_t *held;  /* old_seqs: entries that hold pages */
@@ -564,33 +568,40 @@ typedef struct smq_page_fork {
 } smq_page_fork;
 size_t smq_paged_fork_workspace(const smq_page_fork *fork);
 smq_status smq_paged_fork(const smq_page_fork *fork, void *workspace, size_t workspace_bytes);
-/* The copies of smq_paged_fork in every pool: of row i the first copies[3 i + 2]
- * positions of page copies[3 i] into page copies[3 i + 1], nothing else of that
- * page. No page may be written twice or be read and written. Ids that are no page, or more positions than page_size, raise the numeric
- * flag, and the row is skipped; so is one of no positions, without the flag.
- * shape: kv_heads and head_dim. Pools as
- * smq_paged_compact's. Asynchronous, capturable. */
+/* The copies of smq_paged_fork in every pool: of row i the first copies[3 i +
+ * 2] positions of page copies[3 i] into page copies[3 i + 1], nothing else of
+ * that page. No page may be written twice or be read and written. Ids that are
+ * no page, or more positions than page_size, raise the numeric flag, and the
+ * row is skipped; so is one of no positions, without the flag. shape: kv_heads
+ * and head_dim. Pools as smq_paged_compact's. Asynchronous, capturable. */
 smq_status smq_paged_copy(const int32_t *copies, uint32_t rows, const smq_attn_shape *shape, const smq_paged_kv *pools,
                           uint32_t n_pools);
 /* A step of a beam search: `groups` of `beams` rows of logits each (row r at
- * logits + r * stride), and of each group the `select` best continuations, best
- * first. A continuation of row r by id v is worth
+ * logits + r * stride), and of each group the `select` best continuations,
+ * best first. A continuation of row r by id v is worth
  *   score[r] + (l[v] - log sum_u exp(l[u]))
- * in 64 bits, sum and logarithm included; the results are rounded to f32. Equal ones: the
- * lower row first; of one row, the larger logit, then the lower id. A row that is done has one continuation, by `pad`, worth
- * score[r]. Continuations worth -inf (masked ids) are none. Where a group has
- * fewer than `select`, the rest gets parent -1, token UINT32_MAX, score -inf
- * and counts as done. A row that is not done with a NaN or +inf among its logits, or any with a score that is
- * NaN or +inf, raises the numeric flag and has no continuation.
+ * in 64 bits, sum and logarithm included (each exponential within 1e-12 of its
+ * size); the results are rounded to f32. Equal ones: the lower row first; of
+ * one row, the larger logit, then the lower id. A row that is done has one continuation, by `pad`,
+ * worth score[r]. Continuations worth -inf (masked ids) are none. Where a
+ * group has fewer than `select`, the rest gets parent -1, token UINT32_MAX,
+ * score -inf and counts as done. A row that is not done with a NaN or +inf
+ * among its logits, or any with a score that is NaN or +inf, raises the
+ * numeric flag and has no continuation.
  *
- * parent[i] is the row in 0 .. groups * beams - 1, as smq_paged_fork takes it. done_out[i]: the
- * parent was done or the token is eos. History rows (history_stride ids each,
- * as many as `length` says): row i of history_out has the parent's ids and,
- * unless the parent was done, the token behind them (a row that is full raises the numeric flag and stays as
- * it is); the rest of the row is UINT32_MAX, which smq_logits_adjust skips, so
- * that history_begin may be multiples of history_stride. Lengths outside [0, history_stride] raise the flag and are cut.
- * New arrays must not overlap old ones. select: 1 .. 64, beams 1 .. 64, at most 65535 rows of logits or results. workspace: device, 16-byte
- * aligned; calls that may overlap in time must not share one. Asynchronous, capturable. */
+ * parent[i] is the row in 0 .. groups * beams - 1, as smq_paged_fork takes it.
+ * done_out[i]: the parent was done or the token is eos. History rows
+ * (history_stride ids each, as many as `length` says): row i of history_out
+ * has the parent's ids and, unless the parent was done, the token behind them
+ * (a row that is full raises the numeric flag and stays as it is); the rest of
+ * the row is UINT32_MAX, which smq_logits_adjust skips, so that history_begin
+ * may be multiples of history_stride. Lengths outside [0, history_stride]
+ * raise the flag and are cut. No new array may overlap another one.
+ *
+ * select and beams: 1 .. 64, vocab: at most 1,048,576, at most 65535 rows of
+ * logits or of results. workspace: device, 16-byte aligned, the query's bytes,
+ * which suffice for fewer rows, ids or results too; calls that may overlap in
+ * time must not share one. Asynchronous, capturable. */
 typedef struct smq_beam_step {
     const float *logits;
     size_t stride;

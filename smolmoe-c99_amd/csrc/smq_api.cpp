@@ -1600,6 +1600,36 @@ static bool overlap(const void *p, size_t n, const void *q, size_t m) {
     return n && m && (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n;
 }
 
+/* Ranges that a call reads and ranges that it writes: all there, and none that is written shares a byte with another. */
+struct Range {
+    const void *p;
+    size_t bytes;
+    const char *what;
+};
+static bool ranges_ok(const char *who, const Range *in, int n_in, const Range *to, int n_to) {
+    for (int i = 0; i < n_in; ++i)
+        if (!extent_ok(in[i].p, in[i].bytes, in[i].what)) return false;
+    for (int i = 0; i < n_to; ++i) {
+        if (!extent_ok(to[i].p, to[i].bytes, to[i].what)) return false;
+        for (int j = 0; j < n_in + i; ++j) {
+            const Range &x = j < n_in ? in[j] : to[j - n_in];
+            if (overlap(x.p, x.bytes, to[i].p, to[i].bytes)) {
+                set_status(SMQ_ERR_RANGE, "%s: %s overlaps %s", who, to[i].what, x.what);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+/* A workspace of `need` bytes, 16-byte aligned. */
+static bool workspace_ok(const char *who, const void *p, size_t bytes, size_t need) {
+    if (bytes < need || ((uintptr_t)p & 15)) {
+        set_status(SMQ_ERR_RANGE, "%s: the workspace has %zu bytes of %zu, 16-byte aligned", who, bytes, need);
+        return false;
+    }
+    return extent_ok(p, need, "workspace");
+}
+
 /* Bytes of `rows` rows of `width` floats, `stride` apart (0: width); 0 with an error where they are none. */
 static size_t row_bytes_of(uint32_t rows, size_t width, size_t *stride, const char *who, const char *what) {
     if (!*stride) *stride = width;
@@ -1801,25 +1831,12 @@ smq_status smq_paged_fork(const smq_page_fork *fork, void *workspace, size_t wor
     smq::ForkArgs a;
     if (!fork_args(fork, who, &a)) return t_status;
     const size_t old = (size_t)a.old_seqs * 4, now = (size_t)a.seqs * 4, pages = (size_t)a.pages * 4;
-    const struct {
-        const void *p;
-        size_t bytes;
-        const char *what;
-    } in[6] = {{a.table, old * a.table_stride, "table"}, {a.held, old, "held"}, {a.refs, pages, "refs"},
-               {a.parent, now, "parent"}, {a.keep, now, "keep"}, {a.room, now, "room"}},
-      to[5] = {{a.table_out, now * a.table_stride, "table_out"}, {a.held_out, now, "held_out"},
-               {a.refs_out, pages, "refs_out"}, {a.copies, now * 3, "copies"}, {a.free_out, 4, "free_out"}};
-    for (const auto &x : in)
-        if (!extent_ok(x.p, x.bytes, x.what)) return t_status;
-    const size_t need = smq::fork_workspace(a.pages, a.seqs);
-    if (workspace_bytes < need || ((uintptr_t)workspace & 15))
-        return set_status(SMQ_ERR_RANGE, "%s: the workspace has %zu bytes of %zu, 16-byte aligned", who, workspace_bytes, need);
-    if (!extent_ok(workspace, need, "workspace")) return t_status;
-    for (const auto &y : to) {
-        if (!extent_ok(y.p, y.bytes, y.what)) return t_status;
-        for (const auto &x : in)
-            if (overlap(x.p, x.bytes, y.p, y.bytes)) return set_status(SMQ_ERR_RANGE, "%s: %s overlaps %s", who, y.what, x.what);
-    }
+    const Range in[6] = {{a.table, old * a.table_stride, "table"}, {a.held, old, "held"}, {a.refs, pages, "refs"},
+                         {a.parent, now, "parent"}, {a.keep, now, "keep"}, {a.room, now, "room"}},
+                to[5] = {{a.table_out, now * a.table_stride, "table_out"}, {a.held_out, now, "held_out"},
+                         {a.refs_out, pages, "refs_out"}, {a.copies, now * 3, "copies"}, {a.free_out, 4, "free_out"}};
+    if (!ranges_ok(who, in, 6, to, 5) || !workspace_ok(who, workspace, workspace_bytes, smq::fork_workspace(a.pages, a.seqs)))
+        return t_status;
     return hip_ok(smq::launch_fork(a, workspace, g.cur), who) ? SMQ_OK : t_status;
 }
 
@@ -1860,26 +1877,12 @@ smq_status smq_beam_select(const smq_beam_step *step, void *workspace, size_t wo
     if (a.history && (!a.history_stride || a.history_stride > 0x7fffffffu))
         return set_status(SMQ_ERR_RANGE, "%s: a history_stride of %u", who, a.history_stride);
     const size_t hs = a.history ? a.history_stride : 0, h = a.history ? 4 : 0;
-    const struct {
-        const void *p;
-        size_t bytes;
-        const char *what;
-    } in[5] = {{a.logits, ((rows - 1) * a.stride + a.vocab) * 4, "logits"}, {a.score, rows * 4, "score"},
-               {a.done, a.done ? rows : 0, "done"}, {a.history, rows * hs * 4, "history"}, {a.length, rows * h, "length"}},
-      to[6] = {{a.parent, now * 4, "parent"}, {a.token, now * 4, "token"}, {a.score_out, now * 4, "score_out"},
-               {a.done_out, a.done_out ? now : 0, "done_out"}, {a.history_out, now * hs * 4, "history_out"},
-               {a.length_out, now * h, "length_out"}};
-    for (const auto &x : in)
-        if (!extent_ok(x.p, x.bytes, x.what)) return t_status;
-    for (const auto &y : to) {
-        if (!extent_ok(y.p, y.bytes, y.what)) return t_status;
-        for (const auto &x : in)
-            if (overlap(x.p, x.bytes, y.p, y.bytes)) return set_status(SMQ_ERR_RANGE, "%s: %s overlaps %s", who, y.what, x.what);
-    }
-    const size_t need = smq::beam_workspace(a);
-    if (workspace_bytes < need || ((uintptr_t)workspace & 15))
-        return set_status(SMQ_ERR_RANGE, "%s: the workspace has %zu bytes of %zu, 16-byte aligned", who, workspace_bytes, need);
-    if (!extent_ok(workspace, need, "workspace")) return t_status;
+    const Range in[5] = {{a.logits, ((rows - 1) * a.stride + a.vocab) * 4, "logits"}, {a.score, rows * 4, "score"},
+                         {a.done, a.done ? rows : 0, "done"}, {a.history, rows * hs * 4, "history"}, {a.length, rows * h, "length"}},
+                to[6] = {{a.parent, now * 4, "parent"}, {a.token, now * 4, "token"}, {a.score_out, now * 4, "score_out"},
+                         {a.done_out, a.done_out ? now : 0, "done_out"}, {a.history_out, now * hs * 4, "history_out"},
+                         {a.length_out, now * h, "length_out"}};
+    if (!ranges_ok(who, in, 5, to, 6) || !workspace_ok(who, workspace, workspace_bytes, smq::beam_workspace(a))) return t_status;
     return hip_ok(smq::launch_beam(a, workspace, g.cur), who) ? SMQ_OK : t_status;
 }
 

@@ -258,6 +258,11 @@ def forks():
         for old in ("table", "held", "refs", "parent", "keep", "room"):
             buf = smq.DeviceBuffer(4096)
             refused(lambda: fork(**{out: buf, old: buf}), words=out + " overlaps " + old)
+    outs = ("table_out", "held_out", "refs_out", "copies", "free_out")
+    for i, out in enumerate(outs):
+        for other in outs[:i]:
+            buf = smq.DeviceBuffer(4096)
+            refused(lambda: fork(**{out: buf, other: buf}), words=out + " overlaps " + other)
     for kw in (dict(page=8), dict(page=48), dict(page=512), dict(page=0), dict(stride=0), dict(pages=0), dict(set_old_seqs=65536),
                dict(set_seqs=65536), dict(set_table_stride=(1 << 20) + 1), dict(set_pages=(1 << 24) + 1)):
         refused(lambda: fork(**kw), words="unsupported tables")
@@ -302,6 +307,8 @@ def beams():
         for old in ("logits", "score", "done", "history", "length"):
             buf = smq.DeviceBuffer(1 << 17)
             refused(lambda: beam(**{out: buf, old: buf.at(4)}), words=out + " overlaps " + old)
+    buf = smq.DeviceBuffer(1 << 17)
+    refused(lambda: beam(token=buf, score_out=buf), words="score_out overlaps token")
     for kw in (dict(set_beams=0), dict(set_beams=65), dict(set_select=0), dict(set_select=65), dict(set_vocab=0),
                dict(set_vocab=(1 << 20) + 1), dict(set_groups=16384), dict(set_groups=TOP)):
         refused(lambda: beam(**kw), words="unsupported step")
