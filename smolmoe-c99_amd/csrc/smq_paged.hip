@@ -1,5 +1,7 @@
 /* Paged KV cache on gfx950: RoPE and the store of new tokens (f32, f16, Q8), rows read back, and the attention of a
  * ragged batch of new tokens over the pages (include/smq.h has the layout of a page). */
+#include <cmath>
+
 #include "smq_paged_attend.h"
 
 namespace smq {
@@ -512,7 +514,8 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
  *
  * Cutting costs partial results and a second launch, which joins them. No cuts
  * - where the longest tile exceeds an equal share by about 24 steps or less (64 sequences at 700, 2 KV heads of 64: 11.8 us
- *   whole, 15.4 cut; 8 with a window of 1024, 4 KV heads of 64: 22 whole, 13 cut);
+ *   whole, 15.4 cut; 8 with a window of 1024, 4 KV heads of 64: 22 whole, 13 cut), 10 where waves own a tree's rows (24
+ *   drafts of 40 Q8 tokens at 700, 2 KV heads of 128: 46 whole, 40 cut; at 300 27 and 32);
  * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
  *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
  *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). */
@@ -544,7 +547,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     if (p.owns && tiles > 256) {
         const uint64_t average = steps - (a.window || tree ? 0 : min(rows / G / seqs / 64, steps / 2));
         if (tiles >= 512 || average * (512 - tiles) / 256 <= 24) p.stream = 0;
-    } else if (tiles >= groups || steps * (groups - tiles) / groups <= 24) {
+    } else if (tiles >= groups || steps * (groups - tiles) / groups <= (tree && p.owns ? 10u : 24u)) {
         p.stream = 0;
     }
     const size_t used = attend_used_bytes(a, p), each = attend_piece_bytes(a, p.tile_rows);
@@ -559,18 +562,31 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     return p;
 }
 
-/* A tile's rows for trees, whose tiles all go over the whole context. 16, whose waves share the positions out, while their steps
- * are few in all: 13 drafts at 613 and 3000 (f16, 14 heads on 2 of 64) 12.1 and 15.2 us, 64 rows 15.3 and 17.4; 8 Q8
- * sequences of 16 at 1500 17.9, 20.6; 8064 steps (two f32 ones of 30 at 2000, 32 on 8 of 64) 28.8, 29.7; but 32000 (4 f16 ones of
- * 16 at 8000, 32 on 8 of 128) 73, 35. Else 64 where a sequence has no more (that one 35.3 us, 128 rows 44.3), 128 above (8 f16
- * sequences of 63 at 16384 252, 64 rows 401). */
+/* A tile's rows for trees, whose tiles all go over the whole context: 16, whose waves share the positions out, 64 or 128, by an
+ * estimate of the time (us; the table, q8 and f16 heads of 128 on 2 and 8, 24 drafts of 40, 8 of 16 and 64 of 8). A step of a
+ * tile of 16, 64, 128 rows takes 1 / r of the card once tiles fill it; before, tiles of 16 wait for a quarter of their steps
+ * one after another (or a piece's, and the join), the others for a piece's steps, the batch and the join.
+ *
+ *                        16 rows   64   128                            16 rows   64   128
+ *   q8  24 x 40 at 300        30   27    37      f16  8 x 16 at  700        19   24    29
+ *               at 700        51   40    42                  at 2000        37   28    34
+ *               at 3001      126   89    79      f16 64 x  8 at 2000       139   98   103
+ *   f16 24 x 40 at 700        47   31    35      f16  8 x 63 at 16384      815  401   252
+ *               at 1500       76   38    41      q8   8 x 16 at 1500        18   21    23 (14 heads on 2 of 64) */
 uint32_t tree_rows(const PagedArgs &a) {
-    const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
-    uint64_t reach = a.limit;
-    if (a.window && (uint64_t)a.window + a.sinks + a.tokens < reach) reach = (uint64_t)a.window + a.sinks + a.tokens;
-    const uint64_t tiles = (rows + seqs * 15) / 16 * a.kv_heads;
-    if (rows <= 32 * seqs || tiles * (reach / PA_STEP + 1) <= 8192) return 16;
-    return rows <= 64 * seqs ? 64 : 64 * attend_rt(attend_ks(a.head_dim));
+    const double ks = attend_ks(a.head_dim), rows = (double)a.tokens * (a.heads / a.kv_heads);
+    const double seqs = a.seqs < a.tokens ? a.seqs : a.tokens, each = rows / seqs;
+    double reach = a.limit;
+    if (a.window) reach = min(reach, (double)a.window + a.sinks + a.tokens);
+    const double steps = reach / PA_STEP + 1;
+    static const double rate[3][3] = {{1200, 400, 230}, {1900, 1300, 1080}, {1900, 1020, 660}}; /* by type, of one 32-wide step */
+    const double *r = rate[a.type];
+    auto tiles = [&](double n) { return ceil(each / n) * seqs * a.kv_heads * steps * ks; };
+    const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = tiles(16) / r[0];
+    const double t16 = min(7 + max(chain, fill), 13 + fill);
+    const double t64 = 15 + max(tiles(64) / r[1], 3.0 * ks), t128 = 17 + max(tiles(128) / r[2], 5.0 * ks);
+    const bool wide = attend_rt(attend_ks(a.head_dim)) == 2 && t128 < t64;
+    return t16 <= min(t64, t128) ? 16 : wide ? 128 : 64;
 }
 
 /* Up to 32 rows a sequence and KV head on average (decoding) the tiles have 16 rows; above, a workgroup's waves own theirs,
@@ -578,12 +594,11 @@ uint32_t tree_rows(const PagedArgs &a) {
  * one's chain of steps, and a step of half the rows is shorter (2048 tokens from an empty cache, f16, 8 KV heads of 64: 71
  * us, 58; 1024 of 128: 51, 40; but 2048 of 128: 100, 104). */
 AttendPlan attend_plan(const PagedArgs &a, size_t ws_bytes, bool tree) {
-    if (tree) return plan_tiles(a, ws_bytes, tree_rows(a), true);
     const uint32_t ks = attend_ks(a.head_dim);
     const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), seqs = a.seqs < a.tokens ? a.seqs : a.tokens;
-    if (rows <= 32 * seqs) return plan_tiles(a, ws_bytes, 16, tree);
-    const AttendPlan p = plan_tiles(a, ws_bytes, 64 * attend_rt(ks), tree);
-    return p.stream || p.tile_rows == 64 || rows / 128 * a.kv_heads * ks >= 2048 ? p : plan_tiles(a, 0, 64, tree);
+    const uint32_t tile = tree ? tree_rows(a) : rows <= 32 * seqs ? 16 : 64 * attend_rt(ks);
+    const AttendPlan p = plan_tiles(a, ws_bytes, tile, tree);
+    return p.stream || tile <= 64 || rows / 128 * a.kv_heads * ks >= 2048 ? p : plan_tiles(a, 0, 64, tree);
 }
 
 }  // namespace
@@ -626,16 +641,15 @@ hipError_t launch_paged_read(const PagedArgs &a, float *keys, float *values, hip
 
 size_t paged_attention_workspace(const PagedArgs &given, bool tree) {
     PagedArgs a = given;
+    a.sinks = a.limit; /* the call brings them: a plan of more positions needs no fewer bytes, up to all of the context's */
     auto bytes = [&](const AttendPlan &p) {
         return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
     };
-    a.sinks = a.limit; /* the call brings them: a plan of more positions needs no fewer bytes, up to all of the context's */
-    const size_t most = bytes(attend_plan(a, ~(size_t)0, tree));
-    if (!tree) return most;
-    a.sinks = 0; /* with fewer the tiles may have other rows */
-    const uint32_t rows = tree_rows(a);
-    a.sinks = a.limit;
-    return max(most, bytes(plan_tiles(a, ~(size_t)0, rows, true)));
+    if (!tree) return bytes(attend_plan(a, ~(size_t)0, false));
+    size_t most = 0; /* the call brings the cache's type too: any of the tiles */
+    for (uint32_t rows = 16; rows <= 64 * attend_rt(attend_ks(a.head_dim)); rows *= rows == 16 ? 4 : 2)
+        most = max(most, bytes(plan_tiles(a, ~(size_t)0, rows, true)));
+    return most;
 }
 
 hipError_t launch_paged_attention(const PagedArgs &a, const TreeArgs *tree, const float *q, float *att, void *ws,
