@@ -572,14 +572,15 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
  *               at 700        51   40    42                  at 2000        37   28    34
  *               at 3001      126   89    79      f16 64 x  8 at 2000       139   98   103
  *   f16 24 x 40 at 700        47   31    35      f16  8 x 63 at 16384      815  401   252
- *               at 1500       76   38    41      q8   8 x 16 at 1500        18   21    23 (14 heads on 2 of 64) */
+ *               at 1500       76   38    41      q8   8 x 16 at 1500        18   21    23 (14 heads on 2 of 64)
+ *   f32 24 x 40 at 3001      247  159   156      f32  8 x 16 at 2000        66   53    78 */
 uint32_t tree_rows(const PagedArgs &a) {
     const double ks = attend_ks(a.head_dim), rows = (double)a.tokens * (a.heads / a.kv_heads);
     const double seqs = a.seqs < a.tokens ? a.seqs : a.tokens, each = rows / seqs;
     double reach = a.limit;
     if (a.window) reach = min(reach, (double)a.window + a.sinks + a.tokens);
     const double steps = reach / PA_STEP + 1;
-    static const double rate[3][3] = {{1200, 400, 230}, {1900, 1300, 1080}, {1900, 1020, 660}}; /* by type, of one 32-wide step */
+    static const double rate[3][3] = {{1050, 510, 270}, {1900, 1300, 1080}, {1900, 1020, 660}}; /* by type, of one 32-wide step */
     const double *r = rate[a.type];
     auto tiles = [&](double n) { return ceil(each / n) * seqs * a.kv_heads * steps * ks; };
     const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = tiles(16) / r[0];

@@ -1084,6 +1084,22 @@ struct InLds {
     }
 };
 
+/* A step's keys (or values) out of LDS in registers, all requested before the first is used: 8 f16 drafts of 63 at 16384, 8 KV
+ * heads of 64 152 -> 142 us, of 128 249 -> 239. f32 and Q8, whose registers are full without them, lose (Q8 heads of 128 74 ->
+ * 79). */
+template <uint32_t TYPE, int KS, bool VALUES>
+struct Held {
+    typename Elem<TYPE>::Frag f[2 * KS];
+    template <typename Src>
+    __device__ __forceinline__ Held(const Src &src) {
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) f[i] = VALUES ? src.v(i) : src.k(i & 1, i >> 1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ const typename Elem<TYPE>::Frag &k(int t, int s) const { return f[2 * s + t]; }
+    __device__ __forceinline__ const typename Elem<TYPE>::Frag &v(int t) const { return f[t]; }
+};
+
 /* Where a tile's results go: its rows of att, or the split's partial results. */
 struct Out {
     const PagedArgs &a;
@@ -1199,9 +1215,16 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
                 const Src src = {lds + ((u - u0) & 1) * Src::BUFFER};
                 const bool full = w.full(p0, ok);
                 float x[RT][8];
-                w.scores(src, x);
-                w.weights(p0, ok, full, x);
-                w.product(p0, ok, full, src, x);
+                if constexpr (TREE && TYPE == 1) {
+                    w.scores(Held<TYPE, KS, false>(src), x);
+                    const Held<TYPE, KS, true> v(src);
+                    w.weights(p0, ok, full, x);
+                    w.product(p0, ok, full, v, x);
+                } else {
+                    w.scores(src, x);
+                    w.weights(p0, ok, full, x);
+                    w.product(p0, ok, full, src, x);
+                }
             }
             Src::wait(); /* the next step is there, and this one's buffer free */
         }
