@@ -250,23 +250,14 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
         keys[tid] = mine;
     }
     __syncthreads();
-    uint64_t most = 0;
-    for (uint32_t i = tid % 64; i < columns; i += 64) most = keys[i] > most ? keys[i] : most;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const uint64_t o = __shfl_xor(most, off);
-        most = o > most ? o : most;
-    }
     if (bad && tid == 0) *a.flag = 1;
-    const bool none = bad || score == -INFINITY || (!done && !most);
-    if (none || done) {
+    auto finish = [&](bool some) { /* without a choice: the one of a row that is done, or none */
         for (uint32_t k = tid; k < a.select; k += BM_WG) {
-            value[k] = !none && k == 0 ? (double)score : -INFINITY;
+            value[k] = some && k == 0 ? (double)score : -INFINITY;
             id[k] = a.pad;
         }
-        return;
-    }
-    const double top = (double)logit_of(most);
+    };
+    if (bad || score == -INFINITY || done) return finish(!bad && score > -INFINITY);
     /* the blocks that are no smaller than the select-th of the columns' maxima, and the best of them */
     const uint64_t least = max(kth_of(keys, columns, a.select), (uint64_t)1);
     auto put = [&](float x, uint32_t i) {
@@ -278,6 +269,8 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     for (uint32_t i = tid + BT * BM_WG; i < s.blocks; i += BM_WG) put(bt[i], i);
     __syncthreads();
     const uint32_t listed = counts[0], nb = best_of(list, other, listed, a.select, keys, blocks, &counts[2]);
+    if (!nb) return finish(false); /* all masked */
+    const double top = (double)logit_of(blocks[0]);
     /* their ids, BM_WG / BM_LANES blocks at a time, a lane four */
     const float low = nb == a.select ? logit_of(blocks[nb - 1]) : -FLT_MAX;
     auto load = [&](uint32_t b, float(&l)[4]) {
@@ -313,27 +306,54 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     }
 }
 
-/* A workgroup per result where there are histories, else per group: the best of the group's candidates, and its results. */
+/* A workgroup per result where there are histories, else per group: the best of the group's candidates, and its results. What the
+ * results may need of the candidates and rows is requested with their values. */
+template <bool MANY> /* more than BM_WG candidates */
 __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *value, const uint32_t *id, uint32_t per) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; /* the lists */
-    __shared__ Cand keys[BM_WG], best[MAX_SELECT];
-    __shared__ uint32_t count;
+    __shared__ uint64_t values[BM_WG], best[MAX_SELECT];
+    __shared__ uint32_t which[MAX_SELECT], ids[BM_WG];
+    __shared__ int lengths[MAX_BEAMS];
+    __shared__ uint8_t over_rows[MAX_BEAMS];
     const uint32_t g = blockIdx.x / per, tid = threadIdx.x, n = a.beams * a.select;
     const size_t at = (size_t)g * n;
-    Cand *list = (Cand *)lds, *other = list + (n > BM_WG ? list_next(n, a.select) : BM_WG);
-    const auto cand = [&](uint32_t i) {
-        const double v = value[at + i];
-        return v > -INFINITY ? Cand{order_of(v), ~(uint64_t)i} : Cand{0, 0};
-    };
-    uint32_t m = n;
-    if (n > BM_WG) {
+    if (tid < a.beams) {
+        over_rows[tid] = a.done ? a.done[g * a.beams + tid] : 0;
+        lengths[tid] = a.history ? a.length[g * a.beams + tid] : 0;
+    }
+    uint32_t found;
+    if constexpr (!MANY) {
+        const double x = tid < n ? value[at + tid] : -INFINITY;
+        const uint64_t mine = x > -INFINITY ? order_of(x) : 0;
+        values[tid] = mine;
+        if (tid < n) ids[tid] = id[at + tid];
+        const int all = __syncthreads_count(mine != 0);
+        if (mine) {
+            uint32_t rank = 0;
+#pragma unroll 16
+            for (uint32_t i = 0; i < n; ++i) rank += values[i] > mine || (values[i] == mine && i < tid);
+            if (rank < a.select) {
+                which[rank] = tid;
+                best[rank] = mine;
+            }
+        }
+        __syncthreads();
+        found = min((uint32_t)all, a.select);
+    } else {
+        extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; /* the lists */
+        __shared__ Cand keys[BM_WG], most[MAX_SELECT];
+        __shared__ uint32_t count;
+        if (tid == 0) count = 0;
+        Cand *list = (Cand *)lds, *other = list + list_next(n, a.select);
+        const auto cand = [&](uint32_t i) {
+            const double v = value[at + i];
+            return v > -INFINITY ? Cand{order_of(v), ~(uint64_t)i} : Cand{0, 0};
+        };
         Cand mine = {0, 0};
         for (uint32_t i = tid; i < n; i += BM_WG) {
             const Cand c = cand(i);
             mine = c > mine ? c : mine;
         }
         keys[tid] = mine;
-        if (tid == 0) count = 0;
         __syncthreads();
         const Cand kth = kth_of(keys, BM_WG, a.select), least = some(kth) ? kth : Cand{1, 0};
         for (uint32_t i = tid; i < n; i += BM_WG) {
@@ -341,29 +361,26 @@ __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *v
             if (!(least > c)) list[atomicAdd(&count, 1u)] = c;
         }
         __syncthreads();
-        m = count;
-    } else {
-        if (tid == 0) count = 0;
+        found = best_of(list, other, count, a.select, keys, most, &count);
+        if (tid < found) {
+            which[tid] = (uint32_t)~most[tid].i;
+            best[tid] = most[tid].v;
+        }
         __syncthreads();
-        const Cand c = tid < n ? cand(tid) : Cand{0, 0};
-        if (some(c)) list[atomicAdd(&count, 1u)] = c;
-        __syncthreads();
-        m = count;
     }
-    const uint32_t found = best_of(list, other, m, a.select, keys, best, &count);
     for (uint32_t k = blockIdx.x % per; k < a.select; k += per) {
-        const uint32_t o = g * a.select + k, w = k < found ? (uint32_t)~best[k].i : 0;
+        const uint32_t o = g * a.select + k, w = k < found ? which[k] : 0, row = w / a.select;
         const bool none = k >= found;
-        const uint32_t r = none ? 0 : g * a.beams + w / a.select, token = none ? NONE : id[at + w];
-        const bool over = !none && a.done && a.done[r];
+        const uint32_t r = none ? 0 : g * a.beams + row, token = none ? NONE : MANY ? id[at + w] : ids[w];
+        const bool over = !none && over_rows[row];
         if (tid == 0) {
             a.parent[o] = none ? -1 : (int)r;
             a.token[o] = token;
-            a.score_out[o] = none ? -INFINITY : (float)value_of(best[k].v);
+            a.score_out[o] = none ? -INFINITY : (float)value_of(best[k]);
             if (a.done_out) a.done_out[o] = none || over || (a.eos != NONE && token == a.eos);
         }
         if (!a.history) continue;
-        const int have = none ? 0 : a.length[r];
+        const int have = none ? 0 : lengths[row];
         const uint32_t len = (uint32_t)min(max(have, 0), (int)a.history_stride);
         const bool more = !none && !over && len < a.history_stride;
         if (tid == 0) {
@@ -414,9 +431,13 @@ hipError_t launch_beam(const BeamArgs &a, void *ws, hipStream_t st) {
 #undef SMQ_BEAM
     const uint32_t first = a.select * BM_BLOCK, n = a.beams * a.select;
     hipLaunchKernelGGL(k_beam_rows, dim3(rows), dim3(BM_WG), (first + list_next(first, a.select)) * 8, st, a, s, value, id);
-    const uint32_t per = a.history ? a.select : 1, list = n > BM_WG ? list_next(n, a.select) : BM_WG;
-    hipLaunchKernelGGL(k_beam_join, dim3(a.groups * per), dim3(BM_WG), (list + list_next(list, a.select)) * sizeof(Cand), st, a,
-                       value, id, per);
+    const uint32_t per = a.history ? a.select : 1, list = list_next(n, a.select);
+    const dim3 joins(a.groups * per);
+    if (n > BM_WG)
+        hipLaunchKernelGGL((k_beam_join<true>), joins, dim3(BM_WG), (list + list_next(list, a.select)) * sizeof(Cand), st, a, value,
+                           id, per);
+    else
+        hipLaunchKernelGGL((k_beam_join<false>), joins, dim3(BM_WG), 0, st, a, value, id, per);
     return hipGetLastError();
 }
 
