@@ -105,7 +105,8 @@ struct Sums {
     uint32_t blocks, sums; /* of a row */
 };
 
-/* A wave takes U times 256 ids of the span: no exchange with the others. */
+/* A wave takes U times 256 ids of the row: no exchange with the others. 128 rows of 151936, 78 MB, 20 us, 3.9 TB/s: 13 us of VALU
+ * work, most of it on 64 bits, beside 13.8 of reading alone, which waves in several rounds overlap in part. */
 template <uint32_t U, bool WIDE>
 __global__ __launch_bounds__(BM_WG) void k_beam_sums(BeamArgs a, Sums s) {
     const uint32_t tid = threadIdx.x, lane = tid % 64, wave = blockIdx.x * BM_WAVES + tid / 64, r = blockIdx.y;
@@ -207,7 +208,8 @@ __host__ __device__ inline uint32_t list_next(uint32_t first, uint32_t most) { r
 __host__ __device__ inline uint32_t columns_of(uint32_t blocks, uint32_t select) { return select <= 32 && blocks <= 4096 ? 64 : BM_WG; }
 
 /* A workgroup per row: its `select` best ids and their values. What the row's blocks have is requested at once; the best
- * blocks' logits are on their way while the sums are joined. */
+ * blocks' logits are on their way while the sums are joined. Bound by its chain of two trips to memory, eight barriers and
+ * three rankings: 8 us, for 4 rows or 128. */
 __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double *value, uint32_t *id) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ double sums[BM_WAVES];
@@ -307,7 +309,8 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
 }
 
 /* A workgroup per result where there are histories, else per group: the best of the group's candidates, and its results. What the
- * results may need of the candidates and rows is requested with their values. */
+ * results may need of the candidates and rows is requested with their values. Bound by two trips to memory and the ranking: 4.2 us
+ * for 32 candidates, 7.2 for 128 of each of 16 groups. */
 template <bool MANY> /* more than BM_WG candidates */
 __global__ __launch_bounds__(BM_WG) void k_beam_join(BeamArgs a, const double *value, const uint32_t *id, uint32_t per) {
     __shared__ uint64_t values[BM_WG], best[MAX_SELECT];

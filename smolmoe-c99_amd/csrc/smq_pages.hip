@@ -74,9 +74,10 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *lds, uint32
     return before;
 }
 
-/* Few rows and pages: one workgroup, the pages' holders in LDS. Three trips to memory (row arrays and holders, old entries, the
- * parents' entries) and ten barriers: the launch and 4 us, where the four launches below take 11. */
-constexpr uint32_t SMALL_WG = 1024, SMALL_WAVES = SMALL_WG / 64, SMALL_PAGES = 8192, SMALL_ROWS = 256, SMALL_ENTRIES = 16384;
+/* Few rows and pages: one workgroup, the pages' holders in LDS. Bound by three trips to memory (row arrays, holders and old
+ * entries; the parents' entries; the results) and ten barriers: four rows 6.8 us, where the four launches below take 11; 64 rows
+ * of 14 entries 9.1, 15; 256 of 32, 7118 pages 13.9, 14.2; but 256 of 63 18.6, 14.6. */
+constexpr uint32_t SMALL_WG = 1024, SMALL_WAVES = SMALL_WG / 64, SMALL_PAGES = 8192, SMALL_ROWS = 256, SMALL_ENTRIES = 8192;
 __global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
     __shared__ int holders[SMALL_PAGES];
     __shared__ uint32_t in_part[SMALL_PAGES / 32], free_words[SMALL_PAGES / 32], word_rank[SMALL_PAGES / 32];
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(SMALL_WG) void k_fork_small(ForkArgs a) {
     if (tid < words) in_part[tid] = 0;
     __syncthreads();
     const float inv = 1.0f / (float)a.table_stride;
-    auto row_of = [&](uint32_t i) { return (uint32_t)(((float)i + 0.5f) * inv); }; /* i / stride: below 2^15, where this is exact */
+    auto row_of = [&](uint32_t i) { return (uint32_t)(((float)i + 0.5f) * inv); }; /* i / stride: below 2^14, where this is exact */
     auto give_up = [&](uint32_t i, uint32_t id) {
         const uint32_t s = row_of(i), x = i - s * a.table_stride;
         if (x >= olds[s]) return;
@@ -426,8 +427,9 @@ struct Divide {
 
 /* A workgroup per row of `copies`, pool, KV head and kind (keys, values). Keys are one run of bytes; of a value dim's row the
  * first positions, 16 bytes at a time and a shorter end. Scales go with their codes. CP_BATCH pieces a thread are requested
- * before the first is written. Bound by three trips to memory where pages are few; 64 rows of 12 f16 layers of 2 KV heads of
- * 128 in pages of 128, 29 of them copied, 15 MB. */
+ * before the first is written. Bound by three trips to memory where pages are few (four beams of 24 Q8 layers 4.8 us), by bytes
+ * else: 20 pages of 128 in 12 f16 layers of 2 KV heads of 128, 24 MB read and written, 6.9 us, 3.5 TB/s (4 bytes a piece, keys
+ * and values in one workgroup: 42). */
 constexpr uint32_t CP_BATCH = 4;
 template <typename T, typename At>
 __device__ __forceinline__ void copy_pieces(uint32_t n, const void *from, void *to, At at) {
@@ -488,7 +490,9 @@ __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, 
  * key every 16th piece of 16 bytes, of its value every 16th dim (lanes next to each other have the path's tokens of one dim,
  * which lie in the same lines of memory).
  *
- * Bound by four trips to memory (batch, path, page ids, tokens). */
+ * Bound by four trips to memory (batch, path, page ids, tokens): 8 paths in 24 Q8 layers 5.2 us; then by the lines that hold a
+ * value dim's tokens, 64 bytes for two each way: 64 paths of up to 12 of 60 drafts, four f16 layers of 8 KV heads of 128, 12 us
+ * (through LDS, a workgroup's tokens one pass after another: 15; keys and values in workgroups of their own: 19). */
 constexpr uint32_t CM_TOKENS = 16;
 template <uint32_t EB>
 struct Element;
