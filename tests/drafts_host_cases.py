@@ -1,5 +1,6 @@
 """Cases of tests/test_drafts_host.py, each in a process of its own: drafts_host_cases.py FAKE_HIP_LIBRARY CASE. Refusals and
 empty calls of the operators of drafts and beams over the recording runtime of tests/fake_hip.cpp, without a GPU."""
+import itertools
 import os
 import sys
 
@@ -359,12 +360,12 @@ def widest_split():
     """The bytes that the query of tree attention gives make the launches that boundless ones would, whatever sinks and table the
     call brings."""
     cut = 0
-    for heads, kv, hd, seqs, new, window, context in (
+    for kv_type, (heads, kv, hd, seqs, new, window, context) in itertools.product((0, 1, 2), (
             (32, 4, 64, 8, 1, 64, 5000), (32, 8, 128, 1, 16, 512, 131072), (14, 2, 64, 3, 9, 1000, 32768),
             (4, 1, 64, 1, 1, 16, 1 << 20), (8, 2, 128, 2, 300, 200, 9000), (32, 8, 128, 6, 64, 33, 60000),
             (8, 2, 256, 1, 100, 0, 4000), (4, 1, 64, 1, 1, 0, 1 << 20), (14, 2, 64, 1, 13, 0, 3000), (12, 2, 128, 24, 40, 0, 3001),
-            (14, 2, 64, 8, 16, 100, 2000)):
-        p = Drafts(heads=heads, kv=kv, hd=hd, pairs=0, type=1, page=64, pages=1, seqs=seqs, tokens=seqs * new,
+            (14, 2, 64, 8, 16, 100, 2000))):
+        p = Drafts(heads=heads, kv=kv, hd=hd, pairs=0, type=kv_type, page=64, pages=1, seqs=seqs, tokens=seqs * new,
                    stride=-(-context // 64), window=window, context=context, words=16)
         p.batch.table_stride = table = -(-context // 64)
         p.b["table"] = smq.DeviceBuffer(4 * seqs * table)
@@ -380,9 +381,9 @@ def widest_split():
                     smq.paged_tree_attention(p.b["q"], p.b["att"], p.batch, p.shape, sinks, p.b["depth"], p.b["mask"], 16, p.kv,
                                              large.at(0), n)
                     got.append(base.grids())
-                assert got[0] == got[1], (heads, kv, hd, seqs, new, window, context, sinks, t, need, got)
+                assert got[0] == got[1], (kv_type, heads, kv, hd, seqs, new, window, context, sinks, t, need, got)
                 cut += len(got[0]) == 2
-    assert cut > 50
+    assert cut > 150
 
 
 CASES = [valid_calls, empty_batches, shapes, buffers, forks, beams, beam_workspace_of_the_largest_step, captures, widest_split]

@@ -385,6 +385,21 @@ def test_tree_attention_of_many(kv_type):
     smq.numeric_check()
 
 
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("length,new,page,kind", [(1107, 1100, 16, "tree"), (640, 640, 64, "any")])
+def test_tree_attention_of_many_drafts(kv_type, length, new, page, kind):
+    """Masks of many words, which steps of 32 positions meet anywhere; a context shorter than a step, and none."""
+    heads, kv, hd = 2, 1, 48
+    cache = Cache(kv_type, kv, hd, page, [length, 40], stale="nan").upload()
+    batch = Batch(cache, [new, 40])
+    trees = Trees(batch, kind=kind).upload()
+    q = synth.normal(96, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    want, tol = ref.tree64(cache, batch, q, heads, trees.depth, trees.seen)
+    close(tree_attend(cache, batch, q, heads, trees), want, tol)
+    close(tree_attend(cache, batch, q, heads, trees, split=False), want, tol)
+    smq.numeric_check()
+
+
 def test_tree_attention_of_a_causal_mask():
     """A chain is causal: smq_paged_attention's results, within both bounds; with its window, whose positions are the same."""
     heads, kv, hd = 8, 2, 64
