@@ -1208,6 +1208,17 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
         loader.load(pl, lds);
         w.queries(q);
         Src::wait();
+        /* Drafts see nearly every step of their tile, so a wave either computes all of them or only loads. Each has its loop:
+         * with the branch in one, O is copied to other registers and back in every step (8 f16 drafts of 63 at 16384, 8 KV
+         * heads of 128: 240 us, 232 so; of 64 146 and 143). Both make the same barriers, which count waves and not the
+         * places they wait at. */
+        if (TREE && !mine) {
+            for (uint32_t u = u0; u < u1; ++u) {
+                if (u + 1 < u1) loader.load(pages.locate(st.at(u + 1), span), lds + ((u + 1 - u0) & 1) * Src::BUFFER);
+                Src::wait();
+            }
+            return;
+        }
         for (uint32_t u = u0; u < u1; ++u) {
             const uint32_t p0 = at * PA_STEP, ok = pl.ok;
             if (u + 1 < u1) {
@@ -1216,7 +1227,7 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
                 loader.load(pl, lds + ((u + 1 - u0) & 1) * Src::BUFFER);
             }
             __builtin_amdgcn_sched_barrier(0); /* the loads first: the compiler would sink them behind the products */
-            if (mine && w.span.meets(p0, PA_STEP)) {
+            if (TREE || (mine && w.span.meets(p0, PA_STEP))) {
                 const Src src = {lds + ((u - u0) & 1) * Src::BUFFER};
                 const bool full = w.full(p0, ok);
                 float x[RT][8];
