@@ -149,6 +149,8 @@ __device__ __forceinline__ h8 codes8(u2 w) {
     return r.h - (_Float16)1152.0f;
 }
 
+__device__ __forceinline__ h8 codes8(const h8 &x) { return x; }
+
 template <uint32_t TYPE>
 struct Elem;
 template <>
@@ -984,7 +986,7 @@ struct InLds {
     static constexpr uint32_t K_BYTES = 32 * 32 * KS * EB;
     static constexpr uint32_t W_BYTES = TYPE == 2 ? 128 * KS : 0; /* the scales of keys or of values */
     static constexpr uint32_t K_LOADS = K_BYTES / 1024, W_LOADS = (2 * W_BYTES + 1023) / 1024; /* of a wave */
-    static constexpr uint32_t BUFFER = 2 * K_BYTES + W_LOADS * 1024, EACH = (K_LOADS + PA_WAVES - 1) / PA_WAVES;
+    static constexpr uint32_t BUFFER = 2 * K_BYTES + W_LOADS * 1024, BYTES = 2 * BUFFER, EACH = (K_LOADS + PA_WAVES - 1) / PA_WAVES;
     const unsigned char *b; /* the buffer of the step */
 
     __device__ __forceinline__ Frag k(int t, int s) const {
@@ -1015,7 +1017,7 @@ struct InLds {
         uint32_t wave, koff[EACH], voff[EACH], woff[W_LOADS ? W_LOADS : 1];
         bool ksecond, vsecond, wsecond, wvalues[W_LOADS ? W_LOADS : 1];
 
-        __device__ __forceinline__ Loader(const PagedArgs &a, uint32_t wave_) : wave(wave_) {
+        __device__ __forceinline__ Loader(const PagedArgs &a, uint32_t wave_, unsigned char *) : wave(wave_) {
             const uint32_t lane = threadIdx.x % 64, hd = a.head_dim, m = lane % 16, quad = lane / 16;
             ksecond = SMALL && m >> 3;
             vsecond = SMALL && (TYPE == 2 ? quad & 1 : quad >> 1);
@@ -1062,6 +1064,10 @@ struct InLds {
                                              (__attribute__((address_space(3))) void *)to, 16, 0, 0);
         }
         __device__ __forceinline__ void load(const Place &pl, unsigned char *to) const {
+            codes(pl, to);
+            if constexpr (TYPE == 2) scales(pl, to + 2 * K_BYTES);
+        }
+        __device__ __forceinline__ void codes(const Place &pl, unsigned char *to) const {
             typedef InRegisters<TYPE, KS, SMALL> Pick;
             const unsigned char *k = Pick::pick(pl.k, ksecond), *v = Pick::pick(pl.v, vsecond);
 #pragma unroll
@@ -1072,13 +1078,13 @@ struct InLds {
                     move(v + voff[j], to + K_BYTES + i * 1024);
                 }
             }
-            if constexpr (TYPE == 2) {
-                if (wave == PA_WAVES - 1) {
-                    const unsigned char *kw = Pick::pick(pl.kw, wsecond), *vw = Pick::pick(pl.vw, wsecond);
+        }
+        __device__ __forceinline__ void scales(const Place &pl, unsigned char *to) const {
+            typedef InRegisters<TYPE, KS, SMALL> Pick;
+            if (wave == PA_WAVES - 1) {
+                const unsigned char *kw = Pick::pick(pl.kw, wsecond), *vw = Pick::pick(pl.vw, wsecond);
 #pragma unroll
-                    for (uint32_t j = 0; j < W_LOADS; ++j)
-                        move((wvalues[j] ? vw : kw) + woff[j], to + 2 * K_BYTES + j * 1024);
-                }
+                for (uint32_t j = 0; j < W_LOADS; ++j) move((wvalues[j] ? vw : kw) + woff[j], to + j * 1024);
             }
         }
     };
@@ -1089,9 +1095,60 @@ struct InLds {
     }
 };
 
+/* TREE: Q8 keys and values in LDS as f16, converted once for the workgroup's four waves: a lane's 16 codes of keys (and of
+ * values) are two lanes' fragments. A wave loads codes to its part of `raw`, the next step's while this one is computed, and
+ * converts them behind the products; scales go straight to the next buffer. Where each wave converts what it reads, that is
+ * 160 of its 600 vector instructions a step (heads of 128): 8 drafts of 63 at 16384, 8 KV heads of 128 402 -> 367 us, of 64
+ * 240 -> 230, 24 drafts of 40 at 3001, 2 KV heads of 128 72.7 -> 69.8. Codes that wait in registers, not in LDS: 395 us and 9
+ * registers spilled. */
+template <int KS, bool SMALL>
+struct InLdsCodes {
+    typedef InLds<2, KS, SMALL> Raw;
+    typedef typename Raw::Place Place;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    static constexpr uint32_t K_BYTES = 2048 * KS, BUFFER = 2 * K_BYTES + Raw::W_LOADS * 1024, BYTES = 2 * BUFFER + 2 * Raw::K_BYTES;
+    const unsigned char *b;
+
+    __device__ __forceinline__ h8 k(int t, int s) const { return *(const h8 *)(b + (s * 2 + t) * 1024 + threadIdx.x % 64 * 16); }
+    __device__ __forceinline__ h8 v(int t) const { return *(const h8 *)(b + K_BYTES + t * 1024 + threadIdx.x % 64 * 16); }
+    __device__ __forceinline__ f4 kscale(int s, int h) const {
+        return *(const f4 *)(b + 2 * K_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
+    }
+    __device__ __forceinline__ f4 vscale(int s, int h) const {
+        return *(const f4 *)(b + 2 * K_BYTES + Raw::W_BYTES + s * 128 + (threadIdx.x % 64 / 16) * 32 + h * 16);
+    }
+
+    struct Loader {
+        typename Raw::Loader from;
+        unsigned char *raw;
+        __device__ __forceinline__ Loader(const PagedArgs &a, uint32_t wave, unsigned char *lds) : from(a, wave, lds), raw(lds + 2 * BUFFER) {}
+        __device__ __forceinline__ void load(const Place &pl, unsigned char *to) const {
+            from.codes(pl, raw);
+            from.scales(pl, to + 2 * K_BYTES);
+        }
+        __device__ __forceinline__ void put(unsigned char *to) const {
+            const uint32_t lane = threadIdx.x % 64, m = lane % 16, odd = lane / 16 & 1, half = lane / 32;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (uint32_t j = 0; j < Raw::EACH; ++j) {
+                const uint32_t i = j * PA_WAVES + from.wave;
+                if (KS % PA_WAVES == 0 || i < (uint32_t)KS) {
+                    const u4 kc = *(const u4 *)(raw + i * 1024 + lane * 16), vc = *(const u4 *)(raw + Raw::K_BYTES + i * 1024 + lane * 16);
+                    h8 *k = (h8 *)(to + (i * 2 + odd) * 1024 + half * 512 + m * 16);           /* tile odd, quads 2 half and the next */
+                    h8 *v = (h8 *)(to + K_BYTES + (i * 2 + half) * 1024 + odd * 512 + m * 16); /* dims of half, quads 2 odd and the next */
+                    k[0] = codes8(u2{kc[0], kc[1]});
+                    k[16] = codes8(u2{kc[2], kc[3]});
+                    v[0] = codes8(u2{vc[0], vc[1]});
+                    v[16] = codes8(u2{vc[2], vc[3]});
+                }
+            }
+        }
+    };
+    static __device__ __forceinline__ void wait() { Raw::wait(); }
+};
+
 /* A step's keys (or values) out of LDS in registers, all requested before the first is used: 8 f16 drafts of 63 at 16384, 8 KV
- * heads of 64 152 -> 142 us, of 128 249 -> 239. f32 and Q8, whose registers are full without them, lose (Q8 heads of 128 74 ->
- * 79). */
+ * heads of 64 152 -> 142 us, of 128 249 -> 239. f32 and Q8, whose registers are full without them, lose. */
 template <uint32_t TYPE, int KS, bool VALUES>
 struct Held {
     typename Elem<TYPE>::Frag f[2 * KS];
@@ -1185,12 +1242,23 @@ __device__ __forceinline__ void tile_shared(const PagedArgs &a, const TreeArgs &
 }
 constexpr uint32_t shared_lds(int ks) { return PA_WAVES * 16 * (32 * ks + 4) * 4 + PA_WAVES * 16 * 8; }
 
+/* Where a tile whose waves own rows has its steps. */
+template <uint32_t TYPE, int KS, bool SMALL, bool TREE>
+struct Staged {
+    typedef InLds<TYPE, KS, SMALL> Src;
+};
+template <int KS, bool SMALL>
+struct Staged<2, KS, SMALL, true> {
+    typedef InLdsCodes<KS, SMALL> Src;
+};
+
 /* Each wave has 16 * RT rows of the tile over the steps [u0, u1), whose keys and values the workgroup brings to LDS, the
  * next step's while this one is computed. A wave without rows (or whose rows do not see a step) only loads. */
 template <uint32_t TYPE, int KS, int RT, bool SMALL, bool TREE>
 __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &tree, const float *q, const Seq &sq, uint32_t seq, const Steps &st,
                                            uint32_t u0, uint32_t u1, uint32_t wave, const Out &out, unsigned char *lds) {
-    typedef InLds<TYPE, KS, SMALL> Src;
+    typedef typename Staged<TYPE, KS, SMALL, TREE>::Src Src;
+    constexpr bool CODES = TREE && TYPE == 2;
     const uint32_t first = wave * 16 * RT, G = a.heads / a.kv_heads;
     const bool mine = first < out.n;
     /* the last wave's rows again where there are none: never stored */
@@ -1202,11 +1270,12 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
         w.queries(q);
     } else {
         Pages<TYPE, SMALL> pages(a, seq, out.kh);
-        const typename Src::Loader loader(a, wave);
+        const typename Src::Loader loader(a, wave, lds);
         uint32_t at = st.at(u0);
         auto pl = pages.locate(at, span);
         loader.load(pl, lds);
         w.queries(q);
+        if constexpr (CODES) loader.put(lds);
         Src::wait();
         /* Drafts see nearly every step of their tile, so a wave either computes all of them or only loads. Each has its loop:
          * with the branch in one, O is copied to other registers and back in every step (8 f16 drafts of 63 at 16384, 8 KV
@@ -1214,7 +1283,11 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
          * places they wait at. */
         if (TREE && !mine) {
             for (uint32_t u = u0; u < u1; ++u) {
-                if (u + 1 < u1) loader.load(pages.locate(st.at(u + 1), span), lds + ((u + 1 - u0) & 1) * Src::BUFFER);
+                if (u + 1 < u1) {
+                    unsigned char *next = lds + ((u + 1 - u0) & 1) * Src::BUFFER;
+                    loader.load(pages.locate(st.at(u + 1), span), next);
+                    if constexpr (CODES) loader.put(next);
+                }
                 Src::wait();
             }
             return;
@@ -1242,6 +1315,8 @@ __device__ __forceinline__ void tile_owned(const PagedArgs &a, const TreeArgs &t
                     w.product(p0, ok, full, src, x);
                 }
             }
+            if constexpr (CODES)
+                if (u + 1 < u1) loader.put(lds + ((u + 1 - u0) & 1) * Src::BUFFER);
             Src::wait(); /* the next step is there, and this one's buffer free */
         }
     }
@@ -1295,7 +1370,7 @@ __device__ __forceinline__ void tile_part(const PagedArgs &a, const TreeArgs &tr
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL, bool TREE>
 __device__ __forceinline__ void attend_piece(const PagedArgs &a, const TreeArgs &tree, const float *q, float *att,
                                              const AttendPlan &p, i4 *used, float *part) {
-    constexpr uint32_t OWN_LDS = OWNS ? 2 * InLds<TYPE, KS, SMALL>::BUFFER : 0;
+    constexpr uint32_t OWN_LDS = OWNS ? Staged<TYPE, KS, SMALL, TREE>::Src::BYTES : 0;
     __shared__ __attribute__((aligned(16))) unsigned char lds[OWN_LDS > shared_lds(KS) ? OWN_LDS : shared_lds(KS)];
     const uint32_t kh = blockIdx.x % a.kv_heads, i = blockIdx.x / a.kv_heads;
     if (blockIdx.x == 0) check_begin(a, threadIdx.x, 64 * PA_WAVES);
