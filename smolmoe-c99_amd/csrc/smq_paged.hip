@@ -572,24 +572,29 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
  * one after another (or a piece's, and the join), the others for a piece's steps, the batch and the join.
  *
  *                        16 rows   64   128                            16 rows   64   128
- *   q8  24 x 40 at 300        30   27    37      f16  8 x 16 at  700        19   24    29
- *               at 700        51   40    42                  at 2000        37   28    34
- *               at 3001      126   89    79      f16 64 x  8 at 2000       139   98   103
- *   f16 24 x 40 at 700        47   31    35      f16  8 x 63 at 16384      815  401   252
- *               at 1500       76   38    41      q8   8 x 16 at 1500        18   21    23 (14 heads on 2 of 64)
- *   f32 24 x 40 at 3001      247  159   156      f32  8 x 16 at 2000        66   53    78 */
+ *   q8  24 x 40 at 300        30   25    25      f16  8 x 16 at  700        19   25    28
+ *               at 700        51   37    40                  at 2000        37   29    32
+ *               at 3001      126   75    72      f16 64 x  8 at 2000       137   99    99
+ *   f16 24 x 40 at 700        47   31    33      f16  8 x 63 at 16384      811  435   240
+ *               at 1500       76   38    39      q8   8 x 16 at 1500        18   20    23 (14 heads on 2 of 64)
+ *   f32 24 x 40 at 3001      246  157   156      q8  24 x  8 at 3001        98   74    91
+ *                                                f32  8 x 16 at 2000        66   52    79 */
 uint32_t tree_rows(const PagedArgs &a) {
     const double ks = attend_ks(a.head_dim), rows = (double)a.tokens * (a.heads / a.kv_heads);
     const double seqs = a.seqs < a.tokens ? a.seqs : a.tokens, each = rows / seqs;
     double reach = a.limit;
     if (a.window) reach = min(reach, (double)a.window + a.sinks + a.tokens);
     const double steps = reach / PA_STEP + 1;
-    static const double rate[3][3] = {{1050, 510, 270}, {1900, 1300, 1080}, {1900, 1020, 660}}; /* by type, of one 32-wide step */
-    const double *r = rate[a.type];
-    auto tiles = [&](double n) { return ceil(each / n) * seqs * a.kv_heads * steps * ks; };
-    const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = tiles(16) / r[0];
+    /* by type, of one 32-wide step: tiles of 16 rows (and where heads are of 128), of 64, of 128. Q8 tiles convert a step once,
+     * whatever their rows, and then each wave has its part: their rates and those of its waves' 16 and 32 rows. */
+    constexpr double NONE = HUGE_VAL;
+    static const double rate[3][6] = {
+        {1050, 1050, 510, NONE, 270, NONE}, {1900, 1900, 1300, NONE, 1080, NONE}, {2540, 1580, 3480, 4400, 1700, 2400}};
+    const double *r = rate[a.type], unit = seqs * a.kv_heads * steps * ks;
+    const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = unit * ceil(each / 16) / r[ks == 4];
     const double t16 = min(7 + max(chain, fill), 13 + fill);
-    const double t64 = 15 + max(tiles(64) / r[1], 3.0 * ks), t128 = 17 + max(tiles(128) / r[2], 5.0 * ks);
+    const double t64 = 15 + max(unit * (ceil(each / 64) / r[2] + ceil(each / 16) / r[3]), 3.0 * ks);
+    const double t128 = 17 + max(unit * (ceil(each / 128) / r[4] + ceil(each / 32) / r[5]), 5.0 * ks);
     const bool wide = attend_rt(attend_ks(a.head_dim)) == 2 && t128 < t64;
     return t16 <= min(t64, t128) ? 16 : wide ? 128 : 64;
 }
