@@ -514,7 +514,8 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
 
 /* The pieces that tiles of so many rows are cut into: two a CU for products and for decoding heads of up to 64 (8 KiB of f16
  * a step and wave), one a CU for wider ones (one f16 sequence at 16384, 8 KV heads of 128: 22 us, two a CU 25); by_piece has
- * what becomes of these numbers.
+ * what becomes of these numbers. Three a CU for products of trees whose registers leave room (8 drafts of 63 at 8000, 32 heads
+ * on 8 of 64, tiles of 64 rows: f16 104 -> 73 us, Q8 178 -> 105, f32 391 -> 225; 24 of 8 at 3001 38 -> 33, 53 -> 41, 88 -> 68).
  *
  * Cutting costs partial results and a second launch, which joins them. No cuts
  * - where the longest tile exceeds an equal share by about 24 steps or less (64 sequences at 700, 2 KV heads of 64: 11.8 us
@@ -531,7 +532,8 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     p.tile_rows = tile_rows;
     p.row_shift = p.tile_rows == 128 ? 7 : p.tile_rows == 64 ? 6 : 4;
     p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) >> p.row_shift);
-    const uint32_t groups = p.owns || a.head_dim <= 64 ? 512 : 256;
+    const bool three = tree && p.owns && a.head_dim <= 64 && tree_waves(a.type, attend_ks(a.head_dim), tile_rows / 64) == 3;
+    const uint32_t groups = three ? 768 : p.owns || a.head_dim <= 64 ? 512 : 256;
     p.stream = (groups + a.kv_heads - 1) / a.kv_heads;
     p.tile_tokens = tree ? a.tokens : p.tile_rows / G + 1; /* a tree's tile goes over all new tokens of its sequence */
     p.fixed = 64 * (PA_FIXED + 1);
@@ -542,7 +544,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     }
     most = 2 * most + p.fixed;
     p.unit = 0; /* all units and the last workgroup's end below 2^31 */
-    while (((uint64_t)(p.tiles + 512) * ((most >> p.unit) + 1)) >= 1u << 30) ++p.unit;
+    while (((uint64_t)(p.tiles + max(groups, 512u)) * ((most >> p.unit) + 1)) >= 1u << 30) ++p.unit;
     p.cw = (uint32_t)(most >> p.unit) + 1;
     p.c1 = tree ? 0 : 2 * p.tile_rows / G >> p.unit;
     /* tiles of an even batch, the steps of the longest and of the mean */
@@ -550,7 +552,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
     if (p.owns && tiles > 256) {
         const uint64_t average = steps - (a.window || tree ? 0 : min(rows / G / seqs / 64, steps / 2));
-        if (tiles >= 512 || average * (512 - tiles) / 256 <= 24) p.stream = 0;
+        if (tiles >= groups || average * (groups - tiles) / 256 <= 24) p.stream = 0;
     } else if (tiles >= groups || steps * (groups - tiles) / groups <= (tree && p.owns ? 10u : 24u)) {
         p.stream = 0;
     }
@@ -585,12 +587,15 @@ uint32_t tree_rows(const PagedArgs &a) {
     double reach = a.limit;
     if (a.window) reach = min(reach, (double)a.window + a.sinks + a.tokens);
     const double steps = reach / PA_STEP + 1;
-    /* by type, of one 32-wide step: tiles of 16 rows (and where heads are of 128), of 64, of 128. Q8 tiles convert a step once,
-     * whatever their rows, and then each wave has its part: their rates and those of its waves' 16 and 32 rows. */
+    /* Of one 32-wide step, by type, heads of up to 64 first: tiles of 16 rows (and where heads are of 128), of 64, of 128. A
+     * tile brings a step (and converts Q8 codes) once, whatever its rows, and then each wave has its part: the tiles' rates
+     * and those of their waves' 16 and 32 rows, where one for both is not as good (measured over 300 batches, the choice costs
+     * 1 % of the best tile's time on average, f32 2.5 %). */
     constexpr double NONE = HUGE_VAL;
-    static const double rate[3][6] = {
-        {1050, 1050, 510, NONE, 270, NONE}, {1900, 1900, 1300, NONE, 1080, NONE}, {2540, 1580, 3480, 4400, 1700, 2400}};
-    const double *r = rate[a.type], unit = seqs * a.kv_heads * steps * ks;
+    static const double rate[2][3][6] = {
+        {{1020, 1020, 1110, 3180, 1270, 1000}, {2410, 2410, 4570, 8330, 6000, 3500}, {2800, 2800, 1950, 8820, 1090, 2980}},
+        {{1050, 1050, 510, NONE, 270, NONE}, {1900, 1900, 1300, NONE, 1080, NONE}, {2540, 1580, 3480, 4400, 1700, 2400}}};
+    const double *r = rate[ks > 2][a.type], unit = seqs * a.kv_heads * steps * ks;
     const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = unit * ceil(each / 16) / r[ks == 4];
     const double t16 = min(7 + max(chain, fill), 13 + fill);
     const double t64 = 15 + max(unit * (ceil(each / 64) / r[2] + ceil(each / 16) / r[3]), 3.0 * ks);

@@ -80,6 +80,8 @@ hipError_t launch_attend(const PagedArgs &a, const TreeArgs &t, const AttendPlan
  * chunks of 500 at 3000, 32 heads on 8: f16 0.42 and 0.41 ms, Q8 0.74 and 0.75). */
 constexpr uint32_t attend_rt(uint32_t ks) { return ks <= 4 ? 2 : 1; }
 constexpr int attend_waves(uint32_t ks) { return ks == 8 ? 1 : 2; }
+/* Three of a tree whose heads have up to 64 dims: its tiles need no more than 168 registers, but for 177 of Q8 ones of 128 rows. */
+constexpr int tree_waves(uint32_t type, uint32_t ks, uint32_t rt) { return ks == 1 || (ks == 2 && (rt == 1 || type != 2)) ? 3 : attend_waves(ks); }
 constexpr uint32_t attend_ks(uint32_t hd) { return hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : hd <= 128 ? 4 : 8; }
 
 #ifdef SMQ_ATTEND_KERNELS
@@ -1395,7 +1397,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
     attend_piece<TYPE, KS, RT, OWNS, SMALL, false>(a, TreeArgs{}, q, att, p, used, part);
 }
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
-__global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_tree(PagedArgs a, TreeArgs tree, const float *q,
+__global__ __launch_bounds__(64 * PA_WAVES, tree_waves(TYPE, KS, RT)) void k_paged_tree(PagedArgs a, TreeArgs tree, const float *q,
                                                                                 float *att, AttendPlan p, i4 *used, float *part) {
     attend_piece<TYPE, KS, RT, OWNS, SMALL, true>(a, tree, q, att, p, used, part);
 }
