@@ -514,8 +514,9 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
 
 /* The pieces that tiles of so many rows are cut into: two a CU for products and for decoding heads of up to 64 (8 KiB of f16
  * a step and wave), one a CU for wider ones (one f16 sequence at 16384, 8 KV heads of 128: 22 us, two a CU 25); by_piece has
- * what becomes of these numbers. Three a CU for products of trees whose registers leave room (8 drafts of 63 at 8000, 32 heads
- * on 8 of 64, tiles of 64 rows: f16 104 -> 73 us, Q8 178 -> 105, f32 391 -> 225; 24 of 8 at 3001 38 -> 33, 53 -> 41, 88 -> 68).
+ * what becomes of these numbers. Three a CU for products of trees whose registers leave room (tiles of 64
+ * rows, 32 heads on 8, 8 drafts of 63 at 8000: heads of 64 f16 104 -> 71 us, Q8 178 -> 105, f32 391 -> 225, of 128 f16 176 ->
+ * 115, Q8 304 -> 168; 24 of 8 at 3001, heads of 128: 60 -> 52, 80 -> 58).
  *
  * Cutting costs partial results and a second launch, which joins them. No cuts
  * - where the longest tile exceeds an equal share by about 24 steps or less (64 sequences at 700, 2 KV heads of 64: 11.8 us
@@ -523,7 +524,9 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
  *   drafts of 40 Q8 tokens at 700, 2 KV heads of 128: 46 whole, 40 cut; at 300 27 and 32);
  * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
  *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
- *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). */
+ *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). With three a CU, whole
+ *   f16 tiles of trees stay ahead for longer (24 drafts of 40 at 3001, 576 tiles of 8 KV heads of 128: 100 us whole, 124 cut; of
+ *   96, 384 tiles 87 whole, 74 cut), Q8 and f32 ones not (198 whole, 157 cut). */
 AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, bool tree) {
     AttendPlan p;
     const uint32_t G = a.heads / a.kv_heads;
@@ -532,7 +535,8 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     p.tile_rows = tile_rows;
     p.row_shift = p.tile_rows == 128 ? 7 : p.tile_rows == 64 ? 6 : 4;
     p.tiles = (uint32_t)((rows + seqs * (p.tile_rows - 1)) >> p.row_shift);
-    const bool three = tree && p.owns && a.head_dim <= 64 && tree_waves(a.type, attend_ks(a.head_dim), tile_rows / 64) == 3;
+    const uint32_t ks = attend_ks(a.head_dim);
+    const bool three = tree && p.owns && ks <= 4 && tree_waves(a.type, ks, tile_rows / 64) == 3;
     const uint32_t groups = three ? 768 : p.owns || a.head_dim <= 64 ? 512 : 256;
     p.stream = (groups + a.kv_heads - 1) / a.kv_heads;
     p.tile_tokens = tree ? a.tokens : p.tile_rows / G + 1; /* a tree's tile goes over all new tokens of its sequence */
@@ -552,7 +556,7 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
     if (p.owns && tiles > 256) {
         const uint64_t average = steps - (a.window || tree ? 0 : min(rows / G / seqs / 64, steps / 2));
-        if (tiles >= groups || average * (groups - tiles) / 256 <= 24) p.stream = 0;
+        if (tiles >= groups || average * (groups - tiles) / 256 <= (three && a.type == 1 ? 72 : 24)) p.stream = 0;
     } else if (tiles >= groups || steps * (groups - tiles) / groups <= (tree && p.owns ? 10u : 24u)) {
         p.stream = 0;
     }
@@ -575,12 +579,12 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
  *
  *                        16 rows   64   128                            16 rows   64   128
  *   q8  24 x 40 at 300        30   25    25      f16  8 x 16 at  700        19   25    28
- *               at 700        51   37    40                  at 2000        37   29    32
- *               at 3001      126   75    72      f16 64 x  8 at 2000       137   99    99
- *   f16 24 x 40 at 700        47   31    33      f16  8 x 63 at 16384      811  435   240
- *               at 1500       76   38    39      q8   8 x 16 at 1500        18   20    23 (14 heads on 2 of 64)
- *   f32 24 x 40 at 3001      246  157   156      q8  24 x  8 at 3001        98   74    91
- *                                                f32  8 x 16 at 2000        66   52    79 */
+ *               at 700        50   36    40                  at 2000        37   31    32
+ *               at 3001      126   67    73      f16 64 x  8 at 2000       138   98    98
+ *   f16 24 x 40 at 700        47   32    33      f16  8 x 63 at 16384      812  285   239
+ *               at 1500       75   37    39      q8   8 x 16 at 1500        18   21    23 (14 heads on 2 of 64)
+ *   f32 24 x 40 at 3001      247  157   156      q8  24 x  8 at 3001        98   58    91
+ *                                                f32  8 x 16 at 2000        66   52    78 */
 uint32_t tree_rows(const PagedArgs &a) {
     const double ks = attend_ks(a.head_dim), rows = (double)a.tokens * (a.heads / a.kv_heads);
     const double seqs = a.seqs < a.tokens ? a.seqs : a.tokens, each = rows / seqs;
@@ -589,12 +593,11 @@ uint32_t tree_rows(const PagedArgs &a) {
     const double steps = reach / PA_STEP + 1;
     /* Of one 32-wide step, by type, heads of up to 64 first: tiles of 16 rows (and where heads are of 128), of 64, of 128. A
      * tile brings a step (and converts Q8 codes) once, whatever its rows, and then each wave has its part: the tiles' rates
-     * and those of their waves' 16 and 32 rows, where one for both is not as good (measured over 300 batches, the choice costs
-     * 1 % of the best tile's time on average, f32 2.5 %). */
-    constexpr double NONE = HUGE_VAL;
+     * and those of their waves' 16 and 32 rows. Fitted to 351 batches and tried on 194 others: the choice costs 1 and 2 % of the
+     * best tile's time on average. */
     static const double rate[2][3][6] = {
-        {{1020, 1020, 1110, 3180, 1270, 1000}, {2410, 2410, 4570, 8330, 6000, 3500}, {2800, 2800, 1950, 8820, 1090, 2980}},
-        {{1050, 1050, 510, NONE, 270, NONE}, {1900, 1900, 1300, NONE, 1080, NONE}, {2540, 1580, 3480, 4400, 1700, 2400}}};
+        {{1060, 1060, 870, 4050, 1050, 1080}, {2740, 2740, 3140, 12100, 5600, 3850}, {2800, 2800, 1910, 9100, 820, 6280}},
+        {{1050, 1070, 710, 5800, 320, 4400}, {2480, 1890, 2190, 52000, 2290, 7560}, {2640, 1880, 3890, 5200, 1800, 2750}}};
     const double *r = rate[ks > 2][a.type], unit = seqs * a.kv_heads * steps * ks;
     const double chain = steps / 4 * (1.0 + 0.19 * ks), fill = unit * ceil(each / 16) / r[ks == 4];
     const double t16 = min(7 + max(chain, fill), 13 + fill);

@@ -80,8 +80,12 @@ hipError_t launch_attend(const PagedArgs &a, const TreeArgs &t, const AttendPlan
  * chunks of 500 at 3000, 32 heads on 8: f16 0.42 and 0.41 ms, Q8 0.74 and 0.75). */
 constexpr uint32_t attend_rt(uint32_t ks) { return ks <= 4 ? 2 : 1; }
 constexpr int attend_waves(uint32_t ks) { return ks == 8 ? 1 : 2; }
-/* Three of a tree whose heads have up to 64 dims: its tiles need no more than 168 registers, but for 177 of Q8 ones of 128 rows. */
-constexpr int tree_waves(uint32_t type, uint32_t ks, uint32_t rt) { return ks == 1 || (ks == 2 && (rt == 1 || type != 2)) ? 3 : attend_waves(ks); }
+/* Of a tree's tiles three where 168 registers hold them: of 64 rows all but f32 ones of 128 dims, of 128 rows those of up to 64
+ * dims but Q8's 177. */
+constexpr int tree_waves(uint32_t type, uint32_t ks, uint32_t rt) {
+    const bool three = rt == 1 ? ks <= 3 || (ks == 4 && type != 0) : ks == 1 || (ks == 2 && type != 2);
+    return three ? 3 : attend_waves(ks);
+}
 constexpr uint32_t attend_ks(uint32_t hd) { return hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : hd <= 128 ? 4 : 8; }
 
 #ifdef SMQ_ATTEND_KERNELS
@@ -1357,7 +1361,7 @@ __device__ __forceinline__ void tile_part(const PagedArgs &a, const TreeArgs &tr
         u1 = st.total * (t.piece + 1) / t.pieces;
     }
     if constexpr (OWNS) {
-        if (n > 16) {
+        if (n > 16 || (TREE && RT == 1 && KS <= 4)) { /* tile_shared would take the registers of a third wave */
             tile_owned<TYPE, KS, RT, SMALL, TREE>(a, tree, q, t.sq, t.seq, st, u0, u1, wave, out, lds);
             return;
         }
@@ -1397,7 +1401,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, attend_waves(KS)) void k_paged_atten
     attend_piece<TYPE, KS, RT, OWNS, SMALL, false>(a, TreeArgs{}, q, att, p, used, part);
 }
 template <uint32_t TYPE, int KS, int RT, bool OWNS, bool SMALL>
-__global__ __launch_bounds__(64 * PA_WAVES, tree_waves(TYPE, KS, RT)) void k_paged_tree(PagedArgs a, TreeArgs tree, const float *q,
+__global__ __launch_bounds__(64 * PA_WAVES, OWNS ? tree_waves(TYPE, KS, RT) : attend_waves(KS)) void k_paged_tree(PagedArgs a, TreeArgs tree, const float *q,
                                                                                 float *att, AttendPlan p, i4 *used, float *part) {
     attend_piece<TYPE, KS, RT, OWNS, SMALL, true>(a, tree, q, att, p, used, part);
 }
