@@ -28,7 +28,7 @@
  * TREE: the new tokens see each other by a mask and the context as ever. A step that ends before the new tokens is seen whole as
  * a causal one is; in the others each lane takes its 8 positions' bits out of two words of its row's mask. Every tile goes over
  * all new tokens of its sequence. 8 f16 sequences of 63 drafts at up to 16384, 32 heads on 8 of 128: 238 us, 0.86 PFLOP/s of
- * products with remainders; 24 Q8 ones of 40 at up to 3001, 12 heads on 2: 75 us. */
+ * products with remainders; 24 Q8 ones of 40 at up to 3001, 12 heads on 2: 66 us. */
 #ifndef SMQ_PAGED_ATTEND_H
 #define SMQ_PAGED_ATTEND_H
 
