@@ -386,6 +386,27 @@ def test_tree_attention_of_many(kv_type):
 
 
 @pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("heads,hd,page,window,sinks", [(6, 128, 64, 0, 0), (12, 96, 16, 0, 0), (6, 64, 32, 0, 0), (6, 128, 16, 900, 5),
+                                                       (12, 128, 16, 2500, 5)])
+def test_tree_attention_of_ragged_drafts(kv_type, heads, hd, page, window, sinks):
+    """Tiles that waves own, cut into pieces, with sequences of a token or two between those of many: last tiles of few rows."""
+    kv = 1
+    new = [40, 1, 2, 33, 16, 0, 24, 3, 40, 1, 17, 30]
+    cache = Cache(kv_type, kv, hd, page, [3001 - 97 * s for s in range(12)], stale="nan").upload()
+    batch = Batch(cache, new, padding=1)
+    trees = Trees(batch).upload()
+    q = synth.normal(97, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    want, tol = ref.tree64(cache, batch, q, heads, trees.depth, trees.seen, window, sinks)
+    n = int(batch.begin[-1])
+    got = tree_attend(cache, batch, q, heads, trees, window, sinks)
+    close(got[:n], want[:n], tol[:n])
+    assert (got[n:] == 9.0).all()
+    same(tree_attend(cache, batch, q, heads, trees, window, sinks), got)
+    close(tree_attend(cache, batch, q, heads, trees, window, sinks, split=False)[:n], want[:n], tol[:n])
+    smq.numeric_check()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
 @pytest.mark.parametrize("length,new,page,kind", [(1107, 1100, 16, "tree"), (640, 640, 64, "any")])
 def test_tree_attention_of_many_drafts(kv_type, length, new, page, kind):
     """Masks of many words, which steps of 32 positions meet anywhere; a context shorter than a step, and none."""
