@@ -524,9 +524,14 @@ __global__ __launch_bounds__(JOIN_WG) void k_paged_join(PagedArgs a, float *att,
  *   drafts of 40 Q8 tokens at 700, 2 KV heads of 128: 46 whole, 40 cut; at 300 27 and 32);
  * - where tiles that waves own, which keep two workgroups a CU busy, are 512 or more (2048 tokens of 8 KV heads of 128, 512
  *   tiles, from an empty cache: 100 us whole, 115 cut). Between one and two a CU some CUs have twice the others' work: cut
- *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). With three a CU, whole
- *   f16 tiles of trees stay ahead for longer (24 drafts of 40 at 3001, 576 tiles of 8 KV heads of 128: 100 us whole, 124 cut; of
- *   96, 384 tiles 87 whole, 74 cut), Q8 and f32 ones not (198 whole, 157 cut). */
+ *   unless the tiles' mean is short (2 x 800 tokens at 4000, 8 KV heads of 128: 260 us whole, 210 cut). A tree's tiles with
+ *   three a CU are cut up to 768 of them, f16 ones, which stay ahead whole for longer, from 72 steps beside an equal share on
+ *   (96 dims, 525 tiles of 29 steps 35 us whole, 53 cut; 528 of 220 steps 220 and 166). Heads above 96: f16
+ *   ones gain nothing where two a CU are full (64 drafts of 8 at 4096, 32 heads on 8 of 128, 512 tiles: 181 whole, 197 cut; at
+ *   16384 680 and 684; but 35 of 15 at 7803, 8 heads of 128, 280 tiles, 292 and 166). Q8 ones do, from 36 steps on (64 of 8 at
+ *   4096 223 whole, 180 cut; at 16384 852 and 641; 24 of 40 at 3001 198 and 157; but 290 of 62 at 1538, 2 heads of 112, 116
+ *   and 123), from 116 where tiles have few rows, whose steps leave the CU to others (170 of 27 at 5665, 4 heads of 128, 310
+ *   whole, 339 cut; but 64 of 7 at 4987, 8 heads, 219 and 186). */
 AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, bool tree) {
     AttendPlan p;
     const uint32_t G = a.heads / a.kv_heads;
@@ -556,7 +561,14 @@ AttendPlan plan_tiles(const PagedArgs &a, size_t ws_bytes, uint32_t tile_rows, b
     const uint64_t steps = (most - p.fixed) / 2 / PA_STEP;
     if (p.owns && tiles > 256) {
         const uint64_t average = steps - (a.window || tree ? 0 : min(rows / G / seqs / 64, steps / 2));
-        if (tiles >= groups || average * (groups - tiles) / 256 <= (three && a.type == 1 ? 72 : 24)) p.stream = 0;
+        /* the longest tile exceeds an equal share of so many workgroups by more than `least` steps */
+        auto over = [&](uint32_t full, uint32_t least) { return tiles < full && average * (full - tiles) / 256 > least; };
+        const bool few = rows * a.kv_heads <= 32 * tiles; /* half of a tile's waves, or more, have no rows */
+        const bool cut = !three       ? over(512, 24)
+                         : ks < 4     ? over(768, a.type == 1 ? 72 : 24)
+                         : a.type == 1 ? over(512, 24) && over(768, 72)
+                                       : over(512, 24) || over(768, few ? 116 : 36);
+        if (!cut) p.stream = 0;
     } else if (tiles >= groups || steps * (groups - tiles) / groups <= (tree && p.owns ? 10u : 24u)) {
         p.stream = 0;
     }
@@ -664,9 +676,10 @@ size_t paged_attention_workspace(const PagedArgs &given, bool tree) {
         return p.stream ? attend_used_bytes(a, p) + p.pieces * attend_piece_bytes(a, p.tile_rows) : 0;
     };
     if (!tree) return bytes(attend_plan(a, ~(size_t)0, false));
-    size_t most = 0; /* the call brings the cache's type too: any of the tiles */
-    for (uint32_t rows = 16; rows <= 64 * attend_rt(attend_ks(a.head_dim)); rows *= rows == 16 ? 4 : 2)
-        most = max(most, bytes(plan_tiles(a, ~(size_t)0, rows, true)));
+    size_t most = 0; /* the call brings the cache's type too: any of the tiles, with any type's workgroups a CU */
+    for (a.type = 0; a.type <= 2; ++a.type)
+        for (uint32_t rows = 16; rows <= 64 * attend_rt(attend_ks(a.head_dim)); rows *= rows == 16 ? 4 : 2)
+            most = max(most, bytes(plan_tiles(a, ~(size_t)0, rows, true)));
     return most;
 }
 

@@ -386,7 +386,36 @@ def widest_split():
     assert cut > 150
 
 
-CASES = [valid_calls, empty_batches, shapes, buffers, forks, beams, beam_workspace_of_the_largest_step, captures, widest_split]
+def widest_split_of_many_tiles():
+    """The same where tiles of 64 rows number 512 to 767, whole for one type of cache and cut for another."""
+    cut = set()
+    for kv_type, (heads, kv, hd, seqs, new, window, context) in itertools.product((0, 1, 2), (
+            (32, 8, 128, 64, 8, 0, 4096), (32, 8, 128, 80, 8, 0, 8192), (32, 8, 128, 72, 16, 0, 3001), (32, 8, 128, 70, 16, 0, 16384),
+            (28, 4, 128, 128, 8, 0, 4096), (32, 8, 64, 16, 63, 0, 8192), (12, 2, 128, 300, 8, 0, 4000), (24, 8, 112, 70, 16, 3000, 9000),
+            (24, 8, 96, 72, 20, 0, 8000), (16, 8, 256, 70, 30, 0, 8000))):
+        p = Drafts(heads=heads, kv=kv, hd=hd, pairs=0, type=kv_type, page=64, pages=1, seqs=seqs, tokens=seqs * new,
+                   window=window, context=context, words=2)
+        p.batch.table_stride = -(-context // 64)
+        p.b["table"] = smq.DeviceBuffer(4 * seqs * p.batch.table_stride)
+        p.batch.table = p.b["table"].ptr
+        need = smq.load().smq_paged_tree_attention_workspace(p.batch, p.shape)
+        large = smq.DeviceBuffer(1 << 31)
+        for sinks in (0, 100, TOP):
+            got = []
+            for n in (large.nbytes, need):
+                fake.fake_clear()
+                smq.paged_tree_attention(p.b["q"], p.b["att"], p.batch, p.shape, sinks, p.b["depth"], p.b["mask"], 2, p.kv,
+                                         large.at(0) if n else None, n)
+                got.append(base.grids())
+            assert got[0] == got[1], (kv_type, heads, kv, hd, seqs, new, window, context, sinks, need, got)
+            if len(got[0]) == 2:
+                cut.add((kv_type, heads, kv, seqs, new))
+        large.free()
+    assert {(2, 32, 8, 64, 8), (2, 32, 8, 80, 8), (2, 28, 4, 128, 8), (2, 12, 2, 300, 8), (0, 24, 8, 72, 20)} <= cut, cut
+
+
+CASES = [valid_calls, empty_batches, shapes, buffers, forks, beams, beam_workspace_of_the_largest_step, captures, widest_split,
+         widest_split_of_many_tiles]
 
 if __name__ == "__main__":
     base.load(sys.argv[1])
