@@ -544,8 +544,8 @@ smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape 
  * held_out[d] = ceil(room[d] / page_size); entries behind it are -1. copies:
  * three words a row, the page copied from and to and its positions; -1, -1, 0
  * where nothing is to be copied. free_out: the pages free afterwards; negative
- * where so many were missing: then the numeric flag is raised, entries without
- * a page are -1, and the old arrays still hold.
+ * where so many were missing (-2^31: so many or more): then the numeric flag is
+ * raised, entries without a page are -1, and the old arrays still hold.
  *
  * Raise the flag as well: held, keep or room outside the table's row (cut), a
  * keep above the parent's pages (cut) or above room (room is raised), a parent

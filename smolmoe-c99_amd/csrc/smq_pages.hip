@@ -40,14 +40,14 @@ __device__ __forceinline__ uint32_t old_held(const ForkArgs &a, uint32_t s, bool
     if (flag && (held < 0 || held > (int)a.table_stride)) *a.flag = 1;
     return (uint32_t)min(max(held, 0), (int)a.table_stride);
 }
-template <uint32_t WAVES>
-__device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t *lds) {
+template <uint32_t WAVES, typename T>
+__device__ __forceinline__ T block_sum(T x, T *lds) {
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) x += __shfl_xor(x, off);
     __syncthreads();
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
     __syncthreads();
-    uint32_t t = 0;
+    T t = 0;
 #pragma unroll
     for (uint32_t w = 0; w < WAVES; ++w) t += lds[w];
     return t;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(PG_WG) void k_fork_rows(ForkArgs a, ForkSpace w, ui
     bool lower = false;
     if (last >= 0)
         for (uint32_t i = tid; i < d; i += PG_WG) lower = lower || w.last[i] == last;
-    const uint32_t any = block_sum<PG_WG / 64>(lower, lds);
+    const uint32_t any = block_sum<PG_WG / 64>((uint32_t)lower, lds);
     if (tid == 0) {
         const bool mine = last >= 0 && !any && holders_of(a, w, (uint32_t)last, false) == 0;
         w.from[d] = r.full + mine;
@@ -329,8 +329,10 @@ __global__ __launch_bounds__(PG_WG) void k_fork_rows(ForkArgs a, ForkSpace w, ui
 }
 
 /* A workgroup per new row: its entries. Its fresh pages are the free ones of the numbers that the rows before it leave off at:
- * the chunk where they begin, then the words of eight chunks at a time. */
+ * the chunk where they begin, then the words of eight chunks at a time. What the rows need is summed in 64 bits (65535 of 2^20
+ * entries); numbers past the free pages are all alike. */
 __global__ __launch_bounds__(PG_WG) void k_fork_assign(ForkArgs a, ForkSpace w, uint32_t chunks) {
+    __shared__ unsigned long long wide[PG_WG / 64];
     __shared__ uint32_t lds[PG_WG / 64], begin[2];
     const uint32_t tid = threadIdx.x, d = blockIdx.x;
     const bool row_there = d < a.seqs;
@@ -354,14 +356,14 @@ __global__ __launch_bounds__(PG_WG) void k_fork_assign(ForkArgs a, ForkSpace w, 
     const bool copies = last >= 0 && from == r.full;
     bool copied = false;
     if (need || d == 0) {
-        uint32_t before = 0, sum = 0;
-        for (uint32_t i = tid; i < (d == 0 ? a.seqs : d); i += PG_WG) before += w.need[i];
-        before = block_sum<PG_WG / 64>(before, lds);
-        const uint32_t all = before;
-        if (d == 0) before = 0;
+        unsigned long long needed = 0; /* by the rows before; row 0: by all */
+        uint32_t sum = 0;
+        for (uint32_t i = tid; i < (d == 0 ? a.seqs : d); i += PG_WG) needed += w.need[i];
+        needed = block_sum<PG_WG / 64>(needed, wide);
         const uint32_t each = (chunks + PG_WG - 1) / PG_WG, c0 = tid * each, c1 = min(c0 + each, chunks);
         for (uint32_t c = c0; c < c1; ++c) sum += w.chunk[c];
         uint32_t spare, at = block_scan<PG_WG / 64>(sum, lds, spare);
+        const uint32_t before = d == 0 ? 0 : (uint32_t)min(needed, (unsigned long long)spare);
         if (before >= at && before < at + sum) /* one thread, if any */
             for (uint32_t c = c0; c < c1; at += w.chunk[c++])
                 if (before < at + w.chunk[c]) {
@@ -370,8 +372,8 @@ __global__ __launch_bounds__(PG_WG) void k_fork_assign(ForkArgs a, ForkSpace w, 
                     break;
                 }
         if (d == 0 && tid == 0) {
-            *a.free_out = (int)(spare - all);
-            if (all > spare) *a.flag = 1;
+            *a.free_out = (int)max((long long)spare - (long long)needed, -(1ll << 31));
+            if (needed > spare) *a.flag = 1;
         }
         __syncthreads();
         const uint32_t end = min(before + need, spare), words = chunks * (PG_CHUNK / 32);

@@ -639,6 +639,35 @@ def test_fork_without_enough_pages(big):
     assert not flagged()
 
 
+@pytest.mark.parametrize("rows", [2100, 4200])
+def test_fork_that_needs_more_pages_than_32_bits_count(rows):
+    """2^31 and 2^32 entries without a page: as many as are free go to the first row, none is given twice."""
+    stride, page, pages = 1 << 20, 16, 9000
+    say("paged fork", rows, "rows of", stride)
+    top = stride * page
+    held, refs = dev(np.zeros(1, np.int32)), np.zeros(pages, np.int32)
+    refs[::3] = 1  # a store of prompts
+    bufs = [dev(np.full(stride, -1, np.int32)), held, dev(refs)] + [
+        dev(np.full(rows, x, np.int32)) for x in (-1, 0, top)]
+    outs = [smq.DeviceBuffer(4 * n) for n in (rows * stride, rows, pages, rows * 3, 1)]
+    f = smq.page_fork(*bufs[:3], 1, rows, stride, page, pages, *bufs[3:], *outs)
+    smq.paged_fork(f, smq.DeviceBuffer(smq.paged_fork_workspace(f)))
+    assert flagged()
+    free = np.nonzero(refs == 0)[0]
+    assert outs[4].download(np.int32)[0] == max(len(free) - rows * stride, -2 ** 31)
+    same(outs[2].download(np.int32), np.ones(pages, np.int32))
+    same(outs[1].download(np.int32), np.full(rows, stride, np.int32))
+    none = np.full(stride, -1, np.int32)
+    for r in (0, 1, 2047, 2048, 2049, 4095, 4096, 4097, rows - 1):
+        if r < rows:
+            want = none.copy()
+            if r == 0:
+                want[:len(free)] = free
+            same(outs[0].download(np.int32, stride, 4 * r * stride), want)
+    for b in outs:
+        b.free()
+
+
 def test_fork_of_what_is_not_valid():
     """Flagged and cut; every index stays in range, and the neighbours are as ever."""
     f = Forked(np.random.default_rng(5), 3, 1, [64, 50, 33], 16, 200, stride=8)
