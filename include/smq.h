@@ -518,7 +518,8 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
  * longer than accepted_stride, raises the numeric flag: the sequence stays as
  * it is, its length too. Positions without a place or page raise the flag and
  * are not moved. Sequences must not share a page that the call writes to. At
- * most SMQ_MAX_POOLS pools. Asynchronous, capturable. */
+ * most SMQ_MAX_POOLS pools; one that is named again counts once, others that
+ * share memory are refused. Asynchronous, capturable. */
 #define SMQ_MAX_POOLS 1024u
 smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,
                              uint32_t accepted_stride, const int32_t *count, const smq_paged_kv *pools, uint32_t n_pools,

@@ -7,6 +7,7 @@
  * error model: a status code plus a thread-local message (src/util.c:24-61).
  */
 #include <hip/hip_runtime.h>
+#include <algorithm>
 
 #include <cstdarg>
 #include <cstdio>
@@ -1732,6 +1733,70 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
     return hip_ok(smq::launch_paged_attention(a, &t, q, att, workspace, workspace_bytes, g.cur), who) ? SMQ_OK : t_status;
 }
 
+/* One kind of array of several pools: where each begins, and the bytes of each. */
+struct PoolArrays {
+    uintptr_t at[SMQ_MAX_POOLS];
+    size_t bytes;
+    void sort(uint32_t n) { /* layers mostly ascend */
+        if (!std::is_sorted(at, at + n)) std::sort(at, at + n);
+    }
+    bool apart(uint32_t n) const {
+        for (uint32_t i = 1; i < n; ++i)
+            if (at[i] - at[i - 1] < bytes) return false;
+        return true;
+    }
+    bool apart(const PoolArrays &o, uint32_t n) const {
+        for (uint32_t i = 0, j = 0; i < n && j < n; at[i] < o.at[j] ? ++i : ++j)
+            if (overlap((const void *)at[i], bytes, (const void *)o.at[j], o.bytes)) return false;
+        return true;
+    }
+};
+/* No two pools share memory: two workgroups would move the same tokens. One that is named again has no part in the call, its
+ * keys are NULL; any other that shares a byte is refused. */
+static bool pools_apart(smq::Pool *p, uint32_t n, const smq::PagedArgs &a, const char *who) {
+    const size_t positions = (size_t)a.pages << a.shift, codes = positions * a.kv_heads * a.head_dim * (4u >> a.type),
+                 scales = positions * a.kv_heads * a.nb * 4;
+    const uint32_t kinds = a.type == SMQ_KV_Q8 ? 4 : 2;
+    /* the layers of one buffer for each kind, one after another: looked at once */
+    auto at = [](const smq::Pool &x, uint32_t k) { return (uintptr_t)(k == 0 ? x.keys : k == 1 ? x.values : k == 2 ? x.ks : x.vs); };
+    bool plain = true;
+    for (uint32_t k = 0; k < kinds; ++k) {
+        const size_t bytes = k < 2 ? codes : scales;
+        for (uint32_t i = 1; i < n; ++i) plain = plain && at(p[i], k) >= at(p[i - 1], k) && at(p[i], k) - at(p[i - 1], k) >= bytes;
+        for (uint32_t j = 0; j < k; ++j)
+            plain = plain && (at(p[n - 1], k) + bytes <= at(p[0], j) || at(p[n - 1], j) + (j < 2 ? codes : scales) <= at(p[0], k));
+    }
+    if (plain) return true;
+    auto same = [&](const smq::Pool &x, const smq::Pool &y) {
+        return x.keys == y.keys && x.values == y.values && (kinds == 2 || (x.ks == y.ks && x.vs == y.vs));
+    };
+    uint16_t order[SMQ_MAX_POOLS];
+    auto before = [&](uint16_t i, uint16_t j) { return p[i].keys != p[j].keys ? p[i].keys < p[j].keys : i < j; };
+    for (uint32_t i = 0; i < n; ++i) order[i] = (uint16_t)i;
+    if (!std::is_sorted(order, order + n, before)) std::sort(order, order + n, before);
+    PoolArrays of[4];
+    uint32_t m = 0, last = 0; /* different ones, the last of them */
+    bool fine = true;
+    for (uint32_t i = 0; i < n; ++i) {
+        smq::Pool &x = p[order[i]];
+        if (m && same(x, p[last])) {
+            x.keys = nullptr;
+            continue;
+        }
+        last = order[i];
+        for (uint32_t k = 0; k < kinds; ++k) of[k].at[m] = at(x, k);
+        ++m;
+    }
+    for (uint32_t k = 0; k < kinds; ++k) {
+        of[k].bytes = k < 2 ? codes : scales;
+        of[k].sort(m);
+        fine = fine && of[k].apart(m);
+        for (uint32_t j = 0; j < k; ++j) fine = fine && of[k].apart(of[j], m);
+    }
+    if (!fine) set_status(SMQ_ERR_RANGE, "%s: pools overlap", who);
+    return fine;
+}
+
 /* The pools of a call that goes over all layers: alike, and of a's shape. */
 static bool pool_args(const smq_paged_kv *pools, uint32_t n, const char *who, const smq::PagedArgs *a, smq::Pool *out) {
     if (n > SMQ_MAX_POOLS) {
@@ -1753,7 +1818,7 @@ static bool pool_args(const smq_paged_kv *pools, uint32_t n, const char *who, co
         if (!pool_extents(one, who, in)) return false;
         out[i] = {p.keys, p.values, p.key_scales, p.value_scales};
     }
-    return true;
+    return pools_apart(out, n, *a, who);
 }
 
 smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,

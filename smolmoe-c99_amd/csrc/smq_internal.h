@@ -318,7 +318,7 @@ struct ForkArgs {
     uint32_t old_seqs, seqs, table_stride, shift, pages;
     int *flag;
 };
-struct Pool {
+struct Pool { /* keys null: another one is the same pool */
     void *keys, *values;
     float *ks, *vs;
 };

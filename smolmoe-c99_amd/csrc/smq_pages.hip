@@ -480,6 +480,7 @@ __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, 
     }
     const uint32_t EB = 4 >> a.type;
     const Pool &p = pools.p[l];
+    if (!p.keys) return;
     const size_t f = (size_t)from * a.kv_heads + h, t = (size_t)to * a.kv_heads + h;
     char *x = (char *)(kind ? p.values : p.keys), *w = (char *)(kind ? p.vs : p.ks);
     const size_t head = ((size_t)a.head_dim << a.shift) * EB, scales = ((size_t)a.nb << a.shift) * 4;
@@ -551,6 +552,7 @@ __global__ __launch_bounds__(PG_WG) void k_paged_compact(PagedArgs a, Pools pool
     typedef typename Element<EB>::T T;
     const uint32_t tid = threadIdx.x, h = blockIdx.x % a.kv_heads, y = blockIdx.x / a.kv_heads, s = y / pools.n;
     const Pool &p = pools.p[y % pools.n];
+    if (!p.keys) return; /* never the first pool, which writes length_out */
     const uint32_t kt = tid / 16, kx = tid % 16, vt = tid % 16, vx = tid / 16; /* token and part, of keys and of values */
     const int32_t *path = accepted + (size_t)s * stride;
     /* of the first round, requested with the count */

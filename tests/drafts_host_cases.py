@@ -227,6 +227,63 @@ def buffers():
     lib.smq_clear_error()
 
 
+def pools_that_share_memory():
+    """Refused, whichever kinds of arrays share a byte, in any order; a pool that is named again is not."""
+    for kv_type, codes in ((0, 4), (1, 2), (2, 1)):
+        p = Drafts(type=kv_type)
+        k, w = 20 * 32 * 2 * 64 * codes, 20 * 32 * 2 * 2 * 4  # bytes of keys, of their scales
+        room = smq.DeviceBuffer(40 * (k + w))
+        at = lambda i: [room.ptr + i * 2 * (k + w) + x for x in (0, k, 2 * k, 2 * k + w)]  # noqa: E731
+
+        def call(*arrays):
+            p.pools = smq.paged_pools([smq.paged_kv(*x, kv_type, 32, 20) for x in arrays])
+            fake.fake_clear()
+            p.copy()
+            p.compact()
+            assert launches() == 2
+
+        layers = [at(i) for i in range(12)]
+        call(*layers)
+        call(*layers[::-1])
+        call(*(layers[i] for i in (5, 0, 11, 2, 7, 3)))
+        call(*(layers[i] for i in (5, 0, 5, 11, 0, 0, 5)))
+        call(*([x[1], x[0], x[3], x[2]] if i % 2 else x for i, x in enumerate(layers)))
+        every = range(4 if kv_type == 2 else 2)
+        for i in every:
+            for j in every:
+                for off in (0, 16, -16):
+                    bad = [list(x) for x in layers]
+                    bad[9][i] = bad[4][j] + off
+                    if i != j or off:
+                        for f in (p.copy, p.compact):
+                            for order in (bad, bad[::-1]):
+                                p.pools = smq.paged_pools([smq.paged_kv(*x, kv_type, 32, 20) for x in order])
+                                refused(f, words="pools overlap")
+        for i in every:  # the keys of another pool, but not its values
+            bad = [list(x) for x in layers]
+            bad[9] = list(bad[4])
+            bad[9][i] = layers[9][i]
+            p.pools = smq.paged_pools([smq.paged_kv(*x, kv_type, 32, 20) for x in bad])
+            refused(p.compact, words="pools overlap")
+        # a run of layers for each kind
+        begin = [0, 12 * k, 24 * k, 24 * k + 12 * w]
+        run = lambda i, moved=-1, by=0: [room.ptr + 4096 + b + (by if n == moved else 0) + i * x  # noqa: E731
+                                         for n, (b, x) in enumerate(zip(begin, (k, k, w, w)))]
+        call(*(run(i) for i in range(12)))
+        for i in every:
+            for by in (16, -16):
+                if 0 <= i + (by > 0) - (by < 0) < len(every):  # into the next kind's run
+                    p.pools = smq.paged_pools([smq.paged_kv(*run(x, i, by), kv_type, 32, 20) for x in range(12)])
+                    refused(p.compact, words="pools overlap")
+            for n in (1, 11):
+                p.pools = smq.paged_pools([smq.paged_kv(*run(x, i if x == n else -1, -16), kv_type, 32, 20) for x in range(12)])
+                refused(p.compact, words="pools overlap")
+        if kv_type < 2:  # scales are not looked at
+            for x in layers:
+                x[2:] = layers[0][:2]
+            call(*layers)
+
+
 def fork(short=None, **kw):
     o = dict(old=5, seqs=7, stride=9, page=32, pages=60)
     o.update({k: v for k, v in kw.items() if k in o})
@@ -415,7 +472,7 @@ def widest_split_of_many_tiles():
 
 
 CASES = [valid_calls, empty_batches, shapes, buffers, forks, beams, beam_workspace_of_the_largest_step, captures, widest_split,
-         widest_split_of_many_tiles]
+         widest_split_of_many_tiles, pools_that_share_memory]
 
 if __name__ == "__main__":
     base.load(sys.argv[1])

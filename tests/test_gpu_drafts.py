@@ -762,6 +762,35 @@ def test_compact(kv_type, kv, hd, page, lengths, new, layers, kind):
     assert not flagged()
 
 
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+def test_pools_named_again_count_once(kv_type):
+    """Paths move, and pages are copied, once in a pool that is named several times, in one launch or two."""
+    caches = [Cache(kv_type, 2, 64, 32, [100, 70], seed=4) for _ in range(3)]
+    for i, c in enumerate(caches):
+        for x, _ in ref.pool_parts(c):
+            x[...] = np.roll(x, i, 0)
+        c.upload()
+    names = [0, 1, 0, 2, 2, 0] + [1] * 50 + [2, 0]
+    pools = smq.paged_pools([caches[i].desc for i in names])
+    batch = Batch(caches[0], [60, 50])
+    paths = [list(range(1, 60, 2)), [1, 2, 3, 5, 8, 13, 21, 34, 49]]
+    acc, out = np.zeros((2, 30), np.int32), smq.DeviceBuffer(8)
+    for s, p in enumerate(paths):
+        acc[s, :len(p)] = p
+        for c in caches:
+            ref.compact(c, s, (40, 20)[s], p)
+    shape = smq.attn_shape(2, 2, 64, 0, 0, 100)
+    smq.paged_compact(batch.desc, shape, dev(acc), 30, dev(np.array([30, 9], np.int32)), pools, out)
+    assert list(out.download(np.int32)) == [70, 29]
+    copies = np.array([[0, 5, 32], [1, 6, 17]], np.int32)
+    for c in caches:
+        ref.copy(c, copies)
+    smq.paged_copy(dev(copies), 2, shape, pools)
+    for c in caches:
+        pool_same(c)
+    assert not flagged()
+
+
 def test_compact_of_what_is_not_valid():
     """Lists that do not ascend, leave the draft or are too long: the sequence stays, the others are done."""
     for path, count in (([3, 3], 2), ([4, 2], 2), ([0, 20], 2), ([-1, 2], 2), ([1, 2], 4), ([1, 2], -1), ([1, 2], 2 ** 31 - 1)):
