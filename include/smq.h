@@ -513,10 +513,10 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
  * in every pool (the layers' caches: same type, page_size and pages): for k
  * below count[s] the keys and values of new token accepted[s * accepted_stride
  * + k] go to the place of new token k, as the cache holds them. length_out[s]
- * = the positions before the new tokens + count[s]; it must not overlap
- * length, accepted or count. A list that does not ascend strictly within the sequence's new tokens, or is
- * longer than accepted_stride, raises the numeric flag: the sequence stays as
- * it is, its length too. Positions without a place or page raise the flag and
+ * = the positions before the new tokens + count[s]; it must not overlap the
+ * batch's arrays, accepted or count. A list that does not ascend strictly
+ * within the sequence's new tokens, or is longer than accepted_stride, raises
+ * the numeric flag: the sequence stays as it is, its length too. Positions without a place or page raise the flag and
  * are not moved. Sequences must not share a page that the call writes to. At
  * most SMQ_MAX_POOLS pools; one that is named again counts once, others that
  * share memory are refused. Asynchronous, capturable. */

@@ -1835,12 +1835,10 @@ smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape 
     if (!accepted_stride || accepted_stride > (1u << 22))
         return set_status(SMQ_ERR_RANGE, "%s: an accepted_stride of %u of 1 .. 2^22", who, accepted_stride);
     const size_t n = (size_t)a.seqs * 4;
-    if (!extent_ok(a.begin, n + 4, "begin") || !extent_ok(a.length, n, "length") ||
-        !extent_ok(a.table, n * a.table_stride, "table") || !extent_ok(accepted, n * accepted_stride, "accepted") ||
-        !extent_ok(count, n, "count") || !extent_ok(length_out, n, "length_out"))
-        return t_status;
-    if (overlap(length_out, n, a.length, n) || overlap(length_out, n, count, n) || overlap(length_out, n, accepted, n * accepted_stride))
-        return set_status(SMQ_ERR_RANGE, "%s: length_out overlaps length, accepted or count", who);
+    const Range in[5] = {{a.begin, n + 4, "begin"}, {a.length, n, "length"}, {a.table, n * a.table_stride, "table"},
+                         {accepted, n * accepted_stride, "accepted"}, {count, n, "count"}},
+                to[1] = {{length_out, n, "length_out"}};
+    if (!ranges_ok(who, in, 5, to, 1)) return t_status;
     smq::Pool p[SMQ_MAX_POOLS];
     if (!pool_args(pools, n_pools, who, &a, p)) return t_status;
     return hip_ok(smq::launch_paged_compact(a, p, n_pools, accepted, accepted_stride, count, length_out, g.cur), who)

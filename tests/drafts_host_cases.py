@@ -227,6 +227,14 @@ def buffers():
     lib.smq_clear_error()
 
 
+def results_over_descriptors():
+    """What a call writes shares no byte with what its other workgroups read."""
+    p = Drafts()
+    for name in ("begin", "length", "table", "accepted", "count"):
+        for at in (p.b[name].ptr, p.b[name].ptr + p.b[name].nbytes - 12):
+            refused(lambda: p.compact(out=at), words="length_out overlaps " + name)
+
+
 def pools_that_share_memory():
     """Refused, whichever kinds of arrays share a byte, in any order; a pool that is named again is not."""
     for kv_type, codes in ((0, 4), (1, 2), (2, 1)):
@@ -472,7 +480,8 @@ def widest_split_of_many_tiles():
 
 
 CASES = [valid_calls, empty_batches, shapes, buffers, forks, beams, beam_workspace_of_the_largest_step, captures, widest_split,
-         widest_split_of_many_tiles, pools_that_share_memory]
+         widest_split_of_many_tiles, pools_that_share_memory,
+         results_over_descriptors]
 
 if __name__ == "__main__":
     base.load(sys.argv[1])
