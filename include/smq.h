@@ -489,8 +489,8 @@ smq_status smq_paged_norm_rope_kv(const smq_paged_rows *rows, const smq_paged_ba
  * raises the numeric flag and counts as negative. A sequence of more than
  * 32 * mask_stride new tokens raises the flag; its rows are left as they are,
  * as those of padding. mask_stride: 1 .. 128. One call serves the attention of
- * all layers. depth, mask and parent must not overlap. Asynchronous,
- * capturable. */
+ * all layers. depth and mask must not overlap each other, parent or begin.
+ * Asynchronous, capturable. */
 smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, int32_t *depth, uint32_t *mask,
                            uint32_t mask_stride);
 /* smq_paged_attention where a mask says which of its sequence's new tokens a

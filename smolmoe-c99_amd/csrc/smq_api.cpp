@@ -1698,11 +1698,9 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
     a.tokens = batch->tokens;
     a.flag = g.flag;
     const size_t n = (size_t)a.tokens * 4;
-    if (!extent_ok(a.begin, ((size_t)a.seqs + 1) * 4, "begin") || !extent_ok(parent, n, "parent") ||
-        !extent_ok(depth, n, "depth") || !extent_ok(mask, n * mask_stride, "mask"))
-        return t_status;
-    if (overlap(parent, n, depth, n) || overlap(parent, n, mask, n * mask_stride) || overlap(depth, n, mask, n * mask_stride))
-        return set_status(SMQ_ERR_RANGE, "%s: parent, depth and mask overlap", who);
+    const Range in[2] = {{a.begin, ((size_t)a.seqs + 1) * 4, "begin"}, {parent, n, "parent"}},
+                to[2] = {{depth, n, "depth"}, {mask, n * mask_stride, "mask"}};
+    if (!ranges_ok(who, in, 2, to, 2)) return t_status;
     return hip_ok(smq::launch_draft_masks(a, parent, depth, mask, mask_stride, g.cur), who) ? SMQ_OK : t_status;
 }
 

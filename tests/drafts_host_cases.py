@@ -233,6 +233,11 @@ def results_over_descriptors():
     for name in ("begin", "length", "table", "accepted", "count"):
         for at in (p.b[name].ptr, p.b[name].ptr + p.b[name].nbytes - 12):
             refused(lambda: p.compact(out=at), words="length_out overlaps " + name)
+    b, mask = p.b, p.b["mask"]
+    for out, args in (("depth", lambda at: (at, mask)), ("mask", lambda at: (b["depth"], at))):
+        big = smq.DeviceBuffer(4096)
+        p.batch.begin = big.at(12)
+        refused(lambda: smq.draft_masks(b["parent"], p.batch, *args(big), 2), words=out + " overlaps begin")
 
 
 def pools_that_share_memory():
