@@ -476,8 +476,8 @@ typedef struct smq_paged_rows {
  * rotation and the cache's rounding as smq_paged_rope_kv has them. Keys and
  * values go to the tokens' own places whatever their depth. A row whose rotary
  * position is outside [0, context) raises the numeric flag: its k is not
- * stored and its q not written. q_out must not overlap k, v or, but for in
- * place, q. Asynchronous, capturable. */
+ * stored and its q not written. q_out must not overlap what the call reads, but
+ * for q in place. Asynchronous, capturable. */
 smq_status smq_paged_norm_rope_kv(const smq_paged_rows *rows, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                   const float *cos_table, const float *sin_table, const smq_paged_kv *kv);
 /* Trees of drafted tokens: parent[r], for row r of the batch, is the index
@@ -503,8 +503,8 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
  * as smq_paged_attention's; a depth below 0 or where p is not below the
  * context's size raises the numeric flag, its row is 0, and so are those of a
  * sequence of more than 32 * mask_stride new tokens. All pages of the new
- * tokens must be pages. mask_stride: 1 .. 128. The workspace has a query of
- * its own. Asynchronous, capturable. */
+ * tokens must be pages. mask_stride: 1 .. 128. att must not overlap q, depth
+ * or mask. The workspace has a query of its own. Asynchronous, capturable. */
 size_t smq_paged_tree_attention_workspace(const smq_paged_batch *batch, const smq_attn_shape *shape);
 smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_batch *batch, const smq_attn_shape *shape,
                                     uint32_t sinks, const int32_t *depth, const uint32_t *mask, uint32_t mask_stride,

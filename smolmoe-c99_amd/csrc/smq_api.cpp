@@ -1724,10 +1724,9 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
     const size_t rows = (size_t)a.tokens * a.heads * a.head_dim * 4;
     if (!workspace) workspace_bytes = 0;
     if ((uintptr_t)workspace & 15) return set_status(SMQ_ERR_RANGE, "%s: the workspace must be 16-byte aligned", who);
-    if (!paged_extents(a, who) || !extent_ok(q, rows, "q") || !extent_ok(att, rows, "att") ||
-        !extent_ok(depth, depth ? (size_t)a.tokens * 4 : 0, "depth") ||
-        !extent_ok(mask, (size_t)a.tokens * mask_stride * 4, "mask") || !extent_ok(workspace, workspace_bytes, "workspace"))
-        return t_status;
+    const Range in[3] = {{q, rows, "q"}, {depth, depth ? (size_t)a.tokens * 4 : 0, "depth"}, {mask, (size_t)a.tokens * mask_stride * 4, "mask"}},
+                to[1] = {{att, rows, "att"}};
+    if (!paged_extents(a, who) || !ranges_ok(who, in, 3, to, 1) || !extent_ok(workspace, workspace_bytes, "workspace")) return t_status;
     return hip_ok(smq::launch_paged_attention(a, &t, q, att, workspace, workspace_bytes, g.cur), who) ? SMQ_OK : t_status;
 }
 

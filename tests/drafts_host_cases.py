@@ -238,6 +238,9 @@ def results_over_descriptors():
         big = smq.DeviceBuffer(4096)
         p.batch.begin = big.at(12)
         refused(lambda: smq.draft_masks(b["parent"], p.batch, *args(big), 2), words=out + " overlaps begin")
+    p = Drafts()
+    for name in ("q", "depth", "mask"):
+        refused(lambda: p.tree(**{name: p.b["att"].at(0 if name == "q" else 16)}), words="att overlaps " + name)
 
 
 def pools_that_share_memory():
