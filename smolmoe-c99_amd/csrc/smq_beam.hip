@@ -42,8 +42,9 @@ __device__ __forceinline__ double value_of(uint64_t v) { return __longlong_as_do
 
 /* e^x, x <= 0 (below -700, -infinity too, as at -700: nothing beside the largest term, 1): x log2 e to a whole number, which
  * the sum with 1.5 * 2^52 leaves in its low bits, and f in [-1/2, 1/2], whose 2^f is the polynomial with the least relative
- * error of its degree, 7.8e-13. 14 instructions on 64 bits, which run at the rate of those on 32. lead: the polynomial's first
- * coefficient, in vector registers (an instruction takes one scalar operand). */
+ * error of its degree, 7.8e-13 (a term may have 1e-12: one of these, not a product of two). 14 instructions on 64 bits, which
+ * run at the rate of those on 32. lead: the polynomial's first coefficient, in vector registers (an instruction takes one
+ * scalar operand). */
 constexpr double EXP_LEAD = 0x1.61af6ea7cb2d7p-20;
 __device__ __forceinline__ double exp_of(double x, double lead) {
     x = fmax(x, -700.0);
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(BM_WG) void k_beam_rows(BeamArgs a, Sums s, double 
     float l[4];
     uint32_t i = load(tid / BM_LANES, l);
     double sum = 0.0;
-    auto add = [&](const WaveSum &w) { sum += w.sum * exp_of(w.top - top, EXP_LEAD); };
+    auto add = [&](const WaveSum &w) { sum += w.sum * exp(w.top - top); }; /* a second exp_of would double its error */
 #pragma unroll
     for (uint32_t k = 0; k < ST; ++k) add(ws[k]);
     for (uint32_t i = tid + ST * BM_WG; i < s.sums; i += BM_WG) add(sum_row[i]);

@@ -944,6 +944,25 @@ def test_beam_of_what_is_not_finite():
     beam_check(base * np.float32(1e-42), score, 2, 2, 6)
 
 
+@pytest.mark.parametrize("d", [-0.4326171875, -1.65625])
+def test_beam_sums_are_within_their_bound(d):
+    """A row whose sum of exponentials is mostly one term, at a distance d from the largest of its 256 ids, which is at d from the
+    row's: where the exponential is furthest off. Each is within 1e-12 of its size, so that the sum's logarithm is within 1e-12;
+    64-bit sums and logarithms of this size add less than 1e-14, and the result, near 0, half an f32 step."""
+    vocab = 50000
+    logits = np.full((1, vocab), 2 * d, np.float32)
+    logits[0, ::256] = d
+    logits[0, :256] = -np.inf
+    logits[0, 0] = 0
+    lse = np.log(np.exp(logits[0].astype(np.longdouble)).sum())
+    score = np.array([lse], np.float32)
+    got = beam_call(logits, score, 1, 1, 1)
+    want = float(np.longdouble(score[0]) - lse)
+    assert got[0][0] == 0 and got[1][0] == 0 and abs(want) < 1e-6
+    assert abs(float(got[2][0]) - want) <= 1e-12 + 1e-14 + abs(want) * 2.0 ** -24
+    assert not flagged()
+
+
 def test_beam_histories_that_are_full():
     logits = synth.normal(42, 2 * 500, 3.0).reshape(2, 500)
     history = np.arange(20, dtype=np.uint32).reshape(2, 10)
