@@ -1059,6 +1059,49 @@ def test_drafts_together(kv_type):
         assert not flagged()
 
 
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+def test_drafts_on_a_shared_prompt(kv_type):
+    """Three sequences draft on one prompt that a store holds too: its last page, which they take in part, is copied to each
+    one's own before their tokens are stored, and stays what it was."""
+    heads, kv, hd, page, stride, keep, new = 6, 2, 64, 16, 6, 37, [9, 20, 1]
+    cache = Cache(kv_type, kv, hd, page, [keep], spare=40, stride=stride, stale="nan").upload()
+    refs = np.zeros(cache.pages, np.int32)
+    refs[cache.table[0, :3]] = 2  # the table's row and the store
+    room = np.array([keep + n for n in new], np.int32)
+    parent, kept = np.zeros(3, np.int32), np.full(3, keep, np.int32)
+    want = ref.fork(cache.table, [3], refs, parent, kept, room, page)
+    assert (want[3][:, 2] == 5).all() and want[2][cache.table[0, 2]] == 1
+    bufs = [dev(x) for x in (cache.table, np.array([3], np.int32), refs, parent, kept, room)]
+    outs = [smq.DeviceBuffer(4 * n) for n in (3 * stride, 3, cache.pages, 9, 1)]
+    f = smq.page_fork(*bufs[:3], 1, 3, stride, page, cache.pages, *bufs[3:], *outs)
+    smq.paged_fork(f, smq.DeviceBuffer(smq.paged_fork_workspace(f)))
+    for got, w in zip(outs, want[:4]):
+        same(got.download(np.int32), np.ravel(w))
+    shape = smq.attn_shape(heads, kv, hd, hd // 2, 0, 64)
+    smq.paged_copy(outs[3], 3, shape, smq.paged_pools([cache.desc]))
+    ref.copy(cache, want[3])
+    cache.table, cache.tb = want[0], outs[0]
+    batch = Batch(cache, new, lengths=room)
+    trees = Trees(batch).upload()
+    cos, sin = tables(64, hd // 2)
+    q, k, v = (synth.normal(400 + i, batch.tokens * x * hd, 1.5).reshape(-1, x, hd) for i, x in enumerate((heads, kv, kv)))
+    w = (1 + 0.2 * synth.normal(410, hd)).astype(np.float32)
+    rot = smq.DeviceBuffer(q.nbytes)
+    smq.paged_norm_rope_kv(smq.paged_rows(dev(q), rot, dev(k), dev(v), dev(w), dev(w), depth=trees.db), batch.desc, shape, dev(cos),
+                           dev(sin), cache.desc)
+    turn = keep + trees.depth
+    k = rotate(ref.normed(k, w, 1e-6), cos[turn], sin[turn], 32)
+    for s in range(3):
+        r = slice(batch.begin[s], batch.begin[s + 1])
+        cache.put(s, np.arange(keep, room[s]), k[r], v[r])
+    pool_same(cache)
+    q = rotate(ref.normed(q, w, 1e-6), cos[turn], sin[turn], 32)
+    same(rot.download(np.float32).reshape(q.shape), q)
+    want, tol = ref.tree64(cache, batch, q, heads, trees.depth, trees.seen)
+    close(tree_attend(cache, batch, q, heads, trees), want, tol)
+    assert not flagged()
+
+
 def test_beams_together():
     """A beam search of three prompts' beams over one pool: choice, fork, copy, store and attention of every step against a
     search that keeps each beam's tokens and works its attention out from them in 64 bits."""
