@@ -497,8 +497,11 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
  * row sees: of the positions before them (the context) all, with shape->window
  * w > 0 those with j > p - w or j < sinks, p = the context's positions +
  * depth[r] (not read where there is no window); of the new tokens those whose
- * bit is set, whatever the window, later ones too. mask as smq_draft_masks
- * writes it, or any other: bits behind the last new token do not matter. A row
+ * bit is set, whatever the window, later ones too (smq_draft_masks knows no
+ * window: where drafts reach as deep as one, the caller clears the bits of the
+ * ancestors w or more levels above that are no sinks, and a chain's attention
+ * is smq_paged_attention's). mask as smq_draft_masks writes it, or any other:
+ * bits behind the last new token do not matter. A row
  * that sees nothing is 0. Numbers, errors, workspace and what does not matter
  * as smq_paged_attention's; a depth below 0 or where p is not below the
  * context's size raises the numeric flag, its row is 0, and so are those of a
@@ -516,10 +519,11 @@ smq_status smq_paged_tree_attention(const float *q, float *att, const smq_paged_
  * = the positions before the new tokens + count[s]; it must not overlap the
  * batch's arrays, accepted or count. A list that does not ascend strictly
  * within the sequence's new tokens, or is longer than accepted_stride, raises
- * the numeric flag: the sequence stays as it is, its length too. Positions without a place or page raise the flag and
- * are not moved. Sequences must not share a page that the call writes to. At
- * most SMQ_MAX_POOLS pools; one that is named again counts once, others that
- * share memory are refused. Asynchronous, capturable. */
+ * the numeric flag: the sequence stays as it is, its length too. Positions
+ * without a place or page raise the flag and are not moved. Sequences must not
+ * share a page that the call writes to. At most SMQ_MAX_POOLS pools; one that
+ * is named again counts once, others that share memory are refused.
+ * Asynchronous, capturable. */
 #define SMQ_MAX_POOLS 1024u
 smq_status smq_paged_compact(const smq_paged_batch *batch, const smq_attn_shape *shape, const int32_t *accepted,
                              uint32_t accepted_stride, const int32_t *count, const smq_paged_kv *pools, uint32_t n_pools,

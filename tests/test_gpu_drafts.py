@@ -6,7 +6,7 @@ import torch
 
 import drafts_ref as ref
 from checks import assert_same_f32, say
-from paged_ref import F16, F32, Q8, Batch, Cache, rotate, tables
+from paged_ref import F16, F32, Q8, Batch, Cache, attend64, rotate, tables
 from smq_pkg import smq, synth
 
 pytestmark = pytest.mark.gpu
@@ -439,6 +439,31 @@ def test_tree_attention_of_a_causal_mask():
         att = smq.DeviceBuffer(q.nbytes)
         smq.paged_attention(dev(q), att, batch.desc, shape, sinks, cache.desc)
         close(got, att.download(np.float32).reshape(q.shape), 2 * tol)
+    smq.numeric_check()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("window,sinks", [(16, 4), (1, 0), (20, 70)])
+def test_tree_attention_of_chains_deeper_than_the_window(kv_type, window, sinks):
+    """A window does not clear the mask's bits: where those of the ancestors that it leaves behind are cleared, but for sinks, a
+    chain's attention is smq_paged_attention's with that window."""
+    heads, kv, hd = 8, 2, 64
+    cache = Cache(kv_type, kv, hd, 32, [300, 90, 45]).upload()
+    batch = Batch(cache, [40, 90, 45])
+    trees = Trees(batch)
+    trees.depth = np.concatenate([np.arange(n) for n in batch.new]).astype(np.int32)
+    chain = [np.tril(np.ones((n, n), bool)) for n in batch.new]
+    q = synth.normal(93, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    causal, causal_tol = attend64(cache, batch, q, heads, window, sinks)
+    for cleared in (True, False):
+        trees.seen = [x & ((np.subtract.outer(np.arange(n), np.arange(n)) < window) | (m - n + np.arange(n) < sinks)) if cleared else x
+                      for x, n, m in zip(chain, batch.new, cache.lengths)]
+        trees.words = np.concatenate([ref.words(x, trees.stride) for x in trees.seen])
+        got = tree_attend(cache, batch, q, heads, trees.upload(), window, sinks)
+        want, tol = ref.tree64(cache, batch, q, heads, trees.depth, trees.seen, window, sinks)
+        close(got, want, tol)
+        if cleared:
+            close(got, causal, causal_tol)
     smq.numeric_check()
 
 
