@@ -1757,12 +1757,17 @@ static bool pools_apart(smq::Pool *p, uint32_t n, const smq::PagedArgs &a, const
     /* the layers of one buffer for each kind, one after another: looked at once */
     auto at = [](const smq::Pool &x, uint32_t k) { return (uintptr_t)(k == 0 ? x.keys : k == 1 ? x.values : k == 2 ? x.ks : x.vs); };
     bool plain = true;
-    for (uint32_t k = 0; k < kinds; ++k) {
-        const size_t bytes = k < 2 ? codes : scales;
-        for (uint32_t i = 1; i < n; ++i) plain = plain && at(p[i], k) >= at(p[i - 1], k) && at(p[i], k) - at(p[i - 1], k) >= bytes;
-        for (uint32_t j = 0; j < k; ++j)
-            plain = plain && (at(p[n - 1], k) + bytes <= at(p[0], j) || at(p[n - 1], j) + (j < 2 ? codes : scales) <= at(p[0], k));
+    for (uint32_t i = 1; i < n; ++i) {
+        plain &= at(p[i], 0) >= at(p[i - 1], 0) + codes;
+        plain &= at(p[i], 1) >= at(p[i - 1], 1) + codes;
     }
+    for (uint32_t i = 1; i < n && kinds == 4; ++i) {
+        plain &= at(p[i], 2) >= at(p[i - 1], 2) + scales;
+        plain &= at(p[i], 3) >= at(p[i - 1], 3) + scales;
+    }
+    auto end = [&](uint32_t k) { return at(p[n - 1], k) + (k < 2 ? codes : scales); };
+    for (uint32_t k = 1; k < kinds && plain; ++k)
+        for (uint32_t j = 0; j < k; ++j) plain &= end(k) <= at(p[0], j) || end(j) <= at(p[0], k);
     if (plain) return true;
     auto same = [&](const smq::Pool &x, const smq::Pool &y) {
         return x.keys == y.keys && x.values == y.values && (kinds == 2 || (x.ks == y.ks && x.vs == y.vs));
