@@ -6,8 +6,9 @@ namespace smq {
 namespace {
 
 /* A workgroup per sequence, its parents in LDS; a thread per word of a row walks the row's ancestors, which descend, until
- * they are below the word. Depths by the thread of word 0, which walks them all. Bound by the launch, two trips to memory and the
- * deepest token's walk: 24 trees of 40 3.7 us, one of 13 1.9. */
+ * they are below the word. Depths by the thread of word 0, which walks them all. Trees of drafts are bound by the launch, two
+ * trips to memory and the deepest token's walk: 24 trees of 40 3.7 us, one of 13 1.9. Chains are bound by the walks of all
+ * words on one CU, which grow with tokens * words * depth: of 40 4.7 us, 100 10, 400 240, 1000 3.5 ms, 4096 221 ms. */
 constexpr uint32_t DM_WG = 256, DM_MOST = 32 * MAX_MASK_WORDS;
 __global__ __launch_bounds__(DM_WG) void k_draft_masks(PagedArgs a, const int32_t *parent, int32_t *depth, uint32_t *mask,
                                                        uint32_t words) {

@@ -605,8 +605,9 @@ uint32_t tree_rows(const PagedArgs &a) {
     const double steps = reach / PA_STEP + 1;
     /* Of one 32-wide step, by type, heads of up to 64 first: tiles of 16 rows (and where heads are of 128), of 64, of 128. A
      * tile brings a step (and converts Q8 codes) once, whatever its rows, and then each wave has its part: the tiles' rates
-     * and those of their waves' 16 and 32 rows. Fitted to 351 batches and tried on 194 others: the choice costs 1 and 2 % of the
-     * best tile's time on average. */
+     * and those of their waves' 16 and 32 rows. Fitted to 351 batches and tried on 194 others (profiles/tree_tile_rows.csv): the
+     * choice costs 1.8 and 3.1 % of the best tile's time on average, at most 59 % (24 f32 drafts of 16 at 1000) and, for heads
+     * above 128 at short contexts, 93 %. */
     static const double rate[2][3][6] = {
         {{1060, 1060, 870, 4050, 1050, 1080}, {2740, 2740, 3140, 12100, 5600, 3850}, {2800, 2800, 1910, 9100, 820, 6280}},
         {{1050, 1070, 710, 5800, 320, 4400}, {2480, 1890, 2190, 52000, 2290, 7560}, {2640, 1880, 3890, 5200, 1800, 2750}}};
