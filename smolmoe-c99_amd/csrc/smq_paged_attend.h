@@ -680,8 +680,9 @@ struct Rows {
     /* Products to weights, and their sums. */
     __device__ __forceinline__ void weights(uint32_t p0, uint32_t ok, bool full, float (&x)[RT][8]) {
         if (!full) {
-            /* positions of a page that is none: past every row */
-            const uint32_t p = ok >> (quad >> 1) & 1 ? p0 + quad * 8 : 0xfffffff0u;
+            /* positions of a page that is none: past every row, and far before any token of a tree (whose first one may stand at a
+             * negative position, down to -2^26) */
+            const uint32_t p = ok >> (quad >> 1) & 1 ? p0 + quad * 8 : TREE ? 0xc0000000u : 0xfffffff0u;
 #pragma unroll
             for (int c = 0; c < RT; ++c) {
                 if constexpr (TREE) vis[c] = seen8(p, c);

@@ -521,6 +521,29 @@ def test_tree_rows_that_are_refused_on_the_device(kv_type):
 
 
 @pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("page", [16, 64])
+def test_tree_of_more_tokens_than_positions_without_pages(kv_type, page):
+    """New tokens that begin before position 0, and no page for those that have a place: nothing is seen, and the other
+    sequence is as ever."""
+    heads, kv, hd = 4, 2, 64
+    cache = Cache(kv_type, kv, hd, page, [64, 40]).upload()
+    table = cache.table.copy()
+    for new in (60, 20):  # owned and shared tiles
+        batch = Batch(cache, [new, 7], lengths=[12, 40])
+        trees = Trees(batch)
+        q = synth.normal(95, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+        first = Batch(cache, [0, 7], lengths=[12, 40])
+        want, tol = ref.tree64(cache, first, q[new:], heads, trees.depth[new:], [np.zeros((0, 0), bool), trees.seen[1]])
+        trees.words[:new] = 0xFFFFFFFF
+        table[0] = -1
+        cache.tb.upload(table)
+        got = tree_attend(cache, batch, q, heads, trees.upload(), context=64)
+        assert flagged()
+        assert (got[:new] == 0).all()
+        close(got[new:], want, tol)
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
 def test_tree_values_that_are_not_finite_stay_where_they_are_seen(kv_type):
     """A drafted token's NaN value reaches its descendants and nobody else."""
     heads, kv, hd = 4, 2, 64
