@@ -501,8 +501,8 @@ smq_status smq_draft_masks(const int32_t *parent, const smq_paged_batch *batch, 
  * window: where drafts reach as deep as one, the caller clears the bits of the
  * ancestors w or more levels above that are no sinks, and a chain's attention
  * is smq_paged_attention's). mask as smq_draft_masks writes it, or any other:
- * bits behind the last new token do not matter. A row
- * that sees nothing is 0. Numbers, errors, workspace and what does not matter
+ * bits behind the last new token, and of those without a place, do not matter.
+ * A row that sees nothing is 0. Numbers, errors, workspace and what does not matter
  * as smq_paged_attention's; a depth below 0 or where p is not below the
  * context's size raises the numeric flag, its row is 0, and so are those of a
  * sequence of more than 32 * mask_stride new tokens. All pages of the new

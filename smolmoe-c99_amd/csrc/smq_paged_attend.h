@@ -548,7 +548,7 @@ struct Rows {
         int pmax = __builtin_amdgcn_readfirstlane(hi);
         if constexpr (TREE) {
             ctx = sq.first;
-            count_new = sq.n;
+            count_new = min(sq.n, (int)a.limit - sq.first); /* those that have a place */
             low_last = (uint32_t)pmax;
             span = tree_span(a, sq);
             pmax = span.high;

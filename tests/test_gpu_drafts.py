@@ -544,6 +544,31 @@ def test_tree_of_more_tokens_than_positions_without_pages(kv_type, page):
 
 
 @pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("page,length,new,limit", [(32, 44, 12, 40), (64, 200, 90, 150), (16, 60, 30, 48)])
+def test_tree_tokens_without_a_place_are_not_seen(kv_type, page, length, new, limit):
+    """New tokens past the context, or past a table whose last page ends inside a step: no row sees them, whatever its mask and
+    whatever their slots hold."""
+    heads, kv, hd = 4, 2, 64
+    cache = Cache(kv_type, kv, hd, page, [length, 20])
+    cache.spoil_positions(0, np.arange(limit, length))
+    cache.upload()
+    batch = Batch(cache, [new, 7])
+    short = Batch(cache, [new - (length - limit), 7], lengths=[limit, 20])
+    trees, there = Trees(batch), np.concatenate([np.arange(short.new[0]), np.arange(new, new + 7)])
+    trees.words[:new] = 0xFFFFFFFF
+    q = synth.normal(96, batch.tokens * heads * hd, 1.5).reshape(-1, heads, hd)
+    want, tol = ref.tree64(cache, short, q[there], heads, trees.depth[there], [np.ones((short.new[0],) * 2, bool), trees.seen[1]])
+    if page == 16:  # the table's last page is the third
+        cache.table = np.ascontiguousarray(cache.table[:, :3])
+        cache.tb, cache.stride = dev(cache.table), 3
+        batch = Batch(cache, [new, 7])
+    got = tree_attend(cache, batch, q, heads, trees.upload(), context=limit if page != 16 else 64)
+    assert flagged()
+    close(got[there], want, tol)
+    assert (got[short.new[0]:new] == 0).all()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
 def test_tree_values_that_are_not_finite_stay_where_they_are_seen(kv_type):
     """A drafted token's NaN value reaches its descendants and nobody else."""
     heads, kv, hd = 4, 2, 64
