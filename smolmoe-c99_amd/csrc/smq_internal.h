@@ -324,6 +324,7 @@ struct Pool { /* keys null: another one is the same pool */
 };
 struct Pools { /* of a launch */
     uint32_t n;
+    uint64_t again; /* a bit for each without keys */
     Pool p[POOLS_AT_ONCE];
 };
 size_t fork_workspace(uint32_t pages, uint32_t rows);

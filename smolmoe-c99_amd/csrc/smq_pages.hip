@@ -483,7 +483,7 @@ __global__ __launch_bounds__(PG_WG) void k_paged_copy(PagedArgs a, Pools pools, 
     }
     const uint32_t EB = 4 >> a.type;
     const Pool &p = pools.p[l];
-    if (!p.keys) return;
+    if (pools.again >> l & 1) return;
     const size_t f = (size_t)from * a.kv_heads + h, t = (size_t)to * a.kv_heads + h;
     char *x = (char *)(kind ? p.values : p.keys), *w = (char *)(kind ? p.vs : p.ks);
     const size_t head = ((size_t)a.head_dim << a.shift) * EB, scales = ((size_t)a.nb << a.shift) * 4;
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(PG_WG) void k_paged_compact(PagedArgs a, Pools pool
     good = __syncthreads_and(good);
     if (tid == 0 && !good) *a.flag = 1;
     if (length_out && y % pools.n == 0 && h == 0 && tid == 0) length_out[s] = good ? sq.first + m : a.length[s];
-    if (!good || !__syncthreads_or(moved) || !p.keys) return; /* no keys: the pool is another one's again */
+    if (!good || !__syncthreads_or(moved) || (pools.again >> y % pools.n & 1)) return;
     const uint32_t hd = a.head_dim, shift = a.shift, nb = a.nb, pieces = hd * EB / 16;
     const uint32_t kn = pieces > kx ? (pieces - kx + 15) / 16 : 0, vn = hd / 16, vstep = 16 * EB << shift;
     for (uint32_t k0 = 0; k0 < (uint32_t)m; k0 += CM_TOKENS) {
@@ -642,7 +642,11 @@ hipError_t each_pools(const PagedArgs &a, const Pool *pools, uint32_t n, uint32_
     for (uint32_t i = 0; i < n; i += step) {
         Pools p;
         p.n = n - i < step ? n - i : step;
-        for (uint32_t k = 0; k < p.n; ++k) p.p[k] = pools[i + k];
+        p.again = 0;
+        for (uint32_t k = 0; k < p.n; ++k) {
+            p.p[k] = pools[i + k];
+            p.again |= (uint64_t)!pools[i + k].keys << k;
+        }
         launch(p, i == 0);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
